@@ -462,6 +462,126 @@ size_t ssa_sparse_attention_backward_routed_workspace_bytes(int dtype, int dout_
                                                             int64_t n, int h_q, int h_kv, int d, int top_k,
                                                             int a, int b, int n_c, int64_t bitmap_rows);
 
+/* ---- dense attention with a key interval per row ------------------------ */
+
+/* Key intervals [lo, hi) of the usual masks, int32 [batch][n_q][2], for
+ * ssa_masked_attention: query token i sits at key position q_pos0 + i of n keys.
+ *   doc_starts (nullable) int32 [batch][docs + 1], ascending: document x of a
+ *       sequence is the keys [doc_starts[x], doc_starts[x + 1]) and a token sees
+ *       its own only; one before the first or from the last start on sees none.
+ *       NULL: the sequence is one document (docs = 1).
+ *   causal != 0: keys up to the token's own position; with prefix_lens (nullable
+ *       int32 [batch][docs]) also the first prefix_lens[x] keys of its document,
+ *       whatever its position.  causal == 0: the whole document.
+ * No reference counterpart (the reference's dense attention takes an [n][n] bool
+ * mask, ssa/attention.py:118-158). */
+int ssa_mask_spans(const int32_t* doc_starts, int docs, const int32_t* prefix_lens, int64_t batch, int64_t n,
+                   int64_t n_q, int64_t q_pos0, int causal, int32_t* spans, void* stream);
+
+/* out[b][i][hq] = softmax_j(s) . v[b][j][h], h = hq / (h_q / h_kv), over the keys
+ * lo <= j < hi of spans[b][i] (clamped to [0, n); NULL: j <= q_pos0 + i), with
+ *   s = q[b][i][hq] . k[b][j][h] / scale_div,
+ *   softcap c > 0:  s = c tanh(s / c)   (0: none),
+ *   slopes (nullable) fp32 [h_q]:  s -= slopes[hq] |q_pos0 + i - j|.
+ * A row that sees no key is zeros; a key that a row does not see has no influence
+ * on it, whatever it holds.  Scores, weights' sums and products accumulate in
+ * fp32; bf16 inputs round each weight to bf16 for the product with v.
+ * Replaces dense_attention (ssa/attention.py:118-158) for masks of this form; the
+ * cap and the distance bias have no reference counterpart.
+ *   q [batch][n_q][h_q][d], k, v [batch][n][h_kv][d], out as q, all of type dtype,
+ *   rows aligned to 16 bytes.
+ *   out_low (nullable, out's strides and type) what rounding out to bf16 leaves
+ *       of each value, rounded to bf16 (zeros for fp32), and
+ *   lse (nullable) fp32 [batch][h_q][n_q] log2 of each row's sum of exp(s) (+inf
+ *       for a row without a key): for the backward.
+ *   workspace: ssa_masked_attention_workspace_bytes(...) bytes (0 for most shapes;
+ *       few rows over many keys are split along the keys).
+ * Limits: d a multiple of 8 up to 128, h_q / h_kv <= 16. */
+size_t ssa_masked_attention_workspace_bytes(int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv, int d);
+int ssa_masked_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t n,
+                         int64_t n_q, int64_t q_pos0, int h_q, int h_kv, int d, int64_t q_sb, int64_t q_sn,
+                         int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn,
+                         int64_t v_sh, const int32_t* spans, float scale_div, float softcap, const float* slopes,
+                         void* out, int64_t o_sb, int64_t o_sn, int64_t o_sh, void* out_low, float* lse,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of ssa_masked_attention with respect to q, k and v, given its output,
+ * out_low (nullable: D = dout . out then takes the rounded output), its lse and the
+ * output gradient.  Same arguments for the forward's; dout has
+ * out's shape and type with its own strides.
+ *   dq [batch][n_q][h_q][d], dk, dv [batch][n][h_kv][d], contiguous, of type dtype:
+ *      written whole (a shared head's sums over its group included), each value
+ *      rounded once.  No atomics: the same inputs give the same bits.
+ *   workspace: ssa_masked_attention_backward_workspace_bytes(...) bytes.
+ * Replaces the autograd backward of dense_attention (ssa/attention.py:118-158)
+ * for masks of this form.  slopes get no gradient. */
+size_t ssa_masked_attention_backward_workspace_bytes(int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv,
+                                                     int d);
+int ssa_masked_attention_backward(
+    const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t n, int64_t n_q,
+    int64_t q_pos0, int h_q, int h_kv, int d, int64_t q_sb, int64_t q_sn, int64_t q_sh, int64_t k_sb,
+    int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn, int64_t v_sh, const int32_t* spans,
+    float scale_div, float softcap, const float* slopes, const void* out, const void* out_low,
+    int64_t o_sb, int64_t o_sn, int64_t o_sh, const void* dout, int64_t do_sb, int64_t do_sn, int64_t do_sh,
+    const float* lse, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- paged cache --------------------------------------------------------- */
+
+/* Attention of new tokens over a paged K/V cache, a ragged batch in one call.
+ * Sequence b's new tokens are rows starts[b] .. starts[b + 1] - 1 of q, k, v and
+ * out ([tokens][heads][d], strides *_st, *_sh); its key j is row j % page_size of
+ * page table[b][j / page_size] of the pools k_pages, v_pages
+ * [num_pages][page_size][h_kv][d] (strides *_sp, *_st, *_sh), and cached[b] keys
+ * are there already.  The call writes the new rows of k and v at keys cached[b]
+ * ... (k = v = NULL: they are there) and attends new token t over keys
+ * 0 .. cached[b] + t with ssa_masked_attention's score rule (positions count from
+ * the sequence's first key).
+ *   table int32 [batch][max_pages] (row stride table_stride), starts int32
+ *       [batch + 1] ascending, cached int32 [batch]: device memory, read by the
+ *       kernels, so that a captured call follows their values.
+ *   max_new, max_len: the most new tokens and the most keys (new ones included) of
+ *       a sequence; the launch is sized by them.
+ *   A sequence that breaks them, or the table's or the rows' range, is left out
+ *       (its rows of out and its pages stay as they are), a page outside the pool
+ *       is not touched (keys there read page 0): either sets *error_flag
+ *       (nullable) to 1.  Rows of out of no sequence stay as they are.
+ *   workspace: ssa_paged_step_workspace_bytes(...) bytes; calls that may run at
+ *       once each need their own.
+ * Limits: as ssa_masked_attention; page_size a power of 2 in [8, 4096].
+ * No reference counterpart (ssa_design.md:225-234 describes decoding against a
+ * cache; its code runs whole sequences). */
+size_t ssa_paged_step_workspace_bytes(int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t max_new,
+                                      int64_t max_len);
+int ssa_paged_step(const void* q, const void* k, const void* v, int dtype, int64_t tokens, int64_t batch, int h_q,
+                   int h_kv, int d, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st,
+                   int64_t v_sh, void* k_pages, void* v_pages, int64_t num_pages, int page_size, int64_t kp_sp,
+                   int64_t kp_st, int64_t kp_sh, int64_t vp_sp, int64_t vp_st, int64_t vp_sh,
+                   const int32_t* table, int64_t table_stride, int max_pages, const int32_t* starts,
+                   const int32_t* cached, int64_t max_new, int64_t max_len, float scale_div, float softcap,
+                   const float* slopes, void* out, int64_t o_st, int64_t o_sh, int32_t* error_flag,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- rotary positions with several axes ---------------------------------- */
+
+/* Rotary embedding of q and k (k nullable with h_k = 0) whose tokens have a
+ * position on each of `axes` axes (1 to 4): feature pair (m, m + rot / 2) turns by
+ * positions[axis(m)][b][i] * freqs[m], the first sections[0] pairs by axis 0, the
+ * next sections[1] by axis 1 and so on (sections: int32 [axes] in HOST memory, read
+ * by the call, their sum rot / 2).  Features from rot on pass through.
+ *   q [batch][n][h_q][d], k [batch][n][h_k][d], outputs likewise with their own
+ *       strides; an output may be its input (same strides).
+ *   positions int32 or int64 (SSA_INDEX_*) [axes][batch][n], strides p_sa, p_sb
+ *       (0 to share), contiguous along n; freqs fp64 [rot / 2].
+ *   inverse != 0 applies the transpose (the backward).
+ * Angles are formed and reduced in 64 bits, the rotation is fp32, the result
+ * rounded once.  No reference counterpart (ssa/utils.py:7-41 has one axis). */
+int ssa_rope_axes(const void* q, const void* k, int dtype, int64_t batch, int64_t n, int h_q, int h_k, int d,
+                  int64_t q_sb, int64_t q_sn, int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh,
+                  const void* positions, int pos_dtype, int64_t p_sa, int64_t p_sb, int axes,
+                  const int32_t* sections, const double* freqs, int rot, int inverse, void* q_out, int64_t qo_sb,
+                  int64_t qo_sn, int64_t qo_sh, void* k_out, int64_t ko_sb, int64_t ko_sn, int64_t ko_sh,
+                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,11 +10,21 @@ Re-exports the reference package's public names (ssa/__init__.py:13-28):
     ToyTransformerBlock     LayerNorm + SSAAttention + FFN block
     apply_rope, precompute_rope_freqs, build_causal_mask, expand_kv_for_gqa
 
+and adds, for the dense layers beside it:
+
+    masked_attention, mask_spans      attention over a key interval per row (causal,
+                                      documents, prefixes), capped or biased scores
+    paged_step, PagedKVCache          new tokens over a paged K/V cache
+    rope_axes, axis_rope_freqs        rotary positions with several axes
+
 The hot path runs in libssa_hip.so (hand-written HIP for gfx950) through a C
 ABI (include/ssa_hip.h); there is no CPU or PyTorch fallback for it.
 """
 
 from .attention import dense_attention, sparse_exact_attention
+from .axes import axis_rope_freqs, rope_axes
+from .masked import mask_spans, masked_attention
+from .paged import PagedKVCache, paged_step
 from .router import CodebookRouter
 from .ssa_layer import SSAAttention, ToyTransformerBlock
 from .utils import (
@@ -35,4 +45,10 @@ __all__ = [
     "precompute_rope_freqs",
     "build_causal_mask",
     "expand_kv_for_gqa",
+    "masked_attention",
+    "mask_spans",
+    "paged_step",
+    "PagedKVCache",
+    "rope_axes",
+    "axis_rope_freqs",
 ]

@@ -53,4 +53,16 @@ int attention_entry(const void* q, const void* k, const void* v, int dtype, int6
                     size_t workspace_bytes = 0, const int32_t* row_prefix = nullptr,
                     float* row_stats = nullptr);
 
+namespace tile {
+struct ScoreRule;
+}
+
+// Argument checks and rules of the dense attention entry points (fn names the
+// caller in the message).
+int check_heads(const char* fn, int dtype, int h_q, int h_kv, int d);
+int check_aligned(const char* fn, const char* name, int dtype, const void* ptr, int64_t s0, int64_t s1, int64_t s2);
+int score_rule(const char* fn, float scale_div, float softcap, const float* slopes, tile::ScoreRule* r);
+// Parts of the key axis for a forward of `blocks` row blocks over `keys` keys.
+int dense_splits(int64_t blocks, int64_t keys);
+
 }  // namespace ssa

@@ -1,0 +1,705 @@
+// Gradients of dense attention with a key interval per row
+// (ssa_masked_attention_backward).  With s the score rule's scores, t the cap's
+// tanh (0 without), p = exp(s - lse) over the visible keys, D_i = dO_i . o_i:
+//
+//   dV_j = sum_i p_ij dO_i          dS_ij = p_ij (dO_i . v_j - D_i) (1 - t_ij^2)
+//   dQ_i = sum_j dS_ij k_j / scale  dK_j  = sum_i dS_ij q_i / scale
+//
+// D takes a bf16 output with what its rounding left (out_low): from the rounded
+// one alone, D's error enters every dS of the row, and with few keys a row dq and
+// dk end 1.7 times as far from 64 bits as their own rounding puts them (1.45 with
+// it; 2^-8 roundings of P and dS are the rest).
+//
+// Two kernels and no atomics, so the sums' order is fixed: dq_kernel by rows
+// (S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T), which also writes D and each
+// 32-row group's interval bounds, then dkv_kernel by keys (S = Q K^T, dP = dO
+// V^T, dV^T += dO^T P, dK^T += Q^T dS) over the rows of all g query heads, so a
+// shared head's gradient is summed in its block.  S and dP are computed twice:
+// 7 products for the 5 of a single kernel, whose dQ would need fp32 atomics
+// (read-modify-writes of n x h_q x d floats for every 128 keys, and sums whose
+// order changes from run to run).
+//
+// Masked rows or keys that hold infinities or NaN: as in the forward, sums that
+// end up other than finite are computed again pair by pair, visible pairs only.
+
+#include <math.h>
+
+#include "ssa_internal.h"
+#include "ssa_tile.h"
+
+namespace ssa {
+namespace {
+
+using namespace tile;
+
+struct BwdParams {
+  const void *q, *k, *v, *out, *out_low, *dout;
+  const float* lse;
+  void *dq, *dk, *dv;
+  int64_t q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh, o_sb, o_sn, o_sh, do_sb, do_sn, do_sh;
+  int64_t n, n_q, q_pos0;
+  int batch, h_q, h_kv, g, d;
+  const int2* spans;
+  ScoreRule rule;
+  float inv_scale;
+  float* dsum;    // [batch][h_q][n_q]: D
+  int4* bounds;   // [batch][groups of 32 packed rows]: lo_min, hi_max, lo_max, hi_min
+  int groups;
+  int splits;     // parts of the rows for dK and dV
+  int split_groups;
+  float *part_k, *part_v;  // [splits][batch][n][h_kv][D]
+};
+
+constexpr int kBlk = 128;  // rows or keys of a block
+
+__device__ __forceinline__ int2 row_span(const BwdParams& p, int b, int tok) {
+  int lo = 0, hi;
+  if (p.spans != nullptr) {
+    const int2 s = p.spans[b * p.n_q + tok];
+    lo = max(s.x, 0);
+    hi = static_cast<int>(min(static_cast<int64_t>(s.y), p.n));
+  } else {
+    hi = static_cast<int>(min(p.q_pos0 + tok + 1, p.n));
+  }
+  return hi > lo ? make_int2(lo, hi) : make_int2(0, 0);
+}
+
+// x (log2 units) and 1 - t^2 of a raw product.
+template <typename T, bool RULE>
+__device__ __forceinline__ float score_x(const ScoreRule& r, float dot, float slope, float dist, float& factor) {
+  factor = 1.0f;
+  float x = dot * r.c1;
+  if constexpr (RULE) {
+    if (r.cap) {
+      const float t = cap_tanh<T>(x);
+      factor = fmaf(-t, t, 1.0f);
+      x = r.c2 * t;
+    }
+    x = fmaf(-slope, fabsf(dist), x);
+  }
+  return x;
+}
+
+template <typename T>
+__device__ __forceinline__ float row_dot(const T* a, const T* b, int d) {
+  float s = 0.0f;
+  for (int e = 0; e < d; e += 8) s = Op<T>::dot(Op<T>::load(a + e), Op<T>::load(b + e), s);
+  return s;
+}
+
+__device__ __forceinline__ const void* lane_ptr(const void* x, int src) {
+  const uint64_t u = reinterpret_cast<uint64_t>(x);
+  return reinterpret_cast<const void*>(
+      (static_cast<uint64_t>(static_cast<uint32_t>(lane_value(static_cast<int>(u >> 32), src))) << 32) |
+      static_cast<uint32_t>(lane_value(static_cast<int>(u & 0xFFFFFFFFu), src)));
+}
+
+template <typename T, int D, bool RULE>
+__global__ __launch_bounds__(kThreads, 2) void dq_kernel(BwdParams p) {
+  using O = Op<T>;
+  using Frag = typename O::Frag;
+  constexpr int RB = D * O::kEsize, NCH = RB / 16, E = 16 / O::kEsize;
+  constexpr int KT = sizeof(T) == 2 ? 64 : 32;
+  constexpr int NSUB = KT / 32, NC = D / 16, ND = D / 32;
+  constexpr int RPP = kThreads / NCH, NP = KT / RPP, TB = KT * RB;
+  extern __shared__ __align__(16) char lds[];
+  __shared__ int s_range[4][2];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int nbh = p.batch * p.h_kv;
+  const int bh = blockIdx.x % nbh;
+  const int tiles = static_cast<int>((p.n_q * p.g + kBlk - 1) / kBlk);
+  const int tile = tiles - 1 - static_cast<int>(blockIdx.x / nbh);
+  const int b = bh / p.h_kv, kvh = bh - b * p.h_kv;
+  const int n_keys = static_cast<int>(p.n);
+
+  const int r = tile * kBlk + wave * 32 + (lane & 31);
+  const bool real = r < p.n_q * p.g;
+  const int tok = real ? r / p.g : 0;
+  const int hq = kvh * p.g + (real ? r - tok * p.g : 0);
+  const int pos = static_cast<int>(p.q_pos0) + tok;
+  const int2 sp = real ? row_span(p, b, tok) : make_int2(0, 0);
+  const int lo = sp.x, hi = sp.y;
+  const bool some = real && hi > lo;
+  const float slope = (RULE && p.rule.slopes != nullptr && real) ? p.rule.slopes[hq] * kLog2e : 0.0f;
+  const int lo_min = wave_min_i(some ? lo : 0x7FFFFFFF), hi_max = wave_max_i(some ? hi : 0);
+  const int lo_max = wave_max_i(real ? lo : 0), hi_min = wave_min_i(real ? hi : 0x7FFFFFFF);
+  if (lane == 0) {
+    s_range[wave][0] = lo_min;
+    s_range[wave][1] = hi_max;
+    const int grp = tile * 4 + wave;
+    if (kvh == 0 && grp < p.groups) p.bounds[static_cast<int64_t>(b) * p.groups + grp] = make_int4(lo_min, hi_max, lo_max, hi_min);
+  }
+  __syncthreads();
+  const int k_lo = min(min(s_range[0][0], s_range[1][0]), min(s_range[2][0], s_range[3][0]));
+  const int k_hi = max(max(s_range[0][1], s_range[1][1]), max(s_range[2][1], s_range[3][1]));
+  const int t0 = k_lo / KT, nt = k_hi > k_lo ? (k_hi + KT - 1) / KT - t0 : 0;
+
+  const T* kbase = static_cast<const T*>(p.k) + b * p.k_sb + kvh * p.k_sh;
+  const T* vbase = static_cast<const T*>(p.v) + b * p.v_sb + kvh * p.v_sh;
+  const T* qrow = static_cast<const T*>(p.q) + b * p.q_sb + tok * p.q_sn + hq * p.q_sh;
+  const T* dorow = static_cast<const T*>(p.dout) + b * p.do_sb + tok * p.do_sn + hq * p.do_sh;
+  const T* orow = static_cast<const T*>(p.out) + b * p.o_sb + tok * p.o_sn + hq * p.o_sh;
+  const int64_t stat = (static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok;
+  const float lse = some ? p.lse[stat] : INFINITY;
+  Frag qf[NC], dof[NC];
+  float dsum = 0.0f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int e = 16 * c + 8 * half;
+    const bool in = some && e < p.d;
+    qf[c] = in ? O::load(qrow + e) : O::zero();
+    dof[c] = in ? O::load(dorow + e) : O::zero();
+    const Frag of = in ? O::load(orow + e) : O::zero();
+    dsum = O::dot(dof[c], of, dsum);
+    if (p.out_low != nullptr) {
+      const Frag lf = in ? O::load(static_cast<const T*>(p.out_low) + (orow - static_cast<const T*>(p.out)) + e) : O::zero();
+      dsum = O::dot(dof[c], lf, dsum);
+    }
+  }
+  dsum += other_half(dsum);
+  if (real && half == 0) p.dsum[stat] = dsum;
+
+  const int sc = tid % NCH, sr = tid / NCH;
+  const bool chunk_ok = sc * E < p.d;
+  uint4 kreg[NP], vreg[NP];
+  auto load_tile = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int64_t j = min((t0 + t) * KT + sr + i * RPP, n_keys - 1);
+      kreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(kbase + j * p.k_sn + sc * E) : make_uint4(0u, 0u, 0u, 0u);
+      vreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(vbase + j * p.v_sn + sc * E) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  auto store_tile = [&](int buf) {
+    char* kt = lds + buf * 2 * TB;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int at = chunk_at<RB>(sr + i * RPP, sc);
+      *reinterpret_cast<uint4*>(kt + at) = kreg[i];
+      *reinterpret_cast<uint4*>(kt + TB + at) = vreg[i];
+    }
+  };
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) acc[i] = f32x16{};
+  if (nt > 0) {
+    load_tile(0);
+    store_tile(0);
+  }
+  for (int t = 0; t < nt; ++t) {
+    __syncthreads();
+    if (t + 1 < nt) load_tile(t + 1);
+    const char* kt = lds + (t & 1) * 2 * TB;
+    const char* vt = kt + TB;
+#pragma unroll
+    for (int u = 0; u < NSUB; ++u) {
+      const int k0 = (t0 + t) * KT + 32 * u;
+      if (k0 < hi_max && k0 + 32 > lo_min) {
+        f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          s = O::mfma(O::template row_frag<RB>(kt, 32 * u, c, lane), qf[c], s);
+          dp = O::mfma(O::template row_frag<RB>(vt, 32 * u, c, lane), dof[c], dp);
+        }
+        const int kl = k0 + 4 * half;
+        const float dist = static_cast<float>(kl - pos);
+        const bool whole = k0 >= lo_max && k0 + 32 <= hi_min;
+        const int a = lo - kl, z = hi - kl;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = 8 * (i >> 2) + (i & 3);
+          float f;
+          const float x = score_x<T, RULE>(p.rule, s[i], slope, dist + static_cast<float>(j), f);
+          const float w = exp2_w(x - lse) * (dp[i] - dsum) * f;
+          s[i] = whole || (j >= a && j < z) ? w : 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const Frag df = O::pack(s, c);
+#pragma unroll
+          for (int i = 0; i < ND; ++i) acc[i] = O::mfma(O::template col_frag<RB>(kt, 32 * u + 16 * c, 32 * i, lane), df, acc[i]);
+        }
+      }
+    }
+    if (t + 1 < nt) store_tile((t + 1) & 1);
+  }
+
+  float worst = 0.0f;
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) worst = finite(acc[i][e]) ? worst : 1.0f;
+  worst = fmaxf(worst, other_half(worst));
+  const bool again = some && worst != 0.0f;
+  T* dqrow = static_cast<T*>(p.dq) + ((static_cast<int64_t>(b) * p.n_q + tok) * p.h_q + hq) * p.d;
+  if (real && !again) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int dd = 32 * i + 8 * e + 4 * half;
+        const float z = some ? p.inv_scale : 0.0f;
+        if (dd < p.d)
+          O::store4(dqrow + dd, some ? acc[i][4 * e] * z : 0.0f, some ? acc[i][4 * e + 1] * z : 0.0f,
+                    some ? acc[i][4 * e + 2] * z : 0.0f, some ? acc[i][4 * e + 3] * z : 0.0f);
+      }
+  }
+  uint64_t todo = __ballot(again && half == 0);
+  while (todo != 0) {
+    const int src = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    const int a = lane_value(lo, src), z = lane_value(hi, src), ps = lane_value(pos, src);
+    const float sl = lane_value(slope, src), ls = lane_value(lse, src), ds0 = lane_value(dsum, src);
+    const T* qr = static_cast<const T*>(lane_ptr(qrow, src));
+    const T* dr = static_cast<const T*>(lane_ptr(dorow, src));
+    T* dst = const_cast<T*>(static_cast<const T*>(lane_ptr(dqrow, src)));
+    float o[2] = {0.0f, 0.0f};
+    for (int j0 = a; j0 < z; j0 += 64) {
+      const int j = min(j0 + lane, z - 1);
+      float f;
+      const float x = score_x<T, RULE>(p.rule, row_dot(qr, kbase + j * p.k_sn, p.d), sl, static_cast<float>(j - ps), f);
+      const float w = exp2_w(x - ls) * (row_dot(dr, vbase + j * p.v_sn, p.d) - ds0) * f;
+      for (int t = 0; t < min(64, z - j0); ++t) {
+        const float wt = lane_value(w, t);
+        const T* kr = kbase + static_cast<int64_t>(j0 + t) * p.k_sn;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (lane + 64 * e < p.d) o[e] = fmaf(wt, ld(kr + lane + 64 * e), o[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (lane + 64 * e < p.d) O::store1(dst + lane + 64 * e, o[e] * p.inv_scale);
+  }
+}
+
+// What a staged row needs beside its vectors.
+struct RowStat {
+  float lse, dsum, slope, pos;
+};
+
+template <typename T, int D, bool RULE>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && D == 64 ? 2 : 1) void dkv_kernel(BwdParams p) {
+  using O = Op<T>;
+  using Frag = typename O::Frag;
+  constexpr int RB = D * O::kEsize, NCH = RB / 16, E = 16 / O::kEsize;
+  constexpr int QT = 32;  // rows of a tile: one group
+  constexpr int NC = D / 16, ND = D / 32;
+  constexpr int RPP = kThreads / NCH, NP = (QT + RPP - 1) / RPP, TB = QT * RB;
+  extern __shared__ __align__(16) char lds[];
+  __shared__ __align__(16) float s_lse[2][QT], s_dsum[2][QT], s_slope[2][QT], s_pos[2][QT];
+  __shared__ __align__(16) int s_lo[2][QT], s_hi[2][QT];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int nbh = p.batch * p.h_kv;
+  const int bh = blockIdx.x % nbh;
+  const int rest = blockIdx.x / nbh;
+  const int split = rest % p.splits, tile = rest / p.splits;
+  const int b = bh / p.h_kv, kvh = bh - b * p.h_kv;
+  const int n_keys = static_cast<int>(p.n), n_rows = static_cast<int>(p.n_q * p.g);
+  const int kb0 = tile * kBlk;            // the block's keys
+  const int kw0 = kb0 + wave * 32;        // the wave's
+  const int key = kw0 + (lane & 31);
+  const bool real = key < n_keys;
+
+  const T* krow = static_cast<const T*>(p.k) + b * p.k_sb + kvh * p.k_sh + static_cast<int64_t>(real ? key : 0) * p.k_sn;
+  const T* vrow = static_cast<const T*>(p.v) + b * p.v_sb + kvh * p.v_sh + static_cast<int64_t>(real ? key : 0) * p.v_sn;
+  Frag kf[NC], vf[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int e = 16 * c + 8 * half;
+    const bool in = real && e < p.d;
+    kf[c] = in ? O::load(krow + e) : O::zero();
+    vf[c] = in ? O::load(vrow + e) : O::zero();
+  }
+
+  // the groups of rows that see some key of the block, in ascending order
+  const int g_end = min(p.groups, (split + 1) * p.split_groups);
+  const int4* bounds = p.bounds + static_cast<int64_t>(b) * p.groups;
+  int g_base = split * p.split_groups - 64;
+  uint64_t g_mask = 0;
+  auto next_group = [&]() -> int {
+    while (g_mask == 0) {
+      g_base += 64;
+      if (g_base >= g_end) return -1;
+      bool hit = false;
+      if (g_base + lane < g_end) {
+        const int4 bd = bounds[g_base + lane];
+        hit = bd.x < kb0 + kBlk && bd.y > kb0;
+      }
+      g_mask = __ballot(hit);
+    }
+    const int x = __builtin_ctzll(g_mask);
+    g_mask &= g_mask - 1;
+    return g_base + x;
+  };
+
+  const int sc = tid % NCH, sr = tid / NCH;
+  const bool chunk_ok = sc * E < p.d;
+  const T* qbase = static_cast<const T*>(p.q) + b * p.q_sb;
+  const T* dbase = static_cast<const T*>(p.dout) + b * p.do_sb;
+  uint4 qreg[NP], dreg[NP];
+  RowStat st_reg{};
+  int2 sp_reg{};
+  auto load_group = [&](int grp) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int r = min(grp * QT + min(sr + i * RPP, QT - 1), n_rows - 1);
+      const int tok = r / p.g, hq = kvh * p.g + r - tok * p.g;
+      qreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(qbase + tok * p.q_sn + hq * p.q_sh + sc * E) : make_uint4(0u, 0u, 0u, 0u);
+      dreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(dbase + tok * p.do_sn + hq * p.do_sh + sc * E) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (tid < QT) {
+      const int r = grp * QT + tid;
+      const bool in = r < n_rows;
+      const int tok = in ? r / p.g : 0, hq = kvh * p.g + (in ? r - tok * p.g : 0);
+      sp_reg = in ? row_span(p, b, tok) : make_int2(0, 0);
+      const int64_t stat = (static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok;
+      st_reg.lse = sp_reg.y > sp_reg.x ? p.lse[stat] : INFINITY;
+      st_reg.dsum = p.dsum[stat];
+      if constexpr (RULE) {
+        st_reg.slope = p.rule.slopes != nullptr ? p.rule.slopes[hq] * kLog2e : 0.0f;
+        st_reg.pos = static_cast<float>(static_cast<int>(p.q_pos0) + tok);
+      }
+    }
+  };
+  auto store_group = [&](int buf) {
+    char* qt = lds + buf * 2 * TB;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int row = sr + i * RPP;
+      if (QT % RPP != 0 && row >= QT) break;
+      const int at = chunk_at<RB>(row, sc);
+      *reinterpret_cast<uint4*>(qt + at) = qreg[i];
+      *reinterpret_cast<uint4*>(qt + TB + at) = dreg[i];
+    }
+    if (tid < QT) {
+      s_lse[buf][tid] = st_reg.lse;
+      s_dsum[buf][tid] = st_reg.dsum;
+      s_lo[buf][tid] = sp_reg.x;
+      s_hi[buf][tid] = sp_reg.y;
+      if constexpr (RULE) {
+        s_slope[buf][tid] = st_reg.slope;
+        s_pos[buf][tid] = st_reg.pos;
+      }
+    }
+  };
+
+  f32x16 acck[ND], accv[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    acck[i] = f32x16{};
+    accv[i] = f32x16{};
+  }
+  int grp = next_group();
+  if (grp >= 0) {
+    load_group(grp);
+    store_group(0);
+  }
+  for (int t = 0; grp >= 0; ++t) {
+    __syncthreads();
+    const int nxt = next_group();
+    if (nxt >= 0) load_group(nxt);
+    const int4 bd = bounds[grp];
+    if (bd.x < kw0 + 32 && bd.y > kw0) {
+      const int buf = t & 1;
+      const char* qt = lds + buf * 2 * TB;
+      const char* dt = qt + TB;
+      f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        s = O::mfma(O::template row_frag<RB>(qt, 0, c, lane), kf[c], s);
+        dp = O::mfma(O::template row_frag<RB>(dt, 0, c, lane), vf[c], dp);
+      }
+      const bool whole = bd.z <= kw0 && bd.w >= kw0 + 32 && (grp + 1) * QT <= n_rows;
+      const float fkey = static_cast<float>(key);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r0 = 8 * e + 4 * half;
+        const float4 ls = *reinterpret_cast<const float4*>(&s_lse[buf][r0]);
+        const float4 dd = *reinterpret_cast<const float4*>(&s_dsum[buf][r0]);
+        float4 sl = make_float4(0.f, 0.f, 0.f, 0.f), ps = sl;
+        if constexpr (RULE) {
+          sl = *reinterpret_cast<const float4*>(&s_slope[buf][r0]);
+          ps = *reinterpret_cast<const float4*>(&s_pos[buf][r0]);
+        }
+        int4 lo4 = make_int4(0, 0, 0, 0), hi4 = lo4;
+        if (!whole) {
+          lo4 = *reinterpret_cast<const int4*>(&s_lo[buf][r0]);
+          hi4 = *reinterpret_cast<const int4*>(&s_hi[buf][r0]);
+        }
+        const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dv[4] = {dd.x, dd.y, dd.z, dd.w};
+        const float slv[4] = {sl.x, sl.y, sl.z, sl.w}, psv[4] = {ps.x, ps.y, ps.z, ps.w};
+        const int lov[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hiv[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int i = 4 * e + x;
+          float f;
+          const float y = score_x<T, RULE>(p.rule, s[i], slv[x], fkey - psv[x], f);
+          float w = exp2_w(y - lsv[x]);
+          float ds = w * (dp[i] - dv[x]) * f;
+          const bool see = whole || (key >= lov[x] && key < hiv[x]);
+          s[i] = see ? w : 0.0f;
+          dp[i] = see ? ds : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const Frag pf = O::pack(s, c), df = O::pack(dp, c);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          accv[i] = O::mfma(O::template col_frag<RB>(dt, 16 * c, 32 * i, lane), pf, accv[i]);
+          acck[i] = O::mfma(O::template col_frag<RB>(qt, 16 * c, 32 * i, lane), df, acck[i]);
+        }
+      }
+    }
+    if (nxt >= 0) store_group((t + 1) & 1);
+    grp = nxt;
+  }
+
+  float worst = 0.0f;
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) worst = finite(acck[i][e]) && finite(accv[i][e]) ? worst : 1.0f;
+  worst = fmaxf(worst, other_half(worst));
+  const bool again = real && worst != 0.0f;
+  const int64_t kid = (static_cast<int64_t>(b) * p.n + (real ? key : 0)) * p.h_kv + kvh;
+  const int64_t kids = static_cast<int64_t>(p.batch) * p.n * p.h_kv;
+  T* dkrow = static_cast<T*>(p.dk) + kid * p.d;
+  T* dvrow = static_cast<T*>(p.dv) + kid * p.d;
+  float* pk = p.splits > 1 ? p.part_k + (split * kids + kid) * D : nullptr;
+  float* pv = p.splits > 1 ? p.part_v + (split * kids + kid) * D : nullptr;
+  if (real && !again) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int dd = 32 * i + 8 * e + 4 * half;
+        if (dd >= p.d) continue;
+        const float z = p.inv_scale;
+        const float4 a = make_float4(acck[i][4 * e] * z, acck[i][4 * e + 1] * z, acck[i][4 * e + 2] * z, acck[i][4 * e + 3] * z);
+        const float4 c = make_float4(accv[i][4 * e], accv[i][4 * e + 1], accv[i][4 * e + 2], accv[i][4 * e + 3]);
+        if (p.splits > 1) {
+          *reinterpret_cast<float4*>(pk + dd) = a;
+          *reinterpret_cast<float4*>(pv + dd) = c;
+        } else {
+          O::store4(dkrow + dd, a.x, a.y, a.z, a.w);
+          O::store4(dvrow + dd, c.x, c.y, c.z, c.w);
+        }
+      }
+  }
+  uint64_t todo = __ballot(again && half == 0);
+  while (todo != 0) {  // this key's sums again, over the rows that see it
+    const int src = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    const int kj = lane_value(key, src);
+    const T* kr = static_cast<const T*>(lane_ptr(krow, src));
+    const T* vr = static_cast<const T*>(lane_ptr(vrow, src));
+    float ok[2] = {0.0f, 0.0f}, ov[2] = {0.0f, 0.0f};
+    const int r_end = min(n_rows, g_end * QT);
+    for (int r0 = split * p.split_groups * QT; r0 < r_end; r0 += 64) {
+      const int r = r0 + lane;
+      bool see = false;
+      float w = 0.0f, ds = 0.0f;
+      if (r < r_end) {
+        const int tok = r / p.g, hq = kvh * p.g + r - tok * p.g;
+        const int2 sp = row_span(p, b, tok);
+        see = kj >= sp.x && kj < sp.y;
+        if (see) {
+          const int64_t stat = (static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok;
+          const float sl = RULE && p.rule.slopes != nullptr ? p.rule.slopes[hq] * kLog2e : 0.0f;
+          float f;
+          const float x = score_x<T, RULE>(p.rule, row_dot(qbase + tok * p.q_sn + hq * p.q_sh, kr, p.d), sl,
+                                           static_cast<float>(kj) - static_cast<float>(static_cast<int>(p.q_pos0) + tok), f);
+          w = exp2_w(x - p.lse[stat]);
+          ds = w * (row_dot(dbase + tok * p.do_sn + hq * p.do_sh, vr, p.d) - p.dsum[stat]) * f;
+        }
+      }
+      uint64_t on = __ballot(see);
+      while (on != 0) {
+        const int x = __builtin_ctzll(on);
+        on &= on - 1;
+        const int rr = r0 + x, tok = rr / p.g, hq = kvh * p.g + rr - tok * p.g;
+        const float wx = lane_value(w, x), dx = lane_value(ds, x);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (lane + 64 * e < p.d) {
+            ov[e] = fmaf(wx, ld(dbase + tok * p.do_sn + hq * p.do_sh + lane + 64 * e), ov[e]);
+            ok[e] = fmaf(dx, ld(qbase + tok * p.q_sn + hq * p.q_sh + lane + 64 * e), ok[e]);
+          }
+      }
+    }
+    const int64_t id = (static_cast<int64_t>(b) * p.n + kj) * p.h_kv + kvh;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (lane + 64 * e < p.d) {
+        const int dd = lane + 64 * e;
+        if (p.splits > 1) {
+          p.part_k[(split * kids + id) * D + dd] = ok[e] * p.inv_scale;
+          p.part_v[(split * kids + id) * D + dd] = ov[e];
+        } else {
+          O::store1(static_cast<T*>(p.dk) + id * p.d + dd, ok[e] * p.inv_scale);
+          O::store1(static_cast<T*>(p.dv) + id * p.d + dd, ov[e]);
+        }
+      }
+  }
+}
+
+// dk and dv from the parts, four features a thread, in part order.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void dkv_join_kernel(BwdParams p) {
+  const int per = p.d / 4;
+  const int64_t kids = static_cast<int64_t>(p.batch) * p.n * p.h_kv;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (t >= 2 * kids * per) return;
+  const bool isv = t >= kids * per;
+  const int64_t u = isv ? t - kids * per : t, kid = u / per;
+  const int dd = static_cast<int>(u - kid * per) * 4;
+  const float* part = isv ? p.part_v : p.part_k;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int x = 0; x < p.splits; ++x) {
+    const float4 a = *reinterpret_cast<const float4*>(part + (x * kids + kid) * D + dd);
+    s.x += a.x;
+    s.y += a.y;
+    s.z += a.z;
+    s.w += a.w;
+  }
+  Op<T>::store4(static_cast<T*>(isv ? p.dv : p.dk) + kid * p.d + dd, s.x, s.y, s.z, s.w);
+}
+
+template <typename T, int D, bool RULE>
+int launch_bwd(BwdParams& p, hipStream_t st) {
+  const char* fn = "ssa_masked_attention_backward";
+  constexpr int KT = sizeof(T) == 2 ? 64 : 32;
+  const size_t qbytes = 4 * static_cast<size_t>(KT) * D * sizeof(T), kbytes = 4 * static_cast<size_t>(32) * D * sizeof(T);
+  if (int rc = reserve_lds(reinterpret_cast<const void*>(dq_kernel<T, D, RULE>), qbytes + 1024, fn)) return rc;
+  if (int rc = reserve_lds(reinterpret_cast<const void*>(dkv_kernel<T, D, RULE>), kbytes + 4096, fn)) return rc;
+  const int64_t nbh = static_cast<int64_t>(p.batch) * p.h_kv;
+  const int64_t qblocks = ceil_div(p.n_q * p.g, kBlk) * nbh, kblocks = ceil_div(p.n, kBlk) * nbh * p.splits;
+  if (qblocks > 0x7FFFFFFF || kblocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many rows", fn);
+  if (qblocks > 0) {
+    dq_kernel<T, D, RULE><<<dim3(static_cast<unsigned>(qblocks)), dim3(kThreads), qbytes, st>>>(p);
+    if (int rc = check_launch("ssa_masked_attention_backward dq")) return rc;
+  }
+  if (kblocks > 0) {
+    dkv_kernel<T, D, RULE><<<dim3(static_cast<unsigned>(kblocks)), dim3(kThreads), kbytes, st>>>(p);
+    if (int rc = check_launch("ssa_masked_attention_backward dkv")) return rc;
+    if (p.splits > 1) {
+      const int64_t work = 2 * nbh * p.n * (p.d / 4);
+      dkv_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(work, 256))), dim3(256), 0, st>>>(p);
+      if (int rc = check_launch("ssa_masked_attention_backward join")) return rc;
+    }
+  }
+  return SSA_OK;
+}
+
+template <typename T, int D>
+int launch_rule(BwdParams& p, hipStream_t st) {
+  return p.rule.cap || p.rule.slopes != nullptr ? launch_bwd<T, D, true>(p, st) : launch_bwd<T, D, false>(p, st);
+}
+
+// The workspace: D, the groups' bounds, and the parts of dK and dV.
+struct BwdLayout {
+  int groups, splits, split_groups;
+  size_t dsum, bounds, part, bytes;
+};
+
+BwdLayout bwd_layout(int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv, int d) {
+  BwdLayout l{};
+  const int64_t rows = n_q * (h_q / h_kv);
+  l.groups = static_cast<int>(ceil_div(rows, 32));
+  // Parts of the rows where the keys alone give fewer blocks than CUs, of at
+  // least 256 rows (8 groups) each.
+  const int64_t blocks = ceil_div(n, kBlk) * batch * h_kv;
+  int64_t s = 1;
+  if (blocks > 0 && blocks < 256) {
+    s = (512 + blocks - 1) / blocks;
+    const int64_t most = l.groups / 8;
+    s = s < most ? s : (most > 1 ? most : 1);
+  }
+  l.split_groups = static_cast<int>(ceil_div(l.groups > 0 ? l.groups : 1, s));
+  l.splits = static_cast<int>(ceil_div(l.groups > 0 ? l.groups : 1, l.split_groups));
+  l.dsum = 0;
+  l.bounds = align_up(static_cast<size_t>(batch) * h_q * n_q * sizeof(float), 16);
+  l.part = align_up(l.bounds + static_cast<size_t>(batch) * l.groups * sizeof(int4), 16);
+  l.bytes = l.part;
+  if (l.splits > 1) l.bytes += 2 * static_cast<size_t>(l.splits) * batch * n * h_kv * (d <= 64 ? 64 : 128) * sizeof(float);
+  return l;
+}
+
+}  // namespace
+}  // namespace ssa
+
+using namespace ssa;
+
+extern "C" size_t ssa_masked_attention_backward_workspace_bytes(int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv,
+                                                                int d) {
+  if (batch <= 0 || n <= 0 || n_q <= 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0) return 0;
+  return bwd_layout(batch, n, n_q, h_q, h_kv, d).bytes;
+}
+
+extern "C" int ssa_masked_attention_backward(
+    const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t n, int64_t n_q, int64_t q_pos0, int h_q,
+    int h_kv, int d, int64_t q_sb, int64_t q_sn, int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb,
+    int64_t v_sn, int64_t v_sh, const int32_t* spans, float scale_div, float softcap, const float* slopes, const void* out,
+    const void* out_low, int64_t o_sb, int64_t o_sn, int64_t o_sh, const void* dout, int64_t do_sb, int64_t do_sn, int64_t do_sh,
+    const float* lse, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "ssa_masked_attention_backward";
+  if (int rc = check_heads(fn, dtype, h_q, h_kv, d)) return rc;
+  if (batch < 0 || n < 0 || n_q < 0 || q_pos0 < 0 || batch > 0x7FFFFFFF)
+    return fail(SSA_ERR_INVALID_ARGUMENT, "%s: bad shape batch=%lld n=%lld n_q=%lld q_pos0=%lld", fn, (long long)batch,
+                (long long)n, (long long)n_q, (long long)q_pos0);
+  if (n > 0x7FFFFF00 || q_pos0 + n_q > 0x7FFFFF00 || n_q * (h_q / h_kv) > 0x7FFFFF00)
+    return fail(SSA_ERR_UNSUPPORTED, "%s: sequences must be shorter than 2^31 / group size", fn);
+  BwdParams p{};
+  if (int rc = score_rule(fn, scale_div, softcap, slopes, &p.rule)) return rc;
+  if (batch == 0 || n == 0 || n_q == 0) {
+    if (batch > 0 && (n > 0 || n_q > 0))
+      return fail(SSA_ERR_INVALID_ARGUMENT, "%s: keys without rows, or rows without keys, have no gradient", fn);
+    return SSA_OK;
+  }
+  if (!q || !k || !v || !out || !dout || !lse || !dq || !dk || !dv)
+    return fail(SSA_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+  if (int rc = check_aligned(fn, "q", dtype, q, q_sb, q_sn, q_sh)) return rc;
+  if (int rc = check_aligned(fn, "k", dtype, k, k_sb, k_sn, k_sh)) return rc;
+  if (int rc = check_aligned(fn, "v", dtype, v, v_sb, v_sn, v_sh)) return rc;
+  if (int rc = check_aligned(fn, "out", dtype, out, o_sb, o_sn, o_sh)) return rc;
+  if (int rc = check_aligned(fn, "out_low", dtype, out_low, 0, 0, 0)) return rc;
+  if (int rc = check_aligned(fn, "dout", dtype, dout, do_sb, do_sn, do_sh)) return rc;
+  if (int rc = check_aligned(fn, "dq", dtype, dq, 0, 0, 0)) return rc;
+  if (int rc = check_aligned(fn, "dk", dtype, dk, 0, 0, 0)) return rc;
+  if (int rc = check_aligned(fn, "dv", dtype, dv, 0, 0, 0)) return rc;
+  const BwdLayout l = bwd_layout(batch, n, n_q, h_q, h_kv, d);
+  if (workspace == nullptr || workspace_bytes < l.bytes)
+    return fail(SSA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", fn, l.bytes,
+                workspace == nullptr ? size_t(0) : workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return fail(SSA_ERR_INVALID_ARGUMENT, "%s: workspace must be aligned to 16 bytes", fn);
+  p.q = q; p.k = k; p.v = v; p.out = out; p.out_low = out_low; p.dout = dout; p.lse = lse;
+  p.dq = dq; p.dk = dk; p.dv = dv;
+  p.q_sb = q_sb; p.q_sn = q_sn; p.q_sh = q_sh;
+  p.k_sb = k_sb; p.k_sn = k_sn; p.k_sh = k_sh;
+  p.v_sb = v_sb; p.v_sn = v_sn; p.v_sh = v_sh;
+  p.o_sb = o_sb; p.o_sn = o_sn; p.o_sh = o_sh;
+  p.do_sb = do_sb; p.do_sn = do_sn; p.do_sh = do_sh;
+  p.n = n; p.n_q = n_q; p.q_pos0 = q_pos0;
+  p.batch = static_cast<int>(batch); p.h_q = h_q; p.h_kv = h_kv; p.g = h_q / h_kv; p.d = d;
+  p.spans = reinterpret_cast<const int2*>(spans);
+  p.inv_scale = 1.0f / scale_div;
+  char* ws = static_cast<char*>(workspace);
+  p.dsum = reinterpret_cast<float*>(ws + l.dsum);
+  p.bounds = reinterpret_cast<int4*>(ws + l.bounds);
+  p.groups = l.groups;
+  p.splits = l.splits;
+  p.split_groups = l.split_groups;
+  if (l.splits > 1) {
+    p.part_k = reinterpret_cast<float*>(ws + l.part);
+    p.part_v = p.part_k + static_cast<int64_t>(l.splits) * batch * n * h_kv * (d <= 64 ? 64 : 128);
+  }
+  hipStream_t st = as_stream(stream);
+  if (dtype == SSA_DTYPE_F32) return d <= 64 ? launch_rule<float, 64>(p, st) : launch_rule<float, 128>(p, st);
+  return d <= 64 ? launch_rule<uint16_t, 64>(p, st) : launch_rule<uint16_t, 128>(p, st);
+}

@@ -1,0 +1,489 @@
+// Attention of new tokens over a paged K/V cache (ssa_paged_step): a ragged batch
+// of sequences, each with its new tokens' rows appended to its pages and attended
+// over everything it has cached, causally.
+//
+//   append       a thread copies 16 bytes of a new token's k or v row to its page
+//   few rows     sequences with at most 32 rows (tokens x heads of a group) per KV
+//                head, single tokens above all: few_rows_kernel
+//   many rows    chunks: dense_rows_kernel (ssa_dense_rows.h) over pages
+//
+// few_rows_kernel reads K and V once and is bound by that.  The rows fill one
+// MFMA column block; the block's four waves take every fourth 32-key tile of its
+// part of the sequence, each through LDS of its own (whole rows loaded, so that
+// every load instruction reads contiguous lines; the next tile's loads are in
+// flight while a tile is used, and its pages are looked up a tile earlier still),
+// and join their running sums through LDS at the end.  The parts of a sequence
+// are joined by a second kernel.
+
+#include <math.h>
+
+#include "ssa_dense_rows.h"
+#include "ssa_internal.h"
+
+namespace ssa {
+namespace {
+
+using namespace tile;
+
+constexpr int kFew = 32;  // rows of a few-row block
+
+struct AppendParams {
+  const void *k, *v;
+  int64_t k_st, k_sh, v_st, v_sh;
+};
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void paged_append_kernel(DenseParams p, AppendParams a) {
+  constexpr int E = 16 / static_cast<int>(sizeof(T));
+  const int per = p.d / E;  // chunks of a row
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t total = p.n_q * p.h_kv * per;
+  if (t >= 2 * total) return;
+  const bool isv = t >= total;
+  const int64_t u = isv ? t - total : t, row = u / per;
+  const int c = static_cast<int>(u - row * per);
+  const int tok = static_cast<int>(row / p.h_kv), h = static_cast<int>(row - static_cast<int64_t>(tok) * p.h_kv);
+  int x = 0, y = p.batch + 1;  // the first start past the token
+  while (x < y) {
+    const int mid = (x + y) >> 1;
+    if (p.starts[mid] <= tok)
+      x = mid + 1;
+    else
+      y = mid;
+  }
+  const int b = x - 1;
+  if (b < 0 || b >= p.batch) return;
+  const Seq s = paged_seq(p, b);
+  if (tok < s.first || tok >= s.first + s.m) return;
+  const int j = s.len - s.m + tok - s.first;
+  const int pg = p.table[b * p.table_stride + (j >> p.page_log2)];
+  if (static_cast<unsigned>(pg) >= static_cast<unsigned>(p.num_pages)) {
+    if (p.error_flag != nullptr) atomicOr(p.error_flag, 1);
+    return;
+  }
+  const int64_t r = j & ((1 << p.page_log2) - 1);
+  const T* src = static_cast<const T*>(isv ? a.v : a.k) + tok * (isv ? a.v_st : a.k_st) + h * (isv ? a.v_sh : a.k_sh) + c * E;
+  T* dst = static_cast<T*>(const_cast<void*>(isv ? p.v : p.k)) + pg * (isv ? p.v_sb : p.k_sb) +
+           r * (isv ? p.v_sn : p.k_sn) + h * (isv ? p.v_sh : p.k_sh) + c * E;
+  *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+}
+
+template <typename T, int D, bool RULE>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_kernel(DenseParams p) {
+  using O = Op<T>;
+  using Frag = typename O::Frag;
+  constexpr int RB = D * O::kEsize, NCH = RB / 16, E = 16 / O::kEsize;
+  constexpr int NC = D / 16, ND = D / 32, TB = 32 * RB;
+  constexpr int RPW = 64 / NCH, NP = 32 / RPW;  // rows a wave's load instruction covers; loads of a tile
+  constexpr int PS = D + 4;                     // floats of a row of partial sums
+  extern __shared__ __align__(16) char lds[];   // [4 waves][K, V][TB], then [4][32][PS] sums
+  __shared__ float s_m[4][kFew], s_l[4][kFew];
+  __shared__ int s_bad[4][kFew];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int kvh = blockIdx.x % p.h_kv;
+  const int rest = blockIdx.x / p.h_kv;
+  const int split = rest % p.splits, b = rest / p.splits;
+  const Seq sq = paged_seq(p, b);
+  const int R = sq.m * p.g;
+  if (R == 0 || R > p.few_rows) return;
+  const int k_begin = static_cast<int>(min(split * p.split_len, static_cast<int64_t>(sq.len)));
+  const int k_end = static_cast<int>(min((split + 1) * p.split_len, static_cast<int64_t>(sq.len)));
+  if (k_begin >= k_end) return;  // (a part past the sequence, which the join does not read)
+  const KeyRows<T, true> rows = key_rows<T, true>(p, b, kvh);
+
+  const int rr = lane & 31;
+  const bool real = rr < R;
+  const int tok = real ? rr / p.g : 0;
+  const int hq = kvh * p.g + (real ? rr - tok * p.g : 0);
+  const int pos = sq.len - sq.m + tok;
+  const float slope = (RULE && p.rule.slopes != nullptr && real) ? p.rule.slopes[hq] * kLog2e : 0.0f;
+  const T* qrow = static_cast<const T*>(p.q) + (sq.first + tok) * p.q_sn + hq * p.q_sh;
+  Frag qf[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int e = 16 * c + 8 * half;
+    qf[c] = real && e < p.d ? O::load(qrow + e) : O::zero();
+  }
+
+  char* kt = lds + wave * 2 * TB;
+  char* vt = kt + TB;
+  const int sc = lane % NCH, sr = lane / NCH;
+  const bool chunk_ok = sc * E < p.d;
+  uint4 kreg[NP], vreg[NP];
+  auto pages_at = [&](int k0) { return k0 < k_end ? rows.page_of(min(k0 + rr, k_end - 1)) : 0; };
+  auto load_tile = [&](int k0, int pg) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int r = sr + i * RPW;
+      const int64_t pr = __shfl(pg, r, 64);
+      const int64_t row = min(k0 + r, k_end - 1) & rows.page_mask;
+      const T* kr = rows.k + pr * rows.k_sb + row * rows.k_sn + sc * E;
+      const T* vr = rows.v + pr * rows.v_sb + row * rows.v_sn + sc * E;
+      kreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(kr) : make_uint4(0u, 0u, 0u, 0u);
+      vreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(vr) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) acc[i] = f32x16{};
+  float mref = -INFINITY, lsum = 0.0f;
+
+  int k0 = k_begin + 32 * wave;
+  int pg = pages_at(k0);
+  if (k0 < k_end) load_tile(k0, pg);
+  pg = pages_at(k0 + 128);
+  for (; k0 < k_end; k0 += 128) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int at = chunk_at<RB>(sr + i * RPW, sc);
+      *reinterpret_cast<uint4*>(kt + at) = kreg[i];
+      *reinterpret_cast<uint4*>(vt + at) = vreg[i];
+    }
+    wave_lds_sync();
+    if (k0 + 128 < k_end) load_tile(k0 + 128, pg);
+    pg = pages_at(k0 + 256);
+    f32x16 s = f32x16{};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) s = O::mfma(O::template row_frag<RB>(kt, 0, c, lane), qf[c], s);
+    const int kl = k0 + 4 * half;
+    const float dist = static_cast<float>(kl - pos);
+    const int z = min(pos + 1, k_end) - kl;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int j = 8 * (i >> 2) + (i & 3);
+      float x = s[i] * p.rule.c1;
+      if constexpr (RULE) {
+        if (p.rule.cap) x = p.rule.c2 * cap_tanh<T>(x);
+        x = fmaf(-slope, fabsf(dist + static_cast<float>(j)), x);
+      }
+      s[i] = j < z ? x : -INFINITY;
+      top = fmaxf(top, s[i]);
+    }
+    top = fmaxf(top, other_half(top));
+    if (__ballot(top > mref + 8.0f) != 0) {
+      const float mn = fmaxf(mref, top);
+      const float alpha = mref == mn ? 1.0f : exp2_w(mref - mn);
+      mref = mn;
+      lsum *= alpha;
+#pragma unroll
+      for (int i = 0; i < ND; ++i) acc[i] *= alpha;
+    }
+    const float ref = mref == -INFINITY ? 0.0f : mref;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = exp2_w(s[i] - ref);
+      lsum += s[i];
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const Frag pf = O::pack(s, c);
+#pragma unroll
+      for (int i = 0; i < ND; ++i) acc[i] = O::mfma(O::template col_frag<RB>(vt, 16 * c, 32 * i, lane), pf, acc[i]);
+    }
+    wave_lds_sync();
+  }
+
+  lsum += other_half(lsum);
+  float worst = finite(lsum) ? 0.0f : 1.0f;
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) worst = finite(acc[i][e]) ? worst : 1.0f;
+  worst = fmaxf(worst, other_half(worst));
+  if (half == 0) {
+    s_m[wave][rr] = mref;
+    s_l[wave][rr] = lsum;
+    s_bad[wave][rr] = worst != 0.0f;
+  }
+  __syncthreads();  // every wave is past its tiles: their LDS holds the sums now
+  float* sums = reinterpret_cast<float*>(lds);
+  if (real) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<float4*>(sums + (wave * kFew + rr) * PS + 32 * i + 8 * e + 4 * half) =
+            make_float4(acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]);
+  }
+  __syncthreads();
+  const int64_t part_row = (static_cast<int64_t>(b) * p.h_kv + kvh) * kFew;
+  const int quads = p.d / 4;
+  for (int e = tid; e < R * quads; e += kThreads) {
+    const int r = e / quads, dd = (e - r * quads) * 4;
+    if (s_bad[0][r] | s_bad[1][r] | s_bad[2][r] | s_bad[3][r]) continue;
+    const float m = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float a = exp2_w(s_m[x][r] - ref);
+      const float4 t = *reinterpret_cast<const float4*>(sums + (x * kFew + r) * PS + dd);
+      l = fmaf(a, s_l[x][r], l);
+      o.x = fmaf(a, t.x, o.x);
+      o.y = fmaf(a, t.y, o.y);
+      o.z = fmaf(a, t.z, o.z);
+      o.w = fmaf(a, t.w, o.w);
+    }
+    const int t = r / p.g, h = kvh * p.g + r - t * p.g;
+    if (p.splits > 1) {
+      const int64_t pr = split * p.part_rows + part_row + r;
+      *reinterpret_cast<float4*>(p.part_o + pr * D + dd) = o;
+      if (dd == 0) {
+        // (a part whose visible keys all scored -inf says so by a finite m)
+        const bool here = k_begin < min(k_end, sq.len - sq.m + t + 1);
+        p.part_ml[pr * 2] = here && m == -INFINITY ? -3.0e38f : m;
+        p.part_ml[pr * 2 + 1] = l;
+      }
+    } else {
+      const float inv = 1.0f / l;
+      T* orow = static_cast<T*>(p.out) + (sq.first + t) * p.o_sn + h * p.o_sh;
+      O::store4(orow + dd, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    }
+  }
+  for (int r = wave; r < R; r += 4) {  // rows to compute again, key by key
+    if (!(s_bad[0][r] | s_bad[1][r] | s_bad[2][r] | s_bad[3][r])) continue;
+    const int t = r / p.g, h = kvh * p.g + r - t * p.g, ps = sq.len - sq.m + t;
+    const float sl = RULE && p.rule.slopes != nullptr ? p.rule.slopes[h] * kLog2e : 0.0f;
+    float o[4], m, l;
+    exact_row<T, true>(rows, p.rule, static_cast<const T*>(p.q) + (sq.first + t) * p.q_sn + h * p.q_sh, p.d, k_begin,
+                       min(k_end, ps + 1), sl, ps, o, m, l);
+    const int64_t pr = split * p.part_rows + part_row + r;
+    T* orow = static_cast<T*>(p.out) + (sq.first + t) * p.o_sn + h * p.o_sh;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+      const int dd = lane + 64 * e;
+      if (dd >= p.d) continue;
+      if (p.splits > 1)
+        p.part_o[pr * D + dd] = o[e];
+      else
+        O::store1(orow + dd, o[e] * (1.0f / l));
+    }
+    if (p.splits > 1 && lane == 0) {
+      p.part_ml[pr * 2] = k_begin < min(k_end, ps + 1) && m == -INFINITY ? -3.0e38f : m;
+      p.part_ml[pr * 2 + 1] = l;
+    }
+  }
+}
+
+// One wave a row: the parts of a few-row sequence.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void few_join_kernel(DenseParams p, int row_blocks) {
+  const int lane = threadIdx.x & 63;
+  const int bh = blockIdx.x / row_blocks;
+  const int r = (blockIdx.x - bh * row_blocks) * (kThreads / 64) + (threadIdx.x >> 6);
+  const int b = bh / p.h_kv, kvh = bh - b * p.h_kv;
+  const Seq sq = paged_seq(p, b);
+  const int R = sq.m * p.g;
+  if (R > p.few_rows || r >= R) return;
+  const int parts = static_cast<int>(min(static_cast<int64_t>(p.splits), ceil_div(sq.len, p.split_len)));
+  const int64_t row = static_cast<int64_t>(bh) * kFew + r;
+  float m = -INFINITY;
+  for (int s = lane; s < parts; s += 64) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * p.part_rows + row) * 2);
+    if (ml.y != 0.0f) m = fmaxf(m, ml.x);
+  }
+  m = wave_max(m);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float o[D / 64], l = 0.0f;
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) o[e] = 0.0f;
+  for (int s0 = 0; s0 < parts; s0 += 64) {
+    float a = 0.0f, ls = 0.0f;
+    if (s0 + lane < parts) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((s0 + lane) * p.part_rows + row) * 2);
+      if (ml.y != 0.0f) {
+        a = exp2_w(ml.x - ref);
+        ls = ml.y * a;
+      }
+    }
+    l += wave_sum(ls);
+    uint64_t on = __ballot(ls != 0.0f);
+    while (on != 0) {
+      const int src = __builtin_ctzll(on);
+      on &= on - 1;
+      const float as = lane_value(a, src);
+      const float* pr = p.part_o + ((s0 + src) * p.part_rows + row) * D;
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e)
+        if (lane + 64 * e < p.d) o[e] = fmaf(as, pr[lane + 64 * e], o[e]);
+    }
+  }
+  const int t = r / p.g, h = kvh * p.g + r - t * p.g;
+  T* orow = static_cast<T*>(p.out) + (sq.first + t) * p.o_sn + h * p.o_sh;
+  const float inv = 1.0f / l;  // (a token sees itself: l = 0 only where every score is -inf)
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e)
+    if (lane + 64 * e < p.d) Op<T>::store1(orow + lane + 64 * e, o[e] * inv);
+}
+
+// Parts, tiles and workspace of a call.
+struct PagedPlan {
+  int few_splits, row_splits, row_tiles;
+  int64_t few_len, row_len;
+  size_t few_o, few_ml, row_o, row_ml, bytes;
+};
+
+PagedPlan paged_plan(int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t max_new, int64_t max_len) {
+  PagedPlan l{};
+  const int64_t g = h_q / h_kv, D = d <= 64 ? 64 : 128;
+  // Few rows: parts of at least 256 keys, four blocks a CU where the keys give
+  // them (sequences of unlike lengths even out).
+  const int64_t blocks = batch * h_kv;
+  int64_t s = (1024 + blocks - 1) / blocks, most = ceil_div(max_len, 256);
+  s = s < most ? s : most;
+  s = s > 1 ? s : 1;
+  l.few_len = ceil_div(ceil_div(max_len, s), 128) * 128;
+  l.few_splits = static_cast<int>(ceil_div(max_len, l.few_len));
+  l.row_splits = 1;
+  l.row_len = 0;
+  if (max_new * g > kFew) {
+    const int64_t each = batch * ceil_div(max_new * g, kRows), ragged = tokens * g / kRows + batch;
+    l.row_tiles = static_cast<int>(each < ragged ? each : ragged);
+    l.row_splits = dense_splits(static_cast<int64_t>(l.row_tiles) * h_kv, max_len);
+    l.row_len = ceil_div(ceil_div(max_len, l.row_splits), 64) * 64;
+  }
+  if (l.few_splits > 1) {
+    const size_t rows = static_cast<size_t>(l.few_splits) * batch * h_kv * kFew;
+    l.few_o = l.bytes;
+    l.few_ml = l.few_o + rows * D * sizeof(float);
+    l.bytes = align_up(l.few_ml + rows * 2 * sizeof(float), 16);
+  }
+  if (l.row_splits > 1) {
+    const size_t rows = static_cast<size_t>(l.row_splits) * tokens * h_q;
+    l.row_o = l.bytes;
+    l.row_ml = l.row_o + rows * D * sizeof(float);
+    l.bytes = align_up(l.row_ml + rows * 2 * sizeof(float), 16);
+  }
+  return l;
+}
+
+template <typename T, int D, bool RULE>
+int launch_paged(DenseParams& p, const AppendParams& a, const PagedPlan& l, char* ws, hipStream_t st) {
+  const char* fn = "ssa_paged_step";
+  if (a.k != nullptr) {
+    const int64_t work = 2 * p.n_q * p.h_kv * (p.d / (16 / static_cast<int>(sizeof(T))));
+    if (ceil_div(work, kThreads) > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many tokens", fn);
+    paged_append_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(work, kThreads))), dim3(kThreads), 0, st>>>(p, a);
+    if (int rc = check_launch("ssa_paged_step append")) return rc;
+  }
+  const size_t tiles = static_cast<size_t>(8) * 32 * D * sizeof(T), sums = static_cast<size_t>(4) * kFew * (D + 4) * sizeof(float);
+  const size_t fbytes = tiles > sums ? tiles : sums;
+  if (int rc = reserve_lds(reinterpret_cast<const void*>(few_rows_kernel<T, D, RULE>), fbytes + 2048, fn)) return rc;
+  DenseParams f = p;
+  f.splits = l.few_splits;
+  f.split_len = l.few_len;
+  f.part_rows = static_cast<int64_t>(p.batch) * p.h_kv * kFew;
+  f.part_o = reinterpret_cast<float*>(ws + l.few_o);
+  f.part_ml = reinterpret_cast<float*>(ws + l.few_ml);
+  const int64_t fblocks = static_cast<int64_t>(p.batch) * p.h_kv * f.splits;
+  if (fblocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many sequences", fn);
+  few_rows_kernel<T, D, RULE><<<dim3(static_cast<unsigned>(fblocks)), dim3(kThreads), fbytes, st>>>(f);
+  if (int rc = check_launch("ssa_paged_step few rows")) return rc;
+  if (f.splits > 1) {
+    const int64_t most = p.max_new * p.g < kFew ? p.max_new * p.g : kFew;
+    const int row_blocks = static_cast<int>(ceil_div(most, kThreads / 64));
+    few_join_kernel<T, D><<<dim3(static_cast<unsigned>(p.batch * p.h_kv * row_blocks)), dim3(kThreads), 0, st>>>(f, row_blocks);
+    if (int rc = check_launch("ssa_paged_step join")) return rc;
+  }
+  if (l.row_tiles > 0) {
+    DenseParams r = p;
+    r.splits = l.row_splits;
+    r.split_len = l.row_len;
+    r.part_rows = p.n_q * p.h_q;
+    r.part_o = reinterpret_cast<float*>(ws + l.row_o);
+    r.part_ml = reinterpret_cast<float*>(ws + l.row_ml);
+    const size_t bytes = 4 * static_cast<size_t>(key_tile<T>()) * D * sizeof(T);
+    if (int rc = reserve_lds(reinterpret_cast<const void*>(dense_rows_kernel<T, D, true, RULE>), bytes + 1024, fn)) return rc;
+    const int64_t blocks = static_cast<int64_t>(l.row_tiles) * p.h_kv * r.splits;
+    if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many tokens", fn);
+    dense_rows_kernel<T, D, true, RULE><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(r);
+    if (int rc = check_launch("ssa_paged_step rows")) return rc;
+    if (r.splits > 1) {
+      dense_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(r.part_rows, kThreads / 64))), dim3(kThreads), 0, st>>>(r);
+      if (int rc = check_launch("ssa_paged_step row join")) return rc;
+    }
+  }
+  return SSA_OK;
+}
+
+template <typename T, int D>
+int launch_rule(DenseParams& p, const AppendParams& a, const PagedPlan& l, char* ws, hipStream_t st) {
+  return p.rule.cap || p.rule.slopes != nullptr ? launch_paged<T, D, true>(p, a, l, ws, st)
+                                                : launch_paged<T, D, false>(p, a, l, ws, st);
+}
+
+}  // namespace
+}  // namespace ssa
+
+using namespace ssa;
+
+extern "C" size_t ssa_paged_step_workspace_bytes(int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t max_new,
+                                                 int64_t max_len) {
+  if (tokens <= 0 || batch <= 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0 || max_new <= 0 || max_len <= 0) return 0;
+  return paged_plan(tokens, batch, h_q, h_kv, d, max_new, max_len).bytes;
+}
+
+extern "C" int ssa_paged_step(const void* q, const void* k, const void* v, int dtype, int64_t tokens, int64_t batch, int h_q,
+                              int h_kv, int d, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st,
+                              int64_t v_sh, void* k_pages, void* v_pages, int64_t num_pages, int page_size, int64_t kp_sp,
+                              int64_t kp_st, int64_t kp_sh, int64_t vp_sp, int64_t vp_st, int64_t vp_sh, const int32_t* table,
+                              int64_t table_stride, int max_pages, const int32_t* starts, const int32_t* cached,
+                              int64_t max_new, int64_t max_len, float scale_div, float softcap, const float* slopes, void* out,
+                              int64_t o_st, int64_t o_sh, int32_t* error_flag, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  const char* fn = "ssa_paged_step";
+  if (int rc = check_heads(fn, dtype, h_q, h_kv, d)) return rc;
+  if (tokens < 0 || batch < 0 || num_pages < 0 || max_pages < 0 || max_new < 0 || max_len < 0)
+    return fail(SSA_ERR_INVALID_ARGUMENT, "%s: bad shape tokens=%lld batch=%lld num_pages=%lld max_pages=%d", fn,
+                (long long)tokens, (long long)batch, (long long)num_pages, max_pages);
+  if (page_size < 8 || page_size > 4096 || (page_size & (page_size - 1)) != 0)
+    return fail(SSA_ERR_UNSUPPORTED, "%s: page_size %d must be a power of 2 in [8, 4096]", fn, page_size);
+  if (tokens * (h_q / h_kv) > 0x7FFFFF00 || batch > 0x7FFFFF || num_pages > 0x7FFFFFFF || max_len > 0x7FFFFF00 ||
+      static_cast<int64_t>(max_pages) * page_size > 0x7FFFFF00)
+    return fail(SSA_ERR_UNSUPPORTED, "%s: sequences must be shorter than 2^31 / group size", fn);
+  tile::DenseParams p{};
+  if (int rc = score_rule(fn, scale_div, softcap, slopes, &p.rule)) return rc;
+  if (tokens == 0 || batch == 0) return SSA_OK;
+  if (max_new < 1 || max_len < 1 || num_pages < 1 || max_pages < 1)
+    return fail(SSA_ERR_INVALID_ARGUMENT, "%s: max_new, max_len, num_pages and max_pages must be positive", fn);
+  if (!q || !k_pages || !v_pages || !table || !starts || !cached || !out || (k == nullptr) != (v == nullptr))
+    return fail(SSA_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+  if (int rc = check_aligned(fn, "q", dtype, q, 0, q_st, q_sh)) return rc;
+  if (int rc = check_aligned(fn, "k", dtype, k, 0, k_st, k_sh)) return rc;
+  if (int rc = check_aligned(fn, "v", dtype, v, 0, v_st, v_sh)) return rc;
+  if (int rc = check_aligned(fn, "k_pages", dtype, k_pages, kp_sp, kp_st, kp_sh)) return rc;
+  if (int rc = check_aligned(fn, "v_pages", dtype, v_pages, vp_sp, vp_st, vp_sh)) return rc;
+  if (int rc = check_aligned(fn, "out", dtype, out, 0, o_st, o_sh)) return rc;
+  if (max_new > tokens) max_new = tokens;
+  const int64_t cap = static_cast<int64_t>(max_pages) * page_size;
+  if (max_len > cap) max_len = cap;
+  const PagedPlan l = paged_plan(tokens, batch, h_q, h_kv, d, max_new, max_len);
+  if (l.bytes > 0 && (workspace == nullptr || workspace_bytes < l.bytes))
+    return fail(SSA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", fn, l.bytes,
+                workspace == nullptr ? size_t(0) : workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return fail(SSA_ERR_INVALID_ARGUMENT, "%s: workspace must be aligned to 16 bytes", fn);
+  p.q = q; p.k = k_pages; p.v = v_pages; p.out = out;
+  p.q_sn = q_st; p.q_sh = q_sh;
+  p.k_sb = kp_sp; p.k_sn = kp_st; p.k_sh = kp_sh;
+  p.v_sb = vp_sp; p.v_sn = vp_st; p.v_sh = vp_sh;
+  p.o_sn = o_st; p.o_sh = o_sh;
+  p.n_q = tokens;
+  p.batch = static_cast<int>(batch); p.h_q = h_q; p.h_kv = h_kv; p.g = h_q / h_kv; p.d = d;
+  p.table = table; p.starts = starts; p.cached = cached; p.table_stride = table_stride;
+  p.max_pages = max_pages; p.num_pages = static_cast<int>(num_pages);
+  while ((1 << p.page_log2) < page_size) ++p.page_log2;
+  p.few_rows = kFew;
+  p.max_new = max_new; p.max_len = max_len;
+  p.error_flag = error_flag;
+  const AppendParams a{k, v, k_st, k_sh, v_st, v_sh};
+  hipStream_t st = as_stream(stream);
+  char* ws = static_cast<char*>(workspace);
+  if (dtype == SSA_DTYPE_F32)
+    return d <= 64 ? launch_rule<float, 64>(p, a, l, ws, st) : launch_rule<float, 128>(p, a, l, ws, st);
+  return d <= 64 ? launch_rule<uint16_t, 64>(p, a, l, ws, st) : launch_rule<uint16_t, 128>(p, a, l, ws, st);
+}

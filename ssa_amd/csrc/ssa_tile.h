@@ -1,0 +1,212 @@
+// Matrix-core tiles of the dense attention kernels (ssa_masked.hip,
+// ssa_masked_bwd.hip, ssa_paged.hip): operand fragments, the LDS tile layout and
+// the score rule they share.
+//
+// One layout serves every product.  A wave works on 32 "columns" (query rows,
+// or keys in the dK/dV kernel) of a 32x32 MFMA: lane l holds column l % 32, and
+// accumulator register r holds row 8 (r / 4) + 4 (l / 32) + r % 4.  A product's
+// contraction may visit its index in any order as long as both operands use the
+// same one, so the registers of a score tile are the next product's B operand as
+// they stand: registers 8c .. 8c + 7 are the 16 rows
+//   16 c + 4 (l / 32) + {0, 1, 2, 3, 8, 9, 10, 11}
+// and only the A operand (read from LDS, by columns) follows that order.  No
+// score moves between lanes.
+//
+// LDS tiles are [rows][D] with 16-byte chunks swizzled within 128 bytes:
+// chunk c of row r lies at chunk c ^ f(r), f(r) = 2 (r % 4) + (r / 4) % 2.
+// Eight consecutive rows of one chunk then touch all banks once (row
+// fragments), and so do four rows x two chunks (column fragments by
+// ds_read_b64_tr_b16).
+#pragma once
+
+#include "ssa_common.h"
+
+namespace ssa {
+namespace tile {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+
+constexpr int kThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ int swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+
+// Byte offset of 16-byte chunk c of row r in a tile of rows of RB bytes.
+template <int RB>
+__device__ __forceinline__ int chunk_at(int r, int c) {
+  return r * RB + ((c ^ swz(r)) << 4);
+}
+
+template <typename T>
+struct Op;
+
+// bf16 storage: one 32x32x16 product per fragment.
+template <>
+struct Op<uint16_t> {
+  static constexpr int kEsize = 2;
+  struct Frag {
+    uint4 v;
+  };
+  static __device__ __forceinline__ f32x16 mfma(const Frag& a, const Frag& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v), c,
+                                                   0, 0, 0);
+  }
+  static __device__ __forceinline__ Frag zero() { return Frag{make_uint4(0u, 0u, 0u, 0u)}; }
+  // Eight consecutive elements in global memory (16-byte aligned).
+  static __device__ __forceinline__ Frag load(const uint16_t* p) { return Frag{*reinterpret_cast<const uint4*>(p)}; }
+  // Columns 16c + 8 (l / 32) .. + 7 of tile row row0 + l % 32.
+  template <int RB>
+  static __device__ __forceinline__ Frag row_frag(const char* t, int row0, int c, int lane) {
+    const int r = row0 + (lane & 31);
+    return Frag{*reinterpret_cast<const uint4*>(t + chunk_at<RB>(r, 2 * c + (lane >> 5)))};
+  }
+  // Column d0 + l % 32 of rows row0 + 4 (l / 32) + {0..3, 8..11} (row0 a multiple of 16).
+  template <int RB>
+  static __device__ __forceinline__ Frag col_frag(const char* t, int row0, int d0, int lane) {
+    const int i = lane & 15;
+    const int r = row0 + 4 * (lane >> 5) + (i >> 2);
+    const int ch = (d0 >> 3) + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
+    const char* p = t + chunk_at<RB>(r, ch) + (i & 1) * 8;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 8 * RB));
+    const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+    return Frag{make_uint4(a.x, a.y, b.x, b.y)};
+  }
+  static __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    // v_cvt_pk_bf16_f32, round to nearest even
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+  }
+  // Registers 8c .. 8c + 7 of a score tile as a B operand.  Weights and score
+  // gradients round to bf16 here, once (the products' inputs are bf16; the sums
+  // stay fp32).
+  static __device__ __forceinline__ Frag pack(const f32x16& s, int c) {
+    return Frag{make_uint4(pack2(s[8 * c], s[8 * c + 1]), pack2(s[8 * c + 2], s[8 * c + 3]),
+                           pack2(s[8 * c + 4], s[8 * c + 5]), pack2(s[8 * c + 6], s[8 * c + 7]))};
+  }
+  static __device__ __forceinline__ float dot(const Frag& a, const Frag& b, float s) {
+    const uint32_t x[4] = {a.v.x, a.v.y, a.v.z, a.v.w}, y[4] = {b.v.x, b.v.y, b.v.z, b.v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), s);
+      s = fmaf(__uint_as_float(x[i] & 0xFFFF0000u), __uint_as_float(y[i] & 0xFFFF0000u), s);
+    }
+    return s;
+  }
+  // Four consecutive outputs, rounded once.
+  static __device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, float d) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2(a, b), pack2(c, d));
+  }
+  static __device__ __forceinline__ void store1(uint16_t* p, float a) { *p = f32_to_bf16_rne(a); }
+  // What rounding leaves.
+  static __device__ __forceinline__ float left(float a) { return a - __uint_as_float(pack2(a, 0.0f) << 16); }
+};
+
+// fp32 storage: the same fragments as eight 32x32x2 products.
+template <>
+struct Op<float> {
+  static constexpr int kEsize = 4;
+  struct Frag {
+    float v[8];
+  };
+  static __device__ __forceinline__ f32x16 mfma(const Frag& a, const Frag& b, f32x16 c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[i], b.v[i], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ Frag zero() { return Frag{{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}}; }
+  static __device__ __forceinline__ Frag of(float4 a, float4 b) { return Frag{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}}; }
+  static __device__ __forceinline__ Frag load(const float* p) {
+    return of(*reinterpret_cast<const float4*>(p), *reinterpret_cast<const float4*>(p + 4));
+  }
+  template <int RB>
+  static __device__ __forceinline__ Frag row_frag(const char* t, int row0, int c, int lane) {
+    const int r = row0 + (lane & 31), ch = 4 * c + 2 * (lane >> 5);
+    return of(*reinterpret_cast<const float4*>(t + chunk_at<RB>(r, ch)),
+              *reinterpret_cast<const float4*>(t + chunk_at<RB>(r, ch + 1)));
+  }
+  template <int RB>
+  static __device__ __forceinline__ Frag col_frag(const char* t, int row0, int d0, int lane) {
+    const int d = d0 + (lane & 31);
+    Frag f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = row0 + 4 * (lane >> 5) + (i & 3) + 8 * (i >> 2);
+      f.v[i] = *reinterpret_cast<const float*>(t + chunk_at<RB>(r, d >> 2) + (d & 3) * 4);
+    }
+    return f;
+  }
+  static __device__ __forceinline__ Frag pack(const f32x16& s, int c) {
+    Frag f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.v[i] = s[8 * c + i];
+    return f;
+  }
+  static __device__ __forceinline__ float dot(const Frag& a, const Frag& b, float s) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fmaf(a.v[i], b.v[i], s);
+    return s;
+  }
+  static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
+    *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+  }
+  static __device__ __forceinline__ void store1(float* p, float a) { *p = a; }
+  static __device__ __forceinline__ float left(float) { return 0.0f; }
+};
+
+// The other half-wave's value of a lane's column.
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+  return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+  return x;
+}
+__device__ __forceinline__ int wave_min_i(int x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
+  return x;
+}
+__device__ __forceinline__ int wave_max_i(int x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
+  return x;
+}
+
+__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
+
+// The score rule, in log2 units (weights are exp2 of differences):
+//   no cap:  x = (q.k) c1 - slope |pos - j|,        c1 = log2(e) / scale
+//   cap c:   x = c2 tanh((q.k) c1) - slope |pos - j|, c1 = 1 / (scale c), c2 = c log2(e)
+// slope already carries log2(e).
+struct ScoreRule {
+  float c1, c2;
+  int cap;              // scores go through the tanh
+  const float* slopes;  // null, or [h_q]
+};
+
+// tanh for the bf16 kernels: 1 - 2 / (exp(2y) + 1), absolute error about 2^-22
+// (v_exp_f32 and v_rcp_f32 are good to an ulp), far below a bf16 weight's
+// 2^-9.  The fp32 kernels take the library's.
+template <typename T>
+__device__ __forceinline__ float cap_tanh(float y) {
+  if constexpr (sizeof(T) == 4) return tanhf(y);
+  const float e = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e));
+  return fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+}
+
+// exp2 of a difference of scores: the instruction's (an ulp; a result below
+// 2^-126 is 0, a weight that no fp32 sum of weights up to 1 can hold).
+__device__ __forceinline__ float exp2_w(float x) { return __builtin_amdgcn_exp2f(x); }
+
+}  // namespace tile
+}  // namespace ssa

@@ -1,0 +1,140 @@
+"""Host-side checks of the dense attention, paged cache and axes entry points: every call
+here fails validation or is an empty no-op, so nothing is launched and no pointer is
+dereferenced (sections, which is host memory, is real)."""
+
+import ctypes
+import os
+
+import pytest
+import torch
+
+import ssa_amd
+from ssa_amd import _lib
+
+FAKE = ctypes.c_void_p(1 << 20)
+MISALIGNED = ctypes.c_void_p((1 << 20) + 8)
+OK, INVALID, UNSUPPORTED, WORKSPACE = (_lib.SSA_OK, _lib.SSA_ERR_INVALID_ARGUMENT, _lib.SSA_ERR_UNSUPPORTED,
+                                       _lib.SSA_ERR_WORKSPACE)
+
+
+@pytest.fixture(scope="module")
+def L():
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("libssa_hip.so not built (run __graft_entry__.build())")
+    return _lib.load()
+
+
+def _call(L, name, defaults, kw):
+    a = {**defaults, **kw}
+    assert set(a) == set(defaults)
+    st = getattr(L, name)(*a.values())
+    return st, (L.ssa_last_error() or b"").decode()
+
+
+SPANS = dict(starts=FAKE, docs=3, prefix=FAKE, batch=2, n=100, n_q=100, q_pos0=0, causal=1, spans=FAKE, stream=None)
+HEADS = dict(dtype=_lib.DTYPE_BF16, batch=1, n=1000, n_q=1000, q_pos0=0, h_q=8, h_kv=2, d=64)
+ROWS = {f"{x}_{s}": v for x in "qkv" for s, v in (("sb", 64000 * 8), ("sn", 512), ("sh", 64))}
+FORWARD = dict(q=FAKE, k=FAKE, v=FAKE, **HEADS, **ROWS, spans=None, scale=8.0, cap=0.0, slopes=None, out=FAKE, o_sb=0,
+               o_sn=512, o_sh=64, out_low=None, lse=None, ws=FAKE, ws_bytes=1 << 30, stream=None)
+BACKWARD = dict(q=FAKE, k=FAKE, v=FAKE, **HEADS, **ROWS, spans=None, scale=8.0, cap=0.0, slopes=None, out=FAKE,
+                out_low=None, o_sb=0, o_sn=512, o_sh=64, dout=FAKE, do_sb=0, do_sn=512, do_sh=64, lse=FAKE, dq=FAKE, dk=FAKE, dv=FAKE,
+                ws=FAKE, ws_bytes=1 << 30, stream=None)
+PAGED = dict(q=FAKE, k=FAKE, v=FAKE, dtype=_lib.DTYPE_BF16, tokens=10, batch=3, h_q=8, h_kv=2, d=64, q_st=512, q_sh=64,
+             k_st=128, k_sh=64, v_st=128, v_sh=64, k_pages=FAKE, v_pages=FAKE, num_pages=100, page_size=16, kp_sp=2048,
+             kp_st=128, kp_sh=64, vp_sp=2048, vp_st=128, vp_sh=64, table=FAKE, table_stride=64, max_pages=64, starts=FAKE,
+             cached=FAKE, max_new=8, max_len=1000, scale=8.0, cap=0.0, slopes=None, out=FAKE, o_st=512, o_sh=64, flag=None,
+             ws=FAKE, ws_bytes=1 << 30, stream=None)
+SECTIONS = (ctypes.c_int32 * 4)(8, 12, 12, 0)
+NEGATIVE = (ctypes.c_int32 * 4)(33, -1, 0, 0)
+AXES = dict(q=FAKE, k=FAKE, dtype=_lib.DTYPE_BF16, batch=1, n=100, h_q=8, h_k=2, d=64, q_sb=0, q_sn=512, q_sh=64, k_sb=0,
+            k_sn=128, k_sh=64, pos=FAKE, pos_dtype=_lib.INDEX_I64, p_sa=100, p_sb=100, axes=3, sections=SECTIONS, freqs=FAKE,
+            rot=64, inverse=0, q_out=FAKE, qo_sb=0, qo_sn=512, qo_sh=64, k_out=FAKE, ko_sb=0, ko_sn=128, ko_sh=64,
+            stream=None)
+
+
+@pytest.mark.parametrize("kw,status,text", [
+    (dict(n=-1), INVALID, "shape"), (dict(docs=0), INVALID, "docs"), (dict(starts=None), INVALID, "one document"),
+    (dict(spans=None), INVALID, "null"), (dict(n=1 << 31), INVALID, "shape"), (dict(batch=0, spans=None), OK, ""),
+])
+def test_mask_spans(L, kw, status, text):
+    st, msg = _call(L, "ssa_mask_spans", SPANS, kw)
+    assert st == status and (st == OK or text in msg), msg
+
+
+DENSE = [
+    (dict(dtype=7), UNSUPPORTED, "dtype"), (dict(h_q=9), INVALID, "divisible"), (dict(h_q=34), UNSUPPORTED, "group"),
+    (dict(d=60), UNSUPPORTED, "head_dim"), (dict(d=136), UNSUPPORTED, "head_dim"), (dict(d=0), INVALID, "shape"),
+    (dict(n=-1), INVALID, "shape"), (dict(q_pos0=-1), INVALID, "shape"), (dict(n=1 << 31), UNSUPPORTED, "2^31"),
+    (dict(n_q=1 << 29), UNSUPPORTED, "2^31"), (dict(scale=0.0), INVALID, "scale"),
+    (dict(scale=float("inf")), INVALID, "scale"), (dict(cap=-1.0), INVALID, "softcap"),
+    (dict(cap=float("nan")), INVALID, "softcap"), (dict(q=None), INVALID, "null"), (dict(v=None), INVALID, "null"),
+    (dict(out=None), INVALID, "null"), (dict(q=MISALIGNED), UNSUPPORTED, "q must"), (dict(k_sn=516), UNSUPPORTED, "k must"),
+    (dict(v_sh=4), UNSUPPORTED, "v must"), (dict(o_sn=4), UNSUPPORTED, "out must"),
+    (dict(batch=0, q=None), OK, ""),
+]
+
+
+@pytest.mark.parametrize("kw,status,text", DENSE + [
+    (dict(n_q=4, ws=None), WORKSPACE, "workspace"), (dict(n_q=4, ws_bytes=100), WORKSPACE, "workspace"),
+    (dict(n_q=4, ws=MISALIGNED), INVALID, "workspace"), (dict(n_q=0, q=None), OK, ""),
+])
+def test_masked_attention(L, kw, status, text):
+    if "ws" in kw or "ws_bytes" in kw:
+        assert L.ssa_masked_attention_workspace_bytes(1, 4000, 4, 8, 2, 64) > 100
+        kw = {**kw, "n": 4000}
+    st, msg = _call(L, "ssa_masked_attention", FORWARD, kw)
+    assert st == status and (st == OK or text in msg), msg
+
+
+@pytest.mark.parametrize("kw,status,text", DENSE + [
+    (dict(ws=None), WORKSPACE, "workspace"), (dict(ws_bytes=100), WORKSPACE, "workspace"),
+    (dict(ws=MISALIGNED), INVALID, "workspace"), (dict(lse=None), INVALID, "null"), (dict(dk=None), INVALID, "null"),
+    (dict(do_sn=4), UNSUPPORTED, "dout must"), (dict(dv=MISALIGNED), UNSUPPORTED, "dv must"),
+    (dict(n_q=0), INVALID, "no gradient"),
+])
+def test_masked_attention_backward(L, kw, status, text):
+    st, msg = _call(L, "ssa_masked_attention_backward", BACKWARD, kw)
+    assert st == status and (st == OK or text in msg), msg
+
+
+@pytest.mark.parametrize("kw,status,text", [x for x in DENSE if not {"n", "n_q", "q_pos0", "k_sn", "o_sn", "batch"} & set(x[0])] + [
+    (dict(tokens=-1), INVALID, "shape"), (dict(page_size=24), UNSUPPORTED, "page_size"),
+    (dict(page_size=4), UNSUPPORTED, "page_size"), (dict(page_size=8192), UNSUPPORTED, "page_size"),
+    (dict(tokens=1 << 30), UNSUPPORTED, "2^31"), (dict(max_pages=1 << 28), UNSUPPORTED, "2^31"),
+    (dict(max_new=0), INVALID, "max_new"), (dict(num_pages=0), INVALID, "num_pages"), (dict(k=None), INVALID, "null"),
+    (dict(table=None), INVALID, "null"), (dict(kp_st=4), UNSUPPORTED, "k_pages"), (dict(vp_sp=4), UNSUPPORTED, "v_pages"),
+    (dict(k_st=4), UNSUPPORTED, "k must"), (dict(ws=None), WORKSPACE, "workspace"),
+    (dict(ws=MISALIGNED), INVALID, "workspace"), (dict(tokens=0, q=None), OK, ""), (dict(batch=0, q=None), OK, ""),
+])
+def test_paged_step(L, kw, status, text):
+    st, msg = _call(L, "ssa_paged_step", PAGED, kw)
+    assert st == status and (st == OK or text in msg), msg
+
+
+@pytest.mark.parametrize("kw,status,text", [
+    (dict(dtype=7), UNSUPPORTED, "dtype"), (dict(pos_dtype=5), INVALID, "positions"), (dict(h_q=0), INVALID, "shape"),
+    (dict(rot=63), INVALID, "rot"), (dict(rot=66), INVALID, "rot"), (dict(axes=0), UNSUPPORTED, "axes"),
+    (dict(axes=5), UNSUPPORTED, "axes"), (dict(sections=None), INVALID, "null"), (dict(axes=2), INVALID, "sections"),
+    (dict(sections=NEGATIVE), INVALID, "negative"), (dict(rot=32), INVALID, "sections"), (dict(freqs=None), INVALID, "null"),
+    (dict(k=None), INVALID, "null"), (dict(q_out=None), INVALID, "null"), (dict(n=0, q=None), OK, ""),
+])
+def test_rope_axes(L, kw, status, text):
+    st, msg = _call(L, "ssa_rope_axes", AXES, kw)
+    assert st == status and (st == OK or text in msg), msg
+
+
+def test_python_refuses_host_tensors():
+    q = torch.zeros(1, 4, 2, 8)
+    ints = torch.zeros(1, 4, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="HIP"):
+        ssa_amd.masked_attention(q, q, q)
+    with pytest.raises(RuntimeError, match="HIP"):
+        ssa_amd.mask_spans(4, 1, device="cpu")
+    with pytest.raises(RuntimeError, match="HIP"):
+        ssa_amd.mask_spans(4, 1, doc_starts=ints)
+    with pytest.raises(RuntimeError, match="HIP"):
+        ssa_amd.paged_step(q[0], q[0], q[0], q, q, ints, ints[0], ints[0])
+    with pytest.raises(RuntimeError, match="HIP"):
+        ssa_amd.rope_axes(q, q, ints[None], ssa_amd.axis_rope_freqs(8), (4,))
+    with pytest.raises(ValueError, match="prefix_lens"):
+        ssa_amd.mask_spans(4, 1, causal=False, prefix_lens=ints)
