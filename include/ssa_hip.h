@@ -497,7 +497,8 @@ int ssa_mask_spans(const int32_t* doc_starts, int docs, const int32_t* prefix_le
  *   workspace: ssa_masked_attention_workspace_bytes(...) bytes (0 for most shapes;
  *       few rows over many keys are split along the keys).
  * Limits: d a multiple of 8 up to 128, h_q / h_kv <= 16. */
-size_t ssa_masked_attention_workspace_bytes(int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv, int d);
+size_t ssa_masked_attention_workspace_bytes(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv,
+                                            int d);
 int ssa_masked_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t n,
                          int64_t n_q, int64_t q_pos0, int h_q, int h_kv, int d, int64_t q_sb, int64_t q_sn,
                          int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn,
@@ -515,8 +516,8 @@ int ssa_masked_attention(const void* q, const void* k, const void* v, int dtype,
  *   workspace: ssa_masked_attention_backward_workspace_bytes(...) bytes.
  * Replaces the autograd backward of dense_attention (ssa/attention.py:118-158)
  * for masks of this form.  slopes get no gradient. */
-size_t ssa_masked_attention_backward_workspace_bytes(int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv,
-                                                     int d);
+size_t ssa_masked_attention_backward_workspace_bytes(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q,
+                                                     int h_kv, int d);
 int ssa_masked_attention_backward(
     const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t n, int64_t n_q,
     int64_t q_pos0, int h_q, int h_kv, int d, int64_t q_sb, int64_t q_sn, int64_t q_sh, int64_t k_sb,
@@ -550,8 +551,8 @@ int ssa_masked_attention_backward(
  * Limits: as ssa_masked_attention; page_size a power of 2 in [8, 4096].
  * No reference counterpart (ssa_design.md:225-234 describes decoding against a
  * cache; its code runs whole sequences). */
-size_t ssa_paged_step_workspace_bytes(int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t max_new,
-                                      int64_t max_len);
+size_t ssa_paged_step_workspace_bytes(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv, int d,
+                                      int64_t max_new, int64_t max_len);
 int ssa_paged_step(const void* q, const void* k, const void* v, int dtype, int64_t tokens, int64_t batch, int h_q,
                    int h_kv, int d, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st,
                    int64_t v_sh, void* k_pages, void* v_pages, int64_t num_pages, int page_size, int64_t kp_sp,

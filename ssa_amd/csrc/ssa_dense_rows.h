@@ -5,8 +5,9 @@
 //
 // A block of four waves takes 128 rows of one KV head: a row is a (token, query
 // head of the group) pair, tokens first, so that the g heads that share a key
-// read its tile once and a causal block's diagonal is 128 / g tokens wide.  Each
-// wave keeps 32 rows: Q as B operands in registers, S^T = K Q^T with one row's
+// read its tile once and a causal block's diagonal is 128 / g tokens wide.  Where
+// that leaves CUs idle, KW = 2 or 4 waves share 32 rows and take turns at the keys
+// (64 or 32 rows a block; their sums meet in LDS).  Each wave keeps 32 rows: Q as B operands in registers, S^T = K Q^T with one row's
 // scores down a lane's registers (the running maximum and sum need one exchange
 // with the other half-wave), P^T as the B operand of O^T += V^T P^T without
 // leaving its registers (ssa_tile.h).  K and V tiles of 64 keys (32 in fp32)
@@ -51,12 +52,7 @@ struct DenseParams {
   int64_t part_rows;
 };
 
-constexpr int kRows = 128;  // rows of a block
-
-template <typename T>
-constexpr int key_tile() {
-  return sizeof(T) == 2 ? 64 : 32;
-}
+constexpr int kRows = 128;  // rows of a block of waves of their own
 
 // A sequence of a paged batch: its query tokens [first, first + m) and keys.
 struct Seq {
@@ -98,11 +94,14 @@ struct KeyRows {
     }
     return pg;
   }
+  __device__ __forceinline__ void in_page(int64_t pg, int j, const T*& kr, const T*& vr) const {
+    const int64_t r = j & page_mask;
+    kr = k + pg * k_sb + r * k_sn;
+    vr = v + pg * v_sb + r * v_sn;
+  }
   __device__ __forceinline__ void at(int j, const T*& kr, const T*& vr) const {
     if constexpr (PAGED) {
-      const int64_t pg = page_of(j), r = j & page_mask;
-      kr = k + pg * k_sb + r * k_sn;
-      vr = v + pg * v_sb + r * v_sn;
+      in_page(page_of(j), j, kr, vr);
     } else {
       kr = k + j * k_sn;
       vr = v + j * v_sn;
@@ -182,14 +181,14 @@ __device__ __forceinline__ void exact_row(const KeyRows<T, PAGED>& rows, const S
 // Which (sequence, tile of rows) a block of a ragged batch takes: the idx-th
 // tile in sequence order, sequences with at most few_rows rows left out.
 // Returns false past the last one.
-__device__ __forceinline__ bool find_tile(const DenseParams& p, int idx, int& b, int& tile) {
+__device__ __forceinline__ bool find_tile(const DenseParams& p, int idx, int block_rows, int& b, int& tile) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
     int t = 0;
     if (b0 + lane < p.batch) {
       const int64_t rows = static_cast<int64_t>(paged_seq(p, b0 + lane).m) * p.g;
-      t = rows > p.few_rows ? static_cast<int>((rows + kRows - 1) / kRows) : 0;
+      t = rows > p.few_rows ? static_cast<int>((rows + block_rows - 1) / block_rows) : 0;
     }
     const int incl = wave_incl_scan(t);
     const uint64_t past = __ballot(before + incl > idx);
@@ -204,22 +203,50 @@ __device__ __forceinline__ bool find_tile(const DenseParams& p, int idx, int& b,
   return false;
 }
 
-template <typename T, int D, bool PAGED, bool RULE>
-__global__ __launch_bounds__(kThreads, 2) void dense_rows_kernel(DenseParams p) {
+// Rows of a block whose KW waves share each 32 rows and take the keys in turn.
+constexpr int rows_of(int kw) { return kRows / kw; }
+
+// Keys of a tile: 32 or 64 a wave.
+template <typename T, int KW>
+constexpr int key_tile() {
+  return KW > 1 ? 32 * KW : (sizeof(T) == 2 ? 64 : 32);
+}
+
+// The most waves that may share rows: fp32 rows of 128 features fill the LDS with two.
+template <typename T, int D>
+constexpr int most_kw() {
+  return sizeof(T) == 4 && D == 128 ? 2 : 4;
+}
+
+// LDS of a block: two buffers of K and V, or at the end the waves' sums.
+template <typename T, int D, int KW>
+constexpr size_t rows_lds() {
+  const size_t tiles = static_cast<size_t>(4) * key_tile<T, KW>() * D * sizeof(T);
+  const size_t sums = KW > 1 ? static_cast<size_t>(4) * 32 * (D + 4) * sizeof(float) : 0;
+  return tiles > sums ? tiles : sums;
+}
+
+template <typename T, int D, bool PAGED, bool RULE, int KW>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void dense_rows_kernel(DenseParams p) {
   using O = Op<T>;
   using Frag = typename O::Frag;
   constexpr int RB = D * O::kEsize;      // bytes of a tile row
   constexpr int NCH = RB / 16;           // its chunks
   constexpr int E = 16 / O::kEsize;      // elements of a chunk
-  constexpr int KT = key_tile<T>();
-  constexpr int NSUB = KT / 32, NC = D / 16, ND = D / 32;
+  constexpr int KT = key_tile<T, KW>();  // keys of a tile
+  constexpr int NSUB = KT / (32 * KW), NC = D / 16, ND = D / 32;
   constexpr int RPP = kThreads / NCH;    // tile rows a pass of the block loads
   constexpr int NP = KT / RPP;
   constexpr int TB = KT * RB;            // bytes of a tile
-  extern __shared__ __align__(16) char lds[];  // [2 buffers][K, V][TB]
+  constexpr int BR = rows_of(KW);        // the block's rows
+  constexpr int PS = D + 4;              // floats of a row of sums
+  extern __shared__ __align__(16) char lds[];  // [2 buffers][K, V][TB], then [4 waves][32][PS]
   __shared__ int s_range[4][2];
+  __shared__ float s_m[4][32], s_l[4][32];
+  __shared__ int s_flag[4][32];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int kw = wave % KW, rw = wave / KW;
   const int nbh = PAGED ? p.h_kv : p.batch * p.h_kv;
   const int w = blockIdx.x;
   const int bh = w % nbh;
@@ -230,27 +257,25 @@ __global__ __launch_bounds__(kThreads, 2) void dense_rows_kernel(DenseParams p) 
   int64_t n_keys;
   if constexpr (PAGED) {
     kvh = bh;
-    if (!find_tile(p, rest, b, tile)) return;
+    if (!find_tile(p, rest, BR, b, tile)) return;
     const Seq s = paged_seq(p, b);
     first = s.first;
     m = s.m;
     n_keys = s.len;
     // the longest rows of a chunk first
-    const int tiles = (m * p.g + kRows - 1) / kRows;
-    tile = tiles - 1 - tile;
+    tile = (m * p.g + BR - 1) / BR - 1 - tile;
     if (tile < 0) return;
   } else {
     b = bh / p.h_kv;
     kvh = bh - b * p.h_kv;
     m = static_cast<int>(p.n_q);
     n_keys = p.n;
-    const int tiles = static_cast<int>((p.n_q * p.g + kRows - 1) / kRows);
-    tile = tiles - 1 - rest;
+    tile = static_cast<int>((p.n_q * p.g + BR - 1) / BR) - 1 - rest;
   }
   const KeyRows<T, PAGED> rows = key_rows<T, PAGED>(p, b, kvh);
 
   // this lane's row
-  const int r = tile * kRows + wave * 32 + (lane & 31);
+  const int r = tile * BR + rw * 32 + (lane & 31);
   const bool real = r < m * p.g;
   const int tok = real ? r / p.g : 0;
   const int hq = kvh * p.g + (real ? r - tok * p.g : 0);
@@ -274,6 +299,13 @@ __global__ __launch_bounds__(kThreads, 2) void dense_rows_kernel(DenseParams p) 
     s_range[wave][0] = lo_min;
     s_range[wave][1] = hi_max;
   }
+  const T* qrow = static_cast<const T*>(p.q) + (PAGED ? first * p.q_sn : b * p.q_sb) + tok * p.q_sn + hq * p.q_sh;
+  Frag qf[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int e = 16 * c + 8 * half;
+    qf[c] = real && e < p.d ? O::load(qrow + e) : O::zero();
+  }
   __syncthreads();
   int k_lo = min(min(s_range[0][0], s_range[1][0]), min(s_range[2][0], s_range[3][0]));
   int k_hi = max(max(s_range[0][1], s_range[1][1]), max(s_range[2][1], s_range[3][1]));
@@ -288,24 +320,28 @@ __global__ __launch_bounds__(kThreads, 2) void dense_rows_kernel(DenseParams p) 
   const int t0 = k_lo / KT;
   const int nt = k_hi > k_lo ? (k_hi + KT - 1) / KT - t0 : 0;
 
-  const T* qrow = static_cast<const T*>(p.q) + (PAGED ? first * p.q_sn : b * p.q_sb) + tok * p.q_sn + hq * p.q_sh;
-  Frag qf[NC];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int e = 16 * c + 8 * half;
-    qf[c] = real && e < p.d ? O::load(qrow + e) : O::zero();
-  }
-
-  // staging: chunk sc of tile rows sr, sr + RPP, ...
+  // staging: chunk sc of tile rows sr, sr + RPP, ...; of paged keys a tile's pages
+  // are looked up a tile before its loads
   const int sc = tid % NCH, sr = tid / NCH;
   const bool chunk_ok = sc * E < p.d;
+  const int last = static_cast<int>(n_keys) - 1;
   uint4 kreg[NP], vreg[NP];
+  int pg[PAGED ? NP : 1];
+  auto find_pages = [&](int t) {
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) pg[i] = rows.page_of(min((t0 + t) * KT + sr + i * RPP, last));
+    }
+  };
   auto load_tile = [&](int t) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int j = min((t0 + t) * KT + sr + i * RPP, static_cast<int>(n_keys) - 1);
+      const int j = min((t0 + t) * KT + sr + i * RPP, last);
       const T *kr, *vr;
-      rows.at(j, kr, vr);
+      if constexpr (PAGED)
+        rows.in_page(pg[i], j, kr, vr);
+      else
+        rows.at(j, kr, vr);
       kreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(kr + sc * E) : make_uint4(0u, 0u, 0u, 0u);
       vreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(vr + sc * E) : make_uint4(0u, 0u, 0u, 0u);
     }
@@ -326,15 +362,18 @@ __global__ __launch_bounds__(kThreads, 2) void dense_rows_kernel(DenseParams p) 
   float mref = -INFINITY, lsum = 0.0f;
 
   if (nt > 0) {
+    find_pages(0);
     load_tile(0);
+    if (nt > 1) find_pages(1);
     store_tile(0);
   }
   for (int t = 0; t < nt; ++t) {
     __syncthreads();
     if (t + 1 < nt) load_tile(t + 1);
-    const int k0 = (t0 + t) * KT;
-    if (k0 < hi_max && k0 + KT > lo_min) {
-      const char* kt = lds + (t & 1) * 2 * TB;
+    if (t + 2 < nt) find_pages(t + 2);
+    const int k0 = (t0 + t) * KT + kw * 32 * NSUB;
+    if (k0 < hi_max && k0 + 32 * NSUB > lo_min) {
+      const char* kt = lds + (t & 1) * 2 * TB + kw * 32 * NSUB * RB;
       const char* vt = kt + TB;
       f32x16 s[NSUB];
 #pragma unroll
@@ -366,7 +405,7 @@ __global__ __launch_bounds__(kThreads, 2) void dense_rows_kernel(DenseParams p) 
               s[u][i] = fmaf(-slope, fabsf(dist + static_cast<float>(32 * u + 8 * (i >> 2) + (i & 3))), s[u][i]);
         }
       }
-      const bool whole = k0 >= lo_max && k0 + KT <= hi_min && k0 >= part_lo && k0 + KT <= part_hi;
+      const bool whole = k0 >= lo_max && k0 + 32 * NSUB <= hi_min && k0 >= part_lo && k0 + 32 * NSUB <= part_hi;
       if (!whole) {
         const int a = max(lo, part_lo) - kl, z = min(hi, part_hi) - kl;
 #pragma unroll
@@ -413,96 +452,126 @@ __global__ __launch_bounds__(kThreads, 2) void dense_rows_kernel(DenseParams p) 
 
   // the row's sums, joined over the half-waves (they share the reference)
   lsum += other_half(lsum);
-  float worst = 0.0f;
+  float worst = finite(lsum) ? 0.0f : 1.0f;
 #pragma unroll
   for (int i = 0; i < ND; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) worst = finite(acc[i][e]) ? worst : 1.0f;
   worst = fmaxf(worst, other_half(worst));
-  const bool again = some && (worst != 0.0f || !finite(lsum));
-  const int64_t row_id = PAGED ? static_cast<int64_t>(first + tok) * p.h_q + hq
-                               : (static_cast<int64_t>(b) * p.n_q + tok) * p.h_q + hq;
-  // Where the row's result goes: the output, or its part.
-  T* orow = static_cast<T*>(p.out) + (PAGED ? first * p.o_sn : b * p.o_sb) + tok * p.o_sn + hq * p.o_sh;
-  T* low = p.out_low != nullptr ? static_cast<T*>(p.out_low) + (orow - static_cast<T*>(p.out)) : nullptr;
-  float* prow = p.splits > 1 ? p.part_o + (split * p.part_rows + row_id) * D : nullptr;
-  float* pml = p.splits > 1 ? p.part_ml + (split * p.part_rows + row_id) * 2 : nullptr;
-  float* lrow = p.lse != nullptr ? p.lse + (static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok : nullptr;
-
-  // (a part whose visible keys all scored -inf says so by a finite m)
-  const bool here = some && max(lo, part_lo) < min(hi, part_hi);
-  if (real && !again) {
+  // Where a row's results go: the output, or its part.
+  const int64_t out0 = PAGED ? first * p.o_sn : b * p.o_sb;
+  const int64_t row0 = PAGED ? first : static_cast<int64_t>(b) * p.n_q;
+  auto put = [&](int tk, int h, int dd, float a, float c, float e, float f) {  // four features, normalised unless in parts
     if (p.splits > 1) {
-      if (half == 0) {
-        pml[0] = here && mref == -INFINITY ? -3.0e38f : mref;
-        pml[1] = lsum;
-      }
-      if (lsum != 0.0f) {
-#pragma unroll
-        for (int i = 0; i < ND; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int dd = 32 * i + 8 * e + 4 * half;
-            if (dd < p.d)
-              *reinterpret_cast<float4*>(prow + dd) =
-                  make_float4(acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]);
-          }
-      }
+      *reinterpret_cast<float4*>(p.part_o + (split * p.part_rows + (row0 + tk) * p.h_q + h) * D + dd) = make_float4(a, c, e, f);
     } else {
-      // no key: zeros; only keys of score -inf: NaN, as a softmax of them is
-      const float inv = some ? 1.0f / lsum : 0.0f;
+      const int64_t at = out0 + tk * p.o_sn + h * p.o_sh + dd;
+      O::store4(static_cast<T*>(p.out) + at, a, c, e, f);
+      if (p.out_low != nullptr) O::store4(static_cast<T*>(p.out_low) + at, O::left(a), O::left(c), O::left(e), O::left(f));
+    }
+  };
+  auto put_sums = [&](int tk, int h, float mm, float l, bool any, bool here) {
+    if (p.splits > 1) {
+      // (a part whose visible keys all scored -inf says so by a finite m)
+      float* pml = p.part_ml + (split * p.part_rows + (row0 + tk) * p.h_q + h) * 2;
+      pml[0] = here && mm == -INFINITY ? -3.0e38f : mm;
+      pml[1] = l;
+    } else if (p.lse != nullptr) {
+      p.lse[(static_cast<int64_t>(b) * p.h_q + h) * p.n_q + tk] = any ? mm + __log2f(l) : INFINITY;
+    }
+  };
+  const bool here = some && max(lo, part_lo) < min(hi, part_hi);
+  // no key: zeros; only keys of score -inf: NaN, as a softmax of them is
+  if constexpr (KW == 1) {
+    const bool again = some && worst != 0.0f;
+    if (real && !again) {
+      const float inv = p.splits > 1 ? 1.0f : (some ? 1.0f / lsum : 0.0f);
 #pragma unroll
       for (int i = 0; i < ND; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int dd = 32 * i + 8 * e + 4 * half;
-          if (dd < p.d) {
-            const float a = acc[i][4 * e] * inv, c = acc[i][4 * e + 1] * inv, f = acc[i][4 * e + 2] * inv,
-                        h = acc[i][4 * e + 3] * inv;
-            O::store4(orow + dd, a, c, f, h);
-            if (low != nullptr) O::store4(low + dd, O::left(a), O::left(c), O::left(f), O::left(h));
-          }
+          if (dd < p.d) put(tok, hq, dd, acc[i][4 * e] * inv, acc[i][4 * e + 1] * inv, acc[i][4 * e + 2] * inv, acc[i][4 * e + 3] * inv);
         }
-      if (lrow != nullptr && half == 0) *lrow = some ? mref + __log2f(lsum) : INFINITY;
+      if (half == 0) put_sums(tok, hq, mref, lsum, some, here);
     }
+    worst = again ? 1.0f : 0.0f;
+  } else {
+    if (half == 0) {
+      s_m[wave][lane] = mref;
+      s_l[wave][lane] = lsum;
+      s_flag[wave][lane] = (some && worst != 0.0f ? 1 : 0) | (some ? 2 : 0) | (here ? 4 : 0);
+    }
+    __syncthreads();  // every wave is past its tiles: their LDS holds the sums now
+    float* sums = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<float4*>(sums + (wave * 32 + (lane & 31)) * PS + 32 * i + 8 * e + 4 * half) =
+            make_float4(acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]);
+    __syncthreads();
+    for (int x = tid; x < BR * (D / 4); x += kThreads) {
+      const int rr = x / (D / 4), dd = (x - rr * (D / 4)) * 4, wv = rr / 32 * KW, ln = rr & 31;
+      const int rx = tile * BR + rr;
+      if (dd >= p.d || rx >= m * p.g) continue;
+      int flag = 0;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int y = 0; y < KW; ++y) {
+        flag |= s_flag[wv + y][ln];
+        mm = fmaxf(mm, s_m[wv + y][ln]);
+      }
+      if (flag & 1) continue;
+      const float ref = mm == -INFINITY ? 0.0f : mm;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.0f;
+#pragma unroll
+      for (int y = 0; y < KW; ++y) {
+        const float a = exp2_w(s_m[wv + y][ln] - ref);
+        const float4 v = *reinterpret_cast<const float4*>(sums + ((wv + y) * 32 + ln) * PS + dd);
+        l = fmaf(a, s_l[wv + y][ln], l);
+        o.x = fmaf(a, v.x, o.x);
+        o.y = fmaf(a, v.y, o.y);
+        o.z = fmaf(a, v.z, o.z);
+        o.w = fmaf(a, v.w, o.w);
+      }
+      const int tk = rx / p.g, h = kvh * p.g + rx - tk * p.g;
+      const float inv = p.splits > 1 ? 1.0f : ((flag & 2) ? 1.0f / l : 0.0f);
+      put(tk, h, dd, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+      if (dd == 0) put_sums(tk, h, mm, l, (flag & 2) != 0, (flag & 4) != 0);
+    }
+    int bad = 0;
+#pragma unroll
+    for (int y = 0; y < KW; ++y) bad |= s_flag[rw * KW + y][lane & 31] & 1;
+    worst = bad && (lane & (KW - 1)) == kw ? 1.0f : 0.0f;  // shared out among the waves
   }
-  uint64_t todo = __ballot(again && half == 0);
-  while (todo != 0) {  // rows to compute again, one after the other by the whole wave
+
+  uint64_t todo = __ballot(worst != 0.0f && half == 0);
+  while (todo != 0) {  // rows to compute again, one after the other by a whole wave
     const int src = __builtin_ctzll(todo);
     todo &= todo - 1;
     const int a = max(lane_value(lo, src), part_lo), z = min(lane_value(hi, src), part_hi);
-    const int ps = lane_value(pos, src);
+    const int ps = lane_value(pos, src), tk = lane_value(tok, src), h = lane_value(hq, src);
     const float sl = lane_value(slope, src);
-    auto ptr_of = [&](const void* x) {
-      const uint64_t u = reinterpret_cast<uint64_t>(x);
-      return (static_cast<uint64_t>(static_cast<uint32_t>(lane_value(static_cast<int>(u >> 32), src))) << 32) |
-             static_cast<uint32_t>(lane_value(static_cast<int>(u & 0xFFFFFFFFu), src));
-    };
     float o[4], mm, ll;
-    exact_row<T, PAGED>(rows, p.rule, reinterpret_cast<const T*>(ptr_of(qrow)), p.d, a, z, sl, ps, o, mm, ll);
+    exact_row<T, PAGED>(rows, p.rule,
+                        static_cast<const T*>(p.q) + (PAGED ? first * p.q_sn : b * p.q_sb) + tk * p.q_sn + h * p.q_sh, p.d, a,
+                        z, sl, ps, o, mm, ll);
     const float inv = 1.0f / ll;
-    if (p.splits > 1) {
-      float* pr = reinterpret_cast<float*>(ptr_of(prow));
-      float* pm = reinterpret_cast<float*>(ptr_of(pml));
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < p.d) pr[lane + 64 * e] = o[e];
-      if (lane == 0) {
-        pm[0] = mm == -INFINITY ? -3.0e38f : mm;
-        pm[1] = ll;
+    for (int e = 0; e < 4; ++e) {
+      const int dd = lane + 64 * e;
+      if (dd >= p.d) continue;
+      if (p.splits > 1) {
+        p.part_o[(split * p.part_rows + (row0 + tk) * p.h_q + h) * D + dd] = o[e];
+      } else {
+        const int64_t at = out0 + tk * p.o_sn + h * p.o_sh + dd;
+        O::store1(static_cast<T*>(p.out) + at, o[e] * inv);
+        if (p.out_low != nullptr) O::store1(static_cast<T*>(p.out_low) + at, O::left(o[e] * inv));
       }
-    } else {
-      T* orr = reinterpret_cast<T*>(ptr_of(orow));
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < p.d) {
-          O::store1(orr + lane + 64 * e, o[e] * inv);
-          if (p.out_low != nullptr)
-            O::store1(static_cast<T*>(p.out_low) + (orr - static_cast<T*>(p.out)) + lane + 64 * e, O::left(o[e] * inv));
-        }
-      float* lr = reinterpret_cast<float*>(ptr_of(lrow));
-      if (lr != nullptr && lane == 0) *lr = mm + __log2f(ll);
     }
+    if (lane == 0) put_sums(tk, h, mm, ll, true, a < z);
   }
 }
 

@@ -49,15 +49,15 @@ __global__ __launch_bounds__(256) void mask_spans_kernel(const int32_t* starts, 
   out[t] = hi > lo ? make_int2(static_cast<int>(lo), static_cast<int>(hi)) : make_int2(0, 0);
 }
 
-template <typename T, int D, bool RULE>
+template <typename T, int D, bool RULE, int KW>
 int launch_rows(DenseParams& p, hipStream_t st) {
-  const size_t bytes = 4 * static_cast<size_t>(key_tile<T>()) * D * sizeof(T);
-  if (int rc = reserve_lds(reinterpret_cast<const void*>(dense_rows_kernel<T, D, false, RULE>), bytes + 1024,
+  const size_t bytes = rows_lds<T, D, KW>();
+  if (int rc = reserve_lds(reinterpret_cast<const void*>(dense_rows_kernel<T, D, false, RULE, KW>), bytes + 2048,
                            "ssa_masked_attention"))
     return rc;
-  const int64_t blocks = ceil_div(p.n_q * p.g, kRows) * p.batch * p.h_kv * p.splits;
+  const int64_t blocks = ceil_div(p.n_q * p.g, rows_of(KW)) * p.batch * p.h_kv * p.splits;
   if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "ssa_masked_attention: too many rows");
-  dense_rows_kernel<T, D, false, RULE><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(p);
+  dense_rows_kernel<T, D, false, RULE, KW><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(p);
   if (int rc = check_launch("ssa_masked_attention")) return rc;
   if (p.splits > 1) {
     dense_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(p.part_rows, kThreads / 64))), dim3(kThreads), 0, st>>>(p);
@@ -66,19 +66,34 @@ int launch_rows(DenseParams& p, hipStream_t st) {
   return SSA_OK;
 }
 
+template <typename T, int D, bool RULE>
+int launch_kw(DenseParams& p, int kw, hipStream_t st) {
+  if constexpr (most_kw<T, D>() >= 4)
+    if (kw == 4) return launch_rows<T, D, RULE, 4>(p, st);
+  return kw == 2 ? launch_rows<T, D, RULE, 2>(p, st) : launch_rows<T, D, RULE, 1>(p, st);
+}
+
 template <typename T, int D>
-int launch_rule(DenseParams& p, hipStream_t st) {
-  return p.rule.cap || p.rule.slopes != nullptr ? launch_rows<T, D, true>(p, st) : launch_rows<T, D, false>(p, st);
+int launch_rule(DenseParams& p, int kw, hipStream_t st) {
+  return p.rule.cap || p.rule.slopes != nullptr ? launch_kw<T, D, true>(p, kw, st) : launch_kw<T, D, false>(p, kw, st);
 }
 
 }  // namespace
 
-int dense_splits(int64_t blocks, int64_t keys) {
-  // Parts of the key axis: enough blocks for two on each of the 256 CUs, and at
-  // least 512 keys a part (a part's rows are written and read once more).
-  if (blocks <= 0 || blocks >= 512) return 1;
-  const int64_t s = (512 + blocks - 1) / blocks, most = keys / 512;
-  return static_cast<int>(s < most ? s : (most > 1 ? most : 1));
+DenseSplit dense_split(int64_t rows, int64_t heads, int64_t keys, bool wide_f32) {
+  // Two blocks fit a CU.  Where blocks of 128 rows are fewer than that, the key axis
+  // is cut into parts of at least 1024 keys (a part's rows are written and read once
+  // more, in a second launch), and where keys are fewer too, two or four waves share
+  // each 32 rows and take turns at them.
+  DenseSplit s{1, 1};
+  const int most = wide_f32 ? 2 : 4;
+  const int64_t blocks = ceil_div(rows, 128) * heads;
+  if (blocks > 0 && blocks < 512) {
+    const int64_t want = ceil_div(512, blocks), can = keys / 1024;
+    s.parts = static_cast<int>(want < can ? want : (can > 1 ? can : 1));
+  }
+  while (s.kw < most && ceil_div(rows, 128 / s.kw) * heads * s.parts < 512 && keys > 32 * s.kw) s.kw *= 2;
+  return s;
 }
 
 }  // namespace ssa
@@ -139,9 +154,10 @@ int check_aligned(const char* fn, const char* name, int dtype, const void* ptr, 
 
 }  // namespace ssa
 
-extern "C" size_t ssa_masked_attention_workspace_bytes(int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv, int d) {
+extern "C" size_t ssa_masked_attention_workspace_bytes(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv,
+                                                       int d) {
   if (batch <= 0 || n <= 0 || n_q <= 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0) return 0;
-  const int s = dense_splits(ceil_div(n_q * (h_q / h_kv), kRows) * batch * h_kv, n);
+  const int s = dense_split(n_q * (h_q / h_kv), batch * h_kv, n, dtype == SSA_DTYPE_F32 && d > 64).parts;
   if (s <= 1) return 0;
   return static_cast<size_t>(s) * batch * n_q * h_q * ((d <= 64 ? 64 : 128) + 2) * sizeof(float);
 }
@@ -177,9 +193,10 @@ extern "C" int ssa_masked_attention(const void* q, const void* k, const void* v,
   p.n = n; p.n_q = n_q; p.q_pos0 = q_pos0;
   p.batch = static_cast<int>(batch); p.h_q = h_q; p.h_kv = h_kv; p.g = h_q / h_kv; p.d = d;
   p.spans = reinterpret_cast<const int2*>(spans);
-  p.splits = dense_splits(ceil_div(n_q * p.g, kRows) * batch * h_kv, n);
+  const DenseSplit cut = dense_split(n_q * p.g, batch * h_kv, n, dtype == SSA_DTYPE_F32 && d > 64);
+  p.splits = cut.parts;
   if (p.splits > 1) {
-    const size_t need = ssa_masked_attention_workspace_bytes(batch, n, n_q, h_q, h_kv, d);
+    const size_t need = ssa_masked_attention_workspace_bytes(dtype, batch, n, n_q, h_q, h_kv, d);
     if (workspace == nullptr || workspace_bytes < need)
       return fail(SSA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", fn, need,
                   workspace == nullptr ? size_t(0) : workspace_bytes);
@@ -192,6 +209,6 @@ extern "C" int ssa_masked_attention(const void* q, const void* k, const void* v,
   }
   hipStream_t st = as_stream(stream);
   if (dtype == SSA_DTYPE_F32)
-    return d <= 64 ? launch_rule<float, 64>(p, st) : launch_rule<float, 128>(p, st);
-  return d <= 64 ? launch_rule<uint16_t, 64>(p, st) : launch_rule<uint16_t, 128>(p, st);
+    return d <= 64 ? launch_rule<float, 64>(p, cut.kw, st) : launch_rule<float, 128>(p, cut.kw, st);
+  return d <= 64 ? launch_rule<uint16_t, 64>(p, cut.kw, st) : launch_rule<uint16_t, 128>(p, cut.kw, st);
 }

@@ -42,11 +42,11 @@ struct BwdParams {
   const int2* spans;
   ScoreRule rule;
   float inv_scale;
-  float* dsum;    // [batch][h_q][n_q]: D
+  float4* stats;  // [batch][h_q][n_q]: lse, D, lo, hi (the last two as ints)
   int4* bounds;   // [batch][groups of 32 packed rows]: lo_min, hi_max, lo_max, hi_min
   int groups;
   int splits;     // parts of the rows for dK and dV
-  int split_groups;
+  int split_tiles;
   float *part_k, *part_v;  // [splits][batch][n][h_kv][D]
 };
 
@@ -94,26 +94,44 @@ __device__ __forceinline__ const void* lane_ptr(const void* x, int src) {
       static_cast<uint32_t>(lane_value(static_cast<int>(u & 0xFFFFFFFFu), src)));
 }
 
-template <typename T, int D, bool RULE>
-__global__ __launch_bounds__(kThreads, 2) void dq_kernel(BwdParams p) {
+// Waves of dq_kernel that may share rows: fp32 rows of 128 features fill the LDS with two.
+template <typename T, int D>
+constexpr int most_kw() {
+  return sizeof(T) == 4 && D == 128 ? 2 : 4;
+}
+template <typename T, int D, int KW>
+constexpr int dq_keys() {
+  return KW > 1 ? 32 * KW : (sizeof(T) == 2 ? 64 : 32);
+}
+// LDS: two buffers of K and V, or at the end the sums of the waves that share rows.
+template <typename T, int D, int KW>
+constexpr size_t dq_lds() {
+  const size_t tiles = static_cast<size_t>(4) * dq_keys<T, D, KW>() * D * sizeof(T);
+  const size_t sums = KW > 1 ? static_cast<size_t>(4) * 32 * (D + 4) * sizeof(float) : 0;
+  return tiles > sums ? tiles : sums;
+}
+
+template <typename T, int D, bool RULE, int KW>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void dq_kernel(BwdParams p) {
   using O = Op<T>;
   using Frag = typename O::Frag;
   constexpr int RB = D * O::kEsize, NCH = RB / 16, E = 16 / O::kEsize;
-  constexpr int KT = sizeof(T) == 2 ? 64 : 32;
-  constexpr int NSUB = KT / 32, NC = D / 16, ND = D / 32;
+  constexpr int KT = dq_keys<T, D, KW>();
+  constexpr int NSUB = KT / (32 * KW), NC = D / 16, ND = D / 32, BR = kBlk / KW, PS = D + 4;
   constexpr int RPP = kThreads / NCH, NP = KT / RPP, TB = KT * RB;
   extern __shared__ __align__(16) char lds[];
   __shared__ int s_range[4][2];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int kw = wave % KW, rw = wave / KW;
   const int nbh = p.batch * p.h_kv;
   const int bh = blockIdx.x % nbh;
-  const int tiles = static_cast<int>((p.n_q * p.g + kBlk - 1) / kBlk);
+  const int tiles = static_cast<int>((p.n_q * p.g + BR - 1) / BR);
   const int tile = tiles - 1 - static_cast<int>(blockIdx.x / nbh);
   const int b = bh / p.h_kv, kvh = bh - b * p.h_kv;
   const int n_keys = static_cast<int>(p.n);
 
-  const int r = tile * kBlk + wave * 32 + (lane & 31);
+  const int r = tile * BR + rw * 32 + (lane & 31);
   const bool real = r < p.n_q * p.g;
   const int tok = real ? r / p.g : 0;
   const int hq = kvh * p.g + (real ? r - tok * p.g : 0);
@@ -127,8 +145,8 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(BwdParams p) {
   if (lane == 0) {
     s_range[wave][0] = lo_min;
     s_range[wave][1] = hi_max;
-    const int grp = tile * 4 + wave;
-    if (kvh == 0 && grp < p.groups) p.bounds[static_cast<int64_t>(b) * p.groups + grp] = make_int4(lo_min, hi_max, lo_max, hi_min);
+    const int grp = tile * (BR / 32) + rw;
+    if (kvh == 0 && kw == 0 && grp < p.groups) p.bounds[static_cast<int64_t>(b) * p.groups + grp] = make_int4(lo_min, hi_max, lo_max, hi_min);
   }
   __syncthreads();
   const int k_lo = min(min(s_range[0][0], s_range[1][0]), min(s_range[2][0], s_range[3][0]));
@@ -141,7 +159,7 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(BwdParams p) {
   const T* dorow = static_cast<const T*>(p.dout) + b * p.do_sb + tok * p.do_sn + hq * p.do_sh;
   const T* orow = static_cast<const T*>(p.out) + b * p.o_sb + tok * p.o_sn + hq * p.o_sh;
   const int64_t stat = (static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok;
-  const float lse = some ? p.lse[stat] : INFINITY;
+  const float lse = some ? p.lse[stat] : INFINITY;  // (no key: every weight 0)
   Frag qf[NC], dof[NC];
   float dsum = 0.0f;
 #pragma unroll
@@ -158,7 +176,8 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(BwdParams p) {
     }
   }
   dsum += other_half(dsum);
-  if (real && half == 0) p.dsum[stat] = dsum;
+  if (real && half == 0 && kw == 0)
+    p.stats[stat] = make_float4(lse, dsum, __int_as_float(lo), __int_as_float(hi));
 
   const int sc = tid % NCH, sr = tid / NCH;
   const bool chunk_ok = sc * E < p.d;
@@ -191,11 +210,11 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(BwdParams p) {
   for (int t = 0; t < nt; ++t) {
     __syncthreads();
     if (t + 1 < nt) load_tile(t + 1);
-    const char* kt = lds + (t & 1) * 2 * TB;
+    const char* kt = lds + (t & 1) * 2 * TB + kw * 32 * NSUB * RB;
     const char* vt = kt + TB;
 #pragma unroll
     for (int u = 0; u < NSUB; ++u) {
-      const int k0 = (t0 + t) * KT + 32 * u;
+      const int k0 = (t0 + t) * KT + (kw * NSUB + u) * 32;
       if (k0 < hi_max && k0 + 32 > lo_min) {
         f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
@@ -226,6 +245,32 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(BwdParams p) {
     if (t + 1 < nt) store_tile((t + 1) & 1);
   }
 
+  if constexpr (KW > 1) {  // the first of the waves that share rows adds up
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(lds);
+    if (kw > 0) {
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<float4*>(sums + (wave * 32 + (lane & 31)) * PS + 32 * i + 8 * e + 4 * half) =
+              make_float4(acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]);
+    }
+    __syncthreads();
+    if (kw > 0) return;
+#pragma unroll
+    for (int y = 1; y < KW; ++y)
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4 x = *reinterpret_cast<const float4*>(sums + ((wave + y) * 32 + (lane & 31)) * PS + 32 * i + 8 * e + 4 * half);
+          acc[i][4 * e] += x.x;
+          acc[i][4 * e + 1] += x.y;
+          acc[i][4 * e + 2] += x.z;
+          acc[i][4 * e + 3] += x.w;
+        }
+  }
   float worst = 0.0f;
 #pragma unroll
   for (int i = 0; i < ND; ++i)
@@ -275,98 +320,144 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(BwdParams p) {
   }
 }
 
-// What a staged row needs beside its vectors.
-struct RowStat {
-  float lse, dsum, slope, pos;
+// How dkv_kernel's waves are set: KG groups of 32 keys, RW waves that share a
+// group's keys and take the rows in turn, row tiles of 32 NSUB rows a wave.
+//
+// bf16 at D = 128: dK and dV take 128 registers, so that K and V as operands (64
+// more) would leave one wave on a SIMD, waiting for each of its loads; they lie in
+// LDS instead (half as many LDS reads again), and the block has eight waves.
+template <typename T, int D, int KG_, int RW_>
+struct DkvShape {
+  static constexpr int KG = KG_, RW = RW_, kWaves = KG * RW, kThr = 64 * kWaves;
+  static constexpr bool kInLds = sizeof(T) == 2 && D == 128;
+  static constexpr int NSUB = RW == 1 && sizeof(T) == 2 ? 2 : 1;
+  static constexpr int QT = 32 * RW * NSUB, SG = QT / 32;
+  static constexpr int RB = D * static_cast<int>(sizeof(T)), TB = QT * RB, KB = 32 * KG * RB, PS = D + 4;
+  static constexpr size_t tiles = static_cast<size_t>(4) * TB, keys = kInLds ? static_cast<size_t>(2) * KB : 0;
+  static constexpr size_t sums = static_cast<size_t>(RW - 1) * KG * 32 * PS * sizeof(float);
+  static constexpr size_t lds = keys + tiles > sums ? keys + tiles : sums;
+  // waves a SIMD must hold
+  static constexpr int kPerSimd = sizeof(T) == 2 ? 2 : 1;
 };
 
-template <typename T, int D, bool RULE>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && D == 64 ? 2 : 1) void dkv_kernel(BwdParams p) {
+template <typename T, int D, bool RULE, int KG, int RW>
+__global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4) / (KG * RW) > 0
+                                               ? (DkvShape<T, D, KG, RW>::kPerSimd * 4) / (KG * RW)
+                                               : 1) void dkv_kernel(BwdParams p) {
   using O = Op<T>;
   using Frag = typename O::Frag;
-  constexpr int RB = D * O::kEsize, NCH = RB / 16, E = 16 / O::kEsize;
-  constexpr int QT = 32;  // rows of a tile: one group
-  constexpr int NC = D / 16, ND = D / 32;
-  constexpr int RPP = kThreads / NCH, NP = (QT + RPP - 1) / RPP, TB = QT * RB;
-  extern __shared__ __align__(16) char lds[];
+  using S = DkvShape<T, D, KG, RW>;
+  constexpr int RB = S::RB, NCH = RB / 16, E = 16 / O::kEsize, QT = S::QT, NSUB = S::NSUB, SG = S::SG;
+  constexpr int NC = D / 16, ND = D / 32, TB = S::TB, NT = S::kThr, RPP = NT / NCH, NP = (QT + RPP - 1) / RPP;
+  extern __shared__ __align__(16) char lds[];  // [K, V of the block's keys][2 buffers][Q, dO][TB]
   __shared__ __align__(16) float s_lse[2][QT], s_dsum[2][QT], s_slope[2][QT], s_pos[2][QT];
   __shared__ __align__(16) int s_lo[2][QT], s_hi[2][QT];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int rw = wave % RW, kg = wave / RW;
   const int nbh = p.batch * p.h_kv;
   const int bh = blockIdx.x % nbh;
   const int rest = blockIdx.x / nbh;
   const int split = rest % p.splits, tile = rest / p.splits;
   const int b = bh / p.h_kv, kvh = bh - b * p.h_kv;
   const int n_keys = static_cast<int>(p.n), n_rows = static_cast<int>(p.n_q * p.g);
-  const int kb0 = tile * kBlk;            // the block's keys
-  const int kw0 = kb0 + wave * 32;        // the wave's
+  const int kb0 = tile * 32 * KG;    // the block's keys
+  const int kw0 = kb0 + kg * 32;     // the wave's
   const int key = kw0 + (lane & 31);
   const bool real = key < n_keys;
 
   const T* krow = static_cast<const T*>(p.k) + b * p.k_sb + kvh * p.k_sh + static_cast<int64_t>(real ? key : 0) * p.k_sn;
   const T* vrow = static_cast<const T*>(p.v) + b * p.v_sb + kvh * p.v_sh + static_cast<int64_t>(real ? key : 0) * p.v_sn;
-  Frag kf[NC], vf[NC];
+  char* keys = lds;
+  char* bufs = lds + S::keys;
+  Frag kf[S::kInLds ? 1 : NC], vf[S::kInLds ? 1 : NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int e = 16 * c + 8 * half;
     const bool in = real && e < p.d;
-    kf[c] = in ? O::load(krow + e) : O::zero();
-    vf[c] = in ? O::load(vrow + e) : O::zero();
+    if constexpr (S::kInLds) {
+      if (rw == 0) {
+        const int at = chunk_at<RB>(kg * 32 + (lane & 31), 2 * c + half);
+        *reinterpret_cast<uint4*>(keys + at) = in ? *reinterpret_cast<const uint4*>(krow + e) : make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(keys + S::KB + at) = in ? *reinterpret_cast<const uint4*>(vrow + e) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    } else {
+      kf[c] = in ? O::load(krow + e) : O::zero();
+      vf[c] = in ? O::load(vrow + e) : O::zero();
+    }
   }
 
-  // the groups of rows that see some key of the block, in ascending order
-  const int g_end = min(p.groups, (split + 1) * p.split_groups);
+  // The row tiles that see some key of the block, in ascending order: lane x holds
+  // the bounds of the x-th tile of 64.
+  const int t_end = min((p.groups + SG - 1) / SG, (split + 1) * p.split_tiles);
   const int4* bounds = p.bounds + static_cast<int64_t>(b) * p.groups;
-  int g_base = split * p.split_groups - 64;
-  uint64_t g_mask = 0;
-  auto next_group = [&]() -> int {
-    while (g_mask == 0) {
-      g_base += 64;
-      if (g_base >= g_end) return -1;
-      bool hit = false;
-      if (g_base + lane < g_end) {
-        const int4 bd = bounds[g_base + lane];
-        hit = bd.x < kb0 + kBlk && bd.y > kb0;
+  int t_base = split * p.split_tiles - 64;
+  uint64_t t_mask = 0;
+  int4 bd[SG];
+  struct Pick {
+    int tile;
+    int lo_min[NSUB], hi_max[NSUB], lo_max[NSUB], hi_min[NSUB];  // of this wave's groups
+  };
+  auto next_tile = [&](Pick& pk) {
+    while (t_mask == 0) {
+      t_base += 64;
+      if (t_base >= t_end) {
+        pk.tile = -1;
+        return;
       }
-      g_mask = __ballot(hit);
+      bool hit = false;
+#pragma unroll
+      for (int x = 0; x < SG; ++x) {
+        const int g = (t_base + lane) * SG + x;
+        bd[x] = t_base + lane < t_end && g < p.groups ? bounds[g] : make_int4(0x7FFFFFFF, 0, 0, 0);
+        hit |= bd[x].x < kb0 + 32 * KG && bd[x].y > kb0;
+      }
+      t_mask = __ballot(hit);
     }
-    const int x = __builtin_ctzll(g_mask);
-    g_mask &= g_mask - 1;
-    return g_base + x;
+    const int x = __builtin_ctzll(t_mask);
+    t_mask &= t_mask - 1;
+    pk.tile = t_base + x;
+#pragma unroll
+    for (int u = 0; u < NSUB; ++u) {
+      // (rw is the same for the whole wave)
+      int4 mine = bd[u];
+#pragma unroll
+      for (int y = 1; y < RW; ++y)
+        if (rw == y) mine = bd[y * NSUB + u];
+      pk.lo_min[u] = lane_value(mine.x, x);
+      pk.hi_max[u] = lane_value(mine.y, x);
+      pk.lo_max[u] = lane_value(mine.z, x);
+      pk.hi_min[u] = lane_value(mine.w, x);
+    }
   };
 
   const int sc = tid % NCH, sr = tid / NCH;
   const bool chunk_ok = sc * E < p.d;
-  const T* qbase = static_cast<const T*>(p.q) + b * p.q_sb;
-  const T* dbase = static_cast<const T*>(p.dout) + b * p.do_sb;
+  const T* qbase = static_cast<const T*>(p.q) + b * p.q_sb + sc * E;
+  const T* dbase = static_cast<const T*>(p.dout) + b * p.do_sb + sc * E;
   uint4 qreg[NP], dreg[NP];
-  RowStat st_reg{};
-  int2 sp_reg{};
-  auto load_group = [&](int grp) {
+  float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+  float st_slope = 0.0f, st_pos = 0.0f;
+  auto load_rows = [&](int t) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int r = min(grp * QT + min(sr + i * RPP, QT - 1), n_rows - 1);
-      const int tok = r / p.g, hq = kvh * p.g + r - tok * p.g;
-      qreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(qbase + tok * p.q_sn + hq * p.q_sh + sc * E) : make_uint4(0u, 0u, 0u, 0u);
-      dreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(dbase + tok * p.do_sn + hq * p.do_sh + sc * E) : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t r = min(t * QT + min(sr + i * RPP, QT - 1), n_rows - 1);
+      const uint32_t tok = r / static_cast<uint32_t>(p.g), hq = kvh * p.g + r - tok * p.g;
+      qreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(qbase + tok * p.q_sn + hq * p.q_sh) : make_uint4(0u, 0u, 0u, 0u);
+      dreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(dbase + tok * p.do_sn + hq * p.do_sh) : make_uint4(0u, 0u, 0u, 0u);
     }
     if (tid < QT) {
-      const int r = grp * QT + tid;
-      const bool in = r < n_rows;
-      const int tok = in ? r / p.g : 0, hq = kvh * p.g + (in ? r - tok * p.g : 0);
-      sp_reg = in ? row_span(p, b, tok) : make_int2(0, 0);
-      const int64_t stat = (static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok;
-      st_reg.lse = sp_reg.y > sp_reg.x ? p.lse[stat] : INFINITY;
-      st_reg.dsum = p.dsum[stat];
+      const uint32_t r = min(t * QT + tid, n_rows - 1);
+      const uint32_t tok = r / static_cast<uint32_t>(p.g), hq = kvh * p.g + r - tok * p.g;
+      st = p.stats[(static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok];
       if constexpr (RULE) {
-        st_reg.slope = p.rule.slopes != nullptr ? p.rule.slopes[hq] * kLog2e : 0.0f;
-        st_reg.pos = static_cast<float>(static_cast<int>(p.q_pos0) + tok);
+        st_slope = p.rule.slopes != nullptr ? p.rule.slopes[hq] * kLog2e : 0.0f;
+        st_pos = static_cast<float>(static_cast<int>(p.q_pos0 + tok));
       }
     }
   };
-  auto store_group = [&](int buf) {
-    char* qt = lds + buf * 2 * TB;
+  auto store_rows = [&](int t, int buf) {
+    char* qt = bufs + buf * 2 * TB;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int row = sr + i * RPP;
@@ -376,13 +467,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && D == 64 ? 2 : 1) void d
       *reinterpret_cast<uint4*>(qt + TB + at) = dreg[i];
     }
     if (tid < QT) {
-      s_lse[buf][tid] = st_reg.lse;
-      s_dsum[buf][tid] = st_reg.dsum;
-      s_lo[buf][tid] = sp_reg.x;
-      s_hi[buf][tid] = sp_reg.y;
+      const bool in = t * QT + tid < n_rows;  // a row past the last one sees nothing
+      s_lse[buf][tid] = in ? st.x : INFINITY;
+      s_dsum[buf][tid] = st.y;
+      s_lo[buf][tid] = in ? __float_as_int(st.z) : 0;
+      s_hi[buf][tid] = in ? __float_as_int(st.w) : 0;
       if constexpr (RULE) {
-        s_slope[buf][tid] = st_reg.slope;
-        s_pos[buf][tid] = st_reg.pos;
+        s_slope[buf][tid] = st_slope;
+        s_pos[buf][tid] = st_pos;
       }
     }
   };
@@ -393,31 +485,40 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && D == 64 ? 2 : 1) void d
     acck[i] = f32x16{};
     accv[i] = f32x16{};
   }
-  int grp = next_group();
-  if (grp >= 0) {
-    load_group(grp);
-    store_group(0);
+  Pick cur, nx;
+  next_tile(cur);
+  if (cur.tile >= 0) {
+    load_rows(cur.tile);
+    store_rows(cur.tile, 0);
   }
-  for (int t = 0; grp >= 0; ++t) {
+  for (int t = 0; cur.tile >= 0; ++t) {
     __syncthreads();
-    const int nxt = next_group();
-    if (nxt >= 0) load_group(nxt);
-    const int4 bd = bounds[grp];
-    if (bd.x < kw0 + 32 && bd.y > kw0) {
-      const int buf = t & 1;
-      const char* qt = lds + buf * 2 * TB;
+    next_tile(nx);
+    if (nx.tile >= 0) load_rows(nx.tile);
+    const int buf = t & 1;
+#pragma unroll
+    for (int u = 0; u < NSUB; ++u) {
+      if (cur.lo_min[u] >= kw0 + 32 || cur.hi_max[u] <= kw0) continue;
+      const int row0 = (rw * NSUB + u) * 32;
+      const char* qt = bufs + buf * 2 * TB + row0 * RB;
       const char* dt = qt + TB;
       f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        s = O::mfma(O::template row_frag<RB>(qt, 0, c, lane), kf[c], s);
-        dp = O::mfma(O::template row_frag<RB>(dt, 0, c, lane), vf[c], dp);
+        if constexpr (S::kInLds) {
+          const Frag kk = O::template row_frag<RB>(keys, kg * 32, c, lane), vv = O::template row_frag<RB>(keys + S::KB, kg * 32, c, lane);
+          s = O::mfma(O::template row_frag<RB>(qt, 0, c, lane), kk, s);
+          dp = O::mfma(O::template row_frag<RB>(dt, 0, c, lane), vv, dp);
+        } else {
+          s = O::mfma(O::template row_frag<RB>(qt, 0, c, lane), kf[c], s);
+          dp = O::mfma(O::template row_frag<RB>(dt, 0, c, lane), vf[c], dp);
+        }
       }
-      const bool whole = bd.z <= kw0 && bd.w >= kw0 + 32 && (grp + 1) * QT <= n_rows;
+      const bool whole = cur.lo_max[u] <= kw0 && cur.hi_min[u] >= kw0 + 32 && cur.tile * QT + row0 + 32 <= n_rows;
       const float fkey = static_cast<float>(key);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int r0 = 8 * e + 4 * half;
+        const int r0 = row0 + 8 * e + 4 * half;
         const float4 ls = *reinterpret_cast<const float4*>(&s_lse[buf][r0]);
         const float4 dd = *reinterpret_cast<const float4*>(&s_dsum[buf][r0]);
         float4 sl = make_float4(0.f, 0.f, 0.f, 0.f), ps = sl;
@@ -425,24 +526,26 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && D == 64 ? 2 : 1) void d
           sl = *reinterpret_cast<const float4*>(&s_slope[buf][r0]);
           ps = *reinterpret_cast<const float4*>(&s_pos[buf][r0]);
         }
-        int4 lo4 = make_int4(0, 0, 0, 0), hi4 = lo4;
-        if (!whole) {
-          lo4 = *reinterpret_cast<const int4*>(&s_lo[buf][r0]);
-          hi4 = *reinterpret_cast<const int4*>(&s_hi[buf][r0]);
-        }
         const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dv[4] = {dd.x, dd.y, dd.z, dd.w};
         const float slv[4] = {sl.x, sl.y, sl.z, sl.w}, psv[4] = {ps.x, ps.y, ps.z, ps.w};
-        const int lov[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hiv[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int i = 4 * e + x;
           float f;
           const float y = score_x<T, RULE>(p.rule, s[i], slv[x], fkey - psv[x], f);
-          float w = exp2_w(y - lsv[x]);
-          float ds = w * (dp[i] - dv[x]) * f;
-          const bool see = whole || (key >= lov[x] && key < hiv[x]);
-          s[i] = see ? w : 0.0f;
-          dp[i] = see ? ds : 0.0f;
+          s[i] = exp2_w(y - lsv[x]);
+          dp[i] = s[i] * (dp[i] - dv[x]) * f;
+        }
+        if (!whole) {
+          const int4 lo4 = *reinterpret_cast<const int4*>(&s_lo[buf][r0]);
+          const int4 hi4 = *reinterpret_cast<const int4*>(&s_hi[buf][r0]);
+          const int lov[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hiv[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const bool see = key >= lov[x] && key < hiv[x];
+            s[4 * e + x] = see ? s[4 * e + x] : 0.0f;
+            dp[4 * e + x] = see ? dp[4 * e + x] : 0.0f;
+          }
         }
       }
 #pragma unroll
@@ -455,10 +558,42 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && D == 64 ? 2 : 1) void d
         }
       }
     }
-    if (nxt >= 0) store_group((t + 1) & 1);
-    grp = nxt;
+    if (nx.tile >= 0) store_rows(nx.tile, (t + 1) & 1);
+    cur = nx;
   }
 
+  if constexpr (RW > 1) {  // the first of the waves that share keys adds up, dK and then dV
+    float* sums = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      f32x16(&acc)[ND] = which == 0 ? acck : accv;
+      __syncthreads();
+      if (rw > 0) {
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<float4*>(sums + ((kg * (RW - 1) + rw - 1) * 32 + (lane & 31)) * S::PS + 32 * i + 8 * e + 4 * half) =
+                make_float4(acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]);
+      }
+      __syncthreads();
+      if (rw == 0) {
+#pragma unroll
+        for (int y = 0; y < RW - 1; ++y)
+#pragma unroll
+          for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float4 x = *reinterpret_cast<const float4*>(sums + ((kg * (RW - 1) + y) * 32 + (lane & 31)) * S::PS + 32 * i + 8 * e + 4 * half);
+              acc[i][4 * e] += x.x;
+              acc[i][4 * e + 1] += x.y;
+              acc[i][4 * e + 2] += x.z;
+              acc[i][4 * e + 3] += x.w;
+            }
+      }
+    }
+    if (rw > 0) return;
+  }
   float worst = 0.0f;
 #pragma unroll
   for (int i = 0; i < ND; ++i)
@@ -499,8 +634,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && D == 64 ? 2 : 1) void d
     const T* kr = static_cast<const T*>(lane_ptr(krow, src));
     const T* vr = static_cast<const T*>(lane_ptr(vrow, src));
     float ok[2] = {0.0f, 0.0f}, ov[2] = {0.0f, 0.0f};
-    const int r_end = min(n_rows, g_end * QT);
-    for (int r0 = split * p.split_groups * QT; r0 < r_end; r0 += 64) {
+    const T* qall = static_cast<const T*>(p.q) + b * p.q_sb;
+    const T* dall = static_cast<const T*>(p.dout) + b * p.do_sb;
+    const int r_end = min(n_rows, t_end * QT);
+    for (int r0 = split * p.split_tiles * QT; r0 < r_end; r0 += 64) {
       const int r = r0 + lane;
       bool see = false;
       float w = 0.0f, ds = 0.0f;
@@ -512,10 +649,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && D == 64 ? 2 : 1) void d
           const int64_t stat = (static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok;
           const float sl = RULE && p.rule.slopes != nullptr ? p.rule.slopes[hq] * kLog2e : 0.0f;
           float f;
-          const float x = score_x<T, RULE>(p.rule, row_dot(qbase + tok * p.q_sn + hq * p.q_sh, kr, p.d), sl,
+          const float x = score_x<T, RULE>(p.rule, row_dot(qall + tok * p.q_sn + hq * p.q_sh, kr, p.d), sl,
                                            static_cast<float>(kj) - static_cast<float>(static_cast<int>(p.q_pos0) + tok), f);
-          w = exp2_w(x - p.lse[stat]);
-          ds = w * (row_dot(dbase + tok * p.do_sn + hq * p.do_sh, vr, p.d) - p.dsum[stat]) * f;
+          const float4 rs = p.stats[stat];
+          w = exp2_w(x - rs.x);
+          ds = w * (row_dot(dall + tok * p.do_sn + hq * p.do_sh, vr, p.d) - rs.y) * f;
         }
       }
       uint64_t on = __ballot(see);
@@ -527,8 +665,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && D == 64 ? 2 : 1) void d
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           if (lane + 64 * e < p.d) {
-            ov[e] = fmaf(wx, ld(dbase + tok * p.do_sn + hq * p.do_sh + lane + 64 * e), ov[e]);
-            ok[e] = fmaf(dx, ld(qbase + tok * p.q_sn + hq * p.q_sh + lane + 64 * e), ok[e]);
+            ov[e] = fmaf(wx, ld(dall + tok * p.do_sn + hq * p.do_sh + lane + 64 * e), ov[e]);
+            ok[e] = fmaf(dx, ld(qall + tok * p.q_sn + hq * p.q_sh + lane + 64 * e), ok[e]);
           }
       }
     }
@@ -570,64 +708,90 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(BwdParams p) {
   Op<T>::store4(static_cast<T*>(isv ? p.dv : p.dk) + kid * p.d + dd, s.x, s.y, s.z, s.w);
 }
 
-template <typename T, int D, bool RULE>
-int launch_bwd(BwdParams& p, hipStream_t st) {
-  const char* fn = "ssa_masked_attention_backward";
-  constexpr int KT = sizeof(T) == 2 ? 64 : 32;
-  const size_t qbytes = 4 * static_cast<size_t>(KT) * D * sizeof(T), kbytes = 4 * static_cast<size_t>(32) * D * sizeof(T);
-  if (int rc = reserve_lds(reinterpret_cast<const void*>(dq_kernel<T, D, RULE>), qbytes + 1024, fn)) return rc;
-  if (int rc = reserve_lds(reinterpret_cast<const void*>(dkv_kernel<T, D, RULE>), kbytes + 4096, fn)) return rc;
-  const int64_t nbh = static_cast<int64_t>(p.batch) * p.h_kv;
-  const int64_t qblocks = ceil_div(p.n_q * p.g, kBlk) * nbh, kblocks = ceil_div(p.n, kBlk) * nbh * p.splits;
-  if (qblocks > 0x7FFFFFFF || kblocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many rows", fn);
-  if (qblocks > 0) {
-    dq_kernel<T, D, RULE><<<dim3(static_cast<unsigned>(qblocks)), dim3(kThreads), qbytes, st>>>(p);
-    if (int rc = check_launch("ssa_masked_attention_backward dq")) return rc;
+// How a backward is cut, and its workspace: the rows' stats, the groups' bounds, and
+// the parts of dK and dV.
+struct BwdCut {
+  int kw, key_groups, splits, groups;
+  size_t stats, bounds, part, bytes;
+};
+
+BwdCut bwd_cut(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv, int d) {
+  BwdCut l{};
+  const int64_t rows = n_q * (h_q / h_kv), heads = batch * h_kv;
+  const bool f32 = dtype == SSA_DTYPE_F32, wide = d > 64;
+  l.groups = static_cast<int>(ceil_div(rows, 32));
+  // dQ: as the forward, waves share rows where blocks of 128 leave CUs idle.
+  l.kw = 1;
+  while (l.kw < (f32 && wide ? 2 : 4) && ceil_div(rows, 128 / l.kw) * heads < 512 && n > 32 * l.kw) l.kw *= 2;
+  // dK, dV: likewise waves share keys; then the rows are cut into parts of at least
+  // 256, until each CU has several blocks (causal ones are of unlike lengths).
+  l.key_groups = 4;
+  while (l.key_groups > (wide ? 2 : 1) && ceil_div(n, 32 * l.key_groups) * heads < 256 && rows > 128 / l.key_groups * 2)
+    l.key_groups /= 2;
+  const int64_t blocks = ceil_div(n, 32 * l.key_groups) * heads;
+  l.splits = 1;
+  if (blocks > 0 && blocks < 512) {
+    const int64_t want = ceil_div(1024, blocks), can = rows / 256;
+    l.splits = static_cast<int>(want < can ? want : (can > 1 ? can : 1));
   }
-  if (kblocks > 0) {
-    dkv_kernel<T, D, RULE><<<dim3(static_cast<unsigned>(kblocks)), dim3(kThreads), kbytes, st>>>(p);
-    if (int rc = check_launch("ssa_masked_attention_backward dkv")) return rc;
-    if (p.splits > 1) {
-      const int64_t work = 2 * nbh * p.n * (p.d / 4);
-      dkv_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(work, 256))), dim3(256), 0, st>>>(p);
-      if (int rc = check_launch("ssa_masked_attention_backward join")) return rc;
-    }
+  l.stats = 0;
+  l.bounds = static_cast<size_t>(batch) * h_q * n_q * sizeof(float4);
+  l.part = l.bounds + static_cast<size_t>(batch) * l.groups * sizeof(int4);
+  l.bytes = l.part;
+  if (l.splits > 1) l.bytes += 2 * static_cast<size_t>(l.splits) * batch * n * h_kv * (wide ? 128 : 64) * sizeof(float);
+  return l;
+}
+
+template <typename T, int D, bool RULE, int KW>
+int launch_dq(BwdParams& p, hipStream_t st) {
+  const char* fn = "ssa_masked_attention_backward";
+  const size_t bytes = dq_lds<T, D, KW>();
+  if (int rc = reserve_lds(reinterpret_cast<const void*>(dq_kernel<T, D, RULE, KW>), bytes + 1024, fn)) return rc;
+  const int64_t blocks = ceil_div(p.n_q * p.g, kBlk / KW) * p.batch * p.h_kv;
+  if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many rows", fn);
+  dq_kernel<T, D, RULE, KW><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(p);
+  return check_launch("ssa_masked_attention_backward dq");
+}
+
+template <typename T, int D, bool RULE, int KG, int RW>
+int launch_dkv(BwdParams& p, hipStream_t st) {
+  const char* fn = "ssa_masked_attention_backward";
+  using S = DkvShape<T, D, KG, RW>;
+  if (int rc = reserve_lds(reinterpret_cast<const void*>(dkv_kernel<T, D, RULE, KG, RW>), S::lds + 24 * S::QT * 2 + 1024, fn)) return rc;
+  const int64_t nbh = static_cast<int64_t>(p.batch) * p.h_kv;
+  const int64_t blocks = ceil_div(p.n, 32 * KG) * nbh * p.splits;
+  if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many keys", fn);
+  p.split_tiles = static_cast<int>(ceil_div(ceil_div(p.groups, S::SG), p.splits));
+  dkv_kernel<T, D, RULE, KG, RW><<<dim3(static_cast<unsigned>(blocks)), dim3(S::kThr), S::lds, st>>>(p);
+  if (int rc = check_launch("ssa_masked_attention_backward dkv")) return rc;
+  if (p.splits > 1) {
+    const int64_t work = 2 * nbh * p.n * (p.d / 4);
+    dkv_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(work, 256))), dim3(256), 0, st>>>(p);
+    return check_launch("ssa_masked_attention_backward join");
   }
   return SSA_OK;
 }
 
-template <typename T, int D>
-int launch_rule(BwdParams& p, hipStream_t st) {
-  return p.rule.cap || p.rule.slopes != nullptr ? launch_bwd<T, D, true>(p, st) : launch_bwd<T, D, false>(p, st);
+template <typename T, int D, bool RULE>
+int launch_bwd(BwdParams& p, const BwdCut& cut, hipStream_t st) {
+  int rc;
+  if (most_kw<T, D>() >= 4 && cut.kw == 4)
+    rc = launch_dq<T, D, RULE, most_kw<T, D>()>(p, st);
+  else
+    rc = cut.kw >= 2 ? launch_dq<T, D, RULE, 2>(p, st) : launch_dq<T, D, RULE, 1>(p, st);
+  if (rc) return rc;
+  if constexpr (sizeof(T) == 2 && D == 128) {
+    return cut.key_groups == 4 ? launch_dkv<T, D, RULE, 4, 2>(p, st) : launch_dkv<T, D, RULE, 2, 2>(p, st);
+  } else {
+    if constexpr (D == 64)
+      if (cut.key_groups == 1) return launch_dkv<T, D, RULE, 1, 4>(p, st);
+    return cut.key_groups == 4 ? launch_dkv<T, D, RULE, 4, 1>(p, st) : launch_dkv<T, D, RULE, 2, 2>(p, st);
+  }
 }
 
-// The workspace: D, the groups' bounds, and the parts of dK and dV.
-struct BwdLayout {
-  int groups, splits, split_groups;
-  size_t dsum, bounds, part, bytes;
-};
-
-BwdLayout bwd_layout(int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv, int d) {
-  BwdLayout l{};
-  const int64_t rows = n_q * (h_q / h_kv);
-  l.groups = static_cast<int>(ceil_div(rows, 32));
-  // Parts of the rows where the keys alone give fewer blocks than CUs, of at
-  // least 256 rows (8 groups) each.
-  const int64_t blocks = ceil_div(n, kBlk) * batch * h_kv;
-  int64_t s = 1;
-  if (blocks > 0 && blocks < 256) {
-    s = (512 + blocks - 1) / blocks;
-    const int64_t most = l.groups / 8;
-    s = s < most ? s : (most > 1 ? most : 1);
-  }
-  l.split_groups = static_cast<int>(ceil_div(l.groups > 0 ? l.groups : 1, s));
-  l.splits = static_cast<int>(ceil_div(l.groups > 0 ? l.groups : 1, l.split_groups));
-  l.dsum = 0;
-  l.bounds = align_up(static_cast<size_t>(batch) * h_q * n_q * sizeof(float), 16);
-  l.part = align_up(l.bounds + static_cast<size_t>(batch) * l.groups * sizeof(int4), 16);
-  l.bytes = l.part;
-  if (l.splits > 1) l.bytes += 2 * static_cast<size_t>(l.splits) * batch * n * h_kv * (d <= 64 ? 64 : 128) * sizeof(float);
-  return l;
+template <typename T, int D>
+int launch_rule(BwdParams& p, const BwdCut& cut, hipStream_t st) {
+  return p.rule.cap || p.rule.slopes != nullptr ? launch_bwd<T, D, true>(p, cut, st) : launch_bwd<T, D, false>(p, cut, st);
 }
 
 }  // namespace
@@ -635,10 +799,10 @@ BwdLayout bwd_layout(int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv, i
 
 using namespace ssa;
 
-extern "C" size_t ssa_masked_attention_backward_workspace_bytes(int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv,
-                                                                int d) {
+extern "C" size_t ssa_masked_attention_backward_workspace_bytes(int dtype, int64_t batch, int64_t n, int64_t n_q,
+                                                                int h_q, int h_kv, int d) {
   if (batch <= 0 || n <= 0 || n_q <= 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0) return 0;
-  return bwd_layout(batch, n, n_q, h_q, h_kv, d).bytes;
+  return bwd_cut(dtype, batch, n, n_q, h_q, h_kv, d).bytes;
 }
 
 extern "C" int ssa_masked_attention_backward(
@@ -672,7 +836,7 @@ extern "C" int ssa_masked_attention_backward(
   if (int rc = check_aligned(fn, "dq", dtype, dq, 0, 0, 0)) return rc;
   if (int rc = check_aligned(fn, "dk", dtype, dk, 0, 0, 0)) return rc;
   if (int rc = check_aligned(fn, "dv", dtype, dv, 0, 0, 0)) return rc;
-  const BwdLayout l = bwd_layout(batch, n, n_q, h_q, h_kv, d);
+  const BwdCut l = bwd_cut(dtype, batch, n, n_q, h_q, h_kv, d);
   if (workspace == nullptr || workspace_bytes < l.bytes)
     return fail(SSA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", fn, l.bytes,
                 workspace == nullptr ? size_t(0) : workspace_bytes);
@@ -690,16 +854,15 @@ extern "C" int ssa_masked_attention_backward(
   p.spans = reinterpret_cast<const int2*>(spans);
   p.inv_scale = 1.0f / scale_div;
   char* ws = static_cast<char*>(workspace);
-  p.dsum = reinterpret_cast<float*>(ws + l.dsum);
+  p.stats = reinterpret_cast<float4*>(ws + l.stats);
   p.bounds = reinterpret_cast<int4*>(ws + l.bounds);
   p.groups = l.groups;
   p.splits = l.splits;
-  p.split_groups = l.split_groups;
   if (l.splits > 1) {
     p.part_k = reinterpret_cast<float*>(ws + l.part);
     p.part_v = p.part_k + static_cast<int64_t>(l.splits) * batch * n * h_kv * (d <= 64 ? 64 : 128);
   }
   hipStream_t st = as_stream(stream);
-  if (dtype == SSA_DTYPE_F32) return d <= 64 ? launch_rule<float, 64>(p, st) : launch_rule<float, 128>(p, st);
-  return d <= 64 ? launch_rule<uint16_t, 64>(p, st) : launch_rule<uint16_t, 128>(p, st);
+  if (dtype == SSA_DTYPE_F32) return d <= 64 ? launch_rule<float, 64>(p, l, st) : launch_rule<float, 128>(p, l, st);
+  return d <= 64 ? launch_rule<uint16_t, 64>(p, l, st) : launch_rule<uint16_t, 128>(p, l, st);
 }

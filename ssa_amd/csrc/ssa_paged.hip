@@ -269,71 +269,85 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_ker
   }
 }
 
-// One wave a row: the parts of a few-row sequence.
+// One block a row: the parts of a few-row sequence, every eighth one a wave's, four
+// of its loads in flight; the waves' sums meet in LDS.
+constexpr int kJoinWaves = 8;
+
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void few_join_kernel(DenseParams p, int row_blocks) {
-  const int lane = threadIdx.x & 63;
-  const int bh = blockIdx.x / row_blocks;
-  const int r = (blockIdx.x - bh * row_blocks) * (kThreads / 64) + (threadIdx.x >> 6);
+__global__ __launch_bounds__(kJoinWaves * 64) void few_join_kernel(DenseParams p, int most_rows) {
+  constexpr int L = D / 64;  // features of a lane: lane * L ..
+  __shared__ float s_o[kJoinWaves][D], s_m[kJoinWaves], s_l[kJoinWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int bh = blockIdx.x / most_rows, r = blockIdx.x - bh * most_rows;
   const int b = bh / p.h_kv, kvh = bh - b * p.h_kv;
   const Seq sq = paged_seq(p, b);
   const int R = sq.m * p.g;
   if (R > p.few_rows || r >= R) return;
   const int parts = static_cast<int>(min(static_cast<int64_t>(p.splits), ceil_div(sq.len, p.split_len)));
   const int64_t row = static_cast<int64_t>(bh) * kFew + r;
-  float m = -INFINITY;
-  for (int s = lane; s < parts; s += 64) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * p.part_rows + row) * 2);
-    if (ml.y != 0.0f) m = fmaxf(m, ml.x);
+  float m = -INFINITY, l = 0.0f, o[L];
+#pragma unroll
+  for (int e = 0; e < L; ++e) o[e] = 0.0f;
+  for (int s0 = wave; s0 < parts; s0 += 4 * kJoinWaves) {
+    float2 ml[4];
+    float v[4][L];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = min(s0 + i * kJoinWaves, parts - 1) * p.part_rows + row;
+      ml[i] = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+#pragma unroll
+      for (int e = 0; e < L; ++e) v[i][e] = p.part_o[at * D + lane * L + e];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (s0 + i * kJoinWaves >= parts || ml[i].y == 0.0f) continue;  // (an empty part)
+      const float mn = fmaxf(m, ml[i].x), ref = mn == -INFINITY ? 0.0f : mn;
+      const float a = exp2_w(m - ref), w = exp2_w(ml[i].x - ref);
+      m = mn;
+      l = fmaf(l, a, ml[i].y * w);
+#pragma unroll
+      for (int e = 0; e < L; ++e) o[e] = fmaf(v[i][e], w, o[e] * a);
+    }
   }
-  m = wave_max(m);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float o[D / 64], l = 0.0f;
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) o[e] = 0.0f;
-  for (int s0 = 0; s0 < parts; s0 += 64) {
-    float a = 0.0f, ls = 0.0f;
-    if (s0 + lane < parts) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((s0 + lane) * p.part_rows + row) * 2);
-      if (ml.y != 0.0f) {
-        a = exp2_w(ml.x - ref);
-        ls = ml.y * a;
-      }
-    }
-    l += wave_sum(ls);
-    uint64_t on = __ballot(ls != 0.0f);
-    while (on != 0) {
-      const int src = __builtin_ctzll(on);
-      on &= on - 1;
-      const float as = lane_value(a, src);
-      const float* pr = p.part_o + ((s0 + src) * p.part_rows + row) * D;
+  for (int e = 0; e < L; ++e) s_o[wave][lane * L + e] = o[e];
+  if (lane == 0) {
+    s_m[wave] = m;
+    s_l[wave] = l;
+  }
+  __syncthreads();
+  const int dd = threadIdx.x;
+  if (dd >= p.d) return;
+  float top = s_m[0];
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e)
-        if (lane + 64 * e < p.d) o[e] = fmaf(as, pr[lane + 64 * e], o[e]);
-    }
+  for (int x = 1; x < kJoinWaves; ++x) top = fmaxf(top, s_m[x]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f, val = 0.0f;
+#pragma unroll
+  for (int x = 0; x < kJoinWaves; ++x) {
+    const float a = exp2_w(s_m[x] - ref);
+    sum = fmaf(a, s_l[x], sum);
+    val = fmaf(a, s_o[x][dd], val);
   }
   const int t = r / p.g, h = kvh * p.g + r - t * p.g;
-  T* orow = static_cast<T*>(p.out) + (sq.first + t) * p.o_sn + h * p.o_sh;
-  const float inv = 1.0f / l;  // (a token sees itself: l = 0 only where every score is -inf)
-#pragma unroll
-  for (int e = 0; e < D / 64; ++e)
-    if (lane + 64 * e < p.d) Op<T>::store1(orow + lane + 64 * e, o[e] * inv);
+  // (a token sees itself: the sum is 0 only where every score is -inf)
+  Op<T>::store1(static_cast<T*>(p.out) + (sq.first + t) * p.o_sn + h * p.o_sh + dd, val * (1.0f / sum));
 }
 
 // Parts, tiles and workspace of a call.
 struct PagedPlan {
-  int few_splits, row_splits, row_tiles;
+  int few_splits, row_splits, row_tiles, row_kw;
   int64_t few_len, row_len;
   size_t few_o, few_ml, row_o, row_ml, bytes;
 };
 
-PagedPlan paged_plan(int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t max_new, int64_t max_len) {
+PagedPlan paged_plan(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t max_new, int64_t max_len) {
   PagedPlan l{};
   const int64_t g = h_q / h_kv, D = d <= 64 ? 64 : 128;
-  // Few rows: parts of at least 256 keys, four blocks a CU where the keys give
-  // them (sequences of unlike lengths even out).
+  // Few rows: parts of at least 256 keys, enough for two blocks a CU twice over
+  // where the batch has sequences of unlike lengths to even out, once for one.
   const int64_t blocks = batch * h_kv;
-  int64_t s = (1024 + blocks - 1) / blocks, most = ceil_div(max_len, 256);
+  int64_t s = ceil_div(batch > 1 ? 1024 : 512, blocks), most = ceil_div(max_len, 256);
   s = s < most ? s : most;
   s = s > 1 ? s : 1;
   l.few_len = ceil_div(ceil_div(max_len, s), 128) * 128;
@@ -341,9 +355,14 @@ PagedPlan paged_plan(int64_t tokens, int64_t batch, int h_q, int h_kv, int d, in
   l.row_splits = 1;
   l.row_len = 0;
   if (max_new * g > kFew) {
-    const int64_t each = batch * ceil_div(max_new * g, kRows), ragged = tokens * g / kRows + batch;
-    l.row_tiles = static_cast<int>(each < ragged ? each : ragged);
-    l.row_splits = dense_splits(static_cast<int64_t>(l.row_tiles) * h_kv, max_len);
+    const int64_t each = batch * max_new, rows = (tokens < each ? tokens : each) * g;
+    const DenseSplit cut = dense_split(rows, h_kv, max_len, dtype == SSA_DTYPE_F32 && d > 64);
+    const int block = rows_of(cut.kw);
+    // (a sequence's last block may be part empty)
+    const int64_t by_seq = batch * ceil_div(max_new * g, block), ragged = rows / block + batch;
+    l.row_kw = cut.kw;
+    l.row_tiles = static_cast<int>(by_seq < ragged ? by_seq : ragged);
+    l.row_splits = cut.parts;
     l.row_len = ceil_div(ceil_div(max_len, l.row_splits), 64) * 64;
   }
   if (l.few_splits > 1) {
@@ -359,6 +378,22 @@ PagedPlan paged_plan(int64_t tokens, int64_t batch, int h_q, int h_kv, int d, in
     l.bytes = align_up(l.row_ml + rows * 2 * sizeof(float), 16);
   }
   return l;
+}
+
+template <typename T, int D, bool RULE, int KW>
+int launch_rows(DenseParams& r, int row_tiles, hipStream_t st) {
+  const char* fn = "ssa_paged_step";
+  const size_t bytes = rows_lds<T, D, KW>();
+  if (int rc = reserve_lds(reinterpret_cast<const void*>(dense_rows_kernel<T, D, true, RULE, KW>), bytes + 2048, fn)) return rc;
+  const int64_t blocks = static_cast<int64_t>(row_tiles) * r.h_kv * r.splits;
+  if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many tokens", fn);
+  dense_rows_kernel<T, D, true, RULE, KW><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(r);
+  if (int rc = check_launch("ssa_paged_step rows")) return rc;
+  if (r.splits > 1) {
+    dense_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(r.part_rows, kThreads / 64))), dim3(kThreads), 0, st>>>(r);
+    if (int rc = check_launch("ssa_paged_step row join")) return rc;
+  }
+  return SSA_OK;
 }
 
 template <typename T, int D, bool RULE>
@@ -384,9 +419,10 @@ int launch_paged(DenseParams& p, const AppendParams& a, const PagedPlan& l, char
   few_rows_kernel<T, D, RULE><<<dim3(static_cast<unsigned>(fblocks)), dim3(kThreads), fbytes, st>>>(f);
   if (int rc = check_launch("ssa_paged_step few rows")) return rc;
   if (f.splits > 1) {
-    const int64_t most = p.max_new * p.g < kFew ? p.max_new * p.g : kFew;
-    const int row_blocks = static_cast<int>(ceil_div(most, kThreads / 64));
-    few_join_kernel<T, D><<<dim3(static_cast<unsigned>(p.batch * p.h_kv * row_blocks)), dim3(kThreads), 0, st>>>(f, row_blocks);
+    const int most = static_cast<int>(p.max_new * p.g < kFew ? p.max_new * p.g : kFew);
+    const int64_t jblocks = static_cast<int64_t>(p.batch) * p.h_kv * most;
+    if (jblocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many sequences", fn);
+    few_join_kernel<T, D><<<dim3(static_cast<unsigned>(jblocks)), dim3(kJoinWaves * 64), 0, st>>>(f, most);
     if (int rc = check_launch("ssa_paged_step join")) return rc;
   }
   if (l.row_tiles > 0) {
@@ -396,16 +432,9 @@ int launch_paged(DenseParams& p, const AppendParams& a, const PagedPlan& l, char
     r.part_rows = p.n_q * p.h_q;
     r.part_o = reinterpret_cast<float*>(ws + l.row_o);
     r.part_ml = reinterpret_cast<float*>(ws + l.row_ml);
-    const size_t bytes = 4 * static_cast<size_t>(key_tile<T>()) * D * sizeof(T);
-    if (int rc = reserve_lds(reinterpret_cast<const void*>(dense_rows_kernel<T, D, true, RULE>), bytes + 1024, fn)) return rc;
-    const int64_t blocks = static_cast<int64_t>(l.row_tiles) * p.h_kv * r.splits;
-    if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many tokens", fn);
-    dense_rows_kernel<T, D, true, RULE><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(r);
-    if (int rc = check_launch("ssa_paged_step rows")) return rc;
-    if (r.splits > 1) {
-      dense_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(r.part_rows, kThreads / 64))), dim3(kThreads), 0, st>>>(r);
-      if (int rc = check_launch("ssa_paged_step row join")) return rc;
-    }
+    if constexpr (most_kw<T, D>() >= 4)
+      if (l.row_kw == 4) return launch_rows<T, D, RULE, 4>(r, l.row_tiles, st);
+    return l.row_kw == 2 ? launch_rows<T, D, RULE, 2>(r, l.row_tiles, st) : launch_rows<T, D, RULE, 1>(r, l.row_tiles, st);
   }
   return SSA_OK;
 }
@@ -421,10 +450,10 @@ int launch_rule(DenseParams& p, const AppendParams& a, const PagedPlan& l, char*
 
 using namespace ssa;
 
-extern "C" size_t ssa_paged_step_workspace_bytes(int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t max_new,
-                                                 int64_t max_len) {
+extern "C" size_t ssa_paged_step_workspace_bytes(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv, int d,
+                                                 int64_t max_new, int64_t max_len) {
   if (tokens <= 0 || batch <= 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0 || max_new <= 0 || max_len <= 0) return 0;
-  return paged_plan(tokens, batch, h_q, h_kv, d, max_new, max_len).bytes;
+  return paged_plan(dtype, tokens, batch, h_q, h_kv, d, max_new, max_len).bytes;
 }
 
 extern "C" int ssa_paged_step(const void* q, const void* k, const void* v, int dtype, int64_t tokens, int64_t batch, int h_q,
@@ -461,7 +490,7 @@ extern "C" int ssa_paged_step(const void* q, const void* k, const void* v, int d
   if (max_new > tokens) max_new = tokens;
   const int64_t cap = static_cast<int64_t>(max_pages) * page_size;
   if (max_len > cap) max_len = cap;
-  const PagedPlan l = paged_plan(tokens, batch, h_q, h_kv, d, max_new, max_len);
+  const PagedPlan l = paged_plan(dtype, tokens, batch, h_q, h_kv, d, max_new, max_len);
   if (l.bytes > 0 && (workspace == nullptr || workspace_bytes < l.bytes))
     return fail(SSA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", fn, l.bytes,
                 workspace == nullptr ? size_t(0) : workspace_bytes);

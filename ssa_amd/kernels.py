@@ -570,7 +570,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: O
     out = torch.empty((B, n_q, h_q, d), device=q.device, dtype=q.dtype)
     lse = torch.empty((B, h_q, n_q), device=q.device, dtype=torch.float32) if with_lse else None
     low = torch.empty_like(out) if with_lse and q.dtype == torch.bfloat16 else None
-    nbytes = int(_lib.load().ssa_masked_attention_workspace_bytes(B, n, n_q, h_q, h_kv, d))
+    nbytes = int(_lib.load().ssa_masked_attention_workspace_bytes(_lib.elem_dtype(q), B, n, n_q, h_q, h_kv, d))
     ws = _workspace(nbytes, q.device)
     _call_on(q, "ssa_masked_attention", ptr(q), ptr(k), ptr(v), _lib.elem_dtype(q), B, n, n_q, q_pos0, h_q, h_kv, d,
              *_strides(q), *_strides(k), *_strides(v), ptr(spans), float(math.sqrt(d) if scale_div is None else scale_div),
@@ -604,7 +604,7 @@ def masked_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         raise ValueError("out_low must have out's shape, strides and dtype")
     q, k, v, out, dout = (_aligned_rows(t) for t in (q, k, v, out, dout))
     out_low = None if out_low is None else _aligned_rows(out_low)
-    nbytes = int(_lib.load().ssa_masked_attention_backward_workspace_bytes(B, n, n_q, h_q, h_kv, d))
+    nbytes = int(_lib.load().ssa_masked_attention_backward_workspace_bytes(_lib.elem_dtype(q), B, n, n_q, h_q, h_kv, d))
     ws = _workspace(nbytes, q.device)
     _call_on(q, "ssa_masked_attention_backward", ptr(q), ptr(k), ptr(v), _lib.elem_dtype(q), B, n, n_q, q_pos0, h_q, h_kv,
              d, *_strides(q), *_strides(k), *_strides(v), ptr(spans),
@@ -659,7 +659,7 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
     max_new = T if max_new is None else min(int(max_new), T)
     width = table.shape[1] * page
     max_len = width if max_len is None else min(int(max_len), width)
-    nbytes = int(_lib.load().ssa_paged_step_workspace_bytes(T, B, h_q, h_kv, d, max_new, max_len))
+    nbytes = int(_lib.load().ssa_paged_step_workspace_bytes(_lib.elem_dtype(q), T, B, h_q, h_kv, d, max_new, max_len))
     ws = _workspace(nbytes, q.device)
     ks, vs = ((0, 0) if t is None else _strides(t) for t in (k, v))
     _call_on(q, "ssa_paged_step", ptr(q), ptr(k), ptr(v), _lib.elem_dtype(q), T, B, h_q, h_kv, d, *_strides(q), *ks, *vs,

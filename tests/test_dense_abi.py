@@ -80,7 +80,7 @@ DENSE = [
 ])
 def test_masked_attention(L, kw, status, text):
     if "ws" in kw or "ws_bytes" in kw:
-        assert L.ssa_masked_attention_workspace_bytes(1, 4000, 4, 8, 2, 64) > 100
+        assert L.ssa_masked_attention_workspace_bytes(_lib.DTYPE_BF16, 1, 4000, 4, 8, 2, 64) > 100
         kw = {**kw, "n": 4000}
     st, msg = _call(L, "ssa_masked_attention", FORWARD, kw)
     assert st == status and (st == OK or text in msg), msg
