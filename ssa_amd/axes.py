@@ -10,9 +10,8 @@ from __future__ import annotations
 from typing import Optional, Sequence
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import _lib, kernels
+from . import kernels
 
 
 def axis_rope_freqs(rot: int, theta: float = 10000.0, device=None) -> torch.Tensor:
@@ -21,36 +20,25 @@ def axis_rope_freqs(rot: int, theta: float = 10000.0, device=None) -> torch.Tens
 
 
 class _RopeAxes(torch.autograd.Function):
-    """ssa_rope_axes with its transpose (the turn back) as the backward."""
+    """ssa_rope_axes with its transpose (the turn back) as the backward, to any order."""
 
     @staticmethod
-    def forward(ctx, q, k, positions, freqs, sections):
-        ctx.save_for_backward(positions, freqs)
-        ctx.sections = sections
-        return kernels.rope_axes(q, k, positions, freqs, sections)
+    def forward(ctx, q, k, plan, positions, freqs, inverse):
+        ctx.save_for_backward(positions, freqs)  # (the plan reads them: they must be as they were)
+        ctx.plan, ctx.inverse = plan, inverse
+        q, k = kernels.axes_run(plan, q, k, inverse)
+        return q if k is None else (q, k)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk):
-        positions, freqs = ctx.saved_tensors
-        dq, dk = kernels.rope_axes(dq, dk, positions, freqs, ctx.sections, inverse=True)
-        return dq, dk, None, None, None
-
-
-class _RopeAxesOne(torch.autograd.Function):
-    """The same for q alone."""
-
-    @staticmethod
-    def forward(ctx, q, positions, freqs, sections):
-        ctx.save_for_backward(positions, freqs)
-        ctx.sections = sections
-        return kernels.rope_axes(q, None, positions, freqs, sections)[0]
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq):
-        positions, freqs = ctx.saved_tensors
-        return kernels.rope_axes(dq, None, positions, freqs, ctx.sections, inverse=True)[0], None, None, None
+    def backward(ctx, dq, dk=None):
+        ctx.saved_tensors
+        plan, inverse = ctx.plan, not ctx.inverse
+        if torch.is_grad_enabled():
+            out = _RopeAxes.apply(dq, dk, plan, plan.positions, plan.freqs, inverse)
+            dq, dk = (out, None) if dk is None else out
+        else:
+            dq, dk = kernels.axes_run(plan, dq, dk, inverse)
+        return dq, dk, None, None, None, None
 
 
 def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor,
@@ -67,20 +55,18 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
     unbatched = q.dim() == 3
     if unbatched:
         q, k = q.unsqueeze(0), None if k is None else k.unsqueeze(0)
-    _lib.require_device(q, k, positions, freqs)
-    if positions.dim() == 2:
-        positions = positions[:, None].expand(-1, q.shape[0], -1)
-    dtypes = (q.dtype, None if k is None else k.dtype)
-    if q.dtype == torch.float16:
+    half = q.dtype == torch.float16
+    if half:
+        if k is not None and k.dtype != q.dtype:
+            raise ValueError(f"k must have q's dtype {q.dtype}, got {k.dtype}")
         q, k = q.float(), None if k is None else k.float()
-    sections = tuple(int(x) for x in sections)
-    grad = torch.is_grad_enabled()
-    if k is None:
-        out = ((_RopeAxesOne.apply(q, positions, freqs, sections) if grad and q.requires_grad
-                else kernels.rope_axes(q, None, positions, freqs, sections)[0]),)
-    elif grad and (q.requires_grad or k.requires_grad):
-        out = _RopeAxes.apply(q, k, positions, freqs, sections)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        out = _RopeAxes.apply(q, k, kernels.axes_plan(q, k, positions, freqs, sections), positions, freqs, False)
+        out = (out,) if k is None else out
     else:
         out = kernels.rope_axes(q, k, positions, freqs, sections)
-    out = tuple((x[0] if unbatched else x).to(t) for x, t in zip(out, dtypes))
+    if half:
+        out = tuple(None if x is None else x.half() for x in out)
+    if unbatched:
+        out = tuple(None if x is None else x[0] for x in out)
     return out[0] if k is None else out

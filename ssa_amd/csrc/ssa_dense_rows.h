@@ -45,6 +45,10 @@ struct DenseParams {
   int max_pages, page_log2, num_pages, few_rows;
   int64_t max_new, max_len;  // what a sequence may hold (the launch is sized by them)
   int32_t* error_flag;
+  // new rows of k and v, read from here while they are copied to their pages (null:
+  // they are there)
+  const void *k_new, *v_new;
+  int64_t kn_st, kn_sh, vn_st, vn_sh;
   // the key axis in parts
   int splits;
   int64_t split_len;
@@ -77,7 +81,8 @@ __device__ __forceinline__ Seq paged_seq(const DenseParams& p, int b) {
   return s;
 }
 
-// The row of key j: contiguous keys, or the sequence's pages.
+// The row of key j: contiguous keys, or the sequence's pages (its new rows where the
+// call brought them).
 template <typename T, bool PAGED>
 struct KeyRows {
   const T *k, *v;
@@ -85,6 +90,9 @@ struct KeyRows {
   const int32_t* table;
   int page_log2, page_mask, num_pages;
   int32_t* error_flag;
+  const T *k_new, *v_new;  // row of key new_from
+  int64_t kn_st, vn_st;
+  int new_from;
 
   __device__ __forceinline__ int page_of(int j) const {
     int pg = table[j >> page_log2];
@@ -95,9 +103,10 @@ struct KeyRows {
     return pg;
   }
   __device__ __forceinline__ void in_page(int64_t pg, int j, const T*& kr, const T*& vr) const {
-    const int64_t r = j & page_mask;
-    kr = k + pg * k_sb + r * k_sn;
-    vr = v + pg * v_sb + r * v_sn;
+    const int64_t r = j & page_mask, x = j - new_from;
+    const T *kp = k + pg * k_sb + r * k_sn, *vp = v + pg * v_sb + r * v_sn;
+    kr = x >= 0 ? k_new + x * kn_st : kp;
+    vr = x >= 0 ? v_new + x * vn_st : vp;
   }
   __device__ __forceinline__ void at(int j, const T*& kr, const T*& vr) const {
     if constexpr (PAGED) {
@@ -110,7 +119,7 @@ struct KeyRows {
 };
 
 template <typename T, bool PAGED>
-__device__ __forceinline__ KeyRows<T, PAGED> key_rows(const DenseParams& p, int b, int kvh) {
+__device__ __forceinline__ KeyRows<T, PAGED> key_rows(const DenseParams& p, int b, int kvh, int first, int cached) {
   KeyRows<T, PAGED> r;
   const int64_t kb = PAGED ? 0 : b * p.k_sb, vb = PAGED ? 0 : b * p.v_sb;
   r.k = static_cast<const T*>(p.k) + kb + kvh * p.k_sh;
@@ -124,6 +133,13 @@ __device__ __forceinline__ KeyRows<T, PAGED> key_rows(const DenseParams& p, int 
   r.page_mask = (1 << p.page_log2) - 1;
   r.num_pages = p.num_pages;
   r.error_flag = p.error_flag;
+  if constexpr (PAGED) {
+    r.new_from = p.k_new != nullptr ? cached : 0x7FFFFFFF;
+    r.k_new = static_cast<const T*>(p.k_new) + first * p.kn_st + kvh * p.kn_sh;
+    r.v_new = static_cast<const T*>(p.v_new) + first * p.vn_st + kvh * p.vn_sh;
+    r.kn_st = p.kn_st;
+    r.vn_st = p.vn_st;
+  }
   return r;
 }
 
@@ -226,8 +242,8 @@ constexpr size_t rows_lds() {
   return tiles > sums ? tiles : sums;
 }
 
-template <typename T, int D, bool PAGED, bool RULE, int KW>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void dense_rows_kernel(DenseParams p) {
+template <typename T, int D, bool PAGED, int RULE, int KW>
+__global__ __launch_bounds__(kThreads, (rows_lds<T, D, KW>() > 80 * 1024 || (sizeof(T) == 4 && D == 128) ? 1 : 2)) void dense_rows_kernel(DenseParams p) {
   using O = Op<T>;
   using Frag = typename O::Frag;
   constexpr int RB = D * O::kEsize;      // bytes of a tile row
@@ -272,7 +288,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void d
     n_keys = p.n;
     tile = static_cast<int>((p.n_q * p.g + BR - 1) / BR) - 1 - rest;
   }
-  const KeyRows<T, PAGED> rows = key_rows<T, PAGED>(p, b, kvh);
+  const KeyRows<T, PAGED> rows = key_rows<T, PAGED>(p, b, kvh, first, static_cast<int>(n_keys) - m);
 
   // this lane's row
   const int r = tile * BR + rw * 32 + (lane & 31);
@@ -292,7 +308,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void d
     if (hi <= lo) lo = hi = 0;
   }
   const bool some = real && hi > lo;
-  const float slope = (RULE && p.rule.slopes != nullptr && real) ? p.rule.slopes[hq] * kLog2e : 0.0f;
+  const Rule<T, RULE> rule(p.rule);
+  const float slope = RULE == kBias && real ? p.rule.slopes[hq] * kLog2e : 0.0f;
   const int lo_min = wave_min_i(some ? lo : 0x7FFFFFFF), hi_max = wave_max_i(some ? hi : 0);
   const int lo_max = wave_max_i(real ? lo : 0), hi_min = wave_min_i(real ? hi : 0x7FFFFFFF);
   if (lane == 0) {
@@ -384,27 +401,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void d
         for (int u = 0; u < NSUB; ++u) s[u] = O::mfma(O::template row_frag<RB>(kt, 32 * u, c, lane), qf[c], s[u]);
 
       const int kl = k0 + 4 * half;  // key of register 0
-      float cs = p.rule.c1;          // what is left to multiply the scores by
-      if constexpr (RULE) {
-        cs = 1.0f;
-        if (p.rule.cap) {
+      const float dist = static_cast<float>(kl - pos);
 #pragma unroll
-          for (int u = 0; u < NSUB; ++u)
+      for (int u = 0; u < NSUB; ++u)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[u][i] = p.rule.c2 * cap_tanh<T>(s[u][i] * p.rule.c1);
-        } else {
-#pragma unroll
-          for (int u = 0; u < NSUB; ++u) s[u] *= p.rule.c1;
-        }
-        if (p.rule.slopes != nullptr) {
-          const float dist = static_cast<float>(kl - pos);
-#pragma unroll
-          for (int u = 0; u < NSUB; ++u)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              s[u][i] = fmaf(-slope, fabsf(dist + static_cast<float>(32 * u + 8 * (i >> 2) + (i & 3))), s[u][i]);
-        }
-      }
+        for (int i = 0; i < 16; ++i)
+          s[u][i] = rule.z(p.rule, s[u][i], slope, dist + static_cast<float>(32 * u + 8 * (i >> 2) + (i & 3)));
       const bool whole = k0 >= lo_max && k0 + 32 * NSUB <= hi_min && k0 >= part_lo && k0 + 32 * NSUB <= part_hi;
       if (!whole) {
         const int a = max(lo, part_lo) - kl, z = min(hi, part_hi) - kl;
@@ -413,15 +415,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void d
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int j = 32 * u + 8 * (i >> 2) + (i & 3);
-            if (j < a || j >= z) s[u][i] = -INFINITY;
+            if (j < a || j >= z) s[u][i] = Rule<T, RULE>::kHidden;
           }
       }
-      float top = -INFINITY;
+      float top = Rule<T, RULE>::kHidden;
 #pragma unroll
       for (int u = 0; u < NSUB; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
-      top = fmaxf(top, other_half(top)) * cs;
+        for (int i = 0; i < 16; ++i) top = rule.better(top, s[u][i]);
+      top = fmaf(rule.better(top, other_half(top)), rule.a, rule.b);
       if (__ballot(top > mref + 8.0f) != 0) {
         const float mn = fmaxf(mref, top);
         const float alpha = mref == mn ? 1.0f : exp2_w(mref - mn);
@@ -430,12 +432,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void d
 #pragma unroll
         for (int i = 0; i < ND; ++i) acc[i] *= alpha;
       }
-      const float ref = mref == -INFINITY ? 0.0f : mref;
+      const float nref = rule.b - (mref == -INFINITY ? 0.0f : mref);
 #pragma unroll
       for (int u = 0; u < NSUB; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          s[u][i] = exp2_w(fmaf(s[u][i], cs, -ref));
+          s[u][i] = exp2_w(fmaf(s[u][i], rule.a, nref));
           lsum += s[u][i];
         }
 #pragma unroll
@@ -575,45 +577,39 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void d
   }
 }
 
-// Joins the parts of each row: one wave a row, lane e features e, e + 64, ....
+// Joins the parts of each row: one wave a row.
 // A part without a key has m = -inf and l = 0 and its o is not read.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void dense_join_kernel(DenseParams p) {
   const int lane = threadIdx.x & 63;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
   if (row >= p.part_rows) return;
-  float m = -INFINITY;
+  constexpr int L = D / 64;  // features of a lane: lane * L ..
+  float m = -INFINITY, l = 0.0f, o[L];
   bool seen = false;
-  for (int s = lane; s < p.splits; s += 64) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * p.part_rows + row) * 2);
-    if (ml.y != 0.0f) m = fmaxf(m, ml.x);
-    seen |= ml.x != -INFINITY;
-  }
-  m = wave_max(m);
-  seen = __ballot(seen) != 0;
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float o[D / 64], l = 0.0f;
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) o[e] = 0.0f;
-  for (int s0 = 0; s0 < p.splits; s0 += 64) {
-    float a = 0.0f, ls = 0.0f;
-    if (s0 + lane < p.splits) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((s0 + lane) * p.part_rows + row) * 2);
-      if (ml.y != 0.0f) {
-        a = exp2_w(ml.x - ref);
-        ls = ml.y * a;
-      }
+  for (int e = 0; e < L; ++e) o[e] = 0.0f;
+  for (int s0 = 0; s0 < p.splits; s0 += 4) {  // four parts' loads in flight
+    float2 ml[4];
+    float v[4][L];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = min(s0 + i, p.splits - 1) * p.part_rows + row;
+      ml[i] = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+#pragma unroll
+      for (int e = 0; e < L; ++e) v[i][e] = p.part_o[at * D + lane * L + e];
     }
-    l += wave_sum(ls);
-    uint64_t on = __ballot(ls != 0.0f);
-    while (on != 0) {
-      const int src = __builtin_ctzll(on);
-      on &= on - 1;
-      const float as = lane_value(a, src);
-      const float* pr = p.part_o + ((s0 + src) * p.part_rows + row) * D;
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e)
-        if (lane + 64 * e < p.d) o[e] = fmaf(as, pr[lane + 64 * e], o[e]);
+    for (int i = 0; i < 4; ++i) {
+      if (s0 + i >= p.splits) continue;
+      seen |= ml[i].x != -INFINITY;
+      if (ml[i].y == 0.0f) continue;  // (an empty part: its o was not written)
+      const float mn = fmaxf(m, ml[i].x), ref = mn == -INFINITY ? 0.0f : mn;
+      const float a = exp2_w(m - ref), w = exp2_w(ml[i].x - ref);
+      m = mn;
+      l = fmaf(l, a, ml[i].y * w);
+#pragma unroll
+      for (int e = 0; e < L; ++e) o[e] = fmaf(v[i][e], w, o[e] * a);
     }
   }
   const int64_t tok = row / p.h_q, hq = row - tok * p.h_q;
@@ -634,11 +630,11 @@ __global__ __launch_bounds__(kThreads) void dense_join_kernel(DenseParams p) {
   // no key: zeros; only keys of score -inf: NaN
   const float inv = seen ? 1.0f / l : 0.0f;
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e)
-    if (lane + 64 * e < p.d) {
-      Op<T>::store1(orow + lane + 64 * e, o[e] * inv);
+  for (int e = 0; e < L; ++e)
+    if (lane * L + e < p.d) {
+      Op<T>::store1(orow + lane * L + e, o[e] * inv);
       if (p.out_low != nullptr)
-        Op<T>::store1(static_cast<T*>(p.out_low) + (orow - static_cast<T*>(p.out)) + lane + 64 * e, Op<T>::left(o[e] * inv));
+        Op<T>::store1(static_cast<T*>(p.out_low) + (orow - static_cast<T*>(p.out)) + lane * L + e, Op<T>::left(o[e] * inv));
     }
   if (p.lse != nullptr && lane == 0) p.lse[(b * p.h_q + hq) * p.n_q + t] = seen ? m + __log2f(l) : INFINITY;
 }

@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void mask_spans_kernel(const int32_t* starts, 
   out[t] = hi > lo ? make_int2(static_cast<int>(lo), static_cast<int>(hi)) : make_int2(0, 0);
 }
 
-template <typename T, int D, bool RULE, int KW>
+template <typename T, int D, int RULE, int KW>
 int launch_rows(DenseParams& p, hipStream_t st) {
   const size_t bytes = rows_lds<T, D, KW>();
   if (int rc = reserve_lds(reinterpret_cast<const void*>(dense_rows_kernel<T, D, false, RULE, KW>), bytes + 2048,
@@ -66,7 +66,7 @@ int launch_rows(DenseParams& p, hipStream_t st) {
   return SSA_OK;
 }
 
-template <typename T, int D, bool RULE>
+template <typename T, int D, int RULE>
 int launch_kw(DenseParams& p, int kw, hipStream_t st) {
   if constexpr (most_kw<T, D>() >= 4)
     if (kw == 4) return launch_rows<T, D, RULE, 4>(p, st);
@@ -75,24 +75,36 @@ int launch_kw(DenseParams& p, int kw, hipStream_t st) {
 
 template <typename T, int D>
 int launch_rule(DenseParams& p, int kw, hipStream_t st) {
-  return p.rule.cap || p.rule.slopes != nullptr ? launch_kw<T, D, true>(p, kw, st) : launch_kw<T, D, false>(p, kw, st);
+  switch (rule_kind(p.rule)) {
+    case kPlain: return launch_kw<T, D, kPlain>(p, kw, st);
+    case kCap: return launch_kw<T, D, kCap>(p, kw, st);
+    default: return launch_kw<T, D, kBias>(p, kw, st);
+  }
 }
 
 }  // namespace
 
 DenseSplit dense_split(int64_t rows, int64_t heads, int64_t keys, bool wide_f32) {
-  // Two blocks fit a CU.  Where blocks of 128 rows are fewer than that, the key axis
-  // is cut into parts of at least 1024 keys (a part's rows are written and read once
-  // more, in a second launch), and where keys are fewer too, two or four waves share
-  // each 32 rows and take turns at them.
+  // Two blocks fit a CU, so 512 run at once.  Blocks of 128 rows that are fewer
+  // (us a call, bf16, measured with each cut):
+  //   over many keys, the key axis is cut into as many parts as about 512 blocks
+  //     take, at least 384 keys each; not in two below 8192 keys, where the second
+  //     launch costs more (1200 rows x 8 heads over 16k keys: 1 part 289, 6 parts 138;
+  //     1000 x 8 x 4 rows over 1000 keys: 1 part 47, 2 parts 62);
+  //   and where blocks are few still, two or four waves share each 32 rows and take
+  //     turns at the keys (2048 x 8 rows of 2 x 1024 tokens, d = 64: 32, 28 and 24 us
+  //     with 1, 2 and 4; from 512 blocks on one wave a row is as fast or faster; four
+  //     read each key tile for 32 rows only, twice as slow over 6000 keys).
   DenseSplit s{1, 1};
-  const int most = wide_f32 ? 2 : 4;
   const int64_t blocks = ceil_div(rows, 128) * heads;
-  if (blocks > 0 && blocks < 512) {
-    const int64_t want = ceil_div(512, blocks), can = keys / 1024;
-    s.parts = static_cast<int>(want < can ? want : (can > 1 ? can : 1));
-  }
-  while (s.kw < most && ceil_div(rows, 128 / s.kw) * heads * s.parts < 512 && keys > 32 * s.kw) s.kw *= 2;
+  if (blocks <= 0 || blocks >= 512) return s;
+  const int64_t want = (512 + blocks / 4) / blocks, can = keys / 384;
+  int64_t parts = want < can ? want : can;
+  if (parts < 2 || (parts == 2 && keys < 8192)) parts = 1;
+  s.parts = static_cast<int>(parts);
+  if (blocks * parts < 512 && keys > 32) s.kw = 2;
+  if (blocks * parts < 192 && keys > 64 && keys < 2048 && !wide_f32) s.kw = 4;
+  if (parts > 1 && blocks * parts >= 384) s.kw = 1;
   return s;
 }
 

@@ -46,7 +46,6 @@ struct BwdParams {
   int4* bounds;   // [batch][groups of 32 packed rows]: lo_min, hi_max, lo_max, hi_min
   int groups;
   int splits;     // parts of the rows for dK and dV
-  int split_tiles;
   float *part_k, *part_v;  // [splits][batch][n][h_kv][D]
 };
 
@@ -64,20 +63,10 @@ __device__ __forceinline__ int2 row_span(const BwdParams& p, int b, int tok) {
   return hi > lo ? make_int2(lo, hi) : make_int2(0, 0);
 }
 
-// x (log2 units) and 1 - t^2 of a raw product.
-template <typename T, bool RULE>
+// x (log2 units) and 1 - t^2 of a raw product, one pair at a time.
+template <typename T>
 __device__ __forceinline__ float score_x(const ScoreRule& r, float dot, float slope, float dist, float& factor) {
-  factor = 1.0f;
-  float x = dot * r.c1;
-  if constexpr (RULE) {
-    if (r.cap) {
-      const float t = cap_tanh<T>(x);
-      factor = fmaf(-t, t, 1.0f);
-      x = r.c2 * t;
-    }
-    x = fmaf(-slope, fabsf(dist), x);
-  }
-  return x;
+  return Rule<T, kBias>(r).z(r, dot, slope, dist, factor);
 }
 
 template <typename T>
@@ -111,8 +100,8 @@ constexpr size_t dq_lds() {
   return tiles > sums ? tiles : sums;
 }
 
-template <typename T, int D, bool RULE, int KW>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void dq_kernel(BwdParams p) {
+template <typename T, int D, int RULE, int KW>
+__global__ __launch_bounds__(kThreads, (dq_lds<T, D, KW>() > 80 * 1024 || (sizeof(T) == 4 && D == 128) ? 1 : 2)) void dq_kernel(BwdParams p) {
   using O = Op<T>;
   using Frag = typename O::Frag;
   constexpr int RB = D * O::kEsize, NCH = RB / 16, E = 16 / O::kEsize;
@@ -139,7 +128,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void d
   const int2 sp = real ? row_span(p, b, tok) : make_int2(0, 0);
   const int lo = sp.x, hi = sp.y;
   const bool some = real && hi > lo;
-  const float slope = (RULE && p.rule.slopes != nullptr && real) ? p.rule.slopes[hq] * kLog2e : 0.0f;
+  const Rule<T, RULE> rule(p.rule);
+  const float slope = RULE == kBias && real ? p.rule.slopes[hq] * kLog2e : 0.0f;
   const int lo_min = wave_min_i(some ? lo : 0x7FFFFFFF), hi_max = wave_max_i(some ? hi : 0);
   const int lo_max = wave_max_i(real ? lo : 0), hi_min = wave_min_i(real ? hi : 0x7FFFFFFF);
   if (lane == 0) {
@@ -223,15 +213,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void d
           dp = O::mfma(O::template row_frag<RB>(vt, 32 * u, c, lane), dof[c], dp);
         }
         const int kl = k0 + 4 * half;
-        const float dist = static_cast<float>(kl - pos);
+        const float dist = static_cast<float>(kl - pos), nlse = rule.b - lse;
         const bool whole = k0 >= lo_max && k0 + 32 <= hi_min;
         const int a = lo - kl, z = hi - kl;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int j = 8 * (i >> 2) + (i & 3);
           float f;
-          const float x = score_x<T, RULE>(p.rule, s[i], slope, dist + static_cast<float>(j), f);
-          const float w = exp2_w(x - lse) * (dp[i] - dsum) * f;
+          const float x = rule.z(p.rule, s[i], slope, dist + static_cast<float>(j), f);
+          const float w = exp2_w(fmaf(x, rule.a, nlse)) * (dp[i] - dsum) * f;
           s[i] = whole || (j >= a && j < z) ? w : 0.0f;
         }
 #pragma unroll
@@ -285,7 +275,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void d
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int dd = 32 * i + 8 * e + 4 * half;
-        const float z = some ? p.inv_scale : 0.0f;
+        const float z = p.inv_scale * Rule<T, RULE>::kSlopeUnit;
         if (dd < p.d)
           O::store4(dqrow + dd, some ? acc[i][4 * e] * z : 0.0f, some ? acc[i][4 * e + 1] * z : 0.0f,
                     some ? acc[i][4 * e + 2] * z : 0.0f, some ? acc[i][4 * e + 3] * z : 0.0f);
@@ -304,7 +294,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || D == 64 ? 2 : 1) void d
     for (int j0 = a; j0 < z; j0 += 64) {
       const int j = min(j0 + lane, z - 1);
       float f;
-      const float x = score_x<T, RULE>(p.rule, row_dot(qr, kbase + j * p.k_sn, p.d), sl, static_cast<float>(j - ps), f);
+      const float x = score_x<T>(p.rule, row_dot(qr, kbase + j * p.k_sn, p.d), sl, static_cast<float>(j - ps), f);
       const float w = exp2_w(x - ls) * (row_dot(dr, vbase + j * p.v_sn, p.d) - ds0) * f;
       for (int t = 0; t < min(64, z - j0); ++t) {
         const float wt = lane_value(w, t);
@@ -337,10 +327,10 @@ struct DkvShape {
   static constexpr size_t sums = static_cast<size_t>(RW - 1) * KG * 32 * PS * sizeof(float);
   static constexpr size_t lds = keys + tiles > sums ? keys + tiles : sums;
   // waves a SIMD must hold
-  static constexpr int kPerSimd = sizeof(T) == 2 ? 2 : 1;
+  static constexpr int kPerSimd = sizeof(T) == 2 && (kWaves == 8 || lds <= 80 * 1024) ? 2 : 1;
 };
 
-template <typename T, int D, bool RULE, int KG, int RW>
+template <typename T, int D, int RULE, int KG, int RW>
 __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4) / (KG * RW) > 0
                                                ? (DkvShape<T, D, KG, RW>::kPerSimd * 4) / (KG * RW)
                                                : 1) void dkv_kernel(BwdParams p) {
@@ -365,6 +355,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
   const int kw0 = kb0 + kg * 32;     // the wave's
   const int key = kw0 + (lane & 31);
   const bool real = key < n_keys;
+  const Rule<T, RULE> rule(p.rule);
 
   const T* krow = static_cast<const T*>(p.k) + b * p.k_sb + kvh * p.k_sh + static_cast<int64_t>(real ? key : 0) * p.k_sn;
   const T* vrow = static_cast<const T*>(p.v) + b * p.v_sb + kvh * p.v_sh + static_cast<int64_t>(real ? key : 0) * p.v_sn;
@@ -389,9 +380,11 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
 
   // The row tiles that see some key of the block, in ascending order: lane x holds
   // the bounds of the x-th tile of 64.
-  const int t_end = min((p.groups + SG - 1) / SG, (split + 1) * p.split_tiles);
+  // (of parts, each takes every splits-th one: they are as long as each other
+  // whatever the mask)
+  const int t_end = (p.groups + SG - 1) / SG;
   const int4* bounds = p.bounds + static_cast<int64_t>(b) * p.groups;
-  int t_base = split * p.split_tiles - 64;
+  int t_base = -64, t_seen = 0;
   uint64_t t_mask = 0;
   int4 bd[SG];
   struct Pick {
@@ -413,6 +406,11 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
         hit |= bd[x].x < kb0 + 32 * KG && bd[x].y > kb0;
       }
       t_mask = __ballot(hit);
+      if (p.splits > 1) {
+        const int at = t_seen + __popcll(t_mask & ((uint64_t(1) << lane) - 1));
+        t_seen += __popcll(t_mask);
+        t_mask = __ballot(hit && static_cast<uint32_t>(at) % static_cast<uint32_t>(p.splits) == static_cast<uint32_t>(split));
+      }
     }
     const int x = __builtin_ctzll(t_mask);
     t_mask &= t_mask - 1;
@@ -450,8 +448,8 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
       const uint32_t r = min(t * QT + tid, n_rows - 1);
       const uint32_t tok = r / static_cast<uint32_t>(p.g), hq = kvh * p.g + r - tok * p.g;
       st = p.stats[(static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok];
-      if constexpr (RULE) {
-        st_slope = p.rule.slopes != nullptr ? p.rule.slopes[hq] * kLog2e : 0.0f;
+      if constexpr (RULE == kBias) {
+        st_slope = p.rule.slopes[hq] * kLog2e;
         st_pos = static_cast<float>(static_cast<int>(p.q_pos0 + tok));
       }
     }
@@ -468,11 +466,11 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
     }
     if (tid < QT) {
       const bool in = t * QT + tid < n_rows;  // a row past the last one sees nothing
-      s_lse[buf][tid] = in ? st.x : INFINITY;
+      s_lse[buf][tid] = in ? rule.b - st.x : -INFINITY;
       s_dsum[buf][tid] = st.y;
       s_lo[buf][tid] = in ? __float_as_int(st.z) : 0;
       s_hi[buf][tid] = in ? __float_as_int(st.w) : 0;
-      if constexpr (RULE) {
+      if constexpr (RULE == kBias) {
         s_slope[buf][tid] = st_slope;
         s_pos[buf][tid] = st_pos;
       }
@@ -522,7 +520,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
         const float4 ls = *reinterpret_cast<const float4*>(&s_lse[buf][r0]);
         const float4 dd = *reinterpret_cast<const float4*>(&s_dsum[buf][r0]);
         float4 sl = make_float4(0.f, 0.f, 0.f, 0.f), ps = sl;
-        if constexpr (RULE) {
+        if constexpr (RULE == kBias) {
           sl = *reinterpret_cast<const float4*>(&s_slope[buf][r0]);
           ps = *reinterpret_cast<const float4*>(&s_pos[buf][r0]);
         }
@@ -532,8 +530,8 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
         for (int x = 0; x < 4; ++x) {
           const int i = 4 * e + x;
           float f;
-          const float y = score_x<T, RULE>(p.rule, s[i], slv[x], fkey - psv[x], f);
-          s[i] = exp2_w(y - lsv[x]);
+          const float y = rule.z(p.rule, s[i], slv[x], fkey - psv[x], f);
+          s[i] = exp2_w(fmaf(y, rule.a, lsv[x]));
           dp[i] = s[i] * (dp[i] - dv[x]) * f;
         }
         if (!whole) {
@@ -614,7 +612,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
       for (int e = 0; e < 4; ++e) {
         const int dd = 32 * i + 8 * e + 4 * half;
         if (dd >= p.d) continue;
-        const float z = p.inv_scale;
+        const float z = p.inv_scale * Rule<T, RULE>::kSlopeUnit;
         const float4 a = make_float4(acck[i][4 * e] * z, acck[i][4 * e + 1] * z, acck[i][4 * e + 2] * z, acck[i][4 * e + 3] * z);
         const float4 c = make_float4(accv[i][4 * e], accv[i][4 * e + 1], accv[i][4 * e + 2], accv[i][4 * e + 3]);
         if (p.splits > 1) {
@@ -636,8 +634,15 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
     float ok[2] = {0.0f, 0.0f}, ov[2] = {0.0f, 0.0f};
     const T* qall = static_cast<const T*>(p.q) + b * p.q_sb;
     const T* dall = static_cast<const T*>(p.dout) + b * p.do_sb;
-    const int r_end = min(n_rows, t_end * QT);
-    for (int r0 = split * p.split_tiles * QT; r0 < r_end; r0 += 64) {
+    int at = 0;  // tiles seen, as next_tile counts them
+    for (int t = 0; t < t_end; ++t) {
+      if (p.splits > 1) {
+        bool hit = false;
+        for (int x = t * SG; x < min((t + 1) * SG, p.groups); ++x) hit |= bounds[x].x < kb0 + 32 * KG && bounds[x].y > kb0;
+        if (!hit || at++ % p.splits != split) continue;
+      }
+      const int r_end = min(n_rows, (t + 1) * QT);
+      for (int r0 = t * QT; r0 < r_end; r0 += 64) {
       const int r = r0 + lane;
       bool see = false;
       float w = 0.0f, ds = 0.0f;
@@ -647,9 +652,9 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
         see = kj >= sp.x && kj < sp.y;
         if (see) {
           const int64_t stat = (static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok;
-          const float sl = RULE && p.rule.slopes != nullptr ? p.rule.slopes[hq] * kLog2e : 0.0f;
+          const float sl = RULE == kBias ? p.rule.slopes[hq] * kLog2e : 0.0f;
           float f;
-          const float x = score_x<T, RULE>(p.rule, row_dot(qall + tok * p.q_sn + hq * p.q_sh, kr, p.d), sl,
+          const float x = score_x<T>(p.rule, row_dot(qall + tok * p.q_sn + hq * p.q_sh, kr, p.d), sl,
                                            static_cast<float>(kj) - static_cast<float>(static_cast<int>(p.q_pos0) + tok), f);
           const float4 rs = p.stats[stat];
           w = exp2_w(x - rs.x);
@@ -668,6 +673,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
             ov[e] = fmaf(wx, ld(dall + tok * p.do_sn + hq * p.do_sh + lane + 64 * e), ov[e]);
             ok[e] = fmaf(dx, ld(qall + tok * p.q_sn + hq * p.q_sh + lane + 64 * e), ok[e]);
           }
+      }
       }
     }
     const int64_t id = (static_cast<int64_t>(b) * p.n + kj) * p.h_kv + kvh;
@@ -720,19 +726,28 @@ BwdCut bwd_cut(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q, int h_
   const int64_t rows = n_q * (h_q / h_kv), heads = batch * h_kv;
   const bool f32 = dtype == SSA_DTYPE_F32, wide = d > 64;
   l.groups = static_cast<int>(ceil_div(rows, 32));
-  // dQ: as the forward, waves share rows where blocks of 128 leave CUs idle.
-  l.kw = 1;
-  while (l.kw < (f32 && wide ? 2 : 4) && ceil_div(rows, 128 / l.kw) * heads < 512 && n > 32 * l.kw) l.kw *= 2;
-  // dK, dV: likewise waves share keys; then the rows are cut into parts of at least
-  // 256, until each CU has several blocks (causal ones are of unlike lengths).
+  // dQ: waves share rows where blocks of 128 are few, earlier than in the forward
+  // (no maximum to agree on): 1500 x 8 rows of 4 x 2 heads, 752 blocks, take the
+  // same with one wave a row and with two; 2048 x 7 of 4 heads, 448 blocks, 5% less
+  // with two; 4096 of 4 heads at d = 64, 128 blocks, 9% less with four.
+  const int64_t qblocks = ceil_div(rows, 128) * heads;
+  l.kw = qblocks >= 1024 || n <= 32 ? 1 : (qblocks >= 192 || n <= 64 || (f32 && wide) ? 2 : 4);
+  // dK, dV: blocks of 128 keys, their rows cut into parts until 512 blocks (two a CU
+  // where they fit; 1024 of the smaller ones of bf16 at d = 64, of which four do) fill
+  // the device, at least 128 rows a part, one more part where that fills the last
+  // round better.  With fewer than 256 blocks even so, blocks of 64 or 32 keys, whose
+  // waves share keys.  Parts cost a write and a read of dK and dV in fp32: 64 blocks
+  // (2048 keys, 28 / 4 heads, d = 128) take 395, 330, 266 and 300 us in 3, 4, 8 and 16.
+  const int64_t target = !f32 && !wide ? 1024 : 512;
   l.key_groups = 4;
-  while (l.key_groups > (wide ? 2 : 1) && ceil_div(n, 32 * l.key_groups) * heads < 256 && rows > 128 / l.key_groups * 2)
-    l.key_groups /= 2;
-  const int64_t blocks = ceil_div(n, 32 * l.key_groups) * heads;
-  l.splits = 1;
-  if (blocks > 0 && blocks < 512) {
-    const int64_t want = ceil_div(1024, blocks), can = rows / 256;
-    l.splits = static_cast<int>(want < can ? want : (can > 1 ? can : 1));
+  for (;; l.key_groups /= 2) {
+    const int64_t blocks = ceil_div(n, 32 * l.key_groups) * heads;
+    int64_t s = blocks > 0 ? ceil_div(target, blocks) : 1;
+    auto idle = [&](int64_t x) { return static_cast<double>(ceil_div(blocks * x, 256) * 256) / (blocks * x); };
+    if (s > 1 && blocks > 0 && idle(s + 1) < idle(s) - 0.1) ++s;
+    const int64_t most = rows / 128;
+    l.splits = static_cast<int>(s < most ? s : (most > 1 ? most : 1));
+    if (blocks * l.splits >= 256 || l.key_groups <= (wide ? 2 : 1)) break;
   }
   l.stats = 0;
   l.bounds = static_cast<size_t>(batch) * h_q * n_q * sizeof(float4);
@@ -742,7 +757,7 @@ BwdCut bwd_cut(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q, int h_
   return l;
 }
 
-template <typename T, int D, bool RULE, int KW>
+template <typename T, int D, int RULE, int KW>
 int launch_dq(BwdParams& p, hipStream_t st) {
   const char* fn = "ssa_masked_attention_backward";
   const size_t bytes = dq_lds<T, D, KW>();
@@ -753,7 +768,7 @@ int launch_dq(BwdParams& p, hipStream_t st) {
   return check_launch("ssa_masked_attention_backward dq");
 }
 
-template <typename T, int D, bool RULE, int KG, int RW>
+template <typename T, int D, int RULE, int KG, int RW>
 int launch_dkv(BwdParams& p, hipStream_t st) {
   const char* fn = "ssa_masked_attention_backward";
   using S = DkvShape<T, D, KG, RW>;
@@ -761,7 +776,6 @@ int launch_dkv(BwdParams& p, hipStream_t st) {
   const int64_t nbh = static_cast<int64_t>(p.batch) * p.h_kv;
   const int64_t blocks = ceil_div(p.n, 32 * KG) * nbh * p.splits;
   if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many keys", fn);
-  p.split_tiles = static_cast<int>(ceil_div(ceil_div(p.groups, S::SG), p.splits));
   dkv_kernel<T, D, RULE, KG, RW><<<dim3(static_cast<unsigned>(blocks)), dim3(S::kThr), S::lds, st>>>(p);
   if (int rc = check_launch("ssa_masked_attention_backward dkv")) return rc;
   if (p.splits > 1) {
@@ -772,7 +786,7 @@ int launch_dkv(BwdParams& p, hipStream_t st) {
   return SSA_OK;
 }
 
-template <typename T, int D, bool RULE>
+template <typename T, int D, int RULE>
 int launch_bwd(BwdParams& p, const BwdCut& cut, hipStream_t st) {
   int rc;
   if (most_kw<T, D>() >= 4 && cut.kw == 4)
@@ -791,7 +805,11 @@ int launch_bwd(BwdParams& p, const BwdCut& cut, hipStream_t st) {
 
 template <typename T, int D>
 int launch_rule(BwdParams& p, const BwdCut& cut, hipStream_t st) {
-  return p.rule.cap || p.rule.slopes != nullptr ? launch_bwd<T, D, true>(p, cut, st) : launch_bwd<T, D, false>(p, cut, st);
+  switch (rule_kind(p.rule)) {
+    case kPlain: return launch_bwd<T, D, kPlain>(p, cut, st);
+    case kCap: return launch_bwd<T, D, kCap>(p, cut, st);
+    default: return launch_bwd<T, D, kBias>(p, cut, st);
+  }
 }
 
 }  // namespace

@@ -2,7 +2,9 @@
 // of sequences, each with its new tokens' rows appended to its pages and attended
 // over everything it has cached, causally.
 //
-//   append       a thread copies 16 bytes of a new token's k or v row to its page
+//   append       blocks of the first launch copy the new rows to their pages, 16
+//                bytes a thread; the attention reads them from the call's k and v, so
+//                that nothing waits for the copies
 //   few rows     sequences with at most 32 rows (tokens x heads of a group) per KV
 //                head, single tokens above all: few_rows_kernel
 //   many rows    chunks: dense_rows_kernel (ssa_dense_rows.h) over pages
@@ -27,16 +29,13 @@ using namespace tile;
 
 constexpr int kFew = 32;  // rows of a few-row block
 
-struct AppendParams {
-  const void *k, *v;
-  int64_t k_st, k_sh, v_st, v_sh;
-};
+constexpr int kAppend = 4 * kThreads;  // 16-byte chunks of a block that appends
 
+// One chunk of the new rows: k's first, then v's.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void paged_append_kernel(DenseParams p, AppendParams a) {
+__device__ __forceinline__ void append_chunk(const DenseParams& p, int64_t t) {
   constexpr int E = 16 / static_cast<int>(sizeof(T));
   const int per = p.d / E;  // chunks of a row
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const int64_t total = p.n_q * p.h_kv * per;
   if (t >= 2 * total) return;
   const bool isv = t >= total;
@@ -62,14 +61,15 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(DenseParams p, A
     return;
   }
   const int64_t r = j & ((1 << p.page_log2) - 1);
-  const T* src = static_cast<const T*>(isv ? a.v : a.k) + tok * (isv ? a.v_st : a.k_st) + h * (isv ? a.v_sh : a.k_sh) + c * E;
+  const T* src = static_cast<const T*>(isv ? p.v_new : p.k_new) + tok * (isv ? p.vn_st : p.kn_st) +
+                 h * (isv ? p.vn_sh : p.kn_sh) + c * E;
   T* dst = static_cast<T*>(const_cast<void*>(isv ? p.v : p.k)) + pg * (isv ? p.v_sb : p.k_sb) +
            r * (isv ? p.v_sn : p.k_sn) + h * (isv ? p.v_sh : p.k_sh) + c * E;
   *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
 }
 
-template <typename T, int D, bool RULE>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_kernel(DenseParams p) {
+template <typename T, int D, int RULE>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_kernel(DenseParams p, int row_blocks) {
   using O = Op<T>;
   using Frag = typename O::Frag;
   constexpr int RB = D * O::kEsize, NCH = RB / 16, E = 16 / O::kEsize;
@@ -81,6 +81,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_ker
   __shared__ int s_bad[4][kFew];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  if (static_cast<int>(blockIdx.x) >= row_blocks) {
+    const int64_t t = (static_cast<int64_t>(blockIdx.x) - row_blocks) * kAppend + tid;
+    for (int i = 0; i < kAppend; i += kThreads) append_chunk<T>(p, t + i);
+    return;
+  }
   const int kvh = blockIdx.x % p.h_kv;
   const int rest = blockIdx.x / p.h_kv;
   const int split = rest % p.splits, b = rest / p.splits;
@@ -90,14 +95,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_ker
   const int k_begin = static_cast<int>(min(split * p.split_len, static_cast<int64_t>(sq.len)));
   const int k_end = static_cast<int>(min((split + 1) * p.split_len, static_cast<int64_t>(sq.len)));
   if (k_begin >= k_end) return;  // (a part past the sequence, which the join does not read)
-  const KeyRows<T, true> rows = key_rows<T, true>(p, b, kvh);
+  const KeyRows<T, true> rows = key_rows<T, true>(p, b, kvh, sq.first, sq.len - sq.m);
 
   const int rr = lane & 31;
   const bool real = rr < R;
   const int tok = real ? rr / p.g : 0;
   const int hq = kvh * p.g + (real ? rr - tok * p.g : 0);
   const int pos = sq.len - sq.m + tok;
-  const float slope = (RULE && p.rule.slopes != nullptr && real) ? p.rule.slopes[hq] * kLog2e : 0.0f;
+  const Rule<T, RULE> rule(p.rule);
+  const float slope = RULE == kBias && real ? p.rule.slopes[hq] * kLog2e : 0.0f;
   const T* qrow = static_cast<const T*>(p.q) + (sq.first + tok) * p.q_sn + hq * p.q_sh;
   Frag qf[NC];
 #pragma unroll
@@ -116,12 +122,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_ker
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int r = sr + i * RPW;
-      const int64_t pr = __shfl(pg, r, 64);
-      const int64_t row = min(k0 + r, k_end - 1) & rows.page_mask;
-      const T* kr = rows.k + pr * rows.k_sb + row * rows.k_sn + sc * E;
-      const T* vr = rows.v + pr * rows.v_sb + row * rows.v_sn + sc * E;
-      kreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(kr) : make_uint4(0u, 0u, 0u, 0u);
-      vreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(vr) : make_uint4(0u, 0u, 0u, 0u);
+      const T *kr, *vr;
+      rows.in_page(__shfl(pg, r, 64), min(k0 + r, k_end - 1), kr, vr);
+      kreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(kr + sc * E) : make_uint4(0u, 0u, 0u, 0u);
+      vreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(vr + sc * E) : make_uint4(0u, 0u, 0u, 0u);
     }
   };
 
@@ -150,19 +154,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_ker
     const int kl = k0 + 4 * half;
     const float dist = static_cast<float>(kl - pos);
     const int z = min(pos + 1, k_end) - kl;
-    float top = -INFINITY;
+    float top = Rule<T, RULE>::kHidden;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int j = 8 * (i >> 2) + (i & 3);
-      float x = s[i] * p.rule.c1;
-      if constexpr (RULE) {
-        if (p.rule.cap) x = p.rule.c2 * cap_tanh<T>(x);
-        x = fmaf(-slope, fabsf(dist + static_cast<float>(j)), x);
-      }
-      s[i] = j < z ? x : -INFINITY;
-      top = fmaxf(top, s[i]);
+      s[i] = rule.z(p.rule, s[i], slope, dist + static_cast<float>(j));
+      if (j >= z) s[i] = Rule<T, RULE>::kHidden;
+      top = rule.better(top, s[i]);
     }
-    top = fmaxf(top, other_half(top));
+    top = fmaf(rule.better(top, other_half(top)), rule.a, rule.b);
     if (__ballot(top > mref + 8.0f) != 0) {
       const float mn = fmaxf(mref, top);
       const float alpha = mref == mn ? 1.0f : exp2_w(mref - mn);
@@ -171,10 +171,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_ker
 #pragma unroll
       for (int i = 0; i < ND; ++i) acc[i] *= alpha;
     }
-    const float ref = mref == -INFINITY ? 0.0f : mref;
+    const float nref = rule.b - (mref == -INFINITY ? 0.0f : mref);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      s[i] = exp2_w(s[i] - ref);
+      s[i] = exp2_w(fmaf(s[i], rule.a, nref));
       lsum += s[i];
     }
 #pragma unroll
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_ker
   for (int r = wave; r < R; r += 4) {  // rows to compute again, key by key
     if (!(s_bad[0][r] | s_bad[1][r] | s_bad[2][r] | s_bad[3][r])) continue;
     const int t = r / p.g, h = kvh * p.g + r - t * p.g, ps = sq.len - sq.m + t;
-    const float sl = RULE && p.rule.slopes != nullptr ? p.rule.slopes[h] * kLog2e : 0.0f;
+    const float sl = RULE == kBias ? p.rule.slopes[h] * kLog2e : 0.0f;
     float o[4], m, l;
     exact_row<T, true>(rows, p.rule, static_cast<const T*>(p.q) + (sq.first + t) * p.q_sn + h * p.q_sh, p.d, k_begin,
                        min(k_end, ps + 1), sl, ps, o, m, l);
@@ -380,7 +380,7 @@ PagedPlan paged_plan(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv
   return l;
 }
 
-template <typename T, int D, bool RULE, int KW>
+template <typename T, int D, int RULE, int KW>
 int launch_rows(DenseParams& r, int row_tiles, hipStream_t st) {
   const char* fn = "ssa_paged_step";
   const size_t bytes = rows_lds<T, D, KW>();
@@ -396,15 +396,9 @@ int launch_rows(DenseParams& r, int row_tiles, hipStream_t st) {
   return SSA_OK;
 }
 
-template <typename T, int D, bool RULE>
-int launch_paged(DenseParams& p, const AppendParams& a, const PagedPlan& l, char* ws, hipStream_t st) {
+template <typename T, int D, int RULE>
+int launch_paged(DenseParams& p, const PagedPlan& l, char* ws, hipStream_t st) {
   const char* fn = "ssa_paged_step";
-  if (a.k != nullptr) {
-    const int64_t work = 2 * p.n_q * p.h_kv * (p.d / (16 / static_cast<int>(sizeof(T))));
-    if (ceil_div(work, kThreads) > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many tokens", fn);
-    paged_append_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(work, kThreads))), dim3(kThreads), 0, st>>>(p, a);
-    if (int rc = check_launch("ssa_paged_step append")) return rc;
-  }
   const size_t tiles = static_cast<size_t>(8) * 32 * D * sizeof(T), sums = static_cast<size_t>(4) * kFew * (D + 4) * sizeof(float);
   const size_t fbytes = tiles > sums ? tiles : sums;
   if (int rc = reserve_lds(reinterpret_cast<const void*>(few_rows_kernel<T, D, RULE>), fbytes + 2048, fn)) return rc;
@@ -415,8 +409,10 @@ int launch_paged(DenseParams& p, const AppendParams& a, const PagedPlan& l, char
   f.part_o = reinterpret_cast<float*>(ws + l.few_o);
   f.part_ml = reinterpret_cast<float*>(ws + l.few_ml);
   const int64_t fblocks = static_cast<int64_t>(p.batch) * p.h_kv * f.splits;
-  if (fblocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many sequences", fn);
-  few_rows_kernel<T, D, RULE><<<dim3(static_cast<unsigned>(fblocks)), dim3(kThreads), fbytes, st>>>(f);
+  const int64_t chunks = p.k_new == nullptr ? 0 : 2 * p.n_q * p.h_kv * (p.d / (16 / static_cast<int>(sizeof(T))));
+  const int64_t blocks = fblocks + ceil_div(chunks, kAppend);
+  if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many sequences", fn);
+  few_rows_kernel<T, D, RULE><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), fbytes, st>>>(f, static_cast<int>(fblocks));
   if (int rc = check_launch("ssa_paged_step few rows")) return rc;
   if (f.splits > 1) {
     const int most = static_cast<int>(p.max_new * p.g < kFew ? p.max_new * p.g : kFew);
@@ -440,9 +436,12 @@ int launch_paged(DenseParams& p, const AppendParams& a, const PagedPlan& l, char
 }
 
 template <typename T, int D>
-int launch_rule(DenseParams& p, const AppendParams& a, const PagedPlan& l, char* ws, hipStream_t st) {
-  return p.rule.cap || p.rule.slopes != nullptr ? launch_paged<T, D, true>(p, a, l, ws, st)
-                                                : launch_paged<T, D, false>(p, a, l, ws, st);
+int launch_rule(DenseParams& p, const PagedPlan& l, char* ws, hipStream_t st) {
+  switch (rule_kind(p.rule)) {
+    case kPlain: return launch_paged<T, D, kPlain>(p, l, ws, st);
+    case kCap: return launch_paged<T, D, kCap>(p, l, ws, st);
+    default: return launch_paged<T, D, kBias>(p, l, ws, st);
+  }
 }
 
 }  // namespace
@@ -509,10 +508,11 @@ extern "C" int ssa_paged_step(const void* q, const void* k, const void* v, int d
   p.few_rows = kFew;
   p.max_new = max_new; p.max_len = max_len;
   p.error_flag = error_flag;
-  const AppendParams a{k, v, k_st, k_sh, v_st, v_sh};
+  p.k_new = k; p.v_new = v;
+  p.kn_st = k_st; p.kn_sh = k_sh; p.vn_st = v_st; p.vn_sh = v_sh;
   hipStream_t st = as_stream(stream);
   char* ws = static_cast<char*>(workspace);
   if (dtype == SSA_DTYPE_F32)
-    return d <= 64 ? launch_rule<float, 64>(p, a, l, ws, st) : launch_rule<float, 128>(p, a, l, ws, st);
-  return d <= 64 ? launch_rule<uint16_t, 64>(p, a, l, ws, st) : launch_rule<uint16_t, 128>(p, a, l, ws, st);
+    return d <= 64 ? launch_rule<float, 64>(p, l, ws, st) : launch_rule<float, 128>(p, l, ws, st);
+  return d <= 64 ? launch_rule<uint16_t, 64>(p, l, ws, st) : launch_rule<uint16_t, 128>(p, l, ws, st);
 }

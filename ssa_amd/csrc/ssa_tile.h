@@ -185,8 +185,8 @@ __device__ __forceinline__ int wave_max_i(int x) {
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
 // The score rule, in log2 units (weights are exp2 of differences):
-//   no cap:  x = (q.k) c1 - slope |pos - j|,        c1 = log2(e) / scale
-//   cap c:   x = c2 tanh((q.k) c1) - slope |pos - j|, c1 = 1 / (scale c), c2 = c log2(e)
+//   no cap:  x = (q.k) c1 - slope |pos - j|,          c1 = log2(e) / scale
+//   cap c:   x = c2 tanh((q.k) c1) - slope |pos - j|,  c1 = 1 / (scale c), c2 = c log2(e)
 // slope already carries log2(e).
 struct ScoreRule {
   float c1, c2;
@@ -203,6 +203,59 @@ __device__ __forceinline__ float cap_tanh(float y) {
   const float e = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e));
   return fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
 }
+
+// What the kernels keep of a product until its weight: z with x = a z + b, a and b
+// the same for every score of the call, so that the running maximum, the
+// subtraction of the reference and b cost one fma in the exponent.
+//   kPlain  z = q.k
+//   kCap    bf16: z = 1 / (exp(2y) + 1), of which tanh y = 1 - 2 z and
+//           1 - tanh^2 = 4 (z - z^2); larger scores have smaller z.  fp32: z = tanh y
+//   kBias   z = x (a distance bias, with or without a cap)
+enum RuleKind { kPlain = 0, kCap = 1, kBias = 2 };
+
+template <typename T, int KIND>
+struct Rule {
+  static constexpr bool kDown = KIND == kCap && sizeof(T) == 2;
+  static constexpr float kHidden = kDown ? INFINITY : -INFINITY;  // z of x = -inf
+  // the gradient's factor 1 - tanh^2 is slope() times this
+  static constexpr float kSlopeUnit = kDown ? 4.0f : 1.0f;
+  float c, a, b;
+
+  __device__ __forceinline__ explicit Rule(const ScoreRule& r) {
+    c = kDown ? r.c1 * (2.0f * kLog2e) : r.c1;
+    a = KIND == kPlain ? r.c1 : (kDown ? -2.0f * r.c2 : (KIND == kCap ? r.c2 : 1.0f));
+    b = kDown ? r.c2 : 0.0f;
+  }
+  // dist: |position - key| or its negative (kBias)
+  __device__ __forceinline__ float z(const ScoreRule& r, float dot, float slope, float dist) const {
+    if constexpr (KIND == kPlain) return dot;
+    if constexpr (kDown) return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * c) + 1.0f);
+    if constexpr (KIND == kCap) return tanhf(dot * c);
+    float x = dot * c;
+    if (r.cap) x = r.c2 * cap_tanh<T>(x);
+    return fmaf(-slope, fabsf(dist), x);
+  }
+  // z, and the gradient's factor over kSlopeUnit
+  __device__ __forceinline__ float z(const ScoreRule& r, float dot, float slope, float dist, float& f) const {
+    f = 1.0f;
+    if constexpr (KIND == kBias) {
+      float x = dot * c;
+      if (r.cap) {
+        const float t = cap_tanh<T>(x);
+        f = fmaf(-t, t, 1.0f);
+        x = r.c2 * t;
+      }
+      return fmaf(-slope, fabsf(dist), x);
+    }
+    const float v = z(r, dot, slope, dist);
+    if constexpr (kDown) f = fmaf(-v, v, v);
+    if constexpr (KIND == kCap && !kDown) f = fmaf(-v, v, 1.0f);
+    return v;
+  }
+  static __device__ __forceinline__ float better(float x, float y) { return kDown ? fminf(x, y) : fmaxf(x, y); }
+};
+
+inline RuleKind rule_kind(const ScoreRule& r) { return r.slopes != nullptr ? kBias : (r.cap ? kCap : kPlain); }
 
 // exp2 of a difference of scores: the instruction's (an ulp; a result below
 // 2^-126 is 0, a weight that no fp32 sum of weights up to 1 can hold).

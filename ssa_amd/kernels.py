@@ -10,6 +10,7 @@ every call is enqueued on the current stream without synchronising.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple, Optional, Tuple, Union
 
@@ -465,41 +466,63 @@ def _contig_i32(t: torch.Tensor, name: str) -> torch.Tensor:
 
 
 # ---- dense attention with key intervals, paged cache, axes -------------------
+# A call of these on small tensors takes about as long on the host as on the GPU:
+# raw addresses and the raw stream go to the library, contiguous tensors skip the
+# stride checks, and workspace sizes (functions of the sizes alone) are remembered.
 
 
-def _call_on(t: torch.Tensor, name: str, *args) -> None:
-    """``call`` with t's device current (the launches go to the current device)."""
-    if t.device.index == torch.cuda.current_device():
-        call(name, *args)
+def _on_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> int:
+    """The HIP device all of these tensors are on."""
+    dev = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != dev:
+            _lib.require_device(first, *rest)
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    if dev < 0:
+        _lib.require_device(first)
+    return dev
+
+
+def _call_on(dev: int, name: str, *args) -> None:
+    """``call`` on the current stream of device ``dev``, with it current (launches go to the
+    current device)."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch._C._cuda_getDevice():
+        call(name, *args, stream)
     else:
-        with torch.cuda.device(t.device):
-            call(name, *args)
+        with torch.cuda.device(dev):
+            call(name, *args, stream)
 
 
-def _same_device(**tensors) -> None:
-    _lib.require_device(*tensors.values())
-    first = next(iter(tensors.values())).device
-    for name, t in tensors.items():
-        if t is not None and t.device != first:
-            raise ValueError(f"{name} is on {t.device}, the other tensors on {first}")
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
-def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    """t, or a contiguous copy where its rows are not contiguous or not aligned to 16 bytes."""
+def _rows16(t: torch.Tensor):
+    """(t, its element strides but the last one), t's rows contiguous and aligned to 16 bytes: a
+    contiguous copy where they are not.  A dimension of one element does not step."""
     e = t.element_size()
-    if (t.stride(-1) != 1 and t.shape[-1] > 1) or any(
-            s * e % 16 for s, x in zip(t.stride()[:-1], t.shape[:-1]) if x > 1):
+    if not t.is_contiguous():
+        st = tuple(0 if x == 1 else s for s, x in zip(t.stride(), t.shape))
+        if (st[-1] == 1 or t.shape[-1] == 1) and not any(s * e % 16 for s in st[:-1]) and t.data_ptr() % 16 == 0:
+            return t, st[:-1]
         t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    if t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    if t.dim() == 4:
+        _, n, h, d = t.shape
+        return t, (n * h * d, h * d, d)
+    _, h, d = t.shape
+    return t, (h * d, d)
 
 
-def _strides(t: torch.Tensor):
-    """Element strides of all but the last dimension; a dimension of one element does not step."""
-    return tuple(s if x > 1 else 0 for s, x in zip(t.stride()[:-1], t.shape[:-1]))
+@functools.lru_cache(maxsize=1024)
+def _bytes(name: str, *sizes) -> int:
+    return int(getattr(_lib.load(), name)(*sizes))
 
 
-def _workspace(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
-    return torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
+def _workspace(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, device=like.device, dtype=torch.uint8) if nbytes else None
 
 
 def _check_slopes(slopes: Optional[torch.Tensor], h_q: int) -> Optional[torch.Tensor]:
@@ -516,7 +539,7 @@ def mask_spans(n: int, batch: int, n_q: int, q_pos0: int, causal: bool, doc_star
                prefix_lens: Optional[torch.Tensor], device: torch.device) -> torch.Tensor:
     """Key interval of each row, int32 [batch, n_q, 2] (ssa_mask_spans)."""
     out = torch.empty((batch, n_q, 2), device=device, dtype=torch.int32)
-    _same_device(spans=out, doc_starts=doc_starts, prefix_lens=prefix_lens)
+    dev = _on_device(out, doc_starts, prefix_lens)
     docs = 1 if doc_starts is None else doc_starts.shape[-1] - 1
     if doc_starts is not None:
         if doc_starts.dim() != 2 or doc_starts.shape[0] != batch or docs < 1:
@@ -526,8 +549,8 @@ def mask_spans(n: int, batch: int, n_q: int, q_pos0: int, causal: bool, doc_star
         if tuple(prefix_lens.shape) != (batch, docs):
             raise ValueError(f"prefix_lens must be [{batch}, {docs}], got {tuple(prefix_lens.shape)}")
         prefix_lens = _index32(prefix_lens, "prefix_lens")
-    _call_on(out, "ssa_mask_spans", ptr(doc_starts), docs, ptr(prefix_lens), batch, n, n_q, q_pos0, int(bool(causal)),
-             ptr(out), stream_of(out))
+    _call_on(dev, "ssa_mask_spans", _at(doc_starts), docs, _at(prefix_lens), batch, n, n_q, q_pos0, int(bool(causal)),
+             out.data_ptr())
     return out
 
 
@@ -537,19 +560,21 @@ def _index32(t: torch.Tensor, name: str) -> torch.Tensor:
     return t.to(torch.int32).contiguous()
 
 
-def _check_dense(q, k, v, spans) -> None:
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            raise ValueError(f"{name} must be [B, n, heads, d], got shape {tuple(t.shape)}")
+def _check_dense(q, k, v, spans):
+    """(B, n_q, h_q, d, n, h_kv) of matching q, k, v and spans."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"q, k, v must be [B, n, heads, d], got shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if not (q.dtype == k.dtype == v.dtype):
         raise TypeError(f"q, k, v must share a dtype ({q.dtype}, {k.dtype}, {v.dtype})")
     B, n_q, h_q, d = q.shape
+    _, n, h_kv, _ = k.shape
     if k.shape != v.shape or k.shape[0] != B or k.shape[3] != d:
         raise ValueError(f"k and v must be [{B}, n, h_kv, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    if k.shape[2] == 0 or h_q % k.shape[2] != 0:
-        raise ValueError(f"{h_q} query heads are not divisible by {k.shape[2]} KV heads")
+    if h_kv == 0 or h_q % h_kv != 0:
+        raise ValueError(f"{h_q} query heads are not divisible by {h_kv} KV heads")
     if spans is not None and (spans.dtype != torch.int32 or tuple(spans.shape) != (B, n_q, 2) or not spans.is_contiguous()):
         raise ValueError(f"spans must be a contiguous int32 [{B}, {n_q}, 2] tensor")
+    return B, n_q, h_q, d, n, h_kv
 
 
 def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: Optional[torch.Tensor] = None,
@@ -559,22 +584,24 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: O
     in q's dtype.  ``with_lse`` returns (out, out_low, lse) for the backward: what rounding left of a
     bf16 output (None for float32) and the float32 [B, h_q, n_q] log2 sums.
     ``spans`` None: causal.  Query row i sits at key position ``q_pos0 + i`` (default n - n_q)."""
-    _same_device(q=q, k=k, v=v, spans=spans, slopes=slopes)
-    _check_dense(q, k, v, spans)
-    B, n_q, h_q, d = q.shape
-    n, h_kv = k.shape[1], k.shape[2]
+    dev = _on_device(q, k, v, spans, slopes)
+    B, n_q, h_q, d, n, h_kv = _check_dense(q, k, v, spans)
     slopes = _check_slopes(slopes, h_q)
-    if q_pos0 is None:
-        q_pos0 = n - n_q
-    q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
+    q, qs = _rows16(q)
+    k, ks = _rows16(k)
+    v, vs = _rows16(v)
+    dt = _lib.elem_dtype(q)
     out = torch.empty((B, n_q, h_q, d), device=q.device, dtype=q.dtype)
-    lse = torch.empty((B, h_q, n_q), device=q.device, dtype=torch.float32) if with_lse else None
-    low = torch.empty_like(out) if with_lse and q.dtype == torch.bfloat16 else None
-    nbytes = int(_lib.load().ssa_masked_attention_workspace_bytes(_lib.elem_dtype(q), B, n, n_q, h_q, h_kv, d))
-    ws = _workspace(nbytes, q.device)
-    _call_on(q, "ssa_masked_attention", ptr(q), ptr(k), ptr(v), _lib.elem_dtype(q), B, n, n_q, q_pos0, h_q, h_kv, d,
-             *_strides(q), *_strides(k), *_strides(v), ptr(spans), float(math.sqrt(d) if scale_div is None else scale_div),
-             float(softcap), ptr(slopes), ptr(out), *_strides(out), ptr(low), ptr(lse), ptr(ws), nbytes, stream_of(q))
+    low = lse = None
+    if with_lse:
+        lse = torch.empty((B, h_q, n_q), device=q.device, dtype=torch.float32)
+        low = torch.empty_like(out) if dt == _lib.DTYPE_BF16 else None
+    nbytes = _bytes("ssa_masked_attention_workspace_bytes", dt, B, n, n_q, h_q, h_kv, d)
+    ws = _workspace(nbytes, q)
+    _call_on(dev, "ssa_masked_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, n, n_q,
+             n - n_q if q_pos0 is None else q_pos0, h_q, h_kv, d, *qs, *ks, *vs, _at(spans),
+             math.sqrt(d) if scale_div is None else scale_div, softcap, _at(slopes), out.data_ptr(), n_q * h_q * d, h_q * d, d,
+             _at(low), _at(lse), _at(ws), nbytes)
     return (out, low, lse) if with_lse else out
 
 
@@ -584,32 +611,33 @@ def masked_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                               out_low: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients of masked_attention w.r.t. q, k and v, in their dtype and contiguous, from the
     forward's ``out``, ``lse`` and (bf16) ``out_low`` and the output gradient."""
-    _same_device(q=q, k=k, v=v, out=out, dout=dout, lse=lse, spans=spans, slopes=slopes, out_low=out_low)
-    _check_dense(q, k, v, spans)
-    B, n_q, h_q, d = q.shape
-    n, h_kv = k.shape[1], k.shape[2]
+    dev = _on_device(q, k, v, out, dout, lse, spans, slopes, out_low)
+    B, n_q, h_q, d, n, h_kv = _check_dense(q, k, v, spans)
     if tuple(out.shape) != (B, n_q, h_q, d) or tuple(dout.shape) != (B, n_q, h_q, d):
         raise ValueError("out and dout must have q's shape")
     if out.dtype != q.dtype or dout.dtype != q.dtype:
         raise TypeError(f"out and dout must have q's dtype {q.dtype}")
     if lse.dtype != torch.float32 or tuple(lse.shape) != (B, h_q, n_q) or not lse.is_contiguous():
         raise ValueError(f"lse must be a contiguous float32 [{B}, {h_q}, {n_q}] tensor")
+    if out_low is not None and (out_low.shape != out.shape or out_low.dtype != out.dtype or out_low.stride() != out.stride()):
+        raise ValueError("out_low must have out's shape, strides and dtype")
     slopes = _check_slopes(slopes, h_q)
-    if q_pos0 is None:
-        q_pos0 = n - n_q
     dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    if out_low is not None and (out_low.shape != out.shape or out_low.dtype != out.dtype or out_low.stride() != out.stride()):
-        raise ValueError("out_low must have out's shape, strides and dtype")
-    q, k, v, out, dout = (_aligned_rows(t) for t in (q, k, v, out, dout))
-    out_low = None if out_low is None else _aligned_rows(out_low)
-    nbytes = int(_lib.load().ssa_masked_attention_backward_workspace_bytes(_lib.elem_dtype(q), B, n, n_q, h_q, h_kv, d))
-    ws = _workspace(nbytes, q.device)
-    _call_on(q, "ssa_masked_attention_backward", ptr(q), ptr(k), ptr(v), _lib.elem_dtype(q), B, n, n_q, q_pos0, h_q, h_kv,
-             d, *_strides(q), *_strides(k), *_strides(v), ptr(spans),
-             float(math.sqrt(d) if scale_div is None else scale_div), float(softcap), ptr(slopes), ptr(out), ptr(out_low),
-             *_strides(out), ptr(dout), *_strides(dout), ptr(lse), ptr(dq), ptr(dk), ptr(dv), ptr(ws), nbytes, stream_of(q))
+    q, qs = _rows16(q)
+    k, ks = _rows16(k)
+    v, vs = _rows16(v)
+    out, os = _rows16(out)
+    dout, dos = _rows16(dout)
+    out_low = None if out_low is None else _rows16(out_low)[0]
+    dt = _lib.elem_dtype(q)
+    nbytes = _bytes("ssa_masked_attention_backward_workspace_bytes", dt, B, n, n_q, h_q, h_kv, d)
+    ws = _workspace(nbytes, q)
+    _call_on(dev, "ssa_masked_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, n, n_q,
+             n - n_q if q_pos0 is None else q_pos0, h_q, h_kv, d, *qs, *ks, *vs, _at(spans),
+             math.sqrt(d) if scale_div is None else scale_div, softcap, _at(slopes), out.data_ptr(), _at(out_low), *os,
+             dout.data_ptr(), *dos, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(ws), nbytes)
     return dq, dk, dv
 
 
@@ -623,81 +651,118 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
     [pages, page size, h_kv, d], table int32 [B, width], starts int32 [B + 1], cached int32
     [B].  ``max_new`` and ``max_len`` bound a sequence's new tokens and keys (defaults: T and
     what the table holds)."""
-    _same_device(q=q, k=k, v=v, k_pages=k_pages, v_pages=v_pages, table=table, starts=starts, cached=cached, slopes=slopes,
-                 out=out, error_flag=error_flag)
+    dev = _on_device(q, k, v, k_pages, v_pages, table, starts, cached, slopes, out, error_flag)
     if (k is None) != (v is None):
         raise ValueError("k and v come together")
     if q.dim() != 3 or k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
         raise ValueError("q must be [T, h_q, d] and the pools [pages, page size, h_kv, d]")
     T, h_q, d = q.shape
-    pages, page, h_kv, _ = k_pages.shape
-    if k_pages.shape[3] != d or h_kv == 0 or h_q % h_kv != 0:
+    pages, page, h_kv, dp = k_pages.shape
+    if dp != d or h_kv == 0 or h_q % h_kv != 0:
         raise ValueError(f"q {tuple(q.shape)} does not fit pages {tuple(k_pages.shape)}")
-    for name, t in (("k", k), ("v", v)):
-        if t is not None and tuple(t.shape) != (T, h_kv, d):
-            raise ValueError(f"{name} must be [{T}, {h_kv}, {d}], got {tuple(t.shape)}")
+    dtype = q.dtype
     for name, t in (("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("out", out)):
-        if t is not None and t.dtype != q.dtype:
-            raise TypeError(f"{name} must have q's dtype {q.dtype}, got {t.dtype}")
-    B = table.shape[0]
-    for name, t, shape in (("table", table, (B, table.shape[-1])), ("starts", starts, (B + 1,)), ("cached", cached, (B,))):
-        if t.dtype != torch.int32 or tuple(t.shape) != shape or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        if t is not None and t.dtype != dtype:
+            raise TypeError(f"{name} must have q's dtype {dtype}, got {t.dtype}")
+    B, width = table.shape
+    for name, t, shape in (("table", table, (B, width)), ("starts", starts, (B + 1,)), ("cached", cached, (B,))):
+        if t.dtype != torch.int32 or t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
             raise ValueError(f"{name} must be an int32 {list(shape)} tensor with contiguous rows")
+    pools = []
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        e = t.element_size()
-        if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * e % 16 for s in _strides(t)):
+        rows, st = _rows16(t) if t.numel() else (t, (0, 0, 0))
+        if rows is not t:
             raise ValueError(f"{name} must have contiguous rows aligned to 16 bytes")
+        pools += st
     slopes = _check_slopes(slopes, h_q)
     if error_flag is not None and (error_flag.dtype != torch.int32 or error_flag.numel() != 1):
         raise ValueError("error_flag must be one int32")
-    q = _aligned_rows(q)
-    k, v = (t if t is None else _aligned_rows(t) for t in (k, v))
+    q, qs = _rows16(q)
+    ks = vs = (0, 0)
+    if k is not None:
+        if k.shape != (T, h_kv, d) or v.shape != (T, h_kv, d):
+            raise ValueError(f"k must be [{T}, {h_kv}, {d}] and v too, got {tuple(k.shape)} and {tuple(v.shape)}")
+        k, ks = _rows16(k)
+        v, vs = _rows16(v)
     if out is None:
-        out = torch.empty((T, h_q, d), device=q.device, dtype=q.dtype)
-    elif tuple(out.shape) != (T, h_q, d) or _aligned_rows(out) is not out:
+        out = torch.empty((T, h_q, d), device=q.device, dtype=dtype)
+    elif out.shape != (T, h_q, d) or _rows16(out)[0] is not out:
         raise ValueError(f"out must be [{T}, {h_q}, {d}] with rows aligned to 16 bytes")
     max_new = T if max_new is None else min(int(max_new), T)
-    width = table.shape[1] * page
-    max_len = width if max_len is None else min(int(max_len), width)
-    nbytes = int(_lib.load().ssa_paged_step_workspace_bytes(_lib.elem_dtype(q), T, B, h_q, h_kv, d, max_new, max_len))
-    ws = _workspace(nbytes, q.device)
-    ks, vs = ((0, 0) if t is None else _strides(t) for t in (k, v))
-    _call_on(q, "ssa_paged_step", ptr(q), ptr(k), ptr(v), _lib.elem_dtype(q), T, B, h_q, h_kv, d, *_strides(q), *ks, *vs,
-             ptr(k_pages), ptr(v_pages), pages, page, *_strides(k_pages), *_strides(v_pages), ptr(table),
-             table.stride(0) if B > 1 else 0, table.shape[1], ptr(starts), ptr(cached), max_new, max_len,
-             float(math.sqrt(d) if scale_div is None else scale_div), float(softcap), ptr(slopes), ptr(out), *_strides(out),
-             ptr(error_flag), ptr(ws), nbytes, stream_of(q))
+    max_len = width * page if max_len is None else min(int(max_len), width * page)
+    dt = _lib.elem_dtype(q)
+    nbytes = _bytes("ssa_paged_step_workspace_bytes", dt, T, B, h_q, h_kv, d, max_new, max_len)
+    ws = _workspace(nbytes, q)
+    _call_on(dev, "ssa_paged_step", q.data_ptr(), _at(k), _at(v), dt, T, B, h_q, h_kv, d, *qs, *ks, *vs, k_pages.data_ptr(),
+             v_pages.data_ptr(), pages, page, *pools, table.data_ptr(), table.stride(0) if B > 1 else 0, width,
+             starts.data_ptr(), cached.data_ptr(), max_new, max_len, math.sqrt(d) if scale_div is None else scale_div,
+             softcap, _at(slopes), out.data_ptr(), *_rows16(out)[1], _at(error_flag), _at(ws), nbytes)
     return out
+
+
+def _steps(t: torch.Tensor):
+    """Element strides of [B, n, heads, d] but the last one; a dimension of one element does not step."""
+    if t.is_contiguous():
+        _, n, h, d = t.shape
+        return n * h * d, h * d, d
+    return tuple(0 if x == 1 else s for s, x in zip(t.stride()[:-1], t.shape))
+
+
+class AxesPlan(NamedTuple):
+    """What rope_axes turns a (q, k) pair by, checked: the backward's call takes it as it is."""
+    dev: int
+    dtype: int
+    sizes: Tuple[int, ...]     # B, n, h_q, h_k, d
+    positions: torch.Tensor
+    freqs: torch.Tensor
+    turn: tuple                # positions' type and steps, the axes and their sections
+
+
+def axes_plan(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor,
+              sections) -> AxesPlan:
+    """Checks rope_axes' arguments."""
+    dev = _on_device(q, k, positions, freqs)
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError(f"q and k must be [B, n, heads, d], got {tuple(q.shape)}" + ("" if k is None else f" and {tuple(k.shape)}"))
+    B, n, h_q, d = q.shape
+    h_k = 0 if k is None else k.shape[2]
+    if k is not None and (k.shape != (B, n, h_k, d) or k.dtype != q.dtype):
+        raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
+    axes = len(sections)
+    if positions.shape != (axes, B, n) and positions.shape != (axes, n):
+        raise ValueError(f"positions must be [{axes}, {B}, {n}] or [{axes}, {n}], got {tuple(positions.shape)}")
+    pos_dtype = _lib.index_dtype(positions)
+    if n > 1 and positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    if freqs.dtype != torch.float64 or freqs.dim() != 1:
+        raise TypeError("freqs must be float64 [rot / 2] (axis_rope_freqs)")
+    freqs = freqs.contiguous()
+    return AxesPlan(dev, _lib.elem_dtype(q), (B, n, h_q, h_k, d), positions, freqs,
+                    (pos_dtype, positions.stride(0), positions.stride(1) if positions.dim() == 3 else 0, axes,
+                     (ctypes.c_int32 * axes)(*sections)))
+
+
+def axes_run(plan: AxesPlan, q: torch.Tensor, k: Optional[torch.Tensor], inverse: bool
+             ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """q and k of the plan's sizes turned (ssa_rope_axes); ``inverse`` applies the transpose.  New
+    contiguous tensors of q's dtype."""
+    B, n, h_q, h_k, d = plan.sizes
+    q = q if q.stride(-1) == 1 else q.contiguous()
+    qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    k_at, ks, ko, ko_at = None, (0, 0, 0), None, None
+    if k is not None:
+        k = k if k.stride(-1) == 1 else k.contiguous()
+        ko = torch.empty(k.shape, device=q.device, dtype=q.dtype)
+        k_at, ks, ko_at = k.data_ptr(), _steps(k), ko.data_ptr()
+    _call_on(plan.dev, "ssa_rope_axes", q.data_ptr(), k_at, plan.dtype, B, n, h_q, h_k, d, *_steps(q), *ks,
+             plan.positions.data_ptr(), *plan.turn, plan.freqs.data_ptr(), 2 * plan.freqs.shape[0], inverse, qo.data_ptr(),
+             n * h_q * d, h_q * d, d, ko_at, n * h_k * d, h_k * d, d)
+    return qo, ko
 
 
 def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, sections,
               inverse: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Rotary positions with several axes on q [B, n, h_q, d] and k [B, n, h_k, d] (or None)
-    (ssa_rope_axes): positions int [axes, B, n], freqs float64 [rot / 2], sections the pairs
-    of each axis.  New contiguous tensors of q's dtype; ``inverse`` applies the transpose."""
-    _same_device(q=q, k=k, positions=positions, freqs=freqs)
-    for name, t in (("q", q), ("k", k)):
-        if t is not None and t.dim() != 4:
-            raise ValueError(f"{name} must be [B, n, heads, d], got shape {tuple(t.shape)}")
-    B, n, h_q, d = q.shape
-    if k is not None and (k.shape[:2] != q.shape[:2] or k.shape[3] != d or k.dtype != q.dtype):
-        raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
-    axes = len(sections)
-    if tuple(positions.shape) != (axes, B, n):
-        raise ValueError(f"positions must be [{axes}, {B}, {n}], got {tuple(positions.shape)}")
-    if freqs.dtype != torch.float64 or freqs.dim() != 1:
-        raise TypeError("freqs must be float64 [rot / 2] (axis_rope_freqs)")
-    pos_dtype = _lib.index_dtype(positions)
-    if n > 1 and positions.stride(2) != 1:
-        positions = positions.contiguous()
-    freqs = freqs.contiguous()
-    q, k = (t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (q, k))
-    qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    ko = None if k is None else torch.empty(k.shape, device=q.device, dtype=q.dtype)
-    cuts = (ctypes.c_int32 * axes)(*(int(x) for x in sections))
-    none = (0, 0, 0)
-    _call_on(q, "ssa_rope_axes", ptr(q), ptr(k), _lib.elem_dtype(q), B, n, h_q, 0 if k is None else k.shape[2], d,
-             *_strides(q), *(none if k is None else _strides(k)), ptr(positions), pos_dtype, *_strides(positions), axes,
-             cuts, ptr(freqs), 2 * freqs.shape[0], int(bool(inverse)), ptr(qo), *_strides(qo), ptr(ko),
-             *(none if ko is None else _strides(ko)), stream_of(q))
-    return qo, ko
+    (ssa_rope_axes): positions int [axes, B, n] or [axes, n], freqs float64 [rot / 2], sections the
+    pairs of each axis."""
+    return axes_run(axes_plan(q, k, positions, freqs, sections), q, k, inverse)

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib, kernels
+from . import kernels
 
 
 def mask_spans(seq_len: int, batch: int = 1, *, causal: bool = True, doc_starts: Optional[torch.Tensor] = None,
@@ -87,7 +87,6 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: O
         q, k, v = q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)
         if spans is not None and spans.dim() == 2:
             spans = spans.unsqueeze(0)
-    _lib.require_device(q, k, v)
     out_dtype = q.dtype
     if q.dtype == torch.float16:
         q, k, v = q.float(), k.float(), v.float()

@@ -86,6 +86,25 @@ def test_gradient_against_differences(dev):
     assert abs(float((ends[0] - ends[1]) / 2 - (grad.double() * way).sum())) < 2.0 ** -19 * (mag + float((q.abs() * dq.abs()).sum())) * 2
 
 
+def test_second_order(dev):
+    """The backward is a rotation itself: its gradient is the rotation."""
+    from ssa_amd import axis_rope_freqs, rope_axes
+
+    g = torch.Generator().manual_seed(53)
+    q, k, a, b = (torch.randn(1, 6, 2, 16, generator=g).to(dev).requires_grad_(True) for _ in range(4))
+    pos = torch.randint(0, 500, (2, 1, 6), generator=g).to(dev)
+    freqs = axis_rope_freqs(16, 1e4, dev)
+    x, y = rope_axes(q, k, pos, freqs, (3, 5))
+    dq, dk = torch.autograd.grad((x, y), (q, k), (a, b), create_graph=True)
+    u, w = torch.randn_like(q), torch.randn_like(k)
+    da, db = torch.autograd.grad((dq, dk), (a, b), (u, w))
+    ru, rw = rope_axes(u, w, pos, freqs, (3, 5))
+    assert torch.equal(da, ru) and torch.equal(db, rw)
+    z = rope_axes(q, None, pos, freqs, (3, 5))
+    dq = torch.autograd.grad(z, q, a, create_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(dq, a, u)[0], ru)
+
+
 def test_layouts_streams_graph(dev):
     from ssa_amd import axis_rope_freqs, rope_axes
 
