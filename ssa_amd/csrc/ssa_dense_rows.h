@@ -261,7 +261,8 @@ __global__ __launch_bounds__(kThreads, (rows_lds<T, D, KW>() > 80 * 1024 || (siz
   __shared__ float s_m[4][32], s_l[4][32];
   __shared__ int s_flag[4][32];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kw = wave % KW, rw = wave / KW;
   const int nbh = PAGED ? p.h_kv : p.batch * p.h_kv;
   const int w = blockIdx.x;
@@ -324,8 +325,8 @@ __global__ __launch_bounds__(kThreads, (rows_lds<T, D, KW>() > 80 * 1024 || (siz
     qf[c] = real && e < p.d ? O::load(qrow + e) : O::zero();
   }
   __syncthreads();
-  int k_lo = min(min(s_range[0][0], s_range[1][0]), min(s_range[2][0], s_range[3][0]));
-  int k_hi = max(max(s_range[0][1], s_range[1][1]), max(s_range[2][1], s_range[3][1]));
+  int k_lo = __builtin_amdgcn_readfirstlane(min(min(s_range[0][0], s_range[1][0]), min(s_range[2][0], s_range[3][0])));
+  int k_hi = __builtin_amdgcn_readfirstlane(max(max(s_range[0][1], s_range[1][1]), max(s_range[2][1], s_range[3][1])));
   int part_lo = 0, part_hi = 0x7FFFFFFF;
   if (p.splits > 1) {
     const int64_t s0 = split * p.split_len, s1 = s0 + p.split_len;
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(kThreads, (rows_lds<T, D, KW>() > 80 * 1024 || (siz
           s[u][i] = rule.z(p.rule, s[u][i], slope, dist + static_cast<float>(32 * u + 8 * (i >> 2) + (i & 3)));
       const bool whole = k0 >= lo_max && k0 + 32 * NSUB <= hi_min && k0 >= part_lo && k0 + 32 * NSUB <= part_hi;
       if (!whole) {
-        const int a = max(lo, part_lo) - kl, z = min(hi, part_hi) - kl;
+        const int a = in_branch(max(lo, part_lo) - kl), z = in_branch(min(hi, part_hi) - kl);
 #pragma unroll
         for (int u = 0; u < NSUB; ++u)
 #pragma unroll

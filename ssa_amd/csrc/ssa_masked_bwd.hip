@@ -111,7 +111,8 @@ __global__ __launch_bounds__(kThreads, (dq_lds<T, D, KW>() > 80 * 1024 || (sizeo
   extern __shared__ __align__(16) char lds[];
   __shared__ int s_range[4][2];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kw = wave % KW, rw = wave / KW;
   const int nbh = p.batch * p.h_kv;
   const int bh = blockIdx.x % nbh;
@@ -139,8 +140,8 @@ __global__ __launch_bounds__(kThreads, (dq_lds<T, D, KW>() > 80 * 1024 || (sizeo
     if (kvh == 0 && kw == 0 && grp < p.groups) p.bounds[static_cast<int64_t>(b) * p.groups + grp] = make_int4(lo_min, hi_max, lo_max, hi_min);
   }
   __syncthreads();
-  const int k_lo = min(min(s_range[0][0], s_range[1][0]), min(s_range[2][0], s_range[3][0]));
-  const int k_hi = max(max(s_range[0][1], s_range[1][1]), max(s_range[2][1], s_range[3][1]));
+  const int k_lo = __builtin_amdgcn_readfirstlane(min(min(s_range[0][0], s_range[1][0]), min(s_range[2][0], s_range[3][0])));
+  const int k_hi = __builtin_amdgcn_readfirstlane(max(max(s_range[0][1], s_range[1][1]), max(s_range[2][1], s_range[3][1])));
   const int t0 = k_lo / KT, nt = k_hi > k_lo ? (k_hi + KT - 1) / KT - t0 : 0;
 
   const T* kbase = static_cast<const T*>(p.k) + b * p.k_sb + kvh * p.k_sh;
@@ -215,14 +216,21 @@ __global__ __launch_bounds__(kThreads, (dq_lds<T, D, KW>() > 80 * 1024 || (sizeo
         const int kl = k0 + 4 * half;
         const float dist = static_cast<float>(kl - pos), nlse = rule.b - lse;
         const bool whole = k0 >= lo_max && k0 + 32 <= hi_min;
-        const int a = lo - kl, z = hi - kl;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int j = 8 * (i >> 2) + (i & 3);
           float f;
           const float x = rule.z(p.rule, s[i], slope, dist + static_cast<float>(j), f);
           const float w = exp2_w(fmaf(x, rule.a, nlse)) * (dp[i] - dsum) * f;
-          s[i] = whole || (j >= a && j < z) ? w : 0.0f;
+          s[i] = w;
+        }
+        if (!whole) {
+          const int a = in_branch(lo - kl), z = in_branch(hi - kl);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = 8 * (i >> 2) + (i & 3);
+            if (j < a || j >= z) s[i] = 0.0f;
+          }
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -343,7 +351,8 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
   __shared__ __align__(16) float s_lse[2][QT], s_dsum[2][QT], s_slope[2][QT], s_pos[2][QT];
   __shared__ __align__(16) int s_lo[2][QT], s_hi[2][QT];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = wave % RW, kg = wave / RW;
   const int nbh = p.batch * p.h_kv;
   const int bh = blockIdx.x % nbh;
@@ -535,12 +544,13 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
           dp[i] = s[i] * (dp[i] - dv[x]) * f;
         }
         if (!whole) {
+          const int my = in_branch(key);
           const int4 lo4 = *reinterpret_cast<const int4*>(&s_lo[buf][r0]);
           const int4 hi4 = *reinterpret_cast<const int4*>(&s_hi[buf][r0]);
           const int lov[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hiv[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const bool see = key >= lov[x] && key < hiv[x];
+            const bool see = my >= lov[x] && my < hiv[x];
             s[4 * e + x] = see ? s[4 * e + x] : 0.0f;
             dp[4 * e + x] = see ? dp[4 * e + x] : 0.0f;
           }

@@ -80,7 +80,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_ker
   __shared__ float s_m[4][kFew], s_l[4][kFew];
   __shared__ int s_bad[4][kFew];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (static_cast<int>(blockIdx.x) >= row_blocks) {
     const int64_t t = (static_cast<int64_t>(blockIdx.x) - row_blocks) * kAppend + tid;
     for (int i = 0; i < kAppend; i += kThreads) append_chunk<T>(p, t + i);

@@ -158,6 +158,15 @@ struct Op<float> {
   static __device__ __forceinline__ float left(float) { return 0.0f; }
 };
 
+// Keeps what uses x inside the wave-uniform branch it stands in.  Left alone, the
+// compiler runs the mask's compares and selects for every tile (three instructions
+// a score beside the eight that a score takes) rather than jump over them where a
+// tile is seen whole.
+__device__ __forceinline__ int in_branch(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // The other half-wave's value of a lane's column.
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
@@ -174,12 +183,12 @@ __device__ __forceinline__ float wave_sum(float x) {
 __device__ __forceinline__ int wave_min_i(int x) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
-  return x;
+  return __builtin_amdgcn_readfirstlane(x);  // (a scalar: branches on it are uniform)
 }
 __device__ __forceinline__ int wave_max_i(int x) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
-  return x;
+  return __builtin_amdgcn_readfirstlane(x);
 }
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }

@@ -100,9 +100,12 @@ def test_second_order(dev):
     da, db = torch.autograd.grad((dq, dk), (a, b), (u, w))
     ru, rw = rope_axes(u, w, pos, freqs, (3, 5))
     assert torch.equal(da, ru) and torch.equal(db, rw)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(x, q, a)
     z = rope_axes(q, None, pos, freqs, (3, 5))
     dq = torch.autograd.grad(z, q, a, create_graph=True)[0]
-    assert torch.equal(torch.autograd.grad(dq, a, u)[0], ru)
+    assert torch.equal(torch.autograd.grad(dq, a, u)[0], rope_axes(u, None, pos, freqs, (3, 5)))
 
 
 def test_layouts_streams_graph(dev):
