@@ -338,30 +338,55 @@ __global__ __launch_bounds__(kThreads, (rows_lds<T, D, KW>() > 80 * 1024 || (siz
   const int t0 = k_lo / KT;
   const int nt = k_hi > k_lo ? (k_hi + KT - 1) / KT - t0 : 0;
 
-  // staging: chunk sc of tile rows sr, sr + RPP, ...; of paged keys a tile's pages
-  // are looked up a tile before its loads
+  // staging: chunk sc of tile rows sr, sr + RPP, ....  Of paged keys, a wave's rows of
+  // a load lie in one page, looked up a tile before; tiles that reach past the pages'
+  // keys (the call's own rows, the end) take each row's address.
   const int sc = tid % NCH, sr = tid / NCH;
   const bool chunk_ok = sc * E < p.d;
   const int last = static_cast<int>(n_keys) - 1;
+  const int64_t kst = rows.k_sn * O::kEsize, vst = rows.v_sn * O::kEsize;  // bytes of a row
+  const uint32_t ks = static_cast<uint32_t>(kst), vs = static_cast<uint32_t>(vst);
+  const int my = PAGED ? lane / NCH : sr;
+  const uint32_t koff = chunk_ok ? my * ks + sc * 16 : kNoChunk, voff = chunk_ok ? my * vs + sc * 16 : kNoChunk;
   uint4 kreg[NP], vreg[NP];
   int pg[PAGED ? NP : 1];
+  const int paged_end = PAGED ? min(rows.new_from, static_cast<int>(n_keys)) : 0;
+  constexpr int RPW = 64 / NCH;  // rows of a wave's load
   auto find_pages = [&](int t) {
     if constexpr (PAGED) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) pg[i] = rows.page_of(min((t0 + t) * KT + sr + i * RPP, last));
+      for (int i = 0; i < NP; ++i) pg[i] = rows.page_of(min((t0 + t) * KT + i * RPP + wave * RPW, last));
     }
   };
   auto load_tile = [&](int t) {
+    const int j0 = (t0 + t) * KT;
+    if constexpr (PAGED) {
+      if (j0 + KT <= paged_end) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int j = min((t0 + t) * KT + sr + i * RPP, last);
-      const T *kr, *vr;
-      if constexpr (PAGED)
-        rows.in_page(pg[i], j, kr, vr);
-      else
-        rows.at(j, kr, vr);
-      kreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(kr + sc * E) : make_uint4(0u, 0u, 0u, 0u);
-      vreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(vr + sc * E) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < NP; ++i) {
+          const int64_t page = __builtin_amdgcn_readfirstlane(pg[i]), r0 = (j0 + i * RPP + wave * RPW) & rows.page_mask;
+          kreg[i] = row_load(row_buffer(rows.k + page * rows.k_sb + r0 * rows.k_sn, kAllBytes), koff);
+          vreg[i] = row_load(row_buffer(rows.v + page * rows.v_sb + r0 * rows.v_sn, kAllBytes), voff);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const T *kr, *vr;
+          rows.at(min(j0 + sr + i * RPP, last), kr, vr);
+          kreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(kr + sc * E) : make_uint4(0u, 0u, 0u, 0u);
+          vreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(vr + sc * E) : make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+    } else {
+      const int left = static_cast<int>(n_keys) - j0;  // at least one
+      const int db = p.d * O::kEsize;
+      const auto kb = row_buffer(rows.k + j0 * rows.k_sn, left >= KT ? kAllBytes : static_cast<int>((left - 1) * kst) + db);
+      const auto vb = row_buffer(rows.v + j0 * rows.v_sn, left >= KT ? kAllBytes : static_cast<int>((left - 1) * vst) + db);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        kreg[i] = row_load(kb, koff + i * RPP * ks);
+        vreg[i] = row_load(vb, voff + i * RPP * vs);
+      }
     }
   };
   auto store_tile = [&](int buf) {
@@ -385,6 +410,7 @@ __global__ __launch_bounds__(kThreads, (rows_lds<T, D, KW>() > 80 * 1024 || (siz
     if (nt > 1) find_pages(1);
     store_tile(0);
   }
+  settle(qf);
   for (int t = 0; t < nt; ++t) {
     __syncthreads();
     if (t + 1 < nt) load_tile(t + 1);

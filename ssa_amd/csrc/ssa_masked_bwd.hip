@@ -150,7 +150,7 @@ __global__ __launch_bounds__(kThreads, (dq_lds<T, D, KW>() > 80 * 1024 || (sizeo
   const T* dorow = static_cast<const T*>(p.dout) + b * p.do_sb + tok * p.do_sn + hq * p.do_sh;
   const T* orow = static_cast<const T*>(p.out) + b * p.o_sb + tok * p.o_sn + hq * p.o_sh;
   const int64_t stat = (static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok;
-  const float lse = some ? p.lse[stat] : INFINITY;  // (no key: every weight 0)
+  float lse = some ? p.lse[stat] : INFINITY;  // (no key: every weight 0)
   Frag qf[NC], dof[NC];
   float dsum = 0.0f;
 #pragma unroll
@@ -172,13 +172,18 @@ __global__ __launch_bounds__(kThreads, (dq_lds<T, D, KW>() > 80 * 1024 || (sizeo
 
   const int sc = tid % NCH, sr = tid / NCH;
   const bool chunk_ok = sc * E < p.d;
+  const int64_t kst = p.k_sn * O::kEsize, vst = p.v_sn * O::kEsize;  // bytes of a row
+  const uint32_t ks = static_cast<uint32_t>(kst), vs = static_cast<uint32_t>(vst);
+  const uint32_t koff = chunk_ok ? sr * ks + sc * 16 : kNoChunk, voff = chunk_ok ? sr * vs + sc * 16 : kNoChunk;
   uint4 kreg[NP], vreg[NP];
   auto load_tile = [&](int t) {
+    const int j0 = (t0 + t) * KT, left = n_keys - j0, db = p.d * O::kEsize;
+    const auto kb = row_buffer(kbase + j0 * p.k_sn, left >= KT ? kAllBytes : static_cast<int>((left - 1) * kst) + db);
+    const auto vb = row_buffer(vbase + j0 * p.v_sn, left >= KT ? kAllBytes : static_cast<int>((left - 1) * vst) + db);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int64_t j = min((t0 + t) * KT + sr + i * RPP, n_keys - 1);
-      kreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(kbase + j * p.k_sn + sc * E) : make_uint4(0u, 0u, 0u, 0u);
-      vreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(vbase + j * p.v_sn + sc * E) : make_uint4(0u, 0u, 0u, 0u);
+      kreg[i] = row_load(kb, koff + i * RPP * ks);
+      vreg[i] = row_load(vb, voff + i * RPP * vs);
     }
   };
   auto store_tile = [&](int buf) {
@@ -198,6 +203,9 @@ __global__ __launch_bounds__(kThreads, (dq_lds<T, D, KW>() > 80 * 1024 || (sizeo
     load_tile(0);
     store_tile(0);
   }
+  settle(qf);
+  settle(dof);
+  settle(lse);
   for (int t = 0; t < nt; ++t) {
     __syncthreads();
     if (t + 1 < nt) load_tile(t + 1);
@@ -440,18 +448,23 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
 
   const int sc = tid % NCH, sr = tid / NCH;
   const bool chunk_ok = sc * E < p.d;
-  const T* qbase = static_cast<const T*>(p.q) + b * p.q_sb + sc * E;
-  const T* dbase = static_cast<const T*>(p.dout) + b * p.do_sb + sc * E;
+  const T* qbase = static_cast<const T*>(p.q) + b * p.q_sb;
+  const T* dbase = static_cast<const T*>(p.dout) + b * p.do_sb;
+  const uint32_t qs = static_cast<uint32_t>(p.q_sn * O::kEsize), qh = static_cast<uint32_t>(p.q_sh * O::kEsize);
+  const uint32_t ds = static_cast<uint32_t>(p.do_sn * O::kEsize), dh = static_cast<uint32_t>(p.do_sh * O::kEsize);
   uint4 qreg[NP], dreg[NP];
   float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
   float st_slope = 0.0f, st_pos = 0.0f;
   auto load_rows = [&](int t) {
+    // offsets from the tile's first token
+    const uint32_t tok0 = static_cast<uint32_t>(t * QT) / static_cast<uint32_t>(p.g);
+    const auto qb = row_buffer(qbase + tok0 * p.q_sn, kAllBytes), db = row_buffer(dbase + tok0 * p.do_sn, kAllBytes);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const uint32_t r = min(t * QT + min(sr + i * RPP, QT - 1), n_rows - 1);
       const uint32_t tok = r / static_cast<uint32_t>(p.g), hq = kvh * p.g + r - tok * p.g;
-      qreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(qbase + tok * p.q_sn + hq * p.q_sh) : make_uint4(0u, 0u, 0u, 0u);
-      dreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(dbase + tok * p.do_sn + hq * p.do_sh) : make_uint4(0u, 0u, 0u, 0u);
+      qreg[i] = row_load(qb, chunk_ok ? (tok - tok0) * qs + hq * qh + sc * 16 : kNoChunk);
+      dreg[i] = row_load(db, chunk_ok ? (tok - tok0) * ds + hq * dh + sc * 16 : kNoChunk);
     }
     if (tid < QT) {
       const uint32_t r = min(t * QT + tid, n_rows - 1);
@@ -497,6 +510,10 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
   if (cur.tile >= 0) {
     load_rows(cur.tile);
     store_rows(cur.tile, 0);
+  }
+  if constexpr (!S::kInLds) {
+    settle(kf);
+    settle(vf);
   }
   for (int t = 0; cur.tile >= 0; ++t) {
     __syncthreads();

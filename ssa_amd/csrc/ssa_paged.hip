@@ -139,6 +139,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_ker
   int pg = pages_at(k0);
   if (k0 < k_end) load_tile(k0, pg);
   pg = pages_at(k0 + 128);
+  settle(qf);
   for (; k0 < k_end; k0 += 128) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {

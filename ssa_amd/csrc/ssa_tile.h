@@ -158,6 +158,46 @@ struct Op<float> {
   static __device__ __forceinline__ float left(float) { return 0.0f; }
 };
 
+// Rows read through a buffer resource whose base moves with the tile: the address of
+// a load is one 32-bit offset a thread keeps, and chunks and rows that do not exist
+// (offsets past `bytes`) read as zeros with no branch.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+constexpr uint32_t kNoChunk = 0x80000000u;     // an offset past any resource
+constexpr int kAllBytes = 0x7FFFFFF0;          // a resource whose rows all exist
+constexpr int64_t kMostRowBytes = 1 << 24;     // of a row stride: 64 rows' offsets stay below 2^31
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* base, int bytes) {
+  // (word 3: raw 32-bit data)
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+}
+__device__ __forceinline__ uint4 row_load(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
+  const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, static_cast<int>(offset), 0, 0);
+  return make_uint4(x.x, x.y, x.z, x.w);
+}
+
+// Waits for fragments loaded before a loop.  A load still out at the loop's head makes
+// the compiler wait for every load at its first use in the body, the next tile's that
+// were just issued among them.
+__device__ __forceinline__ void settle(uint32_t& x) { asm volatile("" : "+v"(x)); }
+__device__ __forceinline__ void settle(float& x) { asm volatile("" : "+v"(x)); }
+template <int N>
+__device__ __forceinline__ void settle(Op<uint16_t>::Frag (&f)[N]) {
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    settle(f[c].v.x);
+    settle(f[c].v.y);
+    settle(f[c].v.z);
+    settle(f[c].v.w);
+  }
+}
+template <int N>
+__device__ __forceinline__ void settle(Op<float>::Frag (&f)[N]) {
+#pragma unroll
+  for (int c = 0; c < N; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) settle(f[c].v[i]);
+}
+
 // Keeps what uses x inside the wave-uniform branch it stands in.  Left alone, the
 // compiler runs the mask's compares and selects for every tile (three instructions
 // a score beside the eight that a score takes) rather than jump over them where a

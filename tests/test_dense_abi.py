@@ -68,7 +68,8 @@ DENSE = [
     (dict(n_q=1 << 29), UNSUPPORTED, "2^31"), (dict(scale=0.0), INVALID, "scale"),
     (dict(scale=float("inf")), INVALID, "scale"), (dict(cap=-1.0), INVALID, "softcap"),
     (dict(cap=float("nan")), INVALID, "softcap"), (dict(q=None), INVALID, "null"), (dict(v=None), INVALID, "null"),
-    (dict(out=None), INVALID, "null"), (dict(q=MISALIGNED), UNSUPPORTED, "q must"), (dict(k_sn=516), UNSUPPORTED, "k must"),
+    (dict(out=None), INVALID, "null"), (dict(q_sn=1 << 23 | 8), UNSUPPORTED, "strides"), (dict(q_sh=-64), UNSUPPORTED, "strides"),
+    (dict(q=MISALIGNED), UNSUPPORTED, "q must"), (dict(k_sn=516), UNSUPPORTED, "k must"),
     (dict(v_sh=4), UNSUPPORTED, "v must"), (dict(o_sn=4), UNSUPPORTED, "out must"),
     (dict(batch=0, q=None), OK, ""),
 ]
@@ -97,7 +98,7 @@ def test_masked_attention_backward(L, kw, status, text):
     assert st == status and (st == OK or text in msg), msg
 
 
-@pytest.mark.parametrize("kw,status,text", [x for x in DENSE if not {"n", "n_q", "q_pos0", "k_sn", "o_sn", "batch"} & set(x[0])] + [
+@pytest.mark.parametrize("kw,status,text", [x for x in DENSE if not {"n", "n_q", "q_pos0", "q_sn", "k_sn", "o_sn", "batch"} & set(x[0])] + [
     (dict(tokens=-1), INVALID, "shape"), (dict(page_size=24), UNSUPPORTED, "page_size"),
     (dict(page_size=4), UNSUPPORTED, "page_size"), (dict(page_size=8192), UNSUPPORTED, "page_size"),
     (dict(tokens=1 << 30), UNSUPPORTED, "2^31"), (dict(max_pages=1 << 28), UNSUPPORTED, "2^31"),
