@@ -94,13 +94,12 @@ struct KeyRows {
   int64_t kn_st, vn_st;
   int new_from;
 
-  __device__ __forceinline__ int page_of(int j) const {
-    int pg = table[j >> page_log2];
-    if (static_cast<unsigned>(pg) >= static_cast<unsigned>(num_pages)) {
-      if (error_flag != nullptr) atomicOr(error_flag, 1);
-      pg = 0;
-    }
-    return pg;
+  // The table's entry, to be checked where it is used: a check here would wait for it.
+  __device__ __forceinline__ int entry_of(int j) const { return table[j >> page_log2]; }
+  __device__ __forceinline__ int checked(int pg) const {
+    if (static_cast<unsigned>(pg) < static_cast<unsigned>(num_pages)) return pg;
+    if (error_flag != nullptr) atomicOr(error_flag, 1);
+    return 0;
   }
   __device__ __forceinline__ void in_page(int64_t pg, int j, const T*& kr, const T*& vr) const {
     const int64_t r = j & page_mask, x = j - new_from;
@@ -110,7 +109,7 @@ struct KeyRows {
   }
   __device__ __forceinline__ void at(int j, const T*& kr, const T*& vr) const {
     if constexpr (PAGED) {
-      in_page(page_of(j), j, kr, vr);
+      in_page(checked(entry_of(j)), j, kr, vr);
     } else {
       kr = k + j * k_sn;
       vr = v + j * v_sn;
@@ -355,7 +354,7 @@ __global__ __launch_bounds__(kThreads, (rows_lds<T, D, KW>() > 80 * 1024 || (siz
   auto find_pages = [&](int t) {
     if constexpr (PAGED) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) pg[i] = rows.page_of(min((t0 + t) * KT + i * RPP + wave * RPW, last));
+      for (int i = 0; i < NP; ++i) pg[i] = rows.entry_of(min((t0 + t) * KT + i * RPP + wave * RPW, last));
     }
   };
   auto load_tile = [&](int t) {
@@ -364,7 +363,7 @@ __global__ __launch_bounds__(kThreads, (rows_lds<T, D, KW>() > 80 * 1024 || (siz
       if (j0 + KT <= paged_end) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          const int64_t page = __builtin_amdgcn_readfirstlane(pg[i]), r0 = (j0 + i * RPP + wave * RPW) & rows.page_mask;
+          const int64_t page = rows.checked(__builtin_amdgcn_readfirstlane(pg[i])), r0 = (j0 + i * RPP + wave * RPW) & rows.page_mask;
           kreg[i] = row_load(row_buffer(rows.k + page * rows.k_sb + r0 * rows.k_sn, kAllBytes), koff);
           vreg[i] = row_load(row_buffer(rows.v + page * rows.v_sb + r0 * rows.v_sn, kAllBytes), voff);
         }

@@ -118,8 +118,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_ker
   const int sc = lane % NCH, sr = lane / NCH;
   const bool chunk_ok = sc * E < p.d;
   uint4 kreg[NP], vreg[NP];
-  auto pages_at = [&](int k0) { return k0 < k_end ? rows.page_of(min(k0 + rr, k_end - 1)) : 0; };
-  auto load_tile = [&](int k0, int pg) {
+  auto pages_at = [&](int k0) { return k0 < k_end ? rows.entry_of(min(k0 + rr, k_end - 1)) : 0; };
+  auto load_tile = [&](int k0, int entry) {
+    const int pg = rows.checked(entry);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int r = sr + i * RPW;
