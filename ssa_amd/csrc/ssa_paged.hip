@@ -272,9 +272,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_ker
   }
 }
 
-// One block a row: the parts of a few-row sequence, every eighth one a wave's, four
+// One block a row: the parts of a few-row sequence, every sixteenth one a wave's, four
 // of its loads in flight; the waves' sums meet in LDS.
-constexpr int kJoinWaves = 8;
+constexpr int kJoinWaves = 16;  // (a sequence of 128k keys leaves 256 parts)
 
 template <typename T, int D>
 __global__ __launch_bounds__(kJoinWaves * 64) void few_join_kernel(DenseParams p, int most_rows) {

@@ -10,9 +10,10 @@
 // The angle is formed and reduced to an eighth of a turn in 64 bits, where far
 // positions would lose it in 32, and its sine and cosine are Taylor polynomials
 // in fp32 (the argument is at most pi / 4, the first term left out below 2e-9).
-// A thread takes one 16-byte chunk of pairs of one token for several heads of q
-// and k: the angles are computed once for them, so the kernel is bound by
-// reading and writing q and k.
+// A block takes a few tokens: their angles first, one a thread, into LDS, then all
+// their heads of q and k, 16 bytes of each half of the pairs a thread, neighbouring
+// threads on neighbouring chunks.  The 64-bit work is done once for the heads and
+// the rest is bound by reading and writing q and k.
 
 #include "ssa_tile.h"
 
@@ -26,7 +27,7 @@ struct AxesParams {
   void *q_out, *k_out;
   const double* freqs;
   int64_t n, rows;  // rows = batch * n
-  int h_q, h_k, d, half, rot, items, groups, per;  // items: chunks of a row; groups: thread groups of a token's heads
+  int h_q, h_k, d, half, rot, items, tokens;  // items: chunks of a head; tokens: of a block
   int cut1, cut2, cut3;                            // first pairs of axes 1, 2, 3
   int64_t q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, qo_sb, qo_sn, qo_sh, ko_sb, ko_sn, ko_sh, p_sa, p_sb;
   float sign;  // -1: the transpose
@@ -84,57 +85,72 @@ struct Chunk {
   }
 };
 
+constexpr int kAxUnroll = 4;  // chunks of a thread whose loads are in flight together
+
 template <typename T, typename P, int VEC>
 __global__ __launch_bounds__(kAxThreads) void rope_axes_kernel(AxesParams p) {
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kAxThreads + threadIdx.x;
-  const int64_t all = p.rows * p.groups * p.items;
-  if (t >= all) return;
-  const int64_t u = t / p.items;
-  const int item = static_cast<int>(t - u * p.items);
-  const int64_t row = u / p.groups;
-  const int h0 = static_cast<int>(u - row * p.groups) * p.per;
-  const int64_t b = row / p.n, i = row - b * p.n;
-  const int h1 = min(h0 + p.per, p.h_q + p.h_k);
-  const T* q = static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_sn;
-  const T* k = static_cast<const T*>(p.k) + b * p.k_sb + i * p.k_sn;
-  T* qo = static_cast<T*>(p.q_out) + b * p.qo_sb + i * p.qo_sn;
-  T* ko = static_cast<T*>(p.k_out) + b * p.ko_sb + i * p.ko_sn;
-  const int pairs = p.half / VEC;
-  if (item >= pairs) {  // a chunk that passes through
-    const int j = p.rot + (item - pairs) * VEC;
-    for (int h = h0; h < h1; ++h) {
-      Chunk<T, VEC> x;
-      x.load(h < p.h_q ? q + h * p.q_sh + j : k + (h - p.h_q) * p.k_sh + j);
-      x.store(h < p.h_q ? qo + h * p.qo_sh + j : ko + (h - p.h_q) * p.ko_sh + j);
-    }
-    return;
-  }
-  const int m0 = item * VEC;
-  const P* pos = static_cast<const P*>(p.pos) + b * p.p_sb + i;
-  float c[VEC], s[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const int m = m0 + e;
+  extern __shared__ __align__(16) float lds[];  // [tokens][half] cosines, then sines
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.tokens;
+  const int tokens = static_cast<int>(min(static_cast<int64_t>(p.tokens), p.rows - row0));
+  float *cs = lds, *sn = lds + p.tokens * p.half;
+  for (int x = threadIdx.x; x < tokens * p.half; x += kAxThreads) {
+    const int tk = x / p.half, m = x - tk * p.half;
+    const int64_t row = row0 + tk, b = row / p.n, i = row - b * p.n;
     const int axis = (m >= p.cut1) + (m >= p.cut2) + (m >= p.cut3);
-    const double ang = static_cast<double>(pos[axis * p.p_sa]) * p.freqs[m];
-    turn(ang * 0.15915494309189533577, c[e], s[e]);
-    s[e] *= p.sign;
+    const double ang = static_cast<double>(static_cast<const P*>(p.pos)[axis * p.p_sa + b * p.p_sb + i]) * p.freqs[m];
+    float c, s;
+    turn(ang * 0.15915494309189533577, c, s);
+    cs[x] = c;
+    sn[x] = s * p.sign;
   }
-#pragma unroll 4
-  for (int h = h0; h < h1; ++h) {
-    const bool isq = h < p.h_q;
-    const T* x = isq ? q + h * p.q_sh : k + (h - p.h_q) * p.k_sh;
-    T* y = isq ? qo + h * p.qo_sh : ko + (h - p.h_q) * p.ko_sh;
-    Chunk<T, VEC> x1, x2, y1, y2;
-    x1.load(x + m0);
-    x2.load(x + m0 + p.half);
+  const int pairs = p.half / VEC, heads = p.h_q + p.h_k, all = tokens * heads * p.items;
+  __syncthreads();
+  for (int e0 = threadIdx.x; e0 < all; e0 += kAxThreads * kAxUnroll) {
+    const T* src[kAxUnroll];
+    T* dst[kAxUnroll];
+    int at[kAxUnroll];  // the chunk's first angle, -1 where it passes through
+    Chunk<T, VEC> x1[kAxUnroll], x2[kAxUnroll];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      y1.v[e] = fmaf(x1.v[e], c[e], -(x2.v[e] * s[e]));
-      y2.v[e] = fmaf(x2.v[e], c[e], x1.v[e] * s[e]);
+    for (int u = 0; u < kAxUnroll; ++u) {
+      const uint32_t e = min(e0 + u * kAxThreads, all - 1);
+      const uint32_t w = e / static_cast<uint32_t>(p.items);
+      const int item = static_cast<int>(e - w * p.items);
+      const uint32_t tk = w / static_cast<uint32_t>(heads);
+      const int h = static_cast<int>(w - tk * heads);
+      int64_t b = 0, i = row0 + tk;
+      if (i >= p.n) {
+        b = i / p.n;
+        i -= b * p.n;
+      }
+      const bool isq = h < p.h_q;
+      src[u] = isq ? static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_sn + h * p.q_sh
+                   : static_cast<const T*>(p.k) + b * p.k_sb + i * p.k_sn + (h - p.h_q) * p.k_sh;
+      dst[u] = isq ? static_cast<T*>(p.q_out) + b * p.qo_sb + i * p.qo_sn + h * p.qo_sh
+                   : static_cast<T*>(p.k_out) + b * p.ko_sb + i * p.ko_sn + (h - p.h_q) * p.ko_sh;
+      const int j = item < pairs ? item * VEC : p.rot + (item - pairs) * VEC;
+      at[u] = item < pairs ? static_cast<int>(tk) * p.half + j : -1;
+      src[u] += j;
+      dst[u] += j;
+      x1[u].load(src[u]);
+      if (at[u] >= 0) x2[u].load(src[u] + p.half);
     }
-    y1.store(y + m0);
-    y2.store(y + m0 + p.half);
+#pragma unroll
+    for (int u = 0; u < kAxUnroll; ++u) {
+      if (e0 + u * kAxThreads >= all) break;
+      if (at[u] < 0) {
+        x1[u].store(dst[u]);
+        continue;
+      }
+      Chunk<T, VEC> y1, y2;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        const float c = cs[at[u] + v], s = sn[at[u] + v];
+        y1.v[v] = fmaf(x1[u].v[v], c, -(x2[u].v[v] * s));
+        y2.v[v] = fmaf(x2[u].v[v], c, x1[u].v[v] * s);
+      }
+      y1.store(dst[u]);
+      y2.store(dst[u] + p.half);
+    }
   }
 }
 
@@ -143,18 +159,20 @@ int launch_axes(AxesParams& p, bool wide, hipStream_t st) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
   const int vec = wide ? V : 1;
   p.items = (p.half + p.d - p.rot) / vec;
-  // Heads a thread takes: all of a long call's (angles once), fewer where that
-  // leaves the device idle.
-  const int heads = p.h_q + p.h_k;
-  p.per = heads;
-  while (p.per > 1 && p.rows * p.items * ceil_div(heads, p.per) < 256 * 1024) p.per = (p.per + 1) / 2;
-  p.groups = static_cast<int>(ceil_div(heads, p.per));
-  const int64_t grid = ceil_div(p.rows * p.groups * p.items, kAxThreads);
+  // A token or more of angles for every thread of a block, fewer where that leaves
+  // fewer than four blocks a CU.
+  int64_t tokens = kAxThreads / p.half;
+  if (tokens > p.rows / 1024) tokens = p.rows / 1024;
+  p.tokens = static_cast<int>(tokens > 1 ? tokens : 1);
+  const int64_t grid = ceil_div(p.rows, p.tokens);
   if (grid > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "ssa_rope_axes: too many rows");
+  const size_t bytes = static_cast<size_t>(2) * p.tokens * p.half * sizeof(float);
+  const void* kernel = wide ? reinterpret_cast<const void*>(rope_axes_kernel<T, P, V>) : reinterpret_cast<const void*>(rope_axes_kernel<T, P, 1>);
+  if (int rc = reserve_lds(kernel, bytes, "ssa_rope_axes")) return rc;
   if (wide)
-    rope_axes_kernel<T, P, V><<<dim3(static_cast<unsigned>(grid)), dim3(kAxThreads), 0, st>>>(p);
+    rope_axes_kernel<T, P, V><<<dim3(static_cast<unsigned>(grid)), dim3(kAxThreads), bytes, st>>>(p);
   else
-    rope_axes_kernel<T, P, 1><<<dim3(static_cast<unsigned>(grid)), dim3(kAxThreads), 0, st>>>(p);
+    rope_axes_kernel<T, P, 1><<<dim3(static_cast<unsigned>(grid)), dim3(kAxThreads), bytes, st>>>(p);
   return check_launch("ssa_rope_axes");
 }
 
@@ -178,6 +196,8 @@ extern "C" int ssa_rope_axes(const void* q, const void* k, int dtype, int64_t ba
                 (long long)n, h_q, h_k, d);
   if (rot <= 0 || rot > d || (rot & 1))
     return fail(SSA_ERR_INVALID_ARGUMENT, "%s: rot=%d must be even and in (0, d=%d]", fn, rot, d);
+  if (h_q > 4096 || h_k > 4096 || d > 4096)
+    return fail(SSA_ERR_UNSUPPORTED, "%s: heads and head_dim must be at most 4096", fn);
   if (axes < 1 || axes > 4) return fail(SSA_ERR_UNSUPPORTED, "%s: axes=%d must be in [1, 4]", fn, axes);
   if (!sections) return fail(SSA_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
   int64_t sum = 0;

@@ -114,7 +114,7 @@ def test_paged_step(L, kw, status, text):
 
 @pytest.mark.parametrize("kw,status,text", [
     (dict(dtype=7), UNSUPPORTED, "dtype"), (dict(pos_dtype=5), INVALID, "positions"), (dict(h_q=0), INVALID, "shape"),
-    (dict(rot=63), INVALID, "rot"), (dict(rot=66), INVALID, "rot"), (dict(axes=0), UNSUPPORTED, "axes"),
+    (dict(rot=63), INVALID, "rot"), (dict(rot=66), INVALID, "rot"), (dict(h_k=5000), UNSUPPORTED, "4096"), (dict(axes=0), UNSUPPORTED, "axes"),
     (dict(axes=5), UNSUPPORTED, "axes"), (dict(sections=None), INVALID, "null"), (dict(axes=2), INVALID, "sections"),
     (dict(sections=NEGATIVE), INVALID, "negative"), (dict(rot=32), INVALID, "sections"), (dict(freqs=None), INVALID, "null"),
     (dict(k=None), INVALID, "null"), (dict(q_out=None), INVALID, "null"), (dict(n=0, q=None), OK, ""),
