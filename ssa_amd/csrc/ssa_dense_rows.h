@@ -241,8 +241,14 @@ constexpr size_t rows_lds() {
   return tiles > sums ? tiles : sums;
 }
 
+// Blocks on a CU: by LDS, and fp32 rows of 128 features want the registers of two.
+template <typename T, int D, int KW>
+constexpr int rows_per_cu() {
+  return rows_lds<T, D, KW>() > 80 * 1024 || (sizeof(T) == 4 && D == 128) ? 1 : 2;
+}
+
 template <typename T, int D, bool PAGED, int RULE, int KW>
-__global__ __launch_bounds__(kThreads, (rows_lds<T, D, KW>() > 80 * 1024 || (sizeof(T) == 4 && D == 128) ? 1 : 2)) void dense_rows_kernel(DenseParams p) {
+__device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, char* lds) {
   using O = Op<T>;
   using Frag = typename O::Frag;
   constexpr int RB = D * O::kEsize;      // bytes of a tile row
@@ -255,7 +261,7 @@ __global__ __launch_bounds__(kThreads, (rows_lds<T, D, KW>() > 80 * 1024 || (siz
   constexpr int TB = KT * RB;            // bytes of a tile
   constexpr int BR = rows_of(KW);        // the block's rows
   constexpr int PS = D + 4;              // floats of a row of sums
-  extern __shared__ __align__(16) char lds[];  // [2 buffers][K, V][TB], then [4 waves][32][PS]
+  // lds: [2 buffers][K, V][TB], then [4 waves][32][PS]
   __shared__ int s_range[4][2];
   __shared__ float s_m[4][32], s_l[4][32];
   __shared__ int s_flag[4][32];
@@ -264,7 +270,6 @@ __global__ __launch_bounds__(kThreads, (rows_lds<T, D, KW>() > 80 * 1024 || (siz
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kw = wave % KW, rw = wave / KW;
   const int nbh = PAGED ? p.h_kv : p.batch * p.h_kv;
-  const int w = blockIdx.x;
   const int bh = w % nbh;
   int rest = w / nbh;
   const int split = rest % p.splits;
@@ -603,13 +608,26 @@ __global__ __launch_bounds__(kThreads, (rows_lds<T, D, KW>() > 80 * 1024 || (siz
   }
 }
 
-// Joins the parts of each row: one wave a row.
-// A part without a key has m = -inf and l = 0 and its o is not read.
+// Joins the parts of a row, by one wave.  A part without a key has m = -inf and
+// l = 0 and its o is not read.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void dense_join_kernel(DenseParams p) {
+__device__ __forceinline__ void dense_join(const DenseParams& p, const int64_t row) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
   if (row >= p.part_rows) return;
+  const int64_t tok = row / p.h_q, hq = row - tok * p.h_q;
+  const int64_t b = p.starts != nullptr ? 0 : tok / p.n_q, t = tok - b * p.n_q;
+  if (p.starts != nullptr) {  // a row behind the last sequence, or of one that is refused, stays as it was
+    bool mine = false;
+    for (int s0 = 0; s0 < p.batch; s0 += 64) {
+      bool in = false;
+      if (s0 + lane < p.batch) {
+        const Seq s = paged_seq(p, s0 + lane);
+        in = t >= s.first && t < s.first + s.m && static_cast<int64_t>(s.m) * p.g > p.few_rows;
+      }
+      mine |= __ballot(in) != 0;
+    }
+    if (!mine) return;
+  }
   constexpr int L = D / 64;  // features of a lane: lane * L ..
   float m = -INFINITY, l = 0.0f, o[L];
   bool seen = false;
@@ -637,20 +655,6 @@ __global__ __launch_bounds__(kThreads) void dense_join_kernel(DenseParams p) {
 #pragma unroll
       for (int e = 0; e < L; ++e) o[e] = fmaf(v[i][e], w, o[e] * a);
     }
-  }
-  const int64_t tok = row / p.h_q, hq = row - tok * p.h_q;
-  const int64_t b = p.starts != nullptr ? 0 : tok / p.n_q, t = tok - b * p.n_q;
-  if (p.starts != nullptr) {  // a row behind the last sequence, or of one that is refused, stays as it was
-    bool mine = false;
-    for (int s0 = 0; s0 < p.batch; s0 += 64) {
-      bool in = false;
-      if (s0 + lane < p.batch) {
-        const Seq s = paged_seq(p, s0 + lane);
-        in = t >= s.first && t < s.first + s.m && static_cast<int64_t>(s.m) * p.g > p.few_rows;
-      }
-      mine |= __ballot(in) != 0;
-    }
-    if (!mine) return;
   }
   T* orow = static_cast<T*>(p.out) + b * p.o_sb + t * p.o_sn + hq * p.o_sh;
   // no key: zeros; only keys of score -inf: NaN

@@ -50,14 +50,25 @@ __global__ __launch_bounds__(256) void mask_spans_kernel(const int32_t* starts, 
 }
 
 template <typename T, int D, int RULE, int KW>
+__global__ __launch_bounds__(kThreads, (rows_per_cu<T, D, KW>())) void dense_rows_kernel(DenseParams p) {
+  extern __shared__ __align__(16) char lds[];
+  dense_rows<T, D, false, RULE, KW>(p, blockIdx.x, lds);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void dense_join_kernel(DenseParams p) {
+  dense_join<T, D>(p, static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6));
+}
+
+template <typename T, int D, int RULE, int KW>
 int launch_rows(DenseParams& p, hipStream_t st) {
   const size_t bytes = rows_lds<T, D, KW>();
-  if (int rc = reserve_lds(reinterpret_cast<const void*>(dense_rows_kernel<T, D, false, RULE, KW>), bytes + 2048,
+  if (int rc = reserve_lds(reinterpret_cast<const void*>(dense_rows_kernel<T, D, RULE, KW>), bytes + 2048,
                            "ssa_masked_attention"))
     return rc;
   const int64_t blocks = ceil_div(p.n_q * p.g, rows_of(KW)) * p.batch * p.h_kv * p.splits;
   if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "ssa_masked_attention: too many rows");
-  dense_rows_kernel<T, D, false, RULE, KW><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(p);
+  dense_rows_kernel<T, D, RULE, KW><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(p);
   if (int rc = check_launch("ssa_masked_attention")) return rc;
   if (p.splits > 1) {
     dense_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(p.part_rows, kThreads / 64))), dim3(kThreads), 0, st>>>(p);

@@ -2,20 +2,21 @@
 // of sequences, each with its new tokens' rows appended to its pages and attended
 // over everything it has cached, causally.
 //
-//   append       blocks of the first launch copy the new rows to their pages, 16
+//   append       blocks that copy the new rows to their pages, 16
 //                bytes a thread; the attention reads them from the call's k and v, so
 //                that nothing waits for the copies
 //   few rows     sequences with at most 32 rows (tokens x heads of a group) per KV
-//                head, single tokens above all: few_rows_kernel
-//   many rows    chunks: dense_rows_kernel (ssa_dense_rows.h) over pages
+//                head, single tokens above all: few_rows
+//   many rows    chunks: dense_rows (ssa_dense_rows.h) over pages
 //
-// few_rows_kernel reads K and V once and is bound by that.  The rows fill one
+// all in one launch, and the parts that sequences were cut into joined in a second.
+//
+// few_rows reads K and V once and is bound by that.  The rows fill one
 // MFMA column block; the block's four waves take every fourth 32-key tile of its
 // part of the sequence, each through LDS of its own (whole rows loaded, so that
 // every load instruction reads contiguous lines; the next tile's loads are in
 // flight while a tile is used, and its pages are looked up a tile earlier still),
-// and join their running sums through LDS at the end.  The parts of a sequence
-// are joined by a second kernel.
+// and join their running sums through LDS at the end.
 
 #include <math.h>
 
@@ -69,26 +70,21 @@ __device__ __forceinline__ void append_chunk(const DenseParams& p, int64_t t) {
 }
 
 template <typename T, int D, int RULE>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_kernel(DenseParams p, int row_blocks) {
+__device__ __forceinline__ void few_rows(const DenseParams& p, const int block, char* lds) {
   using O = Op<T>;
   using Frag = typename O::Frag;
   constexpr int RB = D * O::kEsize, NCH = RB / 16, E = 16 / O::kEsize;
   constexpr int NC = D / 16, ND = D / 32, TB = 32 * RB;
   constexpr int RPW = 64 / NCH, NP = 32 / RPW;  // rows a wave's load instruction covers; loads of a tile
   constexpr int PS = D + 4;                     // floats of a row of partial sums
-  extern __shared__ __align__(16) char lds[];   // [4 waves][K, V][TB], then [4][32][PS] sums
+  // lds: [4 waves][K, V][TB], then [4][32][PS] sums
   __shared__ float s_m[4][kFew], s_l[4][kFew];
   __shared__ int s_bad[4][kFew];
 
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (static_cast<int>(blockIdx.x) >= row_blocks) {
-    const int64_t t = (static_cast<int64_t>(blockIdx.x) - row_blocks) * kAppend + tid;
-    for (int i = 0; i < kAppend; i += kThreads) append_chunk<T>(p, t + i);
-    return;
-  }
-  const int kvh = blockIdx.x % p.h_kv;
-  const int rest = blockIdx.x / p.h_kv;
+  const int kvh = block % p.h_kv;
+  const int rest = block / p.h_kv;
   const int split = rest % p.splits, b = rest / p.splits;
   const Seq sq = paged_seq(p, b);
   const int R = sq.m * p.g;
@@ -272,38 +268,63 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void few_rows_ker
   }
 }
 
-// One block a row: the parts of a few-row sequence, every sixteenth one a wave's, four
-// of its loads in flight; the waves' sums meet in LDS.
-constexpr int kJoinWaves = 16;  // (a sequence of 128k keys leaves 256 parts)
+// Everything of a call in one launch: blocks of many rows (the longest) first, then
+// few rows, then the blocks that append.  KW 0: no sequence has many rows.
+template <typename T, int D, int KW>
+constexpr int paged_per_cu() {
+  if constexpr (KW > 0) return rows_per_cu<T, D, KW>();
+  return sizeof(T) == 2 || D == 64 ? 2 : 1;
+}
+
+template <typename T, int D, int RULE, int KW>
+__global__ __launch_bounds__(kThreads, (paged_per_cu<T, D, KW>())) void paged_kernel(DenseParams rows, DenseParams few, int row_blocks,
+                                                                                     int few_blocks) {
+  extern __shared__ __align__(16) char lds[];
+  const int w = blockIdx.x;
+  if (w < row_blocks) {
+    if constexpr (KW > 0) dense_rows<T, D, true, RULE, KW>(rows, w, lds);
+  } else if (w < row_blocks + few_blocks) {
+    few_rows<T, D, RULE>(few, w - row_blocks, lds);
+  } else {
+    const int64_t t = static_cast<int64_t>(w - row_blocks - few_blocks) * kAppend + threadIdx.x;
+    for (int i = 0; i < kAppend; i += kThreads) append_chunk<T>(few, t + i);
+  }
+}
+
+// The parts of few-row sequences: `per` waves a row (1, 4 or 16 of the block's 16),
+// each with every per-th part, four parts' loads in flight; their sums meet in LDS.
+constexpr int kJoinWaves = 16;
 
 template <typename T, int D>
-__global__ __launch_bounds__(kJoinWaves * 64) void few_join_kernel(DenseParams p, int most_rows) {
+__device__ __forceinline__ void few_join(const DenseParams& p, const int block, const int most_rows, const int per) {
   constexpr int L = D / 64;  // features of a lane: lane * L ..
   __shared__ float s_o[kJoinWaves][D], s_m[kJoinWaves], s_l[kJoinWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int bh = blockIdx.x / most_rows, r = blockIdx.x - bh * most_rows;
-  const int b = bh / p.h_kv, kvh = bh - b * p.h_kv;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t x = static_cast<int64_t>(block) * (kJoinWaves / per) + wave / per;
+  const int bh = static_cast<int>(x / most_rows), r = static_cast<int>(x - static_cast<int64_t>(bh) * most_rows);
+  const int b = min(bh / p.h_kv, p.batch - 1), kvh = bh - b * p.h_kv;
   const Seq sq = paged_seq(p, b);
   const int R = sq.m * p.g;
-  if (R > p.few_rows || r >= R) return;
-  const int parts = static_cast<int>(min(static_cast<int64_t>(p.splits), ceil_div(sq.len, p.split_len)));
+  const bool on = bh < p.batch * p.h_kv && R <= p.few_rows && r < R;
+  const int parts = on ? static_cast<int>(min(static_cast<int64_t>(p.splits), ceil_div(sq.len, p.split_len))) : 0;
   const int64_t row = static_cast<int64_t>(bh) * kFew + r;
   float m = -INFINITY, l = 0.0f, o[L];
 #pragma unroll
   for (int e = 0; e < L; ++e) o[e] = 0.0f;
-  for (int s0 = wave; s0 < parts; s0 += 4 * kJoinWaves) {
+  for (int s0 = wave % per; s0 < parts; s0 += 4 * per) {
     float2 ml[4];
     float v[4][L];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t at = min(s0 + i * kJoinWaves, parts - 1) * p.part_rows + row;
+      const int64_t at = min(s0 + i * per, parts - 1) * p.part_rows + row;
       ml[i] = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
 #pragma unroll
       for (int e = 0; e < L; ++e) v[i][e] = p.part_o[at * D + lane * L + e];
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (s0 + i * kJoinWaves >= parts || ml[i].y == 0.0f) continue;  // (an empty part)
+      if (s0 + i * per >= parts || ml[i].y == 0.0f) continue;  // (an empty part)
       const float mn = fmaxf(m, ml[i].x), ref = mn == -INFINITY ? 0.0f : mn;
       const float a = exp2_w(m - ref), w = exp2_w(ml[i].x - ref);
       m = mn;
@@ -312,29 +333,45 @@ __global__ __launch_bounds__(kJoinWaves * 64) void few_join_kernel(DenseParams p
       for (int e = 0; e < L; ++e) o[e] = fmaf(v[i][e], w, o[e] * a);
     }
   }
+  if (per > 1) {
 #pragma unroll
-  for (int e = 0; e < L; ++e) s_o[wave][lane * L + e] = o[e];
-  if (lane == 0) {
-    s_m[wave] = m;
-    s_l[wave] = l;
+    for (int e = 0; e < L; ++e) s_o[wave][lane * L + e] = o[e];
+    if (lane == 0) {
+      s_m[wave] = m;
+      s_l[wave] = l;
+    }
+    __syncthreads();
+    if (wave % per != 0) return;
+    float top = m;
+    for (int y = 1; y < per; ++y) top = fmaxf(top, s_m[wave + y]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < L; ++e) o[e] = 0.0f;
+    for (int y = 0; y < per; ++y) {
+      const float a = exp2_w(s_m[wave + y] - ref);
+      l = fmaf(a, s_l[wave + y], l);
+#pragma unroll
+      for (int e = 0; e < L; ++e) o[e] = fmaf(a, s_o[wave + y][lane * L + e], o[e]);
+    }
   }
-  __syncthreads();
-  const int dd = threadIdx.x;
-  if (dd >= p.d) return;
-  float top = s_m[0];
-#pragma unroll
-  for (int x = 1; x < kJoinWaves; ++x) top = fmaxf(top, s_m[x]);
-  const float ref = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f, val = 0.0f;
-#pragma unroll
-  for (int x = 0; x < kJoinWaves; ++x) {
-    const float a = exp2_w(s_m[x] - ref);
-    sum = fmaf(a, s_l[x], sum);
-    val = fmaf(a, s_o[x][dd], val);
-  }
+  if (!on) return;
   const int t = r / p.g, h = kvh * p.g + r - t * p.g;
-  // (a token sees itself: the sum is 0 only where every score is -inf)
-  Op<T>::store1(static_cast<T*>(p.out) + (sq.first + t) * p.o_sn + h * p.o_sh + dd, val * (1.0f / sum));
+  T* orow = static_cast<T*>(p.out) + (sq.first + t) * p.o_sn + h * p.o_sh;
+  const float inv = 1.0f / l;  // (a token sees itself: the sum is 0 only where every score is -inf)
+#pragma unroll
+  for (int e = 0; e < L; ++e)
+    if (lane * L + e < p.d) Op<T>::store1(orow + lane * L + e, o[e] * inv);
+}
+
+// The parts of both kinds of rows, in one launch.
+template <typename T, int D>
+__global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(DenseParams rows, DenseParams few, int few_blocks, int most_rows,
+                                                                          int per) {
+  if (static_cast<int>(blockIdx.x) < few_blocks)
+    few_join<T, D>(few, blockIdx.x, most_rows, per);
+  else
+    dense_join<T, D>(rows, static_cast<int64_t>(blockIdx.x - few_blocks) * kJoinWaves + (threadIdx.x >> 6));
 }
 
 // Parts, tiles and workspace of a call.
@@ -384,66 +421,58 @@ PagedPlan paged_plan(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv
 }
 
 template <typename T, int D, int RULE, int KW>
-int launch_rows(DenseParams& r, int row_tiles, hipStream_t st) {
-  const char* fn = "ssa_paged_step";
-  const size_t bytes = rows_lds<T, D, KW>();
-  if (int rc = reserve_lds(reinterpret_cast<const void*>(dense_rows_kernel<T, D, true, RULE, KW>), bytes + 2048, fn)) return rc;
-  const int64_t blocks = static_cast<int64_t>(row_tiles) * r.h_kv * r.splits;
-  if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many tokens", fn);
-  dense_rows_kernel<T, D, true, RULE, KW><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(r);
-  if (int rc = check_launch("ssa_paged_step rows")) return rc;
-  if (r.splits > 1) {
-    dense_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(r.part_rows, kThreads / 64))), dim3(kThreads), 0, st>>>(r);
-    if (int rc = check_launch("ssa_paged_step row join")) return rc;
-  }
-  return SSA_OK;
-}
-
-template <typename T, int D, int RULE>
 int launch_paged(DenseParams& p, const PagedPlan& l, char* ws, hipStream_t st) {
   const char* fn = "ssa_paged_step";
-  const size_t tiles = static_cast<size_t>(8) * 32 * D * sizeof(T), sums = static_cast<size_t>(4) * kFew * (D + 4) * sizeof(float);
-  const size_t fbytes = tiles > sums ? tiles : sums;
-  if (int rc = reserve_lds(reinterpret_cast<const void*>(few_rows_kernel<T, D, RULE>), fbytes + 2048, fn)) return rc;
-  DenseParams f = p;
+  DenseParams f = p, r = p;
   f.splits = l.few_splits;
   f.split_len = l.few_len;
   f.part_rows = static_cast<int64_t>(p.batch) * p.h_kv * kFew;
   f.part_o = reinterpret_cast<float*>(ws + l.few_o);
   f.part_ml = reinterpret_cast<float*>(ws + l.few_ml);
+  r.splits = l.row_splits;
+  r.split_len = l.row_len;
+  r.part_rows = p.n_q * p.h_q;
+  r.part_o = reinterpret_cast<float*>(ws + l.row_o);
+  r.part_ml = reinterpret_cast<float*>(ws + l.row_ml);
+  const size_t tiles = static_cast<size_t>(8) * 32 * D * sizeof(T), sums = static_cast<size_t>(4) * kFew * (D + 4) * sizeof(float);
+  size_t bytes = tiles > sums ? tiles : sums;
+  if constexpr (KW > 0) bytes = bytes > rows_lds<T, D, KW>() ? bytes : rows_lds<T, D, KW>();
+  if (int rc = reserve_lds(reinterpret_cast<const void*>(paged_kernel<T, D, RULE, KW>), bytes + 4096, fn)) return rc;
+  const int64_t rblocks = static_cast<int64_t>(l.row_tiles) * p.h_kv * r.splits;
   const int64_t fblocks = static_cast<int64_t>(p.batch) * p.h_kv * f.splits;
   const int64_t chunks = p.k_new == nullptr ? 0 : 2 * p.n_q * p.h_kv * (p.d / (16 / static_cast<int>(sizeof(T))));
-  const int64_t blocks = fblocks + ceil_div(chunks, kAppend);
-  if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many sequences", fn);
-  few_rows_kernel<T, D, RULE><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), fbytes, st>>>(f, static_cast<int>(fblocks));
-  if (int rc = check_launch("ssa_paged_step few rows")) return rc;
-  if (f.splits > 1) {
-    const int most = static_cast<int>(p.max_new * p.g < kFew ? p.max_new * p.g : kFew);
-    const int64_t jblocks = static_cast<int64_t>(p.batch) * p.h_kv * most;
-    if (jblocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many sequences", fn);
-    few_join_kernel<T, D><<<dim3(static_cast<unsigned>(jblocks)), dim3(kJoinWaves * 64), 0, st>>>(f, most);
-    if (int rc = check_launch("ssa_paged_step join")) return rc;
-  }
-  if (l.row_tiles > 0) {
-    DenseParams r = p;
-    r.splits = l.row_splits;
-    r.split_len = l.row_len;
-    r.part_rows = p.n_q * p.h_q;
-    r.part_o = reinterpret_cast<float*>(ws + l.row_o);
-    r.part_ml = reinterpret_cast<float*>(ws + l.row_ml);
-    if constexpr (most_kw<T, D>() >= 4)
-      if (l.row_kw == 4) return launch_rows<T, D, RULE, 4>(r, l.row_tiles, st);
-    return l.row_kw == 2 ? launch_rows<T, D, RULE, 2>(r, l.row_tiles, st) : launch_rows<T, D, RULE, 1>(r, l.row_tiles, st);
+  const int64_t blocks = rblocks + fblocks + ceil_div(chunks, kAppend);
+  if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many tokens", fn);
+  paged_kernel<T, D, RULE, KW><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(
+      r, f, static_cast<int>(rblocks), static_cast<int>(fblocks));
+  if (int rc = check_launch("ssa_paged_step")) return rc;
+  const int most = static_cast<int>(p.max_new * p.g < kFew ? p.max_new * p.g : kFew);
+  const int per = f.splits <= 8 ? 1 : (f.splits <= 32 ? 4 : 16);  // waves a row: two rounds of four parts at most, or 16
+  const int64_t few_join_blocks = f.splits > 1 ? ceil_div(static_cast<int64_t>(p.batch) * p.h_kv * most, kJoinWaves / per) : 0;
+  const int64_t join_blocks = few_join_blocks + (l.row_tiles > 0 && r.splits > 1 ? ceil_div(r.part_rows, kJoinWaves) : 0);
+  if (join_blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many sequences", fn);
+  if (join_blocks > 0) {
+    paged_join_kernel<T, D><<<dim3(static_cast<unsigned>(join_blocks)), dim3(kJoinWaves * 64), 0, st>>>(
+        r, f, static_cast<int>(few_join_blocks), most, per);
+    return check_launch("ssa_paged_step join");
   }
   return SSA_OK;
+}
+
+template <typename T, int D, int RULE>
+int launch_kw(DenseParams& p, const PagedPlan& l, char* ws, hipStream_t st) {
+  if (l.row_tiles == 0) return launch_paged<T, D, RULE, 0>(p, l, ws, st);
+  if constexpr (most_kw<T, D>() >= 4)
+    if (l.row_kw == 4) return launch_paged<T, D, RULE, 4>(p, l, ws, st);
+  return l.row_kw == 2 ? launch_paged<T, D, RULE, 2>(p, l, ws, st) : launch_paged<T, D, RULE, 1>(p, l, ws, st);
 }
 
 template <typename T, int D>
 int launch_rule(DenseParams& p, const PagedPlan& l, char* ws, hipStream_t st) {
   switch (rule_kind(p.rule)) {
-    case kPlain: return launch_paged<T, D, kPlain>(p, l, ws, st);
-    case kCap: return launch_paged<T, D, kCap>(p, l, ws, st);
-    default: return launch_paged<T, D, kBias>(p, l, ws, st);
+    case kPlain: return launch_kw<T, D, kPlain>(p, l, ws, st);
+    case kCap: return launch_kw<T, D, kCap>(p, l, ws, st);
+    default: return launch_kw<T, D, kBias>(p, l, ws, st);
   }
 }
 
