@@ -292,8 +292,8 @@ __global__ __launch_bounds__(kThreads, (paged_per_cu<T, D, KW>())) void paged_ke
 }
 
 // The parts of few-row sequences: `per` waves a row (1, 4 or 16 of the block's 16),
-// each with every per-th part, four parts' loads in flight; their sums meet in LDS.
-constexpr int kJoinWaves = 16;
+// each with every per-th part, eight parts' loads in flight; their sums meet in LDS.
+constexpr int kJoinWaves = 16, kAtOnce = 8;
 
 template <typename T, int D>
 __device__ __forceinline__ void few_join(const DenseParams& p, const int block, const int most_rows, const int per) {
@@ -312,18 +312,18 @@ __device__ __forceinline__ void few_join(const DenseParams& p, const int block, 
   float m = -INFINITY, l = 0.0f, o[L];
 #pragma unroll
   for (int e = 0; e < L; ++e) o[e] = 0.0f;
-  for (int s0 = wave % per; s0 < parts; s0 += 4 * per) {
-    float2 ml[4];
-    float v[4][L];
+  for (int s0 = wave % per; s0 < parts; s0 += kAtOnce * per) {
+    float2 ml[kAtOnce];
+    float v[kAtOnce][L];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kAtOnce; ++i) {
       const int64_t at = min(s0 + i * per, parts - 1) * p.part_rows + row;
       ml[i] = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
 #pragma unroll
       for (int e = 0; e < L; ++e) v[i][e] = p.part_o[at * D + lane * L + e];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kAtOnce; ++i) {
       if (s0 + i * per >= parts || ml[i].y == 0.0f) continue;  // (an empty part)
       const float mn = fmaxf(m, ml[i].x), ref = mn == -INFINITY ? 0.0f : mn;
       const float a = exp2_w(m - ref), w = exp2_w(ml[i].x - ref);
@@ -447,7 +447,7 @@ int launch_paged(DenseParams& p, const PagedPlan& l, char* ws, hipStream_t st) {
       r, f, static_cast<int>(rblocks), static_cast<int>(fblocks));
   if (int rc = check_launch("ssa_paged_step")) return rc;
   const int most = static_cast<int>(p.max_new * p.g < kFew ? p.max_new * p.g : kFew);
-  const int per = f.splits <= 8 ? 1 : (f.splits <= 32 ? 4 : 16);  // waves a row: two rounds of four parts at most, or 16
+  const int per = f.splits <= 8 ? 1 : (f.splits <= 32 ? 4 : 16);  // waves a row: one round of loads, or 16 waves
   const int64_t few_join_blocks = f.splits > 1 ? ceil_div(static_cast<int64_t>(p.batch) * p.h_kv * most, kJoinWaves / per) : 0;
   const int64_t join_blocks = few_join_blocks + (l.row_tiles > 0 && r.splits > 1 ? ceil_div(r.part_rows, kJoinWaves) : 0);
   if (join_blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many sequences", fn);

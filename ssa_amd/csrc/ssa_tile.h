@@ -210,25 +210,37 @@ __device__ __forceinline__ int in_branch(int x) {
 // The other half-wave's value of a lane's column.
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-  return x;
+// Reductions over the 64 lanes of a wave (all lanes active) to a scalar, in six DPP
+// steps: row_shr 1, 2, 4, 8 fold each 16-lane row into its last lane, row_bcast 15
+// and 31 fold the rows into lane 63.  A lane whose source does not exist takes its
+// own value.  (A ladder of shuffles costs an LDS round trip a step: four reductions
+// of one took a microsecond at the head of every block.)
+template <typename F>
+__device__ __forceinline__ int wave_fold(int x, F f) {
+  x = f(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xF, 0xF, false));
+  x = f(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xF, 0xF, false));
+  x = f(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xF, 0xF, false));
+  x = f(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xF, 0xF, false));
+  x = f(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xA, 0xF, false));
+  x = f(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xC, 0xF, false));
+  return __builtin_amdgcn_readlane(x, 63);
 }
+__device__ __forceinline__ int wave_min_i(int x) {
+  return wave_fold(x, [](int a, int b) { return min(a, b); });
+}
+__device__ __forceinline__ int wave_max_i(int x) {
+  return wave_fold(x, [](int a, int b) { return max(a, b); });
+}
+__device__ __forceinline__ float wave_max(float x) {
+  return __int_as_float(wave_fold(__float_as_int(x), [](int a, int b) {
+    return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b)));
+  }));
+}
+// (a sum counts each lane once: lanes without a source add 0)
 __device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
   return x;
-}
-__device__ __forceinline__ int wave_min_i(int x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
-  return __builtin_amdgcn_readfirstlane(x);  // (a scalar: branches on it are uniform)
-}
-__device__ __forceinline__ int wave_max_i(int x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
-  return __builtin_amdgcn_readfirstlane(x);
 }
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
