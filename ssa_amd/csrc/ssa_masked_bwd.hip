@@ -354,6 +354,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
   using Frag = typename O::Frag;
   using S = DkvShape<T, D, KG, RW>;
   constexpr int RB = S::RB, NCH = RB / 16, E = 16 / O::kEsize, QT = S::QT, NSUB = S::NSUB, SG = S::SG;
+  constexpr int SW = sizeof(T) == 2 ? kWide : kNarrow;
   constexpr int NC = D / 16, ND = D / 32, TB = S::TB, NT = S::kThr, RPP = NT / NCH, NP = (QT + RPP - 1) / RPP;
   extern __shared__ __align__(16) char lds[];  // [K, V of the block's keys][2 buffers][Q, dO][TB]
   __shared__ __align__(16) float s_lse[2][QT], s_dsum[2][QT], s_slope[2][QT], s_pos[2][QT];
@@ -385,7 +386,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
     const bool in = real && e < p.d;
     if constexpr (S::kInLds) {
       if (rw == 0) {
-        const int at = chunk_at<RB>(kg * 32 + (lane & 31), 2 * c + half);
+        const int at = chunk_at<RB, SW>(kg * 32 + (lane & 31), 2 * c + half);
         *reinterpret_cast<uint4*>(keys + at) = in ? *reinterpret_cast<const uint4*>(krow + e) : make_uint4(0u, 0u, 0u, 0u);
         *reinterpret_cast<uint4*>(keys + S::KB + at) = in ? *reinterpret_cast<const uint4*>(vrow + e) : make_uint4(0u, 0u, 0u, 0u);
       }
@@ -482,7 +483,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
     for (int i = 0; i < NP; ++i) {
       const int row = sr + i * RPP;
       if (QT % RPP != 0 && row >= QT) break;
-      const int at = chunk_at<RB>(row, sc);
+      const int at = chunk_at<RB, SW>(row, sc);
       *reinterpret_cast<uint4*>(qt + at) = qreg[i];
       *reinterpret_cast<uint4*>(qt + TB + at) = dreg[i];
     }
@@ -530,12 +531,12 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         if constexpr (S::kInLds) {
-          const Frag kk = O::template row_frag<RB>(keys, kg * 32, c, lane), vv = O::template row_frag<RB>(keys + S::KB, kg * 32, c, lane);
-          s = O::mfma(O::template row_frag<RB>(qt, 0, c, lane), kk, s);
-          dp = O::mfma(O::template row_frag<RB>(dt, 0, c, lane), vv, dp);
+          const Frag kk = O::template row_frag<RB, SW>(keys, kg * 32, c, lane), vv = O::template row_frag<RB, SW>(keys + S::KB, kg * 32, c, lane);
+          s = O::mfma(O::template row_frag<RB, SW>(qt, 0, c, lane), kk, s);
+          dp = O::mfma(O::template row_frag<RB, SW>(dt, 0, c, lane), vv, dp);
         } else {
-          s = O::mfma(O::template row_frag<RB>(qt, 0, c, lane), kf[c], s);
-          dp = O::mfma(O::template row_frag<RB>(dt, 0, c, lane), vf[c], dp);
+          s = O::mfma(O::template row_frag<RB, SW>(qt, 0, c, lane), kf[c], s);
+          dp = O::mfma(O::template row_frag<RB, SW>(dt, 0, c, lane), vf[c], dp);
         }
       }
       const bool whole = cur.lo_max[u] <= kw0 && cur.hi_min[u] >= kw0 + 32 && cur.tile * QT + row0 + 32 <= n_rows;
@@ -578,8 +579,8 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
         const Frag pf = O::pack(s, c), df = O::pack(dp, c);
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
-          accv[i] = O::mfma(O::template col_frag<RB>(dt, 16 * c, 32 * i, lane), pf, accv[i]);
-          acck[i] = O::mfma(O::template col_frag<RB>(qt, 16 * c, 32 * i, lane), df, acck[i]);
+          accv[i] = O::mfma(O::template col_frag<RB, SW>(dt, 16 * c, 32 * i, lane), pf, accv[i]);
+          acck[i] = O::mfma(O::template col_frag<RB, SW>(qt, 16 * c, 32 * i, lane), df, acck[i]);
         }
       }
     }

@@ -12,11 +12,18 @@
 // and only the A operand (read from LDS, by columns) follows that order.  No
 // score moves between lanes.
 //
-// LDS tiles are [rows][D] with 16-byte chunks swizzled within 128 bytes:
-// chunk c of row r lies at chunk c ^ f(r), f(r) = 2 (r % 4) + (r / 4) % 2.
-// Eight consecutive rows of one chunk then touch all banks once (row
-// fragments), and so do four rows x two chunks (column fragments by
-// ds_read_b64_tr_b16).
+// LDS tiles are [rows][D] with 16-byte chunks swizzled: chunk c of row r lies at
+// chunk c ^ f(r).  The LDS serves 16 lanes of a 16-byte read and 32 of an 8-byte one
+// at a time, from 64 banks.  Free of conflicts (kWide) is
+//   f = 4 (r % 4) + (r / 4) % 4          rows of 256 bytes and more
+//   f = 4 ((r / 2) % 2) + (r / 4) % 4    rows of 128 bytes, two to the banks' span
+// for row fragments (one chunk of 16 rows) and column fragments (four chunks of four
+// rows, ds_read_b64_tr_b16) alike.  kNarrow, f = 2 (r % 4) + (r / 4) % 2, reads both in
+// twice the cycles but moves only three bits, so that one address serves more chunks
+// by its offset.  The dK/dV kernel of bf16, whose LDS is the busiest, gains from the
+// wide one (backward over 8192 x 8192, 32 heads, d 128: 4020 to 3780 us; d 64: alike);
+// with it the forward spills at d 128 (1125 to 1240 us), the fp32 backward, whose
+// column fragments are single floats, loses 4% or more, and the dQ kernel gains nothing.
 #pragma once
 
 #include "ssa_common.h"
@@ -34,12 +41,19 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ int swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+enum Swizzle { kNarrow = 0, kWide = 1 };  // (see the head of the file)
+
+template <int RB, int SW>
+__device__ __forceinline__ int swz(int r) {
+  if constexpr (SW == kNarrow) return ((r & 3) << 1) | ((r >> 2) & 1);
+  if constexpr (RB >= 256) return ((r & 3) << 2) | ((r >> 2) & 3);
+  return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+}
 
 // Byte offset of 16-byte chunk c of row r in a tile of rows of RB bytes.
-template <int RB>
+template <int RB, int SW = kNarrow>
 __device__ __forceinline__ int chunk_at(int r, int c) {
-  return r * RB + ((c ^ swz(r)) << 4);
+  return r * RB + ((c ^ swz<RB, SW>(r)) << 4);
 }
 
 template <typename T>
@@ -60,20 +74,20 @@ struct Op<uint16_t> {
   // Eight consecutive elements in global memory (16-byte aligned).
   static __device__ __forceinline__ Frag load(const uint16_t* p) { return Frag{*reinterpret_cast<const uint4*>(p)}; }
   // Columns 16c + 8 (l / 32) .. + 7 of tile row row0 + l % 32.
-  template <int RB>
+  template <int RB, int SW = kNarrow>
   static __device__ __forceinline__ Frag row_frag(const char* t, int row0, int c, int lane) {
     const int r = row0 + (lane & 31);
-    return Frag{*reinterpret_cast<const uint4*>(t + chunk_at<RB>(r, 2 * c + (lane >> 5)))};
+    return Frag{*reinterpret_cast<const uint4*>(t + chunk_at<RB, SW>(r, 2 * c + (lane >> 5)))};
   }
   // Column d0 + l % 32 of rows row0 + 4 (l / 32) + {0..3, 8..11} (row0 a multiple of 16).
-  template <int RB>
+  template <int RB, int SW = kNarrow>
   static __device__ __forceinline__ Frag col_frag(const char* t, int row0, int d0, int lane) {
     const int i = lane & 15;
     const int r = row0 + 4 * (lane >> 5) + (i >> 2);
     const int ch = (d0 >> 3) + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
-    const char* p = t + chunk_at<RB>(r, ch) + (i & 1) * 8;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 8 * RB));
+    const char* p = t + (i & 1) * 8;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + chunk_at<RB, SW>(r, ch)));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + chunk_at<RB, SW>(r + 8, ch)));
     const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
     return Frag{make_uint4(a.x, a.y, b.x, b.y)};
   }
@@ -123,20 +137,20 @@ struct Op<float> {
   static __device__ __forceinline__ Frag load(const float* p) {
     return of(*reinterpret_cast<const float4*>(p), *reinterpret_cast<const float4*>(p + 4));
   }
-  template <int RB>
+  template <int RB, int SW = kNarrow>
   static __device__ __forceinline__ Frag row_frag(const char* t, int row0, int c, int lane) {
     const int r = row0 + (lane & 31), ch = 4 * c + 2 * (lane >> 5);
-    return of(*reinterpret_cast<const float4*>(t + chunk_at<RB>(r, ch)),
-              *reinterpret_cast<const float4*>(t + chunk_at<RB>(r, ch + 1)));
+    return of(*reinterpret_cast<const float4*>(t + chunk_at<RB, SW>(r, ch)),
+              *reinterpret_cast<const float4*>(t + chunk_at<RB, SW>(r, ch + 1)));
   }
-  template <int RB>
+  template <int RB, int SW = kNarrow>
   static __device__ __forceinline__ Frag col_frag(const char* t, int row0, int d0, int lane) {
     const int d = d0 + (lane & 31);
     Frag f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = row0 + 4 * (lane >> 5) + (i & 3) + 8 * (i >> 2);
-      f.v[i] = *reinterpret_cast<const float*>(t + chunk_at<RB>(r, d >> 2) + (d & 3) * 4);
+      f.v[i] = *reinterpret_cast<const float*>(t + chunk_at<RB, SW>(r, d >> 2) + (d & 3) * 4);
     }
     return f;
   }
