@@ -235,8 +235,13 @@ constexpr int most_kw() {
 
 // LDS of a block: two buffers of K and V, or at the end the waves' sums.
 template <typename T, int D, int KW>
+constexpr int key_buffers() {
+  return 4 * key_tile<T, KW>() * D * static_cast<int>(sizeof(T)) > 80 * 1024 ? 1 : 2;
+}
+
+template <typename T, int D, int KW>
 constexpr size_t rows_lds() {
-  const size_t tiles = static_cast<size_t>(4) * key_tile<T, KW>() * D * sizeof(T);
+  const size_t tiles = static_cast<size_t>(2) * key_buffers<T, D, KW>() * key_tile<T, KW>() * D * sizeof(T);
   const size_t sums = KW > 1 ? static_cast<size_t>(4) * 32 * (D + 4) * sizeof(float) : 0;
   return tiles > sums ? tiles : sums;
 }
@@ -259,6 +264,7 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
   constexpr int RPP = kThreads / NCH;    // tile rows a pass of the block loads
   constexpr int NP = KT / RPP;
   constexpr int TB = KT * RB;            // bytes of a tile
+  constexpr bool TWO = key_buffers<T, D, KW>() == 2;
   constexpr int BR = rows_of(KW);        // the block's rows
   constexpr int PS = D + 4;              // floats of a row of sums
   // lds: [2 buffers][K, V][TB], then [4 waves][32][PS]
@@ -291,7 +297,8 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
     kvh = bh - b * p.h_kv;
     m = static_cast<int>(p.n_q);
     n_keys = p.n;
-    tile = static_cast<int>((p.n_q * p.g + BR - 1) / BR) - 1 - rest;
+    const int tiles = static_cast<int>((p.n_q * p.g + BR - 1) / BR);
+    tile = tiles - 1 - (rows_per_cu<T, D, KW>() == 2 && tiles * nbh * p.splits <= 512 ? fold_tile(rest, tiles, nbh * p.splits) : rest);
   }
   const KeyRows<T, PAGED> rows = key_rows<T, PAGED>(p, b, kvh, first, static_cast<int>(n_keys) - m);
 
@@ -421,7 +428,7 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
     if (t + 2 < nt) find_pages(t + 2);
     const int k0 = (t0 + t) * KT + kw * 32 * NSUB;
     if (k0 < hi_max && k0 + 32 * NSUB > lo_min) {
-      const char* kt = lds + (t & 1) * 2 * TB + kw * 32 * NSUB * RB;
+      const char* kt = lds + (TWO ? (t & 1) * 2 * TB : 0) + kw * 32 * NSUB * RB;
       const char* vt = kt + TB;
       f32x16 s[NSUB];
 #pragma unroll
@@ -480,7 +487,8 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
           for (int i = 0; i < ND; ++i) acc[i] = O::mfma(O::template col_frag<RB>(vt, 32 * u + 16 * c, 32 * i, lane), pf, acc[i]);
         }
     }
-    if (t + 1 < nt) store_tile((t + 1) & 1);
+    if constexpr (!TWO) __syncthreads();
+    if (t + 1 < nt) store_tile(TWO ? (t + 1) & 1 : 0);
   }
 
   // the row's sums, joined over the half-waves (they share the reference)

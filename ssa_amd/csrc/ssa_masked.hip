@@ -95,27 +95,45 @@ int launch_rule(DenseParams& p, int kw, hipStream_t st) {
 
 }  // namespace
 
-DenseSplit dense_split(int64_t rows, int64_t heads, int64_t keys, bool wide_f32) {
-  // Two blocks fit a CU, so 512 run at once.  Blocks of 128 rows that are fewer
-  // (us a call, bf16, measured with each cut):
-  //   over many keys, the key axis is cut into as many parts as about 512 blocks
-  //     take, at least 384 keys each; not in two below 8192 keys, where the second
-  //     launch costs more (1200 rows x 8 heads over 16k keys: 1 part 289, 6 parts 138;
-  //     1000 x 8 x 4 rows over 1000 keys: 1 part 47, 2 parts 62);
-  //   and where blocks are few still, two or four waves share each 32 rows and take
-  //     turns at the keys (2048 x 8 rows of 2 x 1024 tokens, d = 64: 32, 28 and 24 us
-  //     with 1, 2 and 4; from 512 blocks on one wave a row is as fast or faster; four
-  //     read each key tile for 32 rows only, twice as slow over 6000 keys).
+DenseSplit dense_split(int64_t rows, int64_t heads, int64_t keys, int64_t n_q, bool f32, bool wide) {
+  // Blocks of 128 rows, one wave a row, from 512 blocks on (two a CU).  Where they are
+  // fewer (us a call, both sides measured; of 120 calls of 700 to 5000 keys and 10 to
+  // 500 blocks the rule's cut is 4% slower than the best of 27 in the mean):
   DenseSplit s{1, 1};
   const int64_t blocks = ceil_div(rows, 128) * heads;
-  if (blocks <= 0 || blocks >= 512) return s;
-  const int64_t want = (512 + blocks / 4) / blocks, can = keys / 384;
-  int64_t parts = want < can ? want : can;
-  if (parts < 2 || (parts == 2 && keys < 8192)) parts = 1;
+  if (blocks <= 0 || blocks >= 512 || keys <= 32) return s;
+  // Two or four waves share each 32 rows and take turns at the keys (2500 causal rows of
+  // 8 / 2 heads, d = 64, 158 blocks: 40 with two, 32 with four; 1500 of 32 / 8, d = 128,
+  // 376 blocks: 54 with one or two, 67 with four).  Four read the keys four times as
+  // often as one; bf16 is bound by that over long ones (6000: twice as slow), fp32 never
+  // (4096 causal rows of 8 / 2 heads, d = 64: 194 with two, 187 with four).
+  const bool one_block = f32 && wide;  // a CU holds one block, of two waves a row at most
+  const int64_t four = f32 ? 256 : 176;
+  if (blocks < four && keys > 64 && (f32 || keys < 4096) && !one_block)
+    s.kw = 4;
+  else if (blocks < 400)
+    s.kw = 2;
+  // Parts of the keys, joined by a second launch.  They pay where the rows are few
+  // beside the keys, which each row then sees nearly all of; in a square causal or
+  // document mask most parts of a row are empty (1500 rows of 12 / 4 heads, d = 128:
+  // 35 in one part, 45 in three).  Long keys take as many parts as about 512 blocks
+  // allow, of 384 keys at least, and waves share rows only where those are few still
+  // (1200 x 8 rows over 16384 keys: 289 in one part, 138 in six); not two parts below
+  // 8192 keys, where the join costs more.  Shorter ones take parts only until the blocks
+  // fill the CUs once, of at least 384 keys (fp32 192: 140 x 4 rows of 2 heads over 700
+  // keys 30 and 24 in one and three parts; bf16 18.6 and 20.3).
+  int64_t parts = 1;
+  if (2 * n_q <= keys && keys >= 4096) {
+    const int64_t want = (512 + blocks / 4) / blocks, can = keys / 384;
+    parts = want < can ? want : can;
+    if (parts < 2 || (parts == 2 && keys < 8192)) parts = 1;
+    s.kw = parts > 1 && blocks * parts >= 384 ? 1 : 2;
+  } else if (2 * n_q <= keys || one_block) {
+    const int64_t all = blocks * s.kw, want = (256 + all / 2) / all, can = keys / (f32 ? 192 : 384);
+    parts = want < can ? want : can;
+    if (parts < 1) parts = 1;
+  }
   s.parts = static_cast<int>(parts);
-  if (blocks * parts < 512 && keys > 32) s.kw = 2;
-  if (blocks * parts < 192 && keys > 64 && keys < 2048 && !wide_f32) s.kw = 4;
-  if (parts > 1 && blocks * parts >= 384) s.kw = 1;
   return s;
 }
 
@@ -184,7 +202,7 @@ int check_aligned(const char* fn, const char* name, int dtype, const void* ptr, 
 extern "C" size_t ssa_masked_attention_workspace_bytes(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv,
                                                        int d) {
   if (batch <= 0 || n <= 0 || n_q <= 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0) return 0;
-  const int s = dense_split(n_q * (h_q / h_kv), batch * h_kv, n, dtype == SSA_DTYPE_F32 && d > 64).parts;
+  const int s = dense_split(n_q * (h_q / h_kv), batch * h_kv, n, n_q, dtype == SSA_DTYPE_F32, d > 64).parts;
   if (s <= 1) return 0;
   return static_cast<size_t>(s) * batch * n_q * h_q * ((d <= 64 ? 64 : 128) + 2) * sizeof(float);
 }
@@ -220,7 +238,7 @@ extern "C" int ssa_masked_attention(const void* q, const void* k, const void* v,
   p.n = n; p.n_q = n_q; p.q_pos0 = q_pos0;
   p.batch = static_cast<int>(batch); p.h_q = h_q; p.h_kv = h_kv; p.g = h_q / h_kv; p.d = d;
   p.spans = reinterpret_cast<const int2*>(spans);
-  const DenseSplit cut = dense_split(n_q * p.g, batch * h_kv, n, dtype == SSA_DTYPE_F32 && d > 64);
+  const DenseSplit cut = dense_split(n_q * p.g, batch * h_kv, n, n_q, dtype == SSA_DTYPE_F32, d > 64);
   p.splits = cut.parts;
   if (p.splits > 1) {
     const size_t need = ssa_masked_attention_workspace_bytes(dtype, batch, n, n_q, h_q, h_kv, d);
