@@ -541,7 +541,8 @@ int ssa_masked_attention_backward(
  *       [batch + 1] ascending, cached int32 [batch]: device memory, read by the
  *       kernels, so that a captured call follows their values.
  *   max_new, max_len: the most new tokens and the most keys (new ones included) of
- *       a sequence; the launch is sized by them.
+ *       a sequence; the launch is sized by them (they may say more than the tokens
+ *       or the table hold; the workspace is asked for with the same).
  *   A sequence that breaks them, or the table's or the rows' range, is left out
  *       (its rows of out and its pages stay as they are), a page outside the pool
  *       is not touched (keys there read page 0): either sets *error_flag

@@ -51,10 +51,12 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
     ``sections[0]`` pairs turn by ``positions[0]``, the next by ``positions[1]``, ...;
     features from rot on pass through.  Returns (q, k), or q alone when k is None, in their
     dtype; shapes without B are kept.  Angles are exact for far positions (64 bits), the
-    result is rounded once.  Differentiable in q and k."""
+    result is rounded once.  Differentiable in q and k, not in freqs."""
     unbatched = q.dim() == 3
     if unbatched:
         q, k = q.unsqueeze(0), None if k is None else k.unsqueeze(0)
+    if freqs.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("freqs get no gradient: detach them")
     half = q.dtype == torch.float16
     if half:
         if k is not None and k.dtype != q.dtype:

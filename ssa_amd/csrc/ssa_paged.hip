@@ -387,6 +387,7 @@ struct PagedPlan {
 
 PagedPlan paged_plan(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t max_new, int64_t max_len) {
   PagedPlan l{};
+  max_new = max_new < tokens ? max_new : tokens;
   const int64_t g = h_q / h_kv, D = d <= 64 ? 64 : 128;
   // Few rows: parts of at least 256 keys, enough for two blocks a CU twice over
   // where the batch has sequences of unlike lengths to even out, once for one.
@@ -522,9 +523,6 @@ extern "C" int ssa_paged_step(const void* q, const void* k, const void* v, int d
   if (int rc = check_aligned(fn, "k_pages", dtype, k_pages, kp_sp, kp_st, kp_sh)) return rc;
   if (int rc = check_aligned(fn, "v_pages", dtype, v_pages, vp_sp, vp_st, vp_sh)) return rc;
   if (int rc = check_aligned(fn, "out", dtype, out, 0, o_st, o_sh)) return rc;
-  if (max_new > tokens) max_new = tokens;
-  const int64_t cap = static_cast<int64_t>(max_pages) * page_size;
-  if (max_len > cap) max_len = cap;
   const PagedPlan l = paged_plan(dtype, tokens, batch, h_q, h_kv, d, max_new, max_len);
   if (l.bytes > 0 && (workspace == nullptr || workspace_bytes < l.bytes))
     return fail(SSA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", fn, l.bytes,
@@ -542,7 +540,7 @@ extern "C" int ssa_paged_step(const void* q, const void* k, const void* v, int d
   p.max_pages = max_pages; p.num_pages = static_cast<int>(num_pages);
   while ((1 << p.page_log2) < page_size) ++p.page_log2;
   p.few_rows = kFew;
-  p.max_new = max_new; p.max_len = max_len;
+  p.max_new = max_new < tokens ? max_new : tokens; p.max_len = max_len;
   p.error_flag = error_flag;
   p.k_new = k; p.v_new = v;
   p.kn_st = k_st; p.kn_sh = k_sh; p.vn_st = v_st; p.vn_sh = v_sh;

@@ -530,9 +530,14 @@ def _check_slopes(slopes: Optional[torch.Tensor], h_q: int) -> Optional[torch.Te
         return None
     if slopes.dtype != torch.float32 or tuple(slopes.shape) != (h_q,):
         raise ValueError(f"slopes must be float32 [{h_q}]")
-    if slopes.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError("slopes get no gradient: detach them")
     return slopes.contiguous()
+
+
+def _pos0(q_pos0: Optional[int], n: int, n_q: int, spans, slopes) -> int:
+    """Position of query row 0; where neither mask nor bias reads it, any will do."""
+    if q_pos0 is not None:
+        return q_pos0
+    return n - n_q if n >= n_q or spans is None or slopes is not None else 0
 
 
 def mask_spans(n: int, batch: int, n_q: int, q_pos0: int, causal: bool, doc_starts: Optional[torch.Tensor],
@@ -599,7 +604,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: O
     nbytes = _bytes("ssa_masked_attention_workspace_bytes", dt, B, n, n_q, h_q, h_kv, d)
     ws = _workspace(nbytes, q)
     _call_on(dev, "ssa_masked_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, n, n_q,
-             n - n_q if q_pos0 is None else q_pos0, h_q, h_kv, d, *qs, *ks, *vs, _at(spans),
+             _pos0(q_pos0, n, n_q, spans, slopes), h_q, h_kv, d, *qs, *ks, *vs, _at(spans),
              math.sqrt(d) if scale_div is None else scale_div, softcap, _at(slopes), out.data_ptr(), n_q * h_q * d, h_q * d, d,
              _at(low), _at(lse), _at(ws), nbytes)
     return (out, low, lse) if with_lse else out
@@ -635,7 +640,7 @@ def masked_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     nbytes = _bytes("ssa_masked_attention_backward_workspace_bytes", dt, B, n, n_q, h_q, h_kv, d)
     ws = _workspace(nbytes, q)
     _call_on(dev, "ssa_masked_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, n, n_q,
-             n - n_q if q_pos0 is None else q_pos0, h_q, h_kv, d, *qs, *ks, *vs, _at(spans),
+             _pos0(q_pos0, n, n_q, spans, slopes), h_q, h_kv, d, *qs, *ks, *vs, _at(spans),
              math.sqrt(d) if scale_div is None else scale_div, softcap, _at(slopes), out.data_ptr(), _at(out_low), *os,
              dout.data_ptr(), *dos, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(ws), nbytes)
     return dq, dk, dv

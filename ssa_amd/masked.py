@@ -77,7 +77,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: O
     ``j // (h_q // h_kv)``; unbatched shapes too); ``spans`` from ``mask_spans`` or any int32
     ``[B, n_q, 2]`` of key intervals [lo, hi), None for causal.  Scores are q.k / scale
     (sqrt(d)); ``softcap`` c makes them c tanh(s / c); ``slopes`` (float32 [h_q]) subtracts
-    slopes[h] |position - key|, row i at position ``q_pos0 + i`` (default n - n_q).
+    slopes[h] |position - key|, row i at position ``q_pos0 + i`` (default n - n_q).  Slopes
+    get no gradient.
 
     Rows that see no key are zeros, and keys a row does not see have no influence on it,
     whatever they hold.  float32 and bfloat16, head_dim a multiple of 8 up to 128; float16
@@ -92,6 +93,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: O
         q, k, v = q.float(), k.float(), v.float()
     if softcap is not None and not softcap > 0:
         raise ValueError(f"softcap must be positive, got {softcap}")
+    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("slopes get no gradient: detach them")
     args = (q, k, v, spans, scale, softcap or 0.0)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out = _MaskedAttention.apply(*args, slopes, q_pos0)

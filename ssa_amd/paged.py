@@ -59,6 +59,12 @@ class PagedKVCache:
 
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.bfloat16, device=None):
+        if page_size < 8 or page_size > 4096 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of 2 in [8, 4096], got {page_size}")
+        if head_dim < 8 or head_dim > 128 or head_dim % 8:
+            raise ValueError(f"head_dim must be a multiple of 8 up to 128, got {head_dim}")
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
         device = torch.device("cuda" if device is None else device)
         self.page_size = page_size
         self.k_pages = torch.empty(num_pages, page_size, num_kv_heads, head_dim, device=device, dtype=dtype)

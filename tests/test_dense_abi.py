@@ -124,6 +124,39 @@ def test_rope_axes(L, kw, status, text):
     assert st == status and (st == OK or text in msg), msg
 
 
+@pytest.mark.parametrize("max_new,max_len,max_pages", [(8, 1000, 64), (8, 1025, 64), (1 << 62, 1025, 64), (10, 70000, 64),
+                                                       (1, 1 << 30, 8), (300, 1024, 1)])
+@pytest.mark.parametrize("tokens,batch", [(10, 3), (300, 1), (700, 16)])
+def test_paged_workspace_of_any_bounds(L, max_new, max_len, max_pages, tokens, batch):
+    """Bounds past the tokens and the table are allowed; the call needs what the sizes say."""
+    need = L.ssa_paged_step_workspace_bytes(_lib.DTYPE_BF16, tokens, batch, 8, 2, 64, max_new, max_len)
+    kw = dict(tokens=tokens, batch=batch, max_new=max_new, max_len=max_len, max_pages=max_pages)
+    if need == 0:
+        return
+    for ws, have in ((FAKE, need - 1), (None, need)):
+        st, msg = _call(L, "ssa_paged_step", PAGED, dict(kw, ws=ws, ws_bytes=have))
+        assert st == WORKSPACE and f"workspace of {need} bytes" in msg, msg
+
+
+def test_cache_refuses_pages_that_no_step_takes():
+    for page in (0, 4, 24, 8192):
+        with pytest.raises(ValueError, match="page_size"):
+            ssa_amd.PagedKVCache(4, page, 2, 64, device="cpu")
+    for d in (0, 12, 136):
+        with pytest.raises(ValueError, match="head_dim"):
+            ssa_amd.PagedKVCache(4, 16, 2, d, device="cpu")
+    with pytest.raises(TypeError, match="dtype"):
+        ssa_amd.PagedKVCache(4, 16, 2, 64, dtype=torch.float16, device="cpu")
+
+
+def test_python_refuses_gradients_it_does_not_have():
+    q = torch.zeros(1, 4, 2, 8, requires_grad=True)
+    with pytest.raises(NotImplementedError, match="slopes"):
+        ssa_amd.masked_attention(q, q, q, slopes=torch.ones(2, requires_grad=True))
+    with pytest.raises(NotImplementedError, match="freqs"):
+        ssa_amd.rope_axes(q, q, torch.zeros(1, 1, 4, dtype=torch.int32), ssa_amd.axis_rope_freqs(8).requires_grad_(True), (4,))
+
+
 def test_python_refuses_host_tensors():
     q = torch.zeros(1, 4, 2, 8)
     ints = torch.zeros(1, 4, dtype=torch.int32)

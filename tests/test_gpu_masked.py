@@ -326,3 +326,40 @@ def test_rejects(dev):
         mask_spans(8, 2, doc_starts=torch.zeros(1, 3, device=dev, dtype=torch.int32))
     with pytest.raises(TypeError, match="doc_starts"):
         mask_spans(8, 1, doc_starts=torch.zeros(1, 3, device=dev))
+
+
+def test_more_rows_than_keys(dev):
+    """With intervals and no bias, where the rows sit is not read; else it has to be said."""
+    from ssa_amd import masked_attention
+
+    q, k, v, dout = _inputs(14, BF16, 1, 90, 20, 4, 2, 64)
+    spans = torch.stack((torch.arange(90) % 20, torch.arange(90) % 20 + 1 + torch.arange(90) // 30), 1).clamp(max=20).int()
+    res = _run(dev, q, k, v, dout, spans[None])
+    _check(res, q, k, v, dout, spans[None], 0.0, None, 0)
+    with pytest.raises(RuntimeError, match="q_pos0"):
+        masked_attention(q.to(dev), k.to(dev), v.to(dev))
+    with pytest.raises(RuntimeError, match="q_pos0"):
+        masked_attention(q.to(dev), k.to(dev), v.to(dev), spans[None].to(dev), slopes=_slopes(4).to(dev))
+
+
+@pytest.mark.parametrize("dtype,d", [(F32, 64), (BF16, 64), (BF16, 128)], ids=str)
+def test_far_rows(dev, dtype, d):
+    """Rows of q, k, v and dout 16 MiB apart: offsets past 2^31 elements and 2^32 bytes."""
+    from ssa_amd import masked_attention
+
+    n, h_q, h_kv = 300, 4, 2
+    q, k, v, dout = _inputs(15, dtype, 1, n, n, h_q, h_kv, d)
+    step = (16 << 20) // q.element_size()
+    pool = torch.zeros((n - 1) * step + 32 * d, device=dev, dtype=dtype)
+    at, far = 0, []
+    for t in (q, k, v, dout):
+        x = torch.as_strided(pool, t.shape, (0, step, d, 1), at)
+        x.copy_(t)
+        far.append(x)
+        at += t.shape[2] * d
+    assert (n - 1) * step * q.element_size() > 1 << 32
+    leaves = [t.detach().requires_grad_(True) for t in far[:3]]
+    out = masked_attention(*leaves)
+    grads = torch.autograd.grad(out, leaves, far[3])
+    res = dict(zip(("out", "dq", "dk", "dv"), (out, *grads)))
+    _check(res, q, k, v, dout, spans_of(n, n, 0)[None], 0.0, None, 0)

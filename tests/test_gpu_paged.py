@@ -216,6 +216,43 @@ def test_far_pages(dev):
         check(out[at:at + m], value, bound, f"sequence {b}")
 
 
+@pytest.mark.parametrize("m", [1, 40])
+def test_shared_pages_and_rows_before_the_first_sequence(dev, m):
+    """Sequences that share the pages of a prefix, one of which stands in it twice; rows before
+    the first sequence and behind the last keep what they held."""
+    from ssa_amd import paged_step
+
+    page, h_q, h_kv, d = 16, 8, 2, 64
+    s, keys = _batch(39, BF16, [(m, 64), (m, 64)], h_q, h_kv, d, page)
+    pre = s["table"][0, :3]
+    s["table"][0, 2] = pre[0]          # keys 32..47 are keys 0..15 again
+    s["table"][1, :3] = s["table"][0, :3]
+    for b in range(2):
+        for x, pool in zip(keys[b], (s["k_pages"], s["v_pages"])):
+            for i in range(3):
+                x[16 * i:16 * i + 16] = pool[s["table"][0, i]]
+    edge = 3
+    for n in ("q", "k", "v"):
+        nobody = torch.full((edge, *s[n].shape[1:]), math.nan, dtype=BF16)
+        s[n] = torch.cat((nobody, s[n], nobody))
+    s["starts"] += edge
+    out = torch.full(s["q"].shape, 7.0, dtype=BF16, device=dev)
+    paged_step(**{n: t.to(dev) for n, t in s.items()}, out=out, check=True)
+    assert (out[:edge] == 7).all() and (out[-edge:] == 7).all()
+    for b in range(2):
+        rows = slice(edge + b * m, edge + (b + 1) * m)
+        check(out[rows], *attend(s["q"][rows], *keys[b], spans_of(64 + m, m, 64), 0.0, None, 64)["out"], f"sequence {b}")
+
+
+def test_bounds_past_the_tokens_and_the_table(dev):
+    """max_new and max_len may say more than a sequence can hold."""
+    from ssa_amd import paged_step
+
+    s, _ = _batch(41, BF16, [(1, 300), (50, 70)], 8, 2, 64, 16)
+    x = {n: t.to(dev) for n, t in s.items()}
+    assert torch.equal(paged_step(**x, check=True), paged_step(**x, max_new=10 ** 6, max_len=10 ** 9, check=True))
+
+
 def test_empty(dev):
     from ssa_amd import paged_step
 
