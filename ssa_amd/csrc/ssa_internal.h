@@ -67,6 +67,6 @@ int score_rule(const char* fn, float scale_div, float softcap, const float* slop
 struct DenseSplit {
   int kw, parts;
 };
-DenseSplit dense_split(int64_t rows, int64_t heads, int64_t keys, int64_t n_q, bool f32, bool wide);
+DenseSplit dense_split(int64_t rows, int64_t heads, int64_t keys, int64_t n_q, bool f32, bool wide, bool paged);
 
 }  // namespace ssa

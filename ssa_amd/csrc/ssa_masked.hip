@@ -95,7 +95,7 @@ int launch_rule(DenseParams& p, int kw, hipStream_t st) {
 
 }  // namespace
 
-DenseSplit dense_split(int64_t rows, int64_t heads, int64_t keys, int64_t n_q, bool f32, bool wide) {
+DenseSplit dense_split(int64_t rows, int64_t heads, int64_t keys, int64_t n_q, bool f32, bool wide, bool paged) {
   // Blocks of 128 rows, one wave a row, from 512 blocks on (two a CU).  Where they are
   // fewer (us a call, both sides measured; of 120 calls of 700 to 5000 keys and 10 to
   // 500 blocks the rule's cut is 4% slower than the best of 27 in the mean):
@@ -121,19 +121,25 @@ DenseSplit dense_split(int64_t rows, int64_t heads, int64_t keys, int64_t n_q, b
   // (1200 x 8 rows over 16384 keys: 289 in one part, 138 in six); not two parts below
   // 8192 keys, where the join costs more.  Shorter ones take parts only until the blocks
   // fill the CUs once, of at least 384 keys (fp32 192: 140 x 4 rows of 2 heads over 700
-  // keys 30 and 24 in one and three parts; bf16 18.6 and 20.3).
-  int64_t parts = 1;
-  if (2 * n_q <= keys && keys >= 4096) {
-    const int64_t want = (512 + blocks / 4) / blocks, can = keys / 384;
-    parts = want < can ? want : can;
-    if (parts < 2 || (parts == 2 && keys < 8192)) parts = 1;
-    s.kw = parts > 1 && blocks * parts >= 384 ? 1 : 2;
-  } else if (2 * n_q <= keys || one_block) {
-    const int64_t all = blocks * s.kw, want = (256 + all / 2) / all, can = keys / (f32 ? 192 : 384);
-    parts = want < can ? want : can;
-    if (parts < 1) parts = 1;
+  // keys 30 and 24 in one and three parts; bf16 18.6 and 20.3).  Over pages, whose rows
+  // follow what is cached and whose tiles wait for their pages as well, half as long
+  // parts and twice as many pay (915 x 3 rows of 2 heads over 2470 keys: 68 in one part,
+  // 51 in three; 500 x 7 rows twice of 4 heads over 6500: 188 in three, 165 in four).
+  const bool chunk = paged || 2 * n_q <= keys;
+  int64_t want = 1, can = 1;
+  if (chunk && keys >= 4096) {
+    want = paged ? ceil_div(640, blocks) : (512 + blocks / 4) / blocks;
+    can = keys / 384;
+    if (!paged && (want < can ? want : can) == 2 && keys < 8192) want = 1;
+    const int64_t all = blocks * (want < can ? want : can);
+    s.kw = all > blocks && all >= 384 ? 1 : (paged && all < 64 && !one_block ? 4 : 2);
+  } else if (chunk || one_block) {
+    const int64_t all = blocks * s.kw;
+    want = ((paged ? 512 : 256) + all / 2) / all;
+    can = keys / (f32 || paged ? 192 : 384);
   }
-  s.parts = static_cast<int>(parts);
+  const int64_t parts = want < can ? want : can;
+  s.parts = parts > 1 ? static_cast<int>(parts) : 1;
   return s;
 }
 
@@ -202,7 +208,7 @@ int check_aligned(const char* fn, const char* name, int dtype, const void* ptr, 
 extern "C" size_t ssa_masked_attention_workspace_bytes(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv,
                                                        int d) {
   if (batch <= 0 || n <= 0 || n_q <= 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0) return 0;
-  const int s = dense_split(n_q * (h_q / h_kv), batch * h_kv, n, n_q, dtype == SSA_DTYPE_F32, d > 64).parts;
+  const int s = dense_split(n_q * (h_q / h_kv), batch * h_kv, n, n_q, dtype == SSA_DTYPE_F32, d > 64, false).parts;
   if (s <= 1) return 0;
   return static_cast<size_t>(s) * batch * n_q * h_q * ((d <= 64 ? 64 : 128) + 2) * sizeof(float);
 }
@@ -238,7 +244,7 @@ extern "C" int ssa_masked_attention(const void* q, const void* k, const void* v,
   p.n = n; p.n_q = n_q; p.q_pos0 = q_pos0;
   p.batch = static_cast<int>(batch); p.h_q = h_q; p.h_kv = h_kv; p.g = h_q / h_kv; p.d = d;
   p.spans = reinterpret_cast<const int2*>(spans);
-  const DenseSplit cut = dense_split(n_q * p.g, batch * h_kv, n, n_q, dtype == SSA_DTYPE_F32, d > 64);
+  const DenseSplit cut = dense_split(n_q * p.g, batch * h_kv, n, n_q, dtype == SSA_DTYPE_F32, d > 64, false);
   p.splits = cut.parts;
   if (p.splits > 1) {
     const size_t need = ssa_masked_attention_workspace_bytes(dtype, batch, n, n_q, h_q, h_kv, d);

@@ -401,7 +401,7 @@ PagedPlan paged_plan(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv
   l.row_len = 0;
   if (max_new * g > kFew) {
     const int64_t each = batch * max_new, rows = (tokens < each ? tokens : each) * g;
-    const DenseSplit cut = dense_split(rows, h_kv, max_len, max_new, dtype == SSA_DTYPE_F32, d > 64);
+    const DenseSplit cut = dense_split(rows, h_kv, max_len, max_new, dtype == SSA_DTYPE_F32, d > 64, true);
     const int block = rows_of(cut.kw);
     // (a sequence's last block may be part empty)
     const int64_t by_seq = batch * ceil_div(max_new * g, block), ragged = rows / block + batch;
