@@ -271,7 +271,7 @@ struct ScoreRule {
 
 // tanh for the bf16 kernels: 1 - 2 / (exp(2y) + 1), absolute error about 2^-22
 // (v_exp_f32 and v_rcp_f32 are good to an ulp), far below a bf16 weight's
-// 2^-9.  The fp32 kernels take the library's.
+// 2^-8.  The fp32 kernels take the library's.
 template <typename T>
 __device__ __forceinline__ float cap_tanh(float y) {
   if constexpr (sizeof(T) == 4) return tanhf(y);
