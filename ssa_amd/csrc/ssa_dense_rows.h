@@ -279,7 +279,8 @@ __device__ __forceinline__ int fold_tile(int t, int tiles, int heads) {
   return round * per + (left < per ? left : per) - 1 - at;
 }
 
-template <typename T, int D, bool PAGED, int RULE, int KW>
+// FRESH: tiles of a paged call's own rows are read as contiguous ones are.
+template <typename T, int D, bool PAGED, int RULE, int KW, bool FRESH = false>
 __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, char* lds) {
   using O = Op<T>;
   using Frag = typename O::Frag;
@@ -379,7 +380,8 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
 
   // staging: chunk sc of tile rows sr, sr + RPP, ....  Of paged keys, a wave's rows of
   // a load lie in one page, looked up a tile before; tiles that reach past the pages'
-  // keys (the call's own rows, the end) take each row's address.
+  // keys (the call's own rows unless FRESH, a tile of both, the end) take each row's
+  // address.
   const int sc = tid % NCH, sr = tid / NCH;
   const bool chunk_ok = sc * E < p.d;
   const int last = static_cast<int>(n_keys) - 1;
@@ -406,6 +408,17 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
           const int64_t page = rows.checked(__builtin_amdgcn_readfirstlane(pg[i])), r0 = (j0 + i * RPP + wave * RPW) & rows.page_mask;
           kreg[i] = row_load(row_buffer(rows.k + page * rows.k_sb + r0 * rows.k_sn, kAllBytes), koff);
           vreg[i] = row_load(row_buffer(rows.v + page * rows.v_sb + r0 * rows.v_sn, kAllBytes), voff);
+        }
+      } else if (FRESH && j0 >= rows.new_from) {
+        const int left = static_cast<int>(n_keys) - j0, x = j0 - rows.new_from, db = p.d * O::kEsize;
+        const uint32_t kn = static_cast<uint32_t>(rows.kn_st * O::kEsize), vn = static_cast<uint32_t>(rows.vn_st * O::kEsize);
+        const auto kb = row_buffer(rows.k_new + x * rows.kn_st, left >= KT ? kAllBytes : static_cast<int>((left - 1) * kn) + db);
+        const auto vb = row_buffer(rows.v_new + x * rows.vn_st, left >= KT ? kAllBytes : static_cast<int>((left - 1) * vn) + db);
+        const uint32_t r = in_branch(sr), ko = chunk_ok ? r * kn + sc * 16 : kNoChunk, vo = chunk_ok ? r * vn + sc * 16 : kNoChunk;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          kreg[i] = row_load(kb, ko + i * RPP * kn);
+          vreg[i] = row_load(vb, vo + i * RPP * vn);
         }
       } else {
 #pragma unroll

@@ -115,6 +115,29 @@ def test_strided_pools_and_rows(dev):
     assert torch.equal(paged_step(**x), want)
 
 
+@pytest.mark.parametrize("dtype,h_q,h_kv,d", [(F32, 4, 2, 64), (F32, 4, 2, 128), (BF16, 8, 2, 64), (BF16, 6, 2, 96)], ids=str)
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (3.0, False), (3.0, True)])
+def test_prompts(dev, dtype, h_q, h_kv, d, cap, bias):
+    """Prompts, most of whose keys are the call's own rows: cut out of one projection, behind
+    nothing, behind an odd number of cached keys and behind whole tiles; rows behind the last."""
+    from ssa_amd import paged_step
+
+    seqs, page = [(300, 0), (131, 37), (65, 128), (1, 0)], 16
+    s, keys = _batch(42, dtype, seqs, h_q, h_kv, d, page, behind=2)
+    slopes = torch.tensor([2.0 ** -(i + 1) for i in range(h_q)]) if bias else None
+    x = {n: t.to(dev) for n, t in s.items()}
+    qkv = torch.cat((x["q"], x["k"], x["v"]), 1)
+    x["q"], x["k"], x["v"] = qkv[:, :h_q], qkv[:, h_q:h_q + h_kv], qkv[:, h_q + h_kv:]
+    out = paged_step(**x, softcap=cap or None, slopes=slopes.to(dev) if bias else None, max_new=300, max_len=300, check=True)
+    for b, at, m, (value, bound) in _expect(s, keys, seqs, cap, slopes):
+        check(out[at:at + m], value, bound, f"sequence {b}")
+    for b, (m, c) in enumerate(seqs):  # and they are in their pages
+        j = torch.arange(c + m)
+        for pool, want in zip((x["k_pages"], x["v_pages"]), keys[b]):
+            got = pool.cpu()[s["table"][b].long()[j // page], j % page]
+            assert torch.equal(got, want)
+
+
 def test_values_in_unwritten_rows(dev):
     """_batch leaves NaN in rows of the pages that hold no key: the outputs are finite (test_step);
     a NaN that a sequence does hold reaches its tokens and no other sequence's."""
