@@ -161,11 +161,12 @@ __device__ __forceinline__ float row_dot(const T* a, const T* b, int d) {
   return s;
 }
 
+// A score (log2 units) of one pair.
 template <typename T>
 __device__ __forceinline__ float rule_of(const ScoreRule& r, float dot, float slope, int pos, int j) {
-  float x = dot * r.c1;
-  if (r.cap) x = r.c2 * cap_tanh<T>(x);
-  return x - slope * fabsf(static_cast<float>(j - pos));
+  const float dist = static_cast<float>(j - pos);
+  if (sizeof(T) == 2 && r.cap == kSeries) return Rule<T, kFar>(r).z(r, dot, slope, dist);
+  return Rule<T, kBias>(r).z(r, dot, slope, dist);
 }
 
 // One row by one wave, key by key, touching visible keys only.  Lane e holds
@@ -350,7 +351,7 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
   }
   const bool some = real && hi > lo;
   const Rule<T, RULE> rule(p.rule);
-  const float slope = RULE == kBias && real ? p.rule.slopes[hq] * kLog2e : 0.0f;
+  const float slope = has_bias(RULE) && real ? slope_of(p.rule, hq) : 0.0f;
   const int lo_min = wave_min_i(some ? lo : 0x7FFFFFFF), hi_max = wave_max_i(some ? hi : 0);
   const int lo_max = wave_max_i(real ? lo : 0), hi_min = wave_min_i(real ? hi : 0x7FFFFFFF);
   if (lane == 0) {

@@ -86,11 +86,14 @@ int launch_kw(DenseParams& p, int kw, hipStream_t st) {
 
 template <typename T, int D>
 int launch_rule(DenseParams& p, int kw, hipStream_t st) {
-  switch (rule_kind(p.rule)) {
+  switch (rule_kind<T>(p.rule)) {
     case kPlain: return launch_kw<T, D, kPlain>(p, kw, st);
     case kCap: return launch_kw<T, D, kCap>(p, kw, st);
-    default: return launch_kw<T, D, kBias>(p, kw, st);
+    case kBias: return launch_kw<T, D, kBias>(p, kw, st);
+    case kFar:
+      if constexpr (sizeof(T) == 2) return launch_kw<T, D, kFar>(p, kw, st);
   }
+  return fail(SSA_ERR_UNSUPPORTED, "no kernel for this rule of scores");
 }
 
 }  // namespace
@@ -172,7 +175,7 @@ int score_rule(const char* fn, float scale_div, float softcap, const float* slop
     return fail(SSA_ERR_INVALID_ARGUMENT, "%s: scale_div must be positive and finite", fn);
   if (!(softcap >= 0.0f) || !isfinite(softcap))
     return fail(SSA_ERR_INVALID_ARGUMENT, "%s: softcap must be finite and not negative (0: none)", fn);
-  r->cap = softcap > 0.0f;
+  r->cap = softcap > tile::kMostDirectCap ? tile::kSeries : (softcap > 0.0f ? tile::kDirect : tile::kNoCap);
   r->c1 = r->cap ? static_cast<float>(1.0 / (static_cast<double>(scale_div) * softcap))
                  : static_cast<float>(1.4426950408889634074 / scale_div);
   r->c2 = static_cast<float>(1.4426950408889634074 * softcap);

@@ -73,6 +73,7 @@ __device__ __forceinline__ int2 row_span(const BwdParams& p, int b, int tok) {
 // x (log2 units) and 1 - t^2 of a raw product, one pair at a time.
 template <typename T>
 __device__ __forceinline__ float score_x(const ScoreRule& r, float dot, float slope, float dist, float& factor) {
+  if (sizeof(T) == 2 && r.cap == kSeries) return Rule<T, kFar>(r).z(r, dot, slope, dist, factor);
   return Rule<T, kBias>(r).z(r, dot, slope, dist, factor);
 }
 
@@ -137,7 +138,7 @@ __global__ __launch_bounds__(kThreads, (dq_lds<T, D, KW>() > 80 * 1024 || (sizeo
   const int lo = sp.x, hi = sp.y;
   const bool some = real && hi > lo;
   const Rule<T, RULE> rule(p.rule);
-  const float slope = RULE == kBias && real ? p.rule.slopes[hq] * kLog2e : 0.0f;
+  const float slope = has_bias(RULE) && real ? slope_of(p.rule, hq) : 0.0f;
   const int lo_min = wave_min_i(some ? lo : 0x7FFFFFFF), hi_max = wave_max_i(some ? hi : 0);
   const int lo_max = wave_max_i(real ? lo : 0), hi_min = wave_min_i(real ? hi : 0x7FFFFFFF);
   if (lane == 0) {
@@ -478,8 +479,8 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
       const uint32_t r = min(t * QT + tid, n_rows - 1);
       const uint32_t tok = r / static_cast<uint32_t>(p.g), hq = kvh * p.g + r - tok * p.g;
       st = p.stats[(static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok];
-      if constexpr (RULE == kBias) {
-        st_slope = p.rule.slopes[hq] * kLog2e;
+      if constexpr (has_bias(RULE)) {
+        st_slope = slope_of(p.rule, hq);
         st_pos = static_cast<float>(static_cast<int>(p.q_pos0 + tok));
       }
     }
@@ -500,7 +501,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
       s_dsum[buf][tid] = st.y;
       s_lo[buf][tid] = in ? __float_as_int(st.z) : 0;
       s_hi[buf][tid] = in ? __float_as_int(st.w) : 0;
-      if constexpr (RULE == kBias) {
+      if constexpr (has_bias(RULE)) {
         s_slope[buf][tid] = st_slope;
         s_pos[buf][tid] = st_pos;
       }
@@ -554,7 +555,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
         const float4 ls = *reinterpret_cast<const float4*>(&s_lse[buf][r0]);
         const float4 dd = *reinterpret_cast<const float4*>(&s_dsum[buf][r0]);
         float4 sl = make_float4(0.f, 0.f, 0.f, 0.f), ps = sl;
-        if constexpr (RULE == kBias) {
+        if constexpr (has_bias(RULE)) {
           sl = *reinterpret_cast<const float4*>(&s_slope[buf][r0]);
           ps = *reinterpret_cast<const float4*>(&s_pos[buf][r0]);
         }
@@ -687,7 +688,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
         see = kj >= sp.x && kj < sp.y;
         if (see) {
           const int64_t stat = (static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok;
-          const float sl = RULE == kBias ? p.rule.slopes[hq] * kLog2e : 0.0f;
+          const float sl = has_bias(RULE) ? slope_of(p.rule, hq) : 0.0f;
           float f;
           const float x = score_x<T>(p.rule, row_dot(qall + tok * p.q_sn + hq * p.q_sh, kr, p.d), sl,
                                            static_cast<float>(kj) - static_cast<float>(static_cast<int>(p.q_pos0) + tok), f);
@@ -840,11 +841,14 @@ int launch_bwd(BwdParams& p, const BwdCut& cut, hipStream_t st) {
 
 template <typename T, int D>
 int launch_rule(BwdParams& p, const BwdCut& cut, hipStream_t st) {
-  switch (rule_kind(p.rule)) {
+  switch (rule_kind<T>(p.rule)) {
     case kPlain: return launch_bwd<T, D, kPlain>(p, cut, st);
     case kCap: return launch_bwd<T, D, kCap>(p, cut, st);
-    default: return launch_bwd<T, D, kBias>(p, cut, st);
+    case kBias: return launch_bwd<T, D, kBias>(p, cut, st);
+    case kFar:
+      if constexpr (sizeof(T) == 2) return launch_bwd<T, D, kFar>(p, cut, st);
   }
+  return fail(SSA_ERR_UNSUPPORTED, "no kernel for this rule of scores");
 }
 
 }  // namespace

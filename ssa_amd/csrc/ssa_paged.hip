@@ -104,7 +104,7 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
   const int hq = kvh * p.g + (real ? rr - tok * p.g : 0);
   const int pos = sq.len - sq.m + tok;
   const Rule<T, RULE> rule(p.rule);
-  const float slope = RULE == kBias && real ? p.rule.slopes[hq] * kLog2e : 0.0f;
+  const float slope = has_bias(RULE) && real ? slope_of(p.rule, hq) : 0.0f;
   const T* qrow = static_cast<const T*>(p.q) + (sq.first + tok) * p.q_sn + hq * p.q_sh;
   Frag qf[NC];
 #pragma unroll
@@ -250,7 +250,7 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
   for (int r = wave; r < R; r += 4) {  // rows to compute again, key by key
     if (!(s_bad[0][r] | s_bad[1][r] | s_bad[2][r] | s_bad[3][r])) continue;
     const int t = r / p.g, h = kvh * p.g + r - t * p.g, ps = sq.len - sq.m + t;
-    const float sl = RULE == kBias ? p.rule.slopes[h] * kLog2e : 0.0f;
+    const float sl = has_bias(RULE) ? slope_of(p.rule, h) : 0.0f;
     float o[4], m, l;
     exact_row<T, true>(rows, p.rule, static_cast<const T*>(p.q) + (sq.first + t) * p.q_sn + h * p.q_sh, p.d, k_begin,
                        min(k_end, ps + 1), sl, ps, o, m, l);
@@ -479,11 +479,14 @@ int launch_kw(DenseParams& p, const PagedPlan& l, char* ws, hipStream_t st) {
 
 template <typename T, int D>
 int launch_rule(DenseParams& p, const PagedPlan& l, char* ws, hipStream_t st) {
-  switch (rule_kind(p.rule)) {
+  switch (rule_kind<T>(p.rule)) {
     case kPlain: return launch_kw<T, D, kPlain>(p, l, ws, st);
     case kCap: return launch_kw<T, D, kCap>(p, l, ws, st);
-    default: return launch_kw<T, D, kBias>(p, l, ws, st);
+    case kBias: return launch_kw<T, D, kBias>(p, l, ws, st);
+    case kFar:
+      if constexpr (sizeof(T) == 2) return launch_kw<T, D, kFar>(p, l, ws, st);
   }
+  return fail(SSA_ERR_UNSUPPORTED, "no kernel for this rule of scores");
 }
 
 }  // namespace

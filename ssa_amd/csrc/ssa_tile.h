@@ -265,18 +265,34 @@ __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0
 // slope already carries log2(e).
 struct ScoreRule {
   float c1, c2;
-  int cap;              // scores go through the tanh
+  int cap;              // scores go through the tanh: kDirect or kSeries of bf16's
   const float* slopes;  // null, or [h_q]
 };
+enum CapKind { kNoCap = 0, kDirect = 1, kSeries = 2 };
 
-// tanh for the bf16 kernels: 1 - 2 / (exp(2y) + 1), absolute error about 2^-22
-// (v_exp_f32 and v_rcp_f32 are good to an ulp), far below a bf16 weight's
-// 2^-8.  The fp32 kernels take the library's.
-template <typename T>
+// tanh for the bf16 kernels.  kDirect: 1 - 2 / (exp(2y) + 1), off by 2^-22 (v_exp_f32 and
+// v_rcp_f32 are good to an ulp), which puts a score and its weight off by c 2^-22: up to
+// kMostDirectCap no more than 2^-12, a sixteenth of what rounding the weight to bf16 may
+// leave.  kSeries, for larger caps, is good to a relative 2^-20, so that c tanh(s / c)
+// keeps s however large c is: below 1/4 the series to y^7 (the first term left out is
+// 62 / 2835 y^9), from there on the same as kDirect (8192 causal rows, 32 / 8 heads, d = 64,
+// caps of 1025 and 1024: 745 us against 545, backward 2180 against 1610).  The fp32 kernels
+// take the library's.
+constexpr float kMostDirectCap = 1024.0f;
+
+template <typename T, int CAP>
 __device__ __forceinline__ float cap_tanh(float y) {
   if constexpr (sizeof(T) == 4) return tanhf(y);
   const float e = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e));
-  return fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+  const float t = fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+  if constexpr (CAP == kDirect) return t;
+  const float w = y * y, u = fmaf(w, fmaf(w, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f);
+  return fabsf(y) < 0.25f ? fmaf(y * w, u, y) : t;
+}
+
+// The slope of a query head in log2 units (0: none).
+__device__ __forceinline__ float slope_of(const ScoreRule& r, int hq) {
+  return r.slopes != nullptr ? r.slopes[hq] * kLog2e : 0.0f;
 }
 
 // What the kernels keep of a product until its weight: z with x = a z + b, a and b
@@ -286,7 +302,10 @@ __device__ __forceinline__ float cap_tanh(float y) {
 //   kCap    bf16: z = 1 / (exp(2y) + 1), of which tanh y = 1 - 2 z and
 //           1 - tanh^2 = 4 (z - z^2); larger scores have smaller z.  fp32: z = tanh y
 //   kBias   z = x (a distance bias, with or without a cap)
-enum RuleKind { kPlain = 0, kCap = 1, kBias = 2 };
+//   kFar    bf16: z = x, with a cap past kMostDirectCap and with or without a bias
+enum RuleKind { kPlain = 0, kCap = 1, kBias = 2, kFar = 3 };
+
+constexpr bool has_bias(int kind) { return kind == kBias || kind == kFar; }
 
 template <typename T, int KIND>
 struct Rule {
@@ -301,22 +320,25 @@ struct Rule {
     a = KIND == kPlain ? r.c1 : (kDown ? -2.0f * r.c2 : (KIND == kCap ? r.c2 : 1.0f));
     b = kDown ? r.c2 : 0.0f;
   }
-  // dist: |position - key| or its negative (kBias)
+  // dist: |position - key| or its negative (kBias, kFar)
   __device__ __forceinline__ float z(const ScoreRule& r, float dot, float slope, float dist) const {
     if constexpr (KIND == kPlain) return dot;
     if constexpr (kDown) return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * c) + 1.0f);
     if constexpr (KIND == kCap) return tanhf(dot * c);
     float x = dot * c;
-    if (r.cap) x = r.c2 * cap_tanh<T>(x);
+    if constexpr (KIND == kFar)
+      x = r.c2 * cap_tanh<T, kSeries>(x);
+    else if (r.cap)
+      x = r.c2 * cap_tanh<T, kDirect>(x);
     return fmaf(-slope, fabsf(dist), x);
   }
   // z, and the gradient's factor over kSlopeUnit
   __device__ __forceinline__ float z(const ScoreRule& r, float dot, float slope, float dist, float& f) const {
     f = 1.0f;
-    if constexpr (KIND == kBias) {
+    if constexpr (has_bias(KIND)) {
       float x = dot * c;
-      if (r.cap) {
-        const float t = cap_tanh<T>(x);
+      if (KIND == kFar || r.cap) {
+        const float t = cap_tanh<T, KIND == kFar ? kSeries : kDirect>(x);
         f = fmaf(-t, t, 1.0f);
         x = r.c2 * t;
       }
@@ -330,7 +352,11 @@ struct Rule {
   static __device__ __forceinline__ float better(float x, float y) { return kDown ? fminf(x, y) : fmaxf(x, y); }
 };
 
-inline RuleKind rule_kind(const ScoreRule& r) { return r.slopes != nullptr ? kBias : (r.cap ? kCap : kPlain); }
+template <typename T>
+RuleKind rule_kind(const ScoreRule& r) {
+  if (sizeof(T) == 2 && r.cap == kSeries) return kFar;
+  return r.slopes != nullptr ? kBias : (r.cap ? kCap : kPlain);
+}
 
 // exp2 of a difference of scores: the instruction's (an ulp; a result below
 // 2^-126 is 0, a weight that no fp32 sum of weights up to 1 can hold).

@@ -34,9 +34,10 @@ def spans_of(n, n_q, q_pos0, causal=True, starts=None, prefix=None):
     return torch.tensor(rows, dtype=torch.int32).reshape(n_q, 2)
 
 
-def attend(q, k, v, spans, cap=0.0, slopes=None, q_pos0=0, dout=None, scale=None, round_to=None):
+def attend(q, k, v, spans, cap=0.0, slopes=None, q_pos0=0, dout=None, scale=None, round_to=None, cap_rel=None):
     """One sequence: q [m, h_q, d], k, v [n, h_kv, d] (any dtype), spans [m, 2].  Returns
-    {"out": (value, bound), ...} with dq, dk and dv too where dout is given."""
+    {"out": (value, bound), ...} with dq, dk and dv too where dout is given.  ``cap_rel``: how
+    far a capped score may be off relative to itself, in place of cap 2^-21."""
     r = 0.0 if (round_to or q.dtype) == torch.float32 else 2.0 ** -8
     m, h_q, d = q.shape
     n, h_kv = k.shape[0], k.shape[1]
@@ -65,7 +66,7 @@ def attend(q, k, v, spans, cap=0.0, slopes=None, q_pos0=0, dout=None, scale=None
         t = torch.tanh(raw / cap) if cap else torch.zeros_like(raw)
         s = cap * t if cap else raw
         if cap:
-            ds_bound = ds_bound + cap * 2.0 ** -21
+            ds_bound = ds_bound + (cap * 2.0 ** -21 if cap_rel is None else cap_rel * s.abs())
         if slopes is not None:
             far = (pos[:, None] - j[None]).abs().double()
             s = s - float(slopes[h]) * far
