@@ -457,8 +457,9 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
 
   const int sc = tid % NCH, sr = tid / NCH;
   const bool chunk_ok = sc * E < p.d;
-  const T* qbase = static_cast<const T*>(p.q) + b * p.q_sb;
-  const T* dbase = static_cast<const T*>(p.dout) + b * p.do_sb;
+  // (the group's first head: 32-bit offsets step over a tile's tokens and the group's heads only)
+  const T* qbase = static_cast<const T*>(p.q) + b * p.q_sb + kvh * p.g * p.q_sh;
+  const T* dbase = static_cast<const T*>(p.dout) + b * p.do_sb + kvh * p.g * p.do_sh;
   const uint32_t qs = static_cast<uint32_t>(p.q_sn * O::kEsize), qh = static_cast<uint32_t>(p.q_sh * O::kEsize);
   const uint32_t ds = static_cast<uint32_t>(p.do_sn * O::kEsize), dh = static_cast<uint32_t>(p.do_sh * O::kEsize);
   uint4 qreg[NP], dreg[NP];
@@ -471,9 +472,9 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const uint32_t r = min(t * QT + min(sr + i * RPP, QT - 1), n_rows - 1);
-      const uint32_t tok = r / static_cast<uint32_t>(p.g), hq = kvh * p.g + r - tok * p.g;
-      qreg[i] = row_load(qb, chunk_ok ? (tok - tok0) * qs + hq * qh + sc * 16 : kNoChunk);
-      dreg[i] = row_load(db, chunk_ok ? (tok - tok0) * ds + hq * dh + sc * 16 : kNoChunk);
+      const uint32_t tok = r / static_cast<uint32_t>(p.g), h = r - tok * p.g;
+      qreg[i] = row_load(qb, chunk_ok ? (tok - tok0) * qs + h * qh + sc * 16 : kNoChunk);
+      dreg[i] = row_load(db, chunk_ok ? (tok - tok0) * ds + h * dh + sc * 16 : kNoChunk);
     }
     if (tid < QT) {
       const uint32_t r = min(t * QT + tid, n_rows - 1);

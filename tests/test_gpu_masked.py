@@ -363,3 +363,25 @@ def test_far_rows(dev, dtype, d):
     grads = torch.autograd.grad(out, leaves, far[3])
     res = dict(zip(("out", "dq", "dk", "dv"), (out, *grads)))
     _check(res, q, k, v, dout, spans_of(n, n, 0)[None], 0.0, None, 0)
+
+
+@pytest.mark.parametrize("dtype,d,g", [(F32, 64, 1), (BF16, 64, 4), (BF16, 128, 16)], ids=str)
+def test_far_heads(dev, dtype, d, g):
+    """Heads of q, k, v and dout 16 MiB apart, 144 of them: offsets past 2^31 bytes of a row."""
+    from ssa_amd import masked_attention
+
+    n, h_q = 70, 144
+    q, k, v, dout = _inputs(16, dtype, 1, n, n, h_q, h_q // g, d)
+    step = (16 << 20) // q.element_size()
+    pool = torch.zeros((h_q - 1) * step + 4 * n * d, device=dev, dtype=dtype)
+    assert (h_q - 1) * step * q.element_size() > 1 << 31
+    far = []
+    for i, t in enumerate((q, k, v, dout)):
+        x = torch.as_strided(pool, t.shape, (0, d, step, 1), i * n * d)
+        x.copy_(t)
+        far.append(x)
+    leaves = [t.detach().requires_grad_(True) for t in far[:3]]
+    out = masked_attention(*leaves)
+    grads = torch.autograd.grad(out, leaves, far[3])
+    res = dict(zip(("out", "dq", "dk", "dv"), (out, *grads)))
+    _check(res, q, k, v, dout, spans_of(n, n, 0)[None], 0.0, None, 0)
