@@ -464,7 +464,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
   const uint32_t ds = static_cast<uint32_t>(p.do_sn * O::kEsize), dh = static_cast<uint32_t>(p.do_sh * O::kEsize);
   uint4 qreg[NP], dreg[NP];
   float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-  float st_slope = 0.0f, st_pos = 0.0f;
+  float st_slope = 0.0f, st_pos = 0.0f;  // (positions count from the block's first key: past 2^24 a float holds no odd one)
   auto load_rows = [&](int t) {
     // offsets from the tile's first token
     const uint32_t tok0 = static_cast<uint32_t>(t * QT) / static_cast<uint32_t>(p.g);
@@ -482,7 +482,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
       st = p.stats[(static_cast<int64_t>(b) * p.h_q + hq) * p.n_q + tok];
       if constexpr (has_bias(RULE)) {
         st_slope = slope_of(p.rule, hq);
-        st_pos = static_cast<float>(static_cast<int>(p.q_pos0 + tok));
+        st_pos = static_cast<float>(static_cast<int>(p.q_pos0 + tok) - kb0);
       }
     }
   };
@@ -549,7 +549,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
         }
       }
       const bool whole = cur.lo_max[u] <= kw0 && cur.hi_min[u] >= kw0 + 32 && cur.tile * QT + row0 + 32 <= n_rows;
-      const float fkey = static_cast<float>(key);
+      const float fkey = static_cast<float>(key - kb0);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r0 = row0 + 8 * e + 4 * half;
@@ -692,7 +692,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
           const float sl = has_bias(RULE) ? slope_of(p.rule, hq) : 0.0f;
           float f;
           const float x = score_x<T>(p.rule, row_dot(qall + tok * p.q_sn + hq * p.q_sh, kr, p.d), sl,
-                                           static_cast<float>(kj) - static_cast<float>(static_cast<int>(p.q_pos0) + tok), f);
+                                           static_cast<float>(kj - (static_cast<int>(p.q_pos0) + tok)), f);
           const float4 rs = p.stats[stat];
           w = exp2_w(x - rs.x);
           ds = w * (row_dot(dall + tok * p.do_sn + hq * p.do_sh, vr, p.d) - rs.y) * f;

@@ -385,3 +385,28 @@ def test_far_heads(dev, dtype, d, g):
     grads = torch.autograd.grad(out, leaves, far[3])
     res = dict(zip(("out", "dq", "dk", "dv"), (out, *grads)))
     _check(res, q, k, v, dout, spans_of(n, n, 0)[None], 0.0, None, 0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("bad", [0.0, math.nan])
+def test_distances_past_2_to_the_24(dev, dtype, bad):
+    """A few rows and keys behind 2^24 others: the distance between them is exact in the
+    gradients as in the output, also where a hidden row's NaN has a key's sums formed pair by pair."""
+    from ssa_amd import masked_attention
+
+    far, n_q, n, h_q, h_kv, d = (1 << 24) + 3, 40, 45, 2, 1, 8
+    q, k, v, dout = _inputs(18, dtype, 1, n_q, n, h_q, h_kv, d)
+    spans = spans_of(n, n_q, n - n_q, starts=[0, 30, n])
+    spans[3] = 0
+    if bad != bad:
+        q[0, 3], dout[0, 3] = bad, bad
+    slopes = torch.tensor([1.0, 0.5])
+    pool = torch.zeros(2, 1, far + n, h_kv, d, device=dev, dtype=dtype)
+    pool[0, :, far:], pool[1, :, far:] = k.to(dev), v.to(dev)
+    leaves = [t.detach().requires_grad_(True) for t in (q.to(dev), pool[0], pool[1])]
+    moved = torch.where(spans[:, 1:] > 0, spans + far, spans)[None].to(dev)
+    out = masked_attention(*leaves, moved, slopes=slopes.to(dev))
+    dq, dk, dv = torch.autograd.grad(out, leaves, dout.to(dev))
+    assert not dk[:, :far].any() and not dv[:, :far].any()
+    res = {"out": out, "dq": dq, "dk": dk[:, far:], "dv": dv[:, far:]}
+    _check(res, q, k, v, dout, spans[None], 0.0, slopes, n - n_q)
