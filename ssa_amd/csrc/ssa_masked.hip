@@ -199,9 +199,9 @@ int check_aligned(const char* fn, const char* name, int dtype, const void* ptr, 
   const int64_t e = dtype == SSA_DTYPE_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0 || (s0 * e) % 16 != 0 || (s1 * e) % 16 != 0 || (s2 * e) % 16 != 0)
     return fail(SSA_ERR_UNSUPPORTED, "%s: %s must have rows aligned to 16 bytes", fn, name);
-  // (a tile's 64 rows, or the heads of a token, are addressed by 32-bit offsets)
-  if (s1 < 0 || s2 < 0 || s1 * e > tile::kMostRowBytes || s2 * e > tile::kMostRowBytes)
-    return fail(SSA_ERR_UNSUPPORTED, "%s: %s must have row and head strides of 0 to %lld bytes", fn, name,
+  // (a tile's rows are addressed by 32-bit offsets, heads by 64-bit pointers)
+  if (s1 < 0 || s2 < 0 || s1 > tile::kMostRowBytes / e)
+    return fail(SSA_ERR_UNSUPPORTED, "%s: %s must have row strides of 0 to %lld bytes, and head strides from 0", fn, name,
                 (long long)tile::kMostRowBytes);
   return SSA_OK;
 }

@@ -70,6 +70,15 @@ __device__ __forceinline__ int2 row_span(const BwdParams& p, int b, int tok) {
   return hi > lo ? make_int2(lo, hi) : make_int2(0, 0);
 }
 
+// dkv_kernel's offsets of a tile's 128 packed rows, ceil(127 / g) tokens and g - 1 heads from
+// the first one's, have to stay within its resource.
+int check_group(const char* fn, const char* name, int dtype, int g, int d, int64_t sn, int64_t sh) {
+  const int64_t e = dtype == SSA_DTYPE_F32 ? 4 : 2, room = kAllBytes / e - d - (126 + g) / g * sn;
+  if (g > 1 && sh > room / (g - 1))
+    return fail(SSA_ERR_UNSUPPORTED, "%s: the heads of a group of %s must lie within 2 GiB", fn, name);
+  return SSA_OK;
+}
+
 // x (log2 units) and 1 - t^2 of a raw product, one pair at a time.
 template <typename T>
 __device__ __forceinline__ float score_x(const ScoreRule& r, float dot, float slope, float dist, float& factor) {
@@ -894,6 +903,8 @@ extern "C" int ssa_masked_attention_backward(
   if (int rc = check_aligned(fn, "dq", dtype, dq, 0, 0, 0)) return rc;
   if (int rc = check_aligned(fn, "dk", dtype, dk, 0, 0, 0)) return rc;
   if (int rc = check_aligned(fn, "dv", dtype, dv, 0, 0, 0)) return rc;
+  if (int rc = check_group(fn, "q", dtype, h_q / h_kv, d, q_sn, q_sh)) return rc;
+  if (int rc = check_group(fn, "dout", dtype, h_q / h_kv, d, do_sn, do_sh)) return rc;
   const BwdCut l = bwd_cut(dtype, batch, n, n_q, h_q, h_kv, d);
   if (workspace == nullptr || workspace_bytes < l.bytes)
     return fail(SSA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", fn, l.bytes,

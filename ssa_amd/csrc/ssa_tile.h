@@ -178,9 +178,7 @@ struct Op<float> {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kNoChunk = 0x80000000u;     // an offset past any resource
 constexpr int kAllBytes = 0x7FFFFFF0;          // a resource whose rows all exist
-// Of a row or head stride: the offsets of a tile's 128 rows stay below kAllBytes, and so do
-// those of 128 (token, head) rows of a group of g heads, ceil(127 / g) tokens and g - 1 heads.
-constexpr int64_t kMostRowBytes = 1 << 24;
+constexpr int64_t kMostRowBytes = 1 << 24;     // of a row stride: the offsets of a tile's 128 rows stay below kAllBytes
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* base, int bytes) {
   // (word 3: raw 32-bit data)

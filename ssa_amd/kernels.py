@@ -516,6 +516,17 @@ def _rows16(t: torch.Tensor):
     return t, (h * d, d)
 
 
+def _group_rows16(t: torch.Tensor, g: int):
+    """``_rows16`` of q or dout [B, n, heads, d] for the backward, which wants the heads of a group
+    of g within 2 GiB: a contiguous copy where they lie further apart."""
+    t, st = _rows16(t)
+    _, _, h, d = t.shape
+    if ((126 + g) // g * st[1] + (g - 1) * st[2] + d) * t.element_size() > 0x7FFFFFF0:
+        n = t.shape[1]
+        return t.contiguous(), (n * h * d, h * d, d)
+    return t, st
+
+
 @functools.lru_cache(maxsize=1024)
 def _bytes(name: str, *sizes) -> int:
     return int(getattr(_lib.load(), name)(*sizes))
@@ -630,11 +641,11 @@ def masked_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    q, qs = _rows16(q)
+    q, qs = _group_rows16(q, h_q // h_kv)
     k, ks = _rows16(k)
     v, vs = _rows16(v)
     out, os = _rows16(out)
-    dout, dos = _rows16(dout)
+    dout, dos = _group_rows16(dout, h_q // h_kv)
     out_low = None if out_low is None else _rows16(out_low)[0]
     dt = _lib.elem_dtype(q)
     nbytes = _bytes("ssa_masked_attention_backward_workspace_bytes", dt, B, n, n_q, h_q, h_kv, d)

@@ -172,3 +172,21 @@ def test_python_refuses_host_tensors():
         ssa_amd.rope_axes(q, q, ints[None], ssa_amd.axis_rope_freqs(8), (4,))
     with pytest.raises(ValueError, match="prefix_lens"):
         ssa_amd.mask_spans(4, 1, causal=False, prefix_lens=ints)
+
+
+def test_heads_far_apart(L):
+    """Head strides are 64-bit: what refuses these calls is the missing workspace.  The backward
+    wants a group's heads within 2 GiB."""
+    far = {f"{x}_sh": 1 << 33 for x in "qkv"}
+    st, msg = _call(L, "ssa_masked_attention", FORWARD, dict(far, n=4000, n_q=4, o_sh=1 << 33, ws=None))
+    assert st == WORKSPACE, msg
+    st, msg = _call(L, "ssa_paged_step", PAGED, dict({f"{x}_sh": 1 << 33 for x in ("q", "k", "v", "kp", "vp", "o")}, ws=None))
+    assert st == WORKSPACE, msg
+    room = (0x7FFFFFF0 // 2 - 64 - 32 * 512) // 3  # g = 4: 32 tokens and 3 heads from the tile's first row
+    for x in ("q", "do"):
+        st, msg = _call(L, "ssa_masked_attention_backward", BACKWARD, {f"{x}_sh": room // 8 * 8, "ws": None})
+        assert st == WORKSPACE, msg
+        st, msg = _call(L, "ssa_masked_attention_backward", BACKWARD, {f"{x}_sh": room // 8 * 8 + 8, "ws": None})
+        assert st == UNSUPPORTED and "2 GiB" in msg, msg
+    st, msg = _call(L, "ssa_masked_attention_backward", BACKWARD, dict(h_q=2, q_sh=1 << 40, do_sh=1 << 40, ws=None))
+    assert st == WORKSPACE, msg

@@ -410,3 +410,25 @@ def test_distances_past_2_to_the_24(dev, dtype, bad):
     assert not dk[:, :far].any() and not dv[:, :far].any()
     res = {"out": out, "dq": dq, "dk": dk[:, far:], "dv": dv[:, far:]}
     _check(res, q, k, v, dout, spans[None], 0.0, slopes, n - n_q)
+
+
+@pytest.mark.parametrize("dtype,d,h_q,g,apart", [(F32, 64, 6, 2, 40), (BF16, 128, 8, 4, 100), (BF16, 64, 32, 16, 160)], ids=str)
+def test_heads_of_long_sequences(dev, dtype, d, h_q, g, apart):
+    """Heads ``apart`` MiB from each other, as views [B, n, h, d] of [B, h, n, d] have them past
+    65536 tokens; in the last case a group's heads lie further apart than the backward reads them."""
+    from ssa_amd import masked_attention
+
+    n = 70
+    q, k, v, dout = _inputs(19, dtype, 1, n, n, h_q, h_q // g, d)
+    step = (apart << 20) // q.element_size()
+    pool = torch.zeros((h_q - 1) * step + 4 * n * d, device=dev, dtype=dtype)
+    far = []
+    for i, t in enumerate((q, k, v, dout)):
+        x = torch.as_strided(pool, t.shape, (0, d, step, 1), i * n * d)
+        x.copy_(t)
+        far.append(x)
+    leaves = [t.detach().requires_grad_(True) for t in far[:3]]
+    out = masked_attention(*leaves)
+    grads = torch.autograd.grad(out, leaves, far[3])
+    res = dict(zip(("out", "dq", "dk", "dv"), (out, *grads)))
+    _check(res, q, k, v, dout, spans_of(n, n, 0)[None], 0.0, None, 0)

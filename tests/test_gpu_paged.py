@@ -347,3 +347,24 @@ def test_cache_and_the_operators_together(dev, dtype):
     assert cache.free_pages == 16
     with pytest.raises(ValueError, match="not open"):
         cache.step(*data[0], [seqs[0]], [n])
+
+
+@pytest.mark.parametrize("m", [1, 50])
+def test_pools_with_whole_heads_apart(dev, m):
+    """Pools as [h_kv, pages, page, d] and rows as [h, T, d]: heads more than 16 MiB apart."""
+    from ssa_amd import paged_step
+
+    h_q, h_kv, d, page = 4, 2, 64, 16
+    s, keys = _batch(43, BF16, [(m, 100), (m, 30)], h_q, h_kv, d, page)
+    x = {n: t.to(dev) for n, t in s.items()}
+    want = paged_step(**{**x, "k_pages": x["k_pages"].clone(), "v_pages": x["v_pages"].clone()})
+    step = (40 << 20) // 2
+    for n in ("k_pages", "v_pages"):
+        pool = torch.zeros(h_kv * step, device=dev, dtype=BF16)
+        pages = torch.as_strided(pool, x[n].shape, (page * d, d, step, 1))
+        x[n] = pages.copy_(x[n])
+    for n in ("q", "k", "v"):
+        rows = torch.zeros(h_q * step, device=dev, dtype=BF16)
+        x[n] = torch.as_strided(rows, x[n].shape, (d, step, 1)).copy_(x[n])
+    out = torch.as_strided(torch.zeros(h_q * step, device=dev, dtype=BF16), x["q"].shape, (d, step, 1))
+    assert torch.equal(paged_step(**x, out=out, check=True), want)
