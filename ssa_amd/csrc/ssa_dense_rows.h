@@ -564,17 +564,20 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
     }
   };
   const bool here = some && max(lo, part_lo) < min(hi, part_hi);
-  // no key: zeros; only keys of score -inf: NaN, as a softmax of them is
+  // no key: zeros, whatever hidden values its tiles' sums met; only keys of score -inf: NaN,
+  // as a softmax of them is
   if constexpr (KW == 1) {
     const bool again = some && worst != 0.0f;
     if (real && !again) {
-      const float inv = p.splits > 1 ? 1.0f : (some ? 1.0f / lsum : 0.0f);
+      const float inv = p.splits > 1 ? 1.0f : 1.0f / lsum;
 #pragma unroll
       for (int i = 0; i < ND; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int dd = 32 * i + 8 * e + 4 * half;
-          if (dd < p.d) put(tok, hq, dd, acc[i][4 * e] * inv, acc[i][4 * e + 1] * inv, acc[i][4 * e + 2] * inv, acc[i][4 * e + 3] * inv);
+          if (dd < p.d)
+            put(tok, hq, dd, some ? acc[i][4 * e] * inv : 0.0f, some ? acc[i][4 * e + 1] * inv : 0.0f,
+                some ? acc[i][4 * e + 2] * inv : 0.0f, some ? acc[i][4 * e + 3] * inv : 0.0f);
         }
       if (half == 0) put_sums(tok, hq, mref, lsum, some, here);
     }
@@ -620,9 +623,10 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
         o.w = fmaf(a, v.w, o.w);
       }
       const int tk = rx / p.g, h = kvh * p.g + rx - tk * p.g;
-      const float inv = p.splits > 1 ? 1.0f : ((flag & 2) ? 1.0f / l : 0.0f);
-      put(tk, h, dd, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-      if (dd == 0) put_sums(tk, h, mm, l, (flag & 2) != 0, (flag & 4) != 0);
+      const float inv = p.splits > 1 ? 1.0f : 1.0f / l;
+      const bool any = (flag & 2) != 0;
+      put(tk, h, dd, any ? o.x * inv : 0.0f, any ? o.y * inv : 0.0f, any ? o.z * inv : 0.0f, any ? o.w * inv : 0.0f);
+      if (dd == 0) put_sums(tk, h, mm, l, any, (flag & 4) != 0);
     }
     int bad = 0;
 #pragma unroll

@@ -432,3 +432,25 @@ def test_heads_of_long_sequences(dev, dtype, d, h_q, g, apart):
     grads = torch.autograd.grad(out, leaves, far[3])
     res = dict(zip(("out", "dq", "dk", "dv"), (out, *grads)))
     _check(res, q, k, v, dout, spans_of(n, n, 0)[None], 0.0, None, 0)
+
+
+@pytest.mark.parametrize("dtype,d", [(F32, 64), (BF16, 64), (BF16, 128)], ids=str)
+@pytest.mark.parametrize("cap", [0.0, 3.0])
+def test_rows_without_keys_beside_hidden_values(dev, dtype, d, cap):
+    """Rows that see nothing are zeros also where they share a tile with rows that see keys, and
+    that tile holds hidden values that are not finite.  Few heads and many: waves that share
+    rows, and that do not; few rows over many keys: parts."""
+    for h_kv, n, n_q in ((2, 150, 150), (270, 150, 150), (2, 1600, 21)):
+        q, k, v, dout = _inputs(21, dtype, 1, n_q, n, 2 * h_kv, h_kv, d)
+        p0 = n - n_q
+        spans = spans_of(n, n_q, p0, starts=[0, n - n_q // 2])
+        dead = spans[:, 0] == spans[:, 1]
+        k[0, n - n_q // 2:], v[0, n - n_q // 2:] = math.nan, math.inf
+        q[0, dead], dout[0, dead] = math.inf, math.nan
+        res = _run(dev, q, k, v, dout, spans[None], cap)
+        assert dead.any() and not dead.all()
+        assert (res["out"].cpu()[0, dead] == 0).all() and (res["dq"].cpu()[0, dead] == 0).all()
+        few = slice(0, 4), slice(0, 2)
+        want = attend(q[0, :, few[0]], k[0, :, few[1]], v[0, :, few[1]], spans, cap, None, p0, dout[0, :, few[0]])
+        for name, (value, bound) in want.items():
+            check(res[name][0, :, few[0 if name in ("out", "dq") else 1]], value, bound, f"{name}, {h_kv} heads")
