@@ -62,11 +62,5 @@ struct ScoreRule;
 int check_heads(const char* fn, int dtype, int h_q, int h_kv, int d);
 int check_aligned(const char* fn, const char* name, int dtype, const void* ptr, int64_t s0, int64_t s1, int64_t s2);
 int score_rule(const char* fn, float scale_div, float softcap, const float* slopes, tile::ScoreRule* r);
-// How a dense forward of `rows` rows (tokens x heads of a group) of each of `heads`
-// KV heads over `keys` keys is cut: waves that share 32 rows, and parts of the keys.
-struct DenseSplit {
-  int kw, parts;
-};
-DenseSplit dense_split(int64_t rows, int64_t heads, int64_t keys, int64_t n_q, bool f32, bool wide, bool paged);
 
 }  // namespace ssa

@@ -4,6 +4,7 @@
 
 #include <math.h>
 
+#include "ssa_cuts.h"
 #include "ssa_dense_rows.h"
 #include "ssa_internal.h"
 
@@ -97,55 +98,6 @@ int launch_rule(DenseParams& p, int kw, hipStream_t st) {
 }
 
 }  // namespace
-
-DenseSplit dense_split(int64_t rows, int64_t heads, int64_t keys, int64_t n_q, bool f32, bool wide, bool paged) {
-  // Blocks of 128 rows, one wave a row, from 512 blocks on (two a CU).  Where they are
-  // fewer (us a call, both sides measured; of 120 calls of 700 to 5000 keys and 10 to
-  // 500 blocks the rule's cut is 4% slower than the best of 27 in the mean):
-  DenseSplit s{1, 1};
-  const int64_t blocks = ceil_div(rows, 128) * heads;
-  if (blocks <= 0 || blocks >= 512 || keys <= 32) return s;
-  // Two or four waves share each 32 rows and take turns at the keys (2500 causal rows of
-  // 8 / 2 heads, d = 64, 158 blocks: 40 with two, 32 with four; 1500 of 32 / 8, d = 128,
-  // 376 blocks: 54 with one or two, 67 with four).  Four read the keys four times as
-  // often as one; bf16 is bound by that over long ones (6000: twice as slow), fp32 never
-  // (4096 causal rows of 8 / 2 heads, d = 64: 194 with two, 187 with four).
-  const bool one_block = f32 && wide;  // a CU holds one block, of two waves a row at most
-  const int64_t four = f32 ? 256 : 176;
-  if (blocks < four && keys > 64 && (f32 || keys < 4096) && !one_block)
-    s.kw = 4;
-  else if (blocks < 400)
-    s.kw = 2;
-  // Parts of the keys, joined by a second launch.  They pay where the rows are few
-  // beside the keys, which each row then sees nearly all of; in a square causal or
-  // document mask most parts of a row are empty (1500 rows of 12 / 4 heads, d = 128:
-  // 35 in one part, 45 in three).  Long keys take as many parts as about 512 blocks
-  // allow, of 384 keys at least, and waves share rows only where those are few still
-  // (1200 x 8 rows over 16384 keys: 289 in one part, 138 in six); not two parts below
-  // 8192 keys, where the join costs more.  Shorter ones take parts only until the blocks
-  // fill the CUs once, of at least 384 keys (fp32 192: 140 x 4 rows of 2 heads over 700
-  // keys 30 and 24 in one and three parts; bf16 18.6 and 20.3).  Over pages, whose rows
-  // follow what is cached and whose tiles wait for their pages as well, half as long
-  // parts and twice as many pay (915 x 3 rows of 2 heads over 2470 keys: 68 in one part,
-  // 51 in three; 500 x 7 rows twice of 4 heads over 6500: 188 in three, 165 in four).
-  const bool chunk = paged || 2 * n_q <= keys;
-  int64_t want = 1, can = 1;
-  if (chunk && keys >= 4096) {
-    want = paged ? ceil_div(640, blocks) : (512 + blocks / 4) / blocks;
-    can = keys / 384;
-    if (!paged && (want < can ? want : can) == 2 && keys < 8192) want = 1;
-    const int64_t all = blocks * (want < can ? want : can);
-    s.kw = all > blocks && all >= 384 ? 1 : (paged && all < 64 && !one_block ? 4 : 2);
-  } else if (chunk || one_block) {
-    const int64_t all = blocks * s.kw;
-    want = ((paged ? 512 : 256) + all / 2) / all;
-    can = keys / (f32 || paged ? 192 : 384);
-  }
-  const int64_t parts = want < can ? want : can;
-  s.parts = parts > 1 ? static_cast<int>(parts) : 1;
-  return s;
-}
-
 }  // namespace ssa
 
 using namespace ssa;

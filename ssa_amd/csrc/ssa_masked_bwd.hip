@@ -31,6 +31,7 @@
 
 #include <math.h>
 
+#include "ssa_cuts.h"
 #include "ssa_internal.h"
 #include "ssa_tile.h"
 
@@ -758,49 +759,6 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(BwdParams p) {
     s.w += a.w;
   }
   Op<T>::store4(static_cast<T*>(isv ? p.dv : p.dk) + kid * p.d + dd, s.x, s.y, s.z, s.w);
-}
-
-// How a backward is cut, and its workspace: the rows' stats, the groups' bounds, and
-// the parts of dK and dV.
-struct BwdCut {
-  int kw, key_groups, splits, groups;
-  size_t stats, bounds, part, bytes;
-};
-
-BwdCut bwd_cut(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv, int d) {
-  BwdCut l{};
-  const int64_t rows = n_q * (h_q / h_kv), heads = batch * h_kv;
-  const bool f32 = dtype == SSA_DTYPE_F32, wide = d > 64;
-  l.groups = static_cast<int>(ceil_div(rows, 32));
-  // dQ: waves share rows where blocks of 128 are few, earlier than in the forward
-  // (no maximum to agree on): 1500 x 8 rows of 4 x 2 heads, 752 blocks, take the
-  // same with one wave a row and with two; 2048 x 7 of 4 heads, 448 blocks, 5% less
-  // with two; 4096 of 4 heads at d = 64, 128 blocks, 9% less with four.
-  const int64_t qblocks = ceil_div(rows, 128) * heads;
-  l.kw = qblocks >= 1024 || n <= 32 ? 1 : (qblocks >= 192 || n <= 64 || (f32 && wide) ? 2 : 4);
-  // dK, dV: blocks of 128 keys, their rows cut into parts until 512 blocks (two a CU
-  // where they fit; 1024 of the smaller ones of bf16 at d = 64, of which four do) fill
-  // the device, at least 128 rows a part, one more part where that fills the last
-  // round better.  With fewer than 256 blocks even so, blocks of 64 or 32 keys, whose
-  // waves share keys.  Parts cost a write and a read of dK and dV in fp32: 64 blocks
-  // (2048 keys, 28 / 4 heads, d = 128) take 395, 330, 266 and 300 us in 3, 4, 8 and 16.
-  const int64_t target = !f32 && !wide ? 1024 : 512;
-  l.key_groups = 4;
-  for (;; l.key_groups /= 2) {
-    const int64_t blocks = ceil_div(n, 32 * l.key_groups) * heads;
-    int64_t s = blocks > 0 ? ceil_div(target, blocks) : 1;
-    auto idle = [&](int64_t x) { return static_cast<double>(ceil_div(blocks * x, 256) * 256) / (blocks * x); };
-    if (s > 1 && blocks > 0 && idle(s + 1) < idle(s) - 0.1) ++s;
-    const int64_t most = rows / 128;
-    l.splits = static_cast<int>(s < most ? s : (most > 1 ? most : 1));
-    if (blocks * l.splits >= 256 || l.key_groups <= (wide ? 2 : 1)) break;
-  }
-  l.stats = 0;
-  l.bounds = static_cast<size_t>(batch) * h_q * n_q * sizeof(float4);
-  l.part = l.bounds + static_cast<size_t>(batch) * l.groups * sizeof(int4);
-  l.bytes = l.part;
-  if (l.splits > 1) l.bytes += 2 * static_cast<size_t>(l.splits) * batch * n * h_kv * (wide ? 128 : 64) * sizeof(float);
-  return l;
 }
 
 template <typename T, int D, int RULE, int KW>

@@ -24,6 +24,7 @@
 
 #include <math.h>
 
+#include "ssa_cuts.h"
 #include "ssa_dense_rows.h"
 #include "ssa_internal.h"
 
@@ -31,8 +32,6 @@ namespace ssa {
 namespace {
 
 using namespace tile;
-
-constexpr int kFew = 32;  // rows of a few-row block
 
 constexpr int kAppend = 4 * kThreads;  // 16-byte chunks of a block that appends
 
@@ -376,53 +375,6 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(DenseParams
     few_join<T, D>(few, blockIdx.x, most_rows, per);
   else
     dense_join<T, D>(rows, static_cast<int64_t>(blockIdx.x - few_blocks) * kJoinWaves + (threadIdx.x >> 6));
-}
-
-// Parts, tiles and workspace of a call.
-struct PagedPlan {
-  int few_splits, row_splits, row_tiles, row_kw;
-  int64_t few_len, row_len;
-  size_t few_o, few_ml, row_o, row_ml, bytes;
-};
-
-PagedPlan paged_plan(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t max_new, int64_t max_len) {
-  PagedPlan l{};
-  max_new = max_new < tokens ? max_new : tokens;
-  const int64_t g = h_q / h_kv, D = d <= 64 ? 64 : 128;
-  // Few rows: parts of at least 256 keys, enough for two blocks a CU twice over
-  // where the batch has sequences of unlike lengths to even out, once for one.
-  const int64_t blocks = batch * h_kv;
-  int64_t s = ceil_div(batch > 1 ? 1024 : 512, blocks), most = ceil_div(max_len, 256);
-  s = s < most ? s : most;
-  s = s > 1 ? s : 1;
-  l.few_len = ceil_div(ceil_div(max_len, s), 128) * 128;
-  l.few_splits = static_cast<int>(ceil_div(max_len, l.few_len));
-  l.row_splits = 1;
-  l.row_len = 0;
-  if (max_new * g > kFew) {
-    const int64_t each = batch * max_new, rows = (tokens < each ? tokens : each) * g;
-    const DenseSplit cut = dense_split(rows, h_kv, max_len, max_new, dtype == SSA_DTYPE_F32, d > 64, true);
-    const int block = rows_of(cut.kw);
-    // (a sequence's last block may be part empty)
-    const int64_t by_seq = batch * ceil_div(max_new * g, block), ragged = rows / block + batch;
-    l.row_kw = cut.kw;
-    l.row_tiles = static_cast<int>(by_seq < ragged ? by_seq : ragged);
-    l.row_splits = cut.parts;
-    l.row_len = ceil_div(ceil_div(max_len, l.row_splits), 64) * 64;
-  }
-  if (l.few_splits > 1) {
-    const size_t rows = static_cast<size_t>(l.few_splits) * batch * h_kv * kFew;
-    l.few_o = l.bytes;
-    l.few_ml = l.few_o + rows * D * sizeof(float);
-    l.bytes = align_up(l.few_ml + rows * 2 * sizeof(float), 16);
-  }
-  if (l.row_splits > 1) {
-    const size_t rows = static_cast<size_t>(l.row_splits) * tokens * h_q;
-    l.row_o = l.bytes;
-    l.row_ml = l.row_o + rows * D * sizeof(float);
-    l.bytes = align_up(l.row_ml + rows * 2 * sizeof(float), 16);
-  }
-  return l;
 }
 
 template <typename T, int D, int RULE, int KW, bool FRESH = false>
