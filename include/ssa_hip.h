@@ -563,6 +563,17 @@ int ssa_paged_step(const void* q, const void* k, const void* v, int dtype, int64
                    const float* slopes, void* out, int64_t o_st, int64_t o_sh, int32_t* error_flag,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* ssa_paged_step where out holds nothing yet: rows of no sequence, and of one that is
+ * left out, are written as zeros.  batch must be positive where tokens is. */
+int ssa_paged_step_zeroed(const void* q, const void* k, const void* v, int dtype, int64_t tokens, int64_t batch, int h_q,
+                          int h_kv, int d, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st,
+                          int64_t v_sh, void* k_pages, void* v_pages, int64_t num_pages, int page_size, int64_t kp_sp,
+                          int64_t kp_st, int64_t kp_sh, int64_t vp_sp, int64_t vp_st, int64_t vp_sh, const int32_t* table,
+                          int64_t table_stride, int max_pages, const int32_t* starts, const int32_t* cached,
+                          int64_t max_new, int64_t max_len, float scale_div, float softcap, const float* slopes, void* out,
+                          int64_t o_st, int64_t o_sh, int32_t* error_flag, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
 /* ---- rotary positions with several axes ---------------------------------- */
 
 /* Rotary embedding of q and k (k nullable with h_k = 0) whose tokens have a

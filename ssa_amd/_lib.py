@@ -143,6 +143,11 @@ SIGNATURES = {
         [_vp, _vp, _vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64,
          _i64, _vp, _vp, _i64, _int, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _int,
          _vp, _vp, _i64, _i64, _flt, _flt, _vp, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
+    "ssa_paged_step_zeroed": (
+        _int,
+        [_vp, _vp, _vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64,
+         _i64, _vp, _vp, _i64, _int, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _int,
+         _vp, _vp, _i64, _i64, _flt, _flt, _vp, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
     "ssa_rope_axes": (
         _int,
         [_vp, _vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64,

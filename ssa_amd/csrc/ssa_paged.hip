@@ -9,7 +9,9 @@
 //                head, single tokens above all: few_rows
 //   many rows    chunks: dense_rows (ssa_dense_rows.h) over pages
 //
-// all in one launch, and the parts that sequences were cut into joined in a second.
+// all in one launch, and the parts that sequences were cut into joined in a second.  Where
+// the caller says that out holds nothing, blocks of the second (of the first, of calls
+// without) write zeros to the rows of out that nothing else writes.
 //
 // few_rows reads K and V once and is bound by that.  The rows fill one
 // MFMA column block; the block's four waves take every fourth 32-key tile of its
@@ -35,6 +37,19 @@ using namespace tile;
 
 constexpr int kAppend = 4 * kThreads;  // 16-byte chunks of a block that appends
 
+// The sequence that holds a token: the last one that starts at or before it (-1 or batch: none).
+__device__ __forceinline__ int sequence_of(const DenseParams& p, int tok) {
+  int x = 0, y = p.batch + 1;  // the first start past the token
+  while (x < y) {
+    const int mid = (x + y) >> 1;
+    if (p.starts[mid] <= tok)
+      x = mid + 1;
+    else
+      y = mid;
+  }
+  return x - 1;
+}
+
 // One chunk of the new rows: k's first, then v's.
 template <typename T>
 __device__ __forceinline__ void append_chunk(const DenseParams& p, int64_t t) {
@@ -46,15 +61,7 @@ __device__ __forceinline__ void append_chunk(const DenseParams& p, int64_t t) {
   const int64_t u = isv ? t - total : t, row = u / per;
   const int c = static_cast<int>(u - row * per);
   const int tok = static_cast<int>(row / p.h_kv), h = static_cast<int>(row - static_cast<int64_t>(tok) * p.h_kv);
-  int x = 0, y = p.batch + 1;  // the first start past the token
-  while (x < y) {
-    const int mid = (x + y) >> 1;
-    if (p.starts[mid] <= tok)
-      x = mid + 1;
-    else
-      y = mid;
-  }
-  const int b = x - 1;
+  const int b = sequence_of(p, tok);
   if (b < 0 || b >= p.batch) return;
   const Seq s = paged_seq(p, b);
   if (tok < s.first || tok >= s.first + s.m) return;
@@ -70,6 +77,31 @@ __device__ __forceinline__ void append_chunk(const DenseParams& p, int64_t t) {
   T* dst = static_cast<T*>(const_cast<void*>(isv ? p.v : p.k)) + pg * (isv ? p.v_sb : p.k_sb) +
            r * (isv ? p.v_sn : p.k_sn) + h * (isv ? p.v_sh : p.k_sh) + c * E;
   *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+}
+
+// Zeros to the rows of out of a block's tokens, one a thread, that no sequence has, or one
+// that is left out.
+template <typename T>
+__device__ __forceinline__ void no_rows(const DenseParams& p, const int block) {
+  constexpr int E = 16 / static_cast<int>(sizeof(T));
+  const int lane = threadIdx.x & 63, per = p.d / E;
+  const int64_t tok0 = static_cast<int64_t>(block) * blockDim.x + (threadIdx.x & ~63);
+  bool none = false;
+  if (tok0 + lane < p.n_q) {
+    const int tok = static_cast<int>(tok0) + lane, b = sequence_of(p, tok);
+    none = true;
+    if (b >= 0 && b < p.batch) {
+      const Seq s = paged_seq(p, b);
+      none = tok < s.first || tok >= s.first + s.m;
+    }
+  }
+  for (uint64_t todo = __ballot(none); todo != 0; todo &= todo - 1) {
+    T* row = static_cast<T*>(p.out) + (tok0 + __builtin_ctzll(todo)) * p.o_sn;
+    for (int c = lane; c < p.h_q * per; c += 64) {
+      const int h = c / per;
+      *reinterpret_cast<uint4*>(row + h * p.o_sh + (c - h * per) * E) = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
 }
 
 template <typename T, int D, int RULE>
@@ -272,7 +304,9 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
 }
 
 // Everything of a call in one launch: blocks of many rows (the longest) first, then
-// few rows, then the blocks that append.  KW 0: no sequence has many rows.
+// few rows, then the blocks that append.  KW 0: no sequence has many rows; its call may
+// have no second launch, so that the blocks of no rows stand here (beside dense_rows they
+// cost 2048 rows behind 30720 cached 12%: 1215 to 1350 us).
 template <typename T, int D, int KW>
 constexpr int paged_per_cu() {
   if constexpr (KW > 0) return rows_per_cu<T, D, KW>();
@@ -281,16 +315,18 @@ constexpr int paged_per_cu() {
 
 template <typename T, int D, int RULE, int KW, bool FRESH>
 __global__ __launch_bounds__(kThreads, (paged_per_cu<T, D, KW>())) void paged_kernel(DenseParams rows, DenseParams few, int row_blocks,
-                                                                                     int few_blocks) {
+                                                                                     int few_blocks, int copy_blocks) {
   extern __shared__ __align__(16) char lds[];
   const int w = blockIdx.x;
   if (w < row_blocks) {
     if constexpr (KW > 0) dense_rows<T, D, true, RULE, KW, FRESH>(rows, w, lds);
   } else if (w < row_blocks + few_blocks) {
     few_rows<T, D, RULE>(few, w - row_blocks, lds);
-  } else {
+  } else if (KW > 0 || w < row_blocks + few_blocks + copy_blocks) {
     const int64_t t = static_cast<int64_t>(w - row_blocks - few_blocks) * kAppend + threadIdx.x;
     for (int i = 0; i < kAppend; i += kThreads) append_chunk<T>(few, t + i);
+  } else {
+    if constexpr (KW == 0) no_rows<T>(few, w - row_blocks - few_blocks - copy_blocks);
   }
 }
 
@@ -367,18 +403,20 @@ __device__ __forceinline__ void few_join(const DenseParams& p, const int block, 
     if (lane * L + e < p.d) Op<T>::store1(orow + lane * L + e, o[e] * inv);
 }
 
-// The parts of both kinds of rows, in one launch.
+// The parts of both kinds of rows, in one launch, and the rows without a sequence.
 template <typename T, int D>
-__global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(DenseParams rows, DenseParams few, int few_blocks, int most_rows,
-                                                                          int per) {
+__global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(DenseParams rows, DenseParams few, int few_blocks,
+                                                                          int join_blocks, int most_rows, int per) {
   if (static_cast<int>(blockIdx.x) < few_blocks)
     few_join<T, D>(few, blockIdx.x, most_rows, per);
+  else if (static_cast<int>(blockIdx.x) >= join_blocks)
+    no_rows<T>(few, blockIdx.x - join_blocks);
   else
     dense_join<T, D>(rows, static_cast<int64_t>(blockIdx.x - few_blocks) * kJoinWaves + (threadIdx.x >> 6));
 }
 
 template <typename T, int D, int RULE, int KW, bool FRESH = false>
-int launch_paged(DenseParams& p, const PagedPlan& l, char* ws, hipStream_t st) {
+int launch_paged(DenseParams& p, const PagedPlan& l, bool zero_rows, char* ws, hipStream_t st) {
   const char* fn = "ssa_paged_step";
   DenseParams f = p, r = p;
   f.splits = l.few_splits;
@@ -398,45 +436,48 @@ int launch_paged(DenseParams& p, const PagedPlan& l, char* ws, hipStream_t st) {
   const int64_t rblocks = static_cast<int64_t>(l.row_tiles) * p.h_kv * r.splits;
   const int64_t fblocks = static_cast<int64_t>(p.batch) * p.h_kv * f.splits;
   const int64_t chunks = p.k_new == nullptr ? 0 : 2 * p.n_q * p.h_kv * (p.d / (16 / static_cast<int>(sizeof(T))));
-  const int64_t blocks = rblocks + fblocks + ceil_div(chunks, kAppend);
-  if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many tokens", fn);
-  paged_kernel<T, D, RULE, KW, FRESH><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(
-      r, f, static_cast<int>(rblocks), static_cast<int>(fblocks));
-  if (int rc = check_launch("ssa_paged_step")) return rc;
   const int most = static_cast<int>(p.max_new * p.g < kFew ? p.max_new * p.g : kFew);
   const int per = f.splits <= 8 ? 1 : (f.splits <= 32 ? 4 : 16);  // waves a row: one round of loads, or 16 waves
   const int64_t few_join_blocks = f.splits > 1 ? ceil_div(static_cast<int64_t>(p.batch) * p.h_kv * most, kJoinWaves / per) : 0;
   const int64_t join_blocks = few_join_blocks + (l.row_tiles > 0 && r.splits > 1 ? ceil_div(r.part_rows, kJoinWaves) : 0);
-  if (join_blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many sequences", fn);
-  if (join_blocks > 0) {
-    paged_join_kernel<T, D><<<dim3(static_cast<unsigned>(join_blocks)), dim3(kJoinWaves * 64), 0, st>>>(
-        r, f, static_cast<int>(few_join_blocks), most, per);
+  const bool zero_here = zero_rows && KW == 0 && join_blocks == 0;
+  const int64_t second = join_blocks + (zero_rows && !zero_here ? ceil_div(p.n_q, kJoinWaves * 64) : 0);
+  if (second > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many sequences", fn);
+  const int64_t cblocks = ceil_div(chunks, kAppend);
+  const int64_t blocks = rblocks + fblocks + cblocks + (zero_here ? ceil_div(p.n_q, kThreads) : 0);
+  if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many tokens", fn);
+  paged_kernel<T, D, RULE, KW, FRESH><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(
+      r, f, static_cast<int>(rblocks), static_cast<int>(fblocks), static_cast<int>(cblocks));
+  if (int rc = check_launch("ssa_paged_step")) return rc;
+  if (second > 0) {
+    paged_join_kernel<T, D><<<dim3(static_cast<unsigned>(second)), dim3(kJoinWaves * 64), 0, st>>>(
+        r, f, static_cast<int>(few_join_blocks), static_cast<int>(join_blocks), most, per);
     return check_launch("ssa_paged_step join");
   }
   return SSA_OK;
 }
 
 template <typename T, int D, int RULE>
-int launch_kw(DenseParams& p, const PagedPlan& l, char* ws, hipStream_t st) {
-  if (l.row_tiles == 0) return launch_paged<T, D, RULE, 0>(p, l, ws, st);
+int launch_kw(DenseParams& p, const PagedPlan& l, bool zero, char* ws, hipStream_t st) {
+  if (l.row_tiles == 0) return launch_paged<T, D, RULE, 0>(p, l, zero, ws, st);
   // Where a good part of the keys are the call's own rows, their tiles are read as
   // contiguous ones (four prompts of 1000 tokens, 32 / 8 heads: 111 to 79 us); the
   // branch costs the pages' tiles 5% (2048 tokens behind 30720: 1335 to 1410).
   const bool fresh = p.k_new != nullptr && 3 * p.max_new >= p.max_len;
   if constexpr (most_kw<T, D>() >= 4)
-    if (l.row_kw == 4) return fresh ? launch_paged<T, D, RULE, 4, true>(p, l, ws, st) : launch_paged<T, D, RULE, 4>(p, l, ws, st);
-  if (l.row_kw == 2) return fresh ? launch_paged<T, D, RULE, 2, true>(p, l, ws, st) : launch_paged<T, D, RULE, 2>(p, l, ws, st);
-  return fresh ? launch_paged<T, D, RULE, 1, true>(p, l, ws, st) : launch_paged<T, D, RULE, 1>(p, l, ws, st);
+    if (l.row_kw == 4) return fresh ? launch_paged<T, D, RULE, 4, true>(p, l, zero, ws, st) : launch_paged<T, D, RULE, 4>(p, l, zero, ws, st);
+  if (l.row_kw == 2) return fresh ? launch_paged<T, D, RULE, 2, true>(p, l, zero, ws, st) : launch_paged<T, D, RULE, 2>(p, l, zero, ws, st);
+  return fresh ? launch_paged<T, D, RULE, 1, true>(p, l, zero, ws, st) : launch_paged<T, D, RULE, 1>(p, l, zero, ws, st);
 }
 
 template <typename T, int D>
-int launch_rule(DenseParams& p, const PagedPlan& l, char* ws, hipStream_t st) {
+int launch_rule(DenseParams& p, const PagedPlan& l, bool zero, char* ws, hipStream_t st) {
   switch (rule_kind<T>(p.rule)) {
-    case kPlain: return launch_kw<T, D, kPlain>(p, l, ws, st);
-    case kCap: return launch_kw<T, D, kCap>(p, l, ws, st);
-    case kBias: return launch_kw<T, D, kBias>(p, l, ws, st);
+    case kPlain: return launch_kw<T, D, kPlain>(p, l, zero, ws, st);
+    case kCap: return launch_kw<T, D, kCap>(p, l, zero, ws, st);
+    case kBias: return launch_kw<T, D, kBias>(p, l, zero, ws, st);
     case kFar:
-      if constexpr (sizeof(T) == 2) return launch_kw<T, D, kFar>(p, l, ws, st);
+      if constexpr (sizeof(T) == 2) return launch_kw<T, D, kFar>(p, l, zero, ws, st);
   }
   return fail(SSA_ERR_UNSUPPORTED, "no kernel for this rule of scores");
 }
@@ -452,15 +493,14 @@ extern "C" size_t ssa_paged_step_workspace_bytes(int dtype, int64_t tokens, int6
   return paged_plan(dtype, tokens, batch, h_q, h_kv, d, max_new, max_len).bytes;
 }
 
-extern "C" int ssa_paged_step(const void* q, const void* k, const void* v, int dtype, int64_t tokens, int64_t batch, int h_q,
-                              int h_kv, int d, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st,
-                              int64_t v_sh, void* k_pages, void* v_pages, int64_t num_pages, int page_size, int64_t kp_sp,
-                              int64_t kp_st, int64_t kp_sh, int64_t vp_sp, int64_t vp_st, int64_t vp_sh, const int32_t* table,
-                              int64_t table_stride, int max_pages, const int32_t* starts, const int32_t* cached,
-                              int64_t max_new, int64_t max_len, float scale_div, float softcap, const float* slopes, void* out,
-                              int64_t o_st, int64_t o_sh, int32_t* error_flag, void* workspace, size_t workspace_bytes,
-                              void* stream) {
-  const char* fn = "ssa_paged_step";
+static int paged_step(const char* fn, bool zero_rows, const void* q, const void* k, const void* v, int dtype,
+                      int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t q_st, int64_t q_sh, int64_t k_st,
+                      int64_t k_sh, int64_t v_st, int64_t v_sh, void* k_pages, void* v_pages, int64_t num_pages,
+                      int page_size, int64_t kp_sp, int64_t kp_st, int64_t kp_sh, int64_t vp_sp, int64_t vp_st,
+                      int64_t vp_sh, const int32_t* table, int64_t table_stride, int max_pages, const int32_t* starts,
+                      const int32_t* cached, int64_t max_new, int64_t max_len, float scale_div, float softcap,
+                      const float* slopes, void* out, int64_t o_st, int64_t o_sh, int32_t* error_flag, void* workspace,
+                      size_t workspace_bytes, void* stream) {
   if (int rc = check_heads(fn, dtype, h_q, h_kv, d)) return rc;
   if (tokens < 0 || batch < 0 || num_pages < 0 || max_pages < 0 || max_new < 0 || max_len < 0)
     return fail(SSA_ERR_INVALID_ARGUMENT, "%s: bad shape tokens=%lld batch=%lld num_pages=%lld max_pages=%d", fn,
@@ -507,6 +547,37 @@ extern "C" int ssa_paged_step(const void* q, const void* k, const void* v, int d
   hipStream_t st = as_stream(stream);
   char* ws = static_cast<char*>(workspace);
   if (dtype == SSA_DTYPE_F32)
-    return d <= 64 ? launch_rule<float, 64>(p, l, ws, st) : launch_rule<float, 128>(p, l, ws, st);
-  return d <= 64 ? launch_rule<uint16_t, 64>(p, l, ws, st) : launch_rule<uint16_t, 128>(p, l, ws, st);
+    return d <= 64 ? launch_rule<float, 64>(p, l, zero_rows, ws, st) : launch_rule<float, 128>(p, l, zero_rows, ws, st);
+  return d <= 64 ? launch_rule<uint16_t, 64>(p, l, zero_rows, ws, st) : launch_rule<uint16_t, 128>(p, l, zero_rows, ws, st);
+}
+
+extern "C" int ssa_paged_step(const void* q, const void* k, const void* v, int dtype, int64_t tokens, int64_t batch,
+                              int h_q, int h_kv, int d, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
+                              int64_t v_st, int64_t v_sh, void* k_pages, void* v_pages, int64_t num_pages, int page_size,
+                              int64_t kp_sp, int64_t kp_st, int64_t kp_sh, int64_t vp_sp, int64_t vp_st, int64_t vp_sh,
+                              const int32_t* table, int64_t table_stride, int max_pages, const int32_t* starts,
+                              const int32_t* cached, int64_t max_new, int64_t max_len, float scale_div, float softcap,
+                              const float* slopes, void* out, int64_t o_st, int64_t o_sh, int32_t* error_flag,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  return paged_step("ssa_paged_step", false, q, k, v, dtype, tokens, batch, h_q, h_kv, d, q_st, q_sh, k_st, k_sh, v_st,
+                    v_sh, k_pages, v_pages, num_pages, page_size, kp_sp, kp_st, kp_sh, vp_sp, vp_st, vp_sh, table,
+                    table_stride, max_pages, starts, cached, max_new, max_len, scale_div, softcap, slopes, out, o_st, o_sh,
+                    error_flag, workspace, workspace_bytes, stream);
+}
+
+extern "C" int ssa_paged_step_zeroed(const void* q, const void* k, const void* v, int dtype, int64_t tokens, int64_t batch,
+                                     int h_q, int h_kv, int d, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
+                                     int64_t v_st, int64_t v_sh, void* k_pages, void* v_pages, int64_t num_pages,
+                                     int page_size, int64_t kp_sp, int64_t kp_st, int64_t kp_sh, int64_t vp_sp,
+                                     int64_t vp_st, int64_t vp_sh, const int32_t* table, int64_t table_stride,
+                                     int max_pages, const int32_t* starts, const int32_t* cached, int64_t max_new,
+                                     int64_t max_len, float scale_div, float softcap, const float* slopes, void* out,
+                                     int64_t o_st, int64_t o_sh, int32_t* error_flag, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  if (tokens > 0 && batch == 0)
+    return fail(SSA_ERR_INVALID_ARGUMENT, "ssa_paged_step_zeroed: rows without a sequence");
+  return paged_step("ssa_paged_step_zeroed", true, q, k, v, dtype, tokens, batch, h_q, h_kv, d, q_st, q_sh, k_st, k_sh,
+                    v_st, v_sh, k_pages, v_pages, num_pages, page_size, kp_sp, kp_st, kp_sh, vp_sp, vp_st, vp_sh, table,
+                    table_stride, max_pages, starts, cached, max_new, max_len, scale_div, softcap, slopes, out, o_st, o_sh,
+                    error_flag, workspace, workspace_bytes, stream);
 }

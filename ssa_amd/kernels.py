@@ -700,8 +700,11 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
             raise ValueError(f"k must be [{T}, {h_kv}, {d}] and v too, got {tuple(k.shape)} and {tuple(v.shape)}")
         k, ks = _rows16(k)
         v, vs = _rows16(v)
-    if out is None:
-        out = torch.empty((T, h_q, d), device=q.device, dtype=dtype)
+    name = "ssa_paged_step"
+    if out is None:  # (rows that no sequence has, or that are left out, become zeros)
+        if B == 0:
+            return torch.zeros((T, h_q, d), device=q.device, dtype=dtype)
+        name, out = "ssa_paged_step_zeroed", torch.empty((T, h_q, d), device=q.device, dtype=dtype)
     elif out.shape != (T, h_q, d) or _rows16(out)[0] is not out:
         raise ValueError(f"out must be [{T}, {h_q}, {d}] with rows aligned to 16 bytes")
     max_new = T if max_new is None else min(int(max_new), T)
@@ -709,7 +712,7 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
     dt = _lib.elem_dtype(q)
     nbytes = _bytes("ssa_paged_step_workspace_bytes", dt, T, B, h_q, h_kv, d, max_new, max_len)
     ws = _workspace(nbytes, q)
-    _call_on(dev, "ssa_paged_step", q.data_ptr(), _at(k), _at(v), dt, T, B, h_q, h_kv, d, *qs, *ks, *vs, k_pages.data_ptr(),
+    _call_on(dev, name, q.data_ptr(), _at(k), _at(v), dt, T, B, h_q, h_kv, d, *qs, *ks, *vs, k_pages.data_ptr(),
              v_pages.data_ptr(), pages, page, *pools, table.data_ptr(), table.stride(0) if B > 1 else 0, width,
              starts.data_ptr(), cached.data_ptr(), max_new, max_len, math.sqrt(d) if scale_div is None else scale_div,
              softcap, _at(slopes), out.data_ptr(), *_rows16(out)[1], _at(error_flag), _at(ws), nbytes)

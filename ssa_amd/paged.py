@@ -36,7 +36,8 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
     many new tokens and keys (the new ones included) a sequence has at most: the work is laid
     out for them (defaults: T, and what the table holds).  A sequence that breaks a bound is
     left out; ``check=True`` waits for the device and raises IndexError then, or if a page lies
-    outside the pool.  Rows of no sequence are not written: they keep what ``out`` held.
+    outside the pool.  Rows of no sequence, and of one that is left out, keep what ``out`` held,
+    and are zeros where it was not given.
 
     float32 and bfloat16 (pools of the same dtype), head_dim a multiple of 8 up to 128,
     page_size a power of 2 from 8 to 4096.  No gradient."""

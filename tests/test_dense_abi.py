@@ -190,3 +190,10 @@ def test_heads_far_apart(L):
         assert st == UNSUPPORTED and "2 GiB" in msg, msg
     st, msg = _call(L, "ssa_masked_attention_backward", BACKWARD, dict(h_q=2, q_sh=1 << 40, do_sh=1 << 40, ws=None))
     assert st == WORKSPACE, msg
+
+
+def test_paged_step_zeroed(L):
+    for kw, status, text in ((dict(batch=0), INVALID, "sequence"), (dict(tokens=0, batch=0, q=None), OK, ""),
+                             (dict(out=None), INVALID, "null"), (dict(ws=None), WORKSPACE, "ssa_paged_step_zeroed: workspace")):
+        st, msg = _call(L, "ssa_paged_step_zeroed", PAGED, kw)
+        assert st == status and (st == OK or text in msg), msg

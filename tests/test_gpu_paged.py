@@ -368,3 +368,37 @@ def test_pools_with_whole_heads_apart(dev, m):
         x[n] = torch.as_strided(rows, x[n].shape, (d, step, 1)).copy_(x[n])
     out = torch.as_strided(torch.zeros(h_q * step, device=dev, dtype=BF16), x["q"].shape, (d, step, 1))
     assert torch.equal(paged_step(**x, out=out, check=True), want)
+
+
+@pytest.mark.parametrize("dtype,d", [(F32, 64), (BF16, 80)], ids=str)
+@pytest.mark.parametrize("seqs", [[(1, 40), (1, 30), (90, 20), (70, 5), (3, 0)], [(1, 40), (1, 30), (2, 7), (3, 0)],
+                                  [(1, 1500), (1, 30), (2, 7), (3, 0)], [(50, 2000), (40, 30), (1, 7), (3, 0)]], ids=str)
+def test_rows_that_nothing_writes_are_zeros(dev, dtype, d, seqs):
+    """Without ``out``: rows before the first sequence, behind the last and of sequences that are
+    left out are zeros whatever the memory held; calls with and without chunks and parts."""
+    from ssa_amd import paged_step
+
+    h_q, h_kv, edge = 4, 2, 300
+    s, keys = _batch(44, dtype, seqs, h_q, h_kv, d, 16, behind=edge)
+    for n in ("q", "k", "v"):
+        s[n] = torch.cat((torch.full((edge, *s[n].shape[1:]), math.nan, dtype=dtype), s[n]))
+    s["starts"] += edge
+    for b in (1, 2):
+        s["cached"][b] = 10 ** 6
+    x = {n: t.to(dev) for n, t in s.items()}
+    stale = torch.full(x["q"].shape, 7.0, device=dev, dtype=dtype)  # the next tensor of this size takes its memory
+    torch.cuda.synchronize()
+    at = stale.data_ptr()
+    del stale
+    out = paged_step(**x)
+    assert out.data_ptr() == at
+    rows = torch.zeros(out.shape[0], dtype=torch.bool)
+    for b, i, m, (value, bound) in _expect({**s, "q": s["q"][edge:]}, keys, seqs, 0.0, None):
+        if b not in (1, 2):
+            check(out[edge + i:edge + i + m], value, bound, f"sequence {b}")
+            rows[edge + i:edge + i + m] = True
+    assert (out.cpu()[~rows] == 0).all()
+    none = {**x, "table": x["table"][:0], "starts": x["starts"][:1], "cached": x["cached"][:0]}
+    assert (paged_step(**none) == 0).all()
+    out.fill_(7.0)
+    assert (paged_step(**none, out=out) == 7).all()
