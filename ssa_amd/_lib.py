@@ -13,6 +13,7 @@ import threading
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # In-tree build; SSA_HIP_LIBRARY may point at another build of the same ABI.
@@ -204,6 +205,12 @@ def ptr(t: Optional[torch.Tensor]):
 
 def stream_of(t: torch.Tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """Raises for dual tensors of forward-mode differentiation: a raw call would drop their tangents."""
+    if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def require_device(*tensors: torch.Tensor) -> None:

@@ -118,6 +118,7 @@ def sparse_exact_attention(
     if scale is None:
         scale = head_dim**0.5
     _lib.require_device(q, k, v, indices)
+    _lib.refuse_tangents("sparse_exact_attention", q, k, v)
     out_dtype = q.dtype
     if q.dtype == torch.float16:
         q, k, v = q.float(), k.float(), v.float()

@@ -11,7 +11,7 @@ from typing import Optional, Sequence
 
 import torch
 
-from . import kernels
+from . import _lib, kernels
 
 
 def axis_rope_freqs(rot: int, theta: float = 10000.0, device=None) -> torch.Tensor:
@@ -52,6 +52,7 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
     features from rot on pass through.  Returns (q, k), or q alone when k is None, in their
     dtype; shapes without B are kept.  Angles are exact for far positions (64 bits), the
     result is rounded once.  Differentiable in q and k, not in freqs."""
+    _lib.refuse_tangents("rope_axes", q, k, freqs)
     unbatched = q.dim() == 3
     if unbatched:
         q, k = q.unsqueeze(0), None if k is None else k.unsqueeze(0)

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import kernels
+from . import _lib, kernels
 
 
 def mask_spans(seq_len: int, batch: int = 1, *, causal: bool = True, doc_starts: Optional[torch.Tensor] = None,
@@ -83,6 +83,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: O
     Rows that see no key are zeros, and keys a row does not see have no influence on it,
     whatever they hold.  float32 and bfloat16, head_dim a multiple of 8 up to 128; float16
     is widened to float32.  Differentiable in q, k and v; repeated calls give the same bits."""
+    _lib.refuse_tangents("masked_attention", q, k, v, slopes)
     unbatched = q.dim() == 3
     if unbatched:
         q, k, v = q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)

@@ -13,7 +13,7 @@ from typing import Optional, Sequence
 
 import torch
 
-from . import kernels
+from . import _lib, kernels
 
 
 @torch.no_grad()
@@ -41,6 +41,7 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
 
     float32 and bfloat16 (pools of the same dtype), head_dim a multiple of 8 up to 128,
     page_size a power of 2 from 8 to 4096.  No gradient."""
+    _lib.refuse_tangents("paged_step", q, k, v, k_pages, v_pages, slopes)
     if softcap is not None and not softcap > 0:
         raise ValueError(f"softcap must be positive, got {softcap}")
     flag = torch.zeros(1, device=q.device, dtype=torch.int32) if check else None

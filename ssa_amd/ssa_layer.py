@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import kernels
+from . import _lib, kernels
 from .attention import dense_attention, sparse_exact_attention
 from .router import CodebookRouter
 from .utils import build_causal_mask
@@ -40,6 +40,7 @@ def rope_rows(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, rot: int,
               by_head: bool) -> torch.Tensor:
     """Rotary embedding of x [B, n, h, d] on the HIP kernel (ssa_rope), differentiable
     in x; the result keeps x's dtype."""
+    _lib.refuse_tangents("rope_rows", x)
     if torch.is_grad_enabled() and x.requires_grad:
         return _Rope.apply(x, cos, sin, rot, by_head)
     return kernels.rope(x, cos, sin, rot, by_head)

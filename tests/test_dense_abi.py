@@ -197,3 +197,30 @@ def test_paged_step_zeroed(L):
                              (dict(out=None), INVALID, "null"), (dict(ws=None), WORKSPACE, "ssa_paged_step_zeroed: workspace")):
         st, msg = _call(L, "ssa_paged_step_zeroed", PAGED, kw)
         assert st == status and (st == OK or text in msg), msg
+
+
+def test_python_refuses_tangents_that_it_would_drop():
+    """Forward-mode differentiation, with and without gradients enabled."""
+    import torch.autograd.forward_ad as fwd
+    from ssa_amd.ssa_layer import rope_rows
+
+    x = torch.zeros(1, 4, 2, 8)
+    ints = torch.zeros(1, 4, dtype=torch.int32)
+    freqs = ssa_amd.axis_rope_freqs(8)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        slopes = fwd.make_dual(torch.ones(2), torch.ones(2))
+        calls = [lambda: ssa_amd.masked_attention(dual, x, x), lambda: ssa_amd.masked_attention(x, x, dual),
+                 lambda: ssa_amd.masked_attention(x, x, x, slopes=slopes),
+                 lambda: ssa_amd.rope_axes(dual, None, ints[None], freqs, (4,)), lambda: ssa_amd.rope_axes(x, dual, ints[None], freqs, (4,)),
+                 lambda: ssa_amd.rope_axes(x, x, ints[None], fwd.make_dual(freqs, freqs), (4,)),
+                 lambda: ssa_amd.paged_step(x[0], dual[0], x[0], x, x, ints, ints[0], ints[0]),
+                 lambda: ssa_amd.paged_step(x[0], None, None, x, dual, ints, ints[0], ints[0]),
+                 lambda: rope_rows(dual, x[0, 0], x[0, 0], 8, True)]
+        for enabled in (True, False):
+            with torch.set_grad_enabled(enabled):
+                for call in calls:
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        call()
+        with pytest.raises(RuntimeError, match="HIP"):  # (no tangent: the device is what is wrong)
+            ssa_amd.masked_attention(x, x, x)

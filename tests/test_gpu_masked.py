@@ -454,3 +454,19 @@ def test_rows_without_keys_beside_hidden_values(dev, dtype, d, cap):
         want = attend(q[0, :, few[0]], k[0, :, few[1]], v[0, :, few[1]], spans, cap, None, p0, dout[0, :, few[0]])
         for name, (value, bound) in want.items():
             check(res[name][0, :, few[0 if name in ("out", "dq") else 1]], value, bound, f"{name}, {h_kv} heads")
+
+
+def test_tangents_are_refused(dev):
+    """Forward-mode differentiation, which a raw call would pass by."""
+    import torch.autograd.forward_ad as fwd
+    from ssa_amd import masked_attention, sparse_exact_attention
+
+    q, k, v, _ = (t.to(dev) for t in _inputs(22, F32, 1, 8, 8, 4, 2, 16))
+    idx = torch.zeros(1, 8, 2, 4, device=dev, dtype=torch.int64)
+    want = masked_attention(q, k, v)
+    with fwd.dual_level():
+        dual = fwd.make_dual(q, torch.ones_like(q))
+        for call in (lambda: masked_attention(dual, k, v), lambda: sparse_exact_attention(dual, k, v, idx)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert torch.equal(masked_attention(q, k, v), want)
