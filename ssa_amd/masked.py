@@ -91,6 +91,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: O
             spans = spans.unsqueeze(0)
     out_dtype = q.dtype
     if q.dtype == torch.float16:
+        if k.dtype != q.dtype or v.dtype != q.dtype:
+            raise TypeError(f"q, k, v must share a dtype ({q.dtype}, {k.dtype}, {v.dtype})")
         q, k, v = q.float(), k.float(), v.float()
     if softcap is not None and not softcap > 0:
         raise ValueError(f"softcap must be positive, got {softcap}")

@@ -224,3 +224,11 @@ def test_python_refuses_tangents_that_it_would_drop():
                         call()
         with pytest.raises(RuntimeError, match="HIP"):  # (no tangent: the device is what is wrong)
             ssa_amd.masked_attention(x, x, x)
+
+
+def test_python_refuses_half_precision_beside_other_types():
+    x = torch.zeros(1, 4, 2, 8, dtype=torch.float16)
+    for other in (x.float(), x.bfloat16()):
+        for args in ((x, other, other), (x, x, other), (x, other, x)):
+            with pytest.raises(TypeError, match="share a dtype"):
+                ssa_amd.masked_attention(*args)
