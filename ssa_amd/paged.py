@@ -16,7 +16,6 @@ import torch
 from . import _lib, kernels
 
 
-@torch.no_grad()
 def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Tensor], k_pages: torch.Tensor,
                v_pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, cached: torch.Tensor, *,
                scale: Optional[float] = None, softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
@@ -40,7 +39,10 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
     and are zeros where it was not given.
 
     float32 and bfloat16 (pools of the same dtype), head_dim a multiple of 8 up to 128,
-    page_size a power of 2 from 8 to 4096.  No gradient."""
+    page_size a power of 2 from 8 to 4096.  No gradient: inputs that want one are refused (call
+    it under ``torch.no_grad()``, or detach them)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, k_pages, v_pages, slopes, out)):
+        raise NotImplementedError("paged_step has no gradient: call it under torch.no_grad(), or detach its inputs")
     _lib.refuse_tangents("paged_step", q, k, v, k_pages, v_pages, slopes)
     if softcap is not None and not softcap > 0:
         raise ValueError(f"softcap must be positive, got {softcap}")

@@ -232,3 +232,23 @@ def test_python_refuses_half_precision_beside_other_types():
         for args in ((x, other, other), (x, x, other), (x, other, x)):
             with pytest.raises(TypeError, match="share a dtype"):
                 ssa_amd.masked_attention(*args)
+
+
+def test_paged_step_refuses_gradients_it_does_not_have():
+    """With gradients enabled only: under no_grad it goes on to the next check, the device."""
+    x = torch.zeros(4, 2, 8)
+    ints = torch.zeros(1, 4, dtype=torch.int32)
+    args = dict(q=x, k=x, v=x, k_pages=x[None], v_pages=x[None], table=ints, starts=ints[0], cached=ints[0], slopes=torch.ones(2))
+    for name in ("q", "k", "v", "k_pages", "v_pages", "slopes"):
+        leaf = {**args, name: args[name].clone().requires_grad_(True)}
+        with pytest.raises(NotImplementedError, match="no gradient"):
+            ssa_amd.paged_step(**leaf)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="HIP"):
+            ssa_amd.paged_step(**leaf)
+    with pytest.raises(RuntimeError, match="HIP"):
+        ssa_amd.paged_step(**args)
+    cache = ssa_amd.PagedKVCache(8, 8, 2, 8, dtype=torch.float32, device="cpu")
+    seq = cache.add()
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        cache.step(x.clone().requires_grad_(True), x, x, [seq], [4])
+    assert cache.free_pages == 8 and cache.length(seq) == 0
