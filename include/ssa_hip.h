@@ -496,7 +496,8 @@ int ssa_mask_spans(const int32_t* doc_starts, int docs, const int32_t* prefix_le
  *       for a row without a key): for the backward.
  *   workspace: ssa_masked_attention_workspace_bytes(...) bytes (0 for most shapes;
  *       few rows over many keys are split along the keys).
- * Limits: d a multiple of 8 up to 128, h_q / h_kv <= 16. */
+ * Limits: d a multiple of 8 up to 128, h_q / h_kv <= 16; scale_div, a softcap and their
+ * product between 1e-30 and 1e30. */
 size_t ssa_masked_attention_workspace_bytes(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv,
                                             int d);
 int ssa_masked_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t n,

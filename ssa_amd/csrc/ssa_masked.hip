@@ -127,6 +127,11 @@ int score_rule(const char* fn, float scale_div, float softcap, const float* slop
     return fail(SSA_ERR_INVALID_ARGUMENT, "%s: scale_div must be positive and finite", fn);
   if (!(softcap >= 0.0f) || !isfinite(softcap))
     return fail(SSA_ERR_INVALID_ARGUMENT, "%s: softcap must be finite and not negative (0: none)", fn);
+  // (so that c1, c2 and a score times c1 are normal fp32 numbers)
+  const double both = softcap > 0.0f ? static_cast<double>(scale_div) * softcap : scale_div;
+  auto out = [](double x) { return x < 1e-30 || x > 1e30; };
+  if (out(scale_div) || out(both) || (softcap > 0.0f && out(softcap)))
+    return fail(SSA_ERR_INVALID_ARGUMENT, "%s: scale_div, softcap and their product must lie in the range of 1e-30 to 1e30", fn);
   r->cap = softcap > tile::kMostDirectCap ? tile::kSeries : (softcap > 0.0f ? tile::kDirect : tile::kNoCap);
   r->c1 = r->cap ? static_cast<float>(1.0 / (static_cast<double>(scale_div) * softcap))
                  : static_cast<float>(1.4426950408889634074 / scale_div);

@@ -252,3 +252,16 @@ def test_paged_step_refuses_gradients_it_does_not_have():
     with pytest.raises(NotImplementedError, match="no gradient"):
         cache.step(x.clone().requires_grad_(True), x, x, [seq], [4])
     assert cache.free_pages == 8 and cache.length(seq) == 0
+
+
+@pytest.mark.parametrize("name,args", [("ssa_masked_attention", FORWARD), ("ssa_masked_attention_backward", BACKWARD),
+                                       ("ssa_paged_step", PAGED)])
+def test_scales_and_caps_that_fp32_does_not_hold(L, name, args):
+    """1 / (scale cap) and a score times it have to be fp32 numbers of full precision."""
+    for kw in (dict(cap=3e38), dict(cap=1e-40), dict(scale=1e-31), dict(scale=1e31), dict(scale=1e20, cap=1e11), dict(scale=1e-20, cap=1e-11)):
+        st, msg = _call(L, name, args, kw)
+        assert st == INVALID and "range" in msg, msg
+    tight = {} if name != "ssa_masked_attention" else dict(n=4000, n_q=4)
+    for kw in (dict(cap=1e29), dict(cap=2e-30), dict(scale=2e-30), dict(scale=9e29), dict(scale=1e20, cap=1e-30)):
+        st, msg = _call(L, name, args, {**tight, **kw, "ws": None})
+        assert st == WORKSPACE, msg

@@ -10,7 +10,8 @@ pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
 # Up to a cap of 1024 the bf16 kernels may be off by cap 2^-22 (the oracle's own bound is twice
 # that), beyond it by 2^-20 of the score; the fp32 kernels' tanh by a few 2^-24 of it.
-CAPS = [(1024.0, None), (1030.0, 2.0 ** -20), (1e5, 2.0 ** -20), (1e6, 2.0 ** -20), (1e12, 2.0 ** -20)]
+CAPS = [(1024.0, None), (1030.0, 2.0 ** -20), (1e5, 2.0 ** -20), (1e6, 2.0 ** -20), (1e12, 2.0 ** -20),
+        (5e28, 2.0 ** -20), (1e-30, None)]
 
 
 def _inputs(seed, dtype, n_q, n, h_q, h_kv, d):
