@@ -652,6 +652,8 @@ def masked_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ws = _workspace(nbytes, q)
     _call_on(dev, "ssa_masked_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, n, n_q,
              _pos0(q_pos0, n, n_q, spans, slopes), h_q, h_kv, d, *qs, *ks, *vs, _at(spans),
+    if out_low is not None and not out.is_contiguous():  # (one may be copied and not the other: they share strides)
+        out, out_low = out.contiguous(), out_low.contiguous()
              math.sqrt(d) if scale_div is None else scale_div, softcap, _at(slopes), out.data_ptr(), _at(out_low), *os,
              dout.data_ptr(), *dos, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(ws), nbytes)
     return dq, dk, dv

@@ -470,3 +470,18 @@ def test_tangents_are_refused(dev):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
         assert torch.equal(masked_attention(q, k, v), want)
+
+
+def test_backward_from_views_of_the_output(dev):
+    """kernels.masked_attention_backward with out and out_low as strided views, one of them off alignment."""
+    from ssa_amd import kernels
+
+    q, k, v, dout = (t.to(dev) for t in _inputs(23, BF16, 1, 50, 50, 4, 2, 64))
+    out, low, lse = kernels.masked_attention(q, k, v, with_lse=True)
+    want = kernels.masked_attention_backward(q, k, v, out, dout, lse, out_low=low)
+    for first, second in ((4, 8), (8, 4)):
+        o, l = (torch.nn.functional.pad(t, (at, 16 - at))[..., at:at + 64] for t, at in ((out, first), (low, second)))
+        assert o.stride() == l.stride() and (o.data_ptr() % 16 != 0) != (l.data_ptr() % 16 != 0)
+        got = kernels.masked_attention_backward(q, k, v, o, dout, lse, out_low=l)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
