@@ -579,6 +579,8 @@ def _index32(t: torch.Tensor, name: str) -> torch.Tensor:
 def _check_dense(q, k, v, spans):
     """(B, n_q, h_q, d, n, h_kv) of matching q, k, v and spans."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+    if t.dtype == torch.int64:  # (a bound far past the keys stays past them)
+        t = t.clamp(-(1 << 31), (1 << 31) - 1)
         raise ValueError(f"q, k, v must be [B, n, heads, d], got shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if not (q.dtype == k.dtype == v.dtype):
         raise TypeError(f"q, k, v must share a dtype ({q.dtype}, {k.dtype}, {v.dtype})")

@@ -485,3 +485,16 @@ def test_backward_from_views_of_the_output(dev):
         got = kernels.masked_attention_backward(q, k, v, o, dout, lse, out_low=l)
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+def test_mask_spans_of_64_bit_bounds(dev):
+    """Starts and prefixes of int64 that 32 bits do not hold stay past every key."""
+    from ssa_amd import mask_spans
+
+    n = 20
+    starts = torch.tensor([[0, 5, 1 << 32], [3, 1 << 33, (1 << 63) - 1]], device=dev)
+    got = mask_spans(n, 2, doc_starts=starts, prefix_lens=torch.tensor([[1 << 32, 0], [(1 << 62) + 7, 0]], device=dev)).cpu()
+    assert torch.equal(got[0], spans_of(n, n, 0, starts=[0, 5, n], prefix=[n, 0]))
+    assert torch.equal(got[1], spans_of(n, n, 0, starts=[3, n, n], prefix=[n, 0]))
+    whole = mask_spans(n, 2, causal=False, doc_starts=starts).cpu()
+    assert torch.equal(whole[0], spans_of(n, n, 0, False, starts=[0, 5, n])) and torch.equal(whole[1], spans_of(n, n, 0, False, starts=[3, n, n]))
