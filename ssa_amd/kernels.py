@@ -536,6 +536,12 @@ def _workspace(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, device=like.device, dtype=torch.uint8) if nbytes else None
 
 
+def _once(t: torch.Tensor, name: str) -> None:
+    """Refuses a tensor to write to whose elements share memory (an expanded one)."""
+    if any(s == 0 and x > 1 for s, x in zip(t.stride(), t.shape)):
+        raise ValueError(f"{name} is written to, but some of its elements are the same memory")
+
+
 def _check_slopes(slopes: Optional[torch.Tensor], h_q: int) -> Optional[torch.Tensor]:
     if slopes is None:
         return None
@@ -693,6 +699,8 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
         rows, st = _rows16(t) if t.numel() else (t, (0, 0, 0))
         if rows is not t:
             raise ValueError(f"{name} must have contiguous rows aligned to 16 bytes")
+        if k is not None:
+            _once(t, name)
         pools += st
     slopes = _check_slopes(slopes, h_q)
     if error_flag is not None and (error_flag.dtype != torch.int32 or error_flag.numel() != 1):
@@ -709,8 +717,10 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
         if B == 0:
             return torch.zeros((T, h_q, d), device=q.device, dtype=dtype)
         name, out = "ssa_paged_step_zeroed", torch.empty((T, h_q, d), device=q.device, dtype=dtype)
-    elif out.shape != (T, h_q, d) or _rows16(out)[0] is not out:
-        raise ValueError(f"out must be [{T}, {h_q}, {d}] with rows aligned to 16 bytes")
+    else:
+        if out.shape != (T, h_q, d) or _rows16(out)[0] is not out:
+            raise ValueError(f"out must be [{T}, {h_q}, {d}] with rows aligned to 16 bytes")
+        _once(out, "out")
     max_new = T if max_new is None else min(int(max_new), T)
     max_len = width * page if max_len is None else min(int(max_len), width * page)
     dt = _lib.elem_dtype(q)

@@ -402,3 +402,20 @@ def test_rows_that_nothing_writes_are_zeros(dev, dtype, d, seqs):
     assert (paged_step(**none) == 0).all()
     out.fill_(7.0)
     assert (paged_step(**none, out=out) == 7).all()
+
+
+def test_expanded_tensors_are_not_written_to(dev):
+    """Pools that hold one head for several take no new rows, but are read; out is a tensor of its own."""
+    from ssa_amd import paged_step
+
+    s, keys = _batch(45, BF16, [(1, 40), (2, 10)], 4, 2, 64, 16)
+    x = {n: t.to(dev) for n, t in s.items()}
+    paged_step(**x)
+    one = {n: x[n][:, :, :1].expand(-1, -1, 2, -1) for n in ("k_pages", "v_pages")}
+    with pytest.raises(ValueError, match="k_pages"):
+        paged_step(**{**x, **one})
+    with pytest.raises(ValueError, match="out"):
+        paged_step(**x, out=torch.zeros(3, 1, 64, device=dev, dtype=BF16).expand(-1, 4, -1))
+    got = paged_step(**{**x, **one, "k": None, "v": None})
+    want = paged_step(**{**x, **{n: t.contiguous() for n, t in one.items()}, "k": None, "v": None})
+    assert torch.equal(got, want)
