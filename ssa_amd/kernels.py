@@ -579,14 +579,14 @@ def mask_spans(n: int, batch: int, n_q: int, q_pos0: int, causal: bool, doc_star
 def _index32(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
+    if t.dtype == torch.int64:  # (a bound far past the keys stays past them)
+        t = t.clamp(-(1 << 31), (1 << 31) - 1)
     return t.to(torch.int32).contiguous()
 
 
 def _check_dense(q, k, v, spans):
     """(B, n_q, h_q, d, n, h_kv) of matching q, k, v and spans."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
-    if t.dtype == torch.int64:  # (a bound far past the keys stays past them)
-        t = t.clamp(-(1 << 31), (1 << 31) - 1)
         raise ValueError(f"q, k, v must be [B, n, heads, d], got shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if not (q.dtype == k.dtype == v.dtype):
         raise TypeError(f"q, k, v must share a dtype ({q.dtype}, {k.dtype}, {v.dtype})")
@@ -652,6 +652,8 @@ def masked_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     q, qs = _group_rows16(q, h_q // h_kv)
     k, ks = _rows16(k)
     v, vs = _rows16(v)
+    if out_low is not None and not out.is_contiguous():  # (one may be copied and not the other: they share strides)
+        out, out_low = out.contiguous(), out_low.contiguous()
     out, os = _rows16(out)
     dout, dos = _group_rows16(dout, h_q // h_kv)
     out_low = None if out_low is None else _rows16(out_low)[0]
@@ -660,8 +662,6 @@ def masked_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ws = _workspace(nbytes, q)
     _call_on(dev, "ssa_masked_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, n, n_q,
              _pos0(q_pos0, n, n_q, spans, slopes), h_q, h_kv, d, *qs, *ks, *vs, _at(spans),
-    if out_low is not None and not out.is_contiguous():  # (one may be copied and not the other: they share strides)
-        out, out_low = out.contiguous(), out_low.contiguous()
              math.sqrt(d) if scale_div is None else scale_div, softcap, _at(slopes), out.data_ptr(), _at(out_low), *os,
              dout.data_ptr(), *dos, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(ws), nbytes)
     return dq, dk, dv
