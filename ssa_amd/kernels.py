@@ -538,7 +538,7 @@ def _workspace(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:
 
 def _once(t: torch.Tensor, name: str) -> None:
     """Refuses a tensor to write to whose elements share memory (an expanded one)."""
-    if any(s == 0 and x > 1 for s, x in zip(t.stride(), t.shape)):
+    if not t.is_contiguous() and any(s == 0 and x > 1 for s, x in zip(t.stride(), t.shape)):
         raise ValueError(f"{name} is written to, but some of its elements are the same memory")
 
 

@@ -41,7 +41,8 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
     float32 and bfloat16 (pools of the same dtype), head_dim a multiple of 8 up to 128,
     page_size a power of 2 from 8 to 4096.  No gradient: inputs that want one are refused (call
     it under ``torch.no_grad()``, or detach them)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, k_pages, v_pages, slopes, out)):
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or
+                                    any([t.requires_grad for t in (k, v, slopes, out) if t is not None])):
         raise NotImplementedError("paged_step has no gradient: call it under torch.no_grad(), or detach its inputs")
     _lib.refuse_tangents("paged_step", q, k, v, k_pages, v_pages, slopes)
     if softcap is not None and not softcap > 0:
