@@ -18,10 +18,10 @@
 // Two waves a SIMD (250 registers each at d = 128) overlap one's products with the
 // other's softmax, and the long calls run near the matrix cores' rate under the
 // card's power limit (32 / 8 heads, bf16; an 8192^3 library product: 1.13 PFLOP/s):
-//   16384 causal rows, d = 128        2.2 ms, 1.0 PFLOP/s
+//   16384 causal rows, d = 128        2.14 to 2.39 ms from card to card, 1.03 to 0.92 PFLOP/s
 //   8192 x 8192, d = 128              1.12 ms, 0.98; d = 64 0.64 ms, 0.86 (the softmax is
 //                                     the same work beside half the products)
-//   2048 rows over 32768 paged keys   1.19 ms, 0.90
+//   2048 rows over 32768 paged keys   1.18 to 1.28 ms, 0.91 to 0.83
 //   4096 x 4096, 16 / 4 heads, fp32   0.56 ms (d = 64), 123 of the product's 154 TFLOP/s
 // Short ones are bound by each block's start (spans, Q, the first tile: 2 to 3 us) and
 // by blocks of unlike lengths: twelve documents of 8192 tokens 155 us, 0.52 PFLOP/s.

@@ -461,8 +461,8 @@ template <typename T, int D, int RULE>
 int launch_kw(DenseParams& p, const PagedPlan& l, bool zero, char* ws, hipStream_t st) {
   if (l.row_tiles == 0) return launch_paged<T, D, RULE, 0>(p, l, zero, ws, st);
   // Where a good part of the keys are the call's own rows, their tiles are read as
-  // contiguous ones (four prompts of 1000 tokens, 32 / 8 heads: 111 to 79 us); the
-  // branch costs the pages' tiles 5% (2048 tokens behind 30720: 1335 to 1410).
+  // contiguous ones (four prompts of 1000 tokens, 32 / 8 heads: 117 to 81 us); the
+  // branch costs the pages' tiles 16% (2048 tokens behind 30720: 1220 to 1410).
   const bool fresh = p.k_new != nullptr && 3 * p.max_new >= p.max_len;
   if constexpr (most_kw<T, D>() >= 4)
     if (l.row_kw == 4) return fresh ? launch_paged<T, D, RULE, 4, true>(p, l, zero, ws, st) : launch_paged<T, D, RULE, 4>(p, l, zero, ws, st);
