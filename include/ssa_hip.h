@@ -514,6 +514,7 @@ int ssa_masked_attention(const void* q, const void* k, const void* v, int dtype,
  *   dq [batch][n_q][h_q][d], dk, dv [batch][n][h_kv][d], contiguous, of type dtype:
  *      written whole (a shared head's sums over its group included), each value
  *      rounded once.  No atomics: the same inputs give the same bits.
+ *   q and dout: the heads of a group within 2 GiB of each other.
  *   workspace: ssa_masked_attention_backward_workspace_bytes(...) bytes.
  * Replaces the autograd backward of dense_attention (ssa/attention.py:118-158)
  * for masks of this form.  slopes get no gradient. */
