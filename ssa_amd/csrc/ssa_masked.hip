@@ -168,6 +168,7 @@ int check_aligned(const char* fn, const char* name, int dtype, const void* ptr, 
 extern "C" size_t ssa_masked_attention_workspace_bytes(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q, int h_kv,
                                                        int d) {
   if (batch <= 0 || n <= 0 || n_q <= 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0) return 0;
+  if (batch > 0x7FFFFFFF || n > 0x7FFFFF00 || n_q > 0x7FFFFF00) return 0;  // (what the call refuses)
   const int s = dense_split(n_q * (h_q / h_kv), batch * h_kv, n, n_q, dtype == SSA_DTYPE_F32, d > 64, false).parts;
   if (s <= 1) return 0;
   return static_cast<size_t>(s) * batch * n_q * h_q * ((d <= 64 ? 64 : 128) + 2) * sizeof(float);

@@ -827,6 +827,7 @@ using namespace ssa;
 extern "C" size_t ssa_masked_attention_backward_workspace_bytes(int dtype, int64_t batch, int64_t n, int64_t n_q,
                                                                 int h_q, int h_kv, int d) {
   if (batch <= 0 || n <= 0 || n_q <= 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0) return 0;
+  if (batch > 0x7FFFFFFF || n > 0x7FFFFF00 || n_q > 0x7FFFFF00) return 0;  // (what the call refuses)
   return bwd_cut(dtype, batch, n, n_q, h_q, h_kv, d).bytes;
 }
 

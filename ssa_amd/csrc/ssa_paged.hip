@@ -490,6 +490,8 @@ using namespace ssa;
 extern "C" size_t ssa_paged_step_workspace_bytes(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv, int d,
                                                  int64_t max_new, int64_t max_len) {
   if (tokens <= 0 || batch <= 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0 || max_new <= 0 || max_len <= 0) return 0;
+  // (what the call refuses: products of these would overflow, to a division by zero at worst)
+  if (tokens > 0x7FFFFF00 || batch > 0x7FFFFF || max_len > 0x7FFFFF00) return 0;
   return paged_plan(dtype, tokens, batch, h_q, h_kv, d, max_new, max_len).bytes;
 }
 
@@ -507,7 +509,7 @@ static int paged_step(const char* fn, bool zero_rows, const void* q, const void*
                 (long long)tokens, (long long)batch, (long long)num_pages, max_pages);
   if (page_size < 8 || page_size > 4096 || (page_size & (page_size - 1)) != 0)
     return fail(SSA_ERR_UNSUPPORTED, "%s: page_size %d must be a power of 2 in [8, 4096]", fn, page_size);
-  if (tokens * (h_q / h_kv) > 0x7FFFFF00 || batch > 0x7FFFFF || num_pages > 0x7FFFFFFF || max_len > 0x7FFFFF00 ||
+  if (tokens > 0x7FFFFF00 || tokens * (h_q / h_kv) > 0x7FFFFF00 || batch > 0x7FFFFF || num_pages > 0x7FFFFFFF || max_len > 0x7FFFFF00 ||
       static_cast<int64_t>(max_pages) * page_size > 0x7FFFFF00)
     return fail(SSA_ERR_UNSUPPORTED, "%s: sequences must be shorter than 2^31 / group size", fn);
   tile::DenseParams p{};

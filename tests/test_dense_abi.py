@@ -265,3 +265,16 @@ def test_scales_and_caps_that_fp32_does_not_hold(L, name, args):
     for kw in (dict(cap=1e29), dict(cap=2e-30), dict(scale=2e-30), dict(scale=9e29), dict(scale=1e20, cap=1e-30)):
         st, msg = _call(L, name, args, {**tight, **kw, "ws": None})
         assert st == WORKSPACE, msg
+
+
+def test_workspaces_of_sizes_that_no_call_takes(L):
+    """Products of the sizes overflow; a batch of 2^62 on 4 heads would divide by 0, and as many
+    tokens in groups of 4 would count as none."""
+    huge = 1 << 62
+    st, msg = _call(L, "ssa_paged_step", PAGED, dict(tokens=huge))
+    assert st == UNSUPPORTED and "2^31" in msg, msg
+    for a in ((10, huge, 8, 4, 64, 8, 1000), (huge, 3, 8, 4, 64, 8, 1000), (10, 3, 8, 4, 64, 8, (1 << 63) - 1)):
+        assert L.ssa_paged_step_workspace_bytes(_lib.DTYPE_BF16, *a) == 0
+    for name in ("ssa_masked_attention_workspace_bytes", "ssa_masked_attention_backward_workspace_bytes"):
+        for B, n, n_q in ((huge, 100, 100), (1, huge, 4), (1, 100, huge)):
+            assert getattr(L, name)(_lib.DTYPE_BF16, B, n, n_q, 8, 4, 64) == 0
