@@ -128,3 +128,51 @@ def test_paged(dev, case, rule):
                           None if slopes is None else slopes[of], c)["out"]
             check(out[at:at + m, of], *want, f"sequence {b}, KV head {kv}")
             at += m
+
+
+# Sums formed again go key by key, without rounding weights to bf16, in another order.  fp32: two scores
+# of d products are (d + 8) 2^-24 sum |q k| / sqrt(d) apart at most, the sum about 0.64 sqrt(d)
+# (128: 6e-5), twice for the weight's and the sum's, from both sides: 2^-12 of the largest value.
+# bf16: a weight's rounding (2^-8 of the values' mean) and the outputs' on both sides.
+TIGHT = {F32: 2.0 ** -12, BF16: 2.0 ** -7}
+
+
+@pytest.mark.parametrize("case", [c for c, _ in MASKED], ids=str)
+def test_masked_values_of_later_tokens(dev, case):
+    """A key near the end whose scores and values are not finite: the rows before it, whose tiles hold
+    it, are as they were, and the rows behind it are not finite."""
+    from ssa_amd import masked_attention
+
+    dtype, B, n, n_q, h_kv, g, d = case
+    gen = torch.Generator().manual_seed(73)
+    q, k, v = (torch.randn(B, m, h, d, generator=gen).to(dtype).to(dev) for m, h in ((n_q, h_kv * g), (n, h_kv), (n, h_kv)))
+    print(f"masked {case}", flush=True)
+    want = masked_attention(q, k, v)
+    at = n - 7
+    k[:, at], v[:, at] = math.nan, math.inf
+    out = masked_attention(q, k, v)
+    row = at - (n - n_q)
+    assert torch.isfinite(out[:, :row]).all() and not torch.isfinite(out[:, row:]).any()
+    assert ((out[:, :row].float() - want[:, :row].float()).abs() <= TIGHT[dtype] * (want[:, :row].float().abs() + v.float().abs().nan_to_num(posinf=0).amax())).all()
+
+
+@pytest.mark.parametrize("case", [c for c, _, _ in PAGED], ids=str)
+def test_paged_values_of_later_tokens(dev, case):
+    """The same of a chunk's last token: its row alone is not finite."""
+    from ssa_amd import paged_step
+
+    dtype, seqs, h_kv, g, d = case
+    s, _ = _batch(74, dtype, seqs, h_kv * g, h_kv, d, 16)
+    x = {n: t.to(dev) for n, t in s.items()}
+    kw = dict(max_new=max(m for m, _ in seqs), max_len=max(m + c for m, c in seqs))
+    print(f"paged {case}", flush=True)
+    want = paged_step(**x, **kw)
+    last = [int(e) - 1 for e, (m, _) in zip(s["starts"][1:], seqs) if m > 1]
+    for i in last:
+        x["k"][i], x["v"][i] = math.nan, math.inf
+    out = paged_step(**x, **kw)
+    bad = torch.zeros(out.shape[0], dtype=torch.bool, device=dev)
+    bad[last] = True
+    assert not torch.isfinite(out[bad]).any() and torch.isfinite(out[~bad]).all()
+    most = max(float(t.float().nan_to_num(posinf=0, neginf=0).abs().max()) for t in (s["v"], s["v_pages"]))
+    assert ((out[~bad].float() - want[~bad].float()).abs() <= TIGHT[dtype] * (want[~bad].float().abs() + most)).all()
