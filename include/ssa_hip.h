@@ -42,6 +42,9 @@ extern "C" {
 /* element types of q / k / v / attention output */
 #define SSA_DTYPE_F32 0
 #define SSA_DTYPE_BF16 1
+/* of pages of a K/V cache, beside the two above: 8-bit codes with a scale a row */
+#define SSA_DTYPE_I8 2
+#define SSA_DTYPE_E4M3 3
 
 /* index element types */
 #define SSA_INDEX_I32 0
@@ -575,6 +578,67 @@ int ssa_paged_step_zeroed(const void* q, const void* k, const void* v, int dtype
                           int64_t max_new, int64_t max_len, float scale_div, float softcap, const float* slopes, void* out,
                           int64_t o_st, int64_t o_sh, int32_t* error_flag, void* workspace, size_t workspace_bytes,
                           void* stream);
+
+/* ssa_paged_step with a sliding window, drafted trees and pages of 8 bits, each by itself
+ * or together.
+ *   window > 0: a token at position p sees the keys at positions p - window + 1 .. p and
+ *       the first `sinks` positions (up to its own); the pages (table entries) between are
+ *       not read.  0: none (sinks 0 too).
+ *   parents (nullable) int32 [tokens]: new token i of a sequence is drafted behind its
+ *       new token parents[starts[b] + i] < i, or behind the cached ones (-1).  It sees
+ *       the cached keys, its ancestors and itself, and its position is cached[b] + its
+ *       number of ancestors; its key is written at cached[b] + i as ever (ssa_paged_keep
+ *       puts a path in order).  max_new (or tokens) at most 64.  Any other value of a
+ *       parent counts as -1 and sets *error_flag.
+ *   page_dtype: dtype, SSA_DTYPE_I8 or SSA_DTYPE_E4M3.  Of 8 bits a page row of a head is d
+ *       codes, and k_scales, v_scales fp32 [num_pages][page_size][h_kv] (strides ks_*, vs_*
+ *       in elements) say what one stands for: code * scale.  Rows written get scale =
+ *       max |x| / 127 (or / 448) and the codes nearest to x / scale (ties to even); below
+ *       2^-100 they are zeros, and one with an infinity or NaN has the scale NaN.  The
+ *       call's own rows are attended as they are given.  Rows aligned to 8 bytes.
+ *   zero_rows != 0: as ssa_paged_step_zeroed.
+ * The other arguments and what is refused as ssa_paged_step; the workspace is
+ * ssa_paged_step_general_workspace_bytes(...) bytes.  No reference counterpart. */
+size_t ssa_paged_step_general_workspace_bytes(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv, int d,
+                                              int64_t max_new, int64_t max_len, int64_t window, int64_t sinks);
+int ssa_paged_step_general(const void* q, const void* k, const void* v, int dtype, int64_t tokens, int64_t batch,
+                           int h_q, int h_kv, int d, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
+                           int64_t v_st, int64_t v_sh, void* k_pages, void* v_pages, int page_dtype,
+                           float* k_scales, float* v_scales, int64_t num_pages, int page_size, int64_t kp_sp,
+                           int64_t kp_st, int64_t kp_sh, int64_t vp_sp, int64_t vp_st, int64_t vp_sh,
+                           int64_t ks_sp, int64_t ks_st, int64_t ks_sh, int64_t vs_sp, int64_t vs_st, int64_t vs_sh,
+                           const int32_t* table, int64_t table_stride, int max_pages, const int32_t* starts,
+                           const int32_t* cached, const int32_t* parents, int64_t max_new, int64_t max_len,
+                           int64_t window, int64_t sinks, float scale_div, float softcap, const float* slopes,
+                           void* out, int64_t o_st, int64_t o_sh, int zero_rows, int32_t* error_flag,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows of a paged cache read back: row starts[b] + i of k_out and v_out
+ * ([tokens][h_kv][d], contiguous, of type out_dtype) is key first[b] + i of sequence b,
+ * for the rows up to starts[b + 1].  Pages of 8 bits are read as what they stand for,
+ * rounded once; others as they are (out_dtype = page_dtype).  Rows of no sequence, and
+ * keys past the table or in a page outside the pool, are zeros (the latter set
+ * *error_flag, nullable). */
+int ssa_paged_read(const void* k_pages, const void* v_pages, int page_dtype, const float* k_scales,
+                   const float* v_scales, int64_t num_pages, int page_size, int h_kv, int d, int64_t kp_sp,
+                   int64_t kp_st, int64_t kp_sh, int64_t vp_sp, int64_t vp_st, int64_t vp_sh, int64_t ks_sp,
+                   int64_t ks_st, int64_t ks_sh, int64_t vs_sp, int64_t vs_st, int64_t vs_sh, int64_t batch,
+                   const int32_t* table, int64_t table_stride, int max_pages, const int32_t* starts,
+                   const int32_t* first, int64_t tokens, int out_dtype, void* k_out, void* v_out,
+                   int32_t* error_flag, void* stream);
+
+/* Keeps some of the tokens behind a sequence's cached ones, of a drafted tree the path that
+ * was accepted: key cached[b] + kept[b][t] (codes and scale) goes to key cached[b] + t, for
+ * t up to the first kept[b][t] below 0 or most_kept (at most 64).  kept int32
+ * [batch][most_kept] (row stride kept_stride) ascends; from the first one that does not on,
+ * nothing moves, and *error_flag (nullable) is set, as for pages outside the pool and keys
+ * past the table, which are left out. */
+int ssa_paged_keep(void* k_pages, void* v_pages, int page_dtype, float* k_scales, float* v_scales,
+                   int64_t num_pages, int page_size, int h_kv, int d, int64_t kp_sp, int64_t kp_st, int64_t kp_sh,
+                   int64_t vp_sp, int64_t vp_st, int64_t vp_sh, int64_t ks_sp, int64_t ks_st, int64_t ks_sh,
+                   int64_t vs_sp, int64_t vs_st, int64_t vs_sh, int64_t batch, const int32_t* table,
+                   int64_t table_stride, int max_pages, const int32_t* cached, const int32_t* kept,
+                   int64_t kept_stride, int most_kept, int32_t* error_flag, void* stream);
 
 /* ---- rotary positions with several axes ---------------------------------- */
 

@@ -27,6 +27,8 @@ SSA_ERR_HIP = 4
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_I8 = 2      # pages of 8-bit codes
+DTYPE_E4M3 = 3
 INDEX_I32 = 0
 INDEX_I64 = 1
 MASK_NONE = 0
@@ -149,6 +151,21 @@ SIGNATURES = {
         [_vp, _vp, _vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64,
          _i64, _vp, _vp, _i64, _int, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _int,
          _vp, _vp, _i64, _i64, _flt, _flt, _vp, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
+    "ssa_paged_step_general_workspace_bytes": (_sz, [_int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64]),
+    "ssa_paged_step_general": (
+        _int,
+        [_vp, _vp, _vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64,
+         _i64, _vp, _vp, _int, _vp, _vp, _i64, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _i64, _vp, _i64, _int, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _flt, _flt, _vp, _vp,
+         _i64, _i64, _int, _vp, _vp, _sz, _vp]),
+    "ssa_paged_read": (
+        _int,
+        [_vp, _vp, _int, _vp, _vp, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i64, _i64, _vp, _i64, _int, _vp, _vp, _i64, _int, _vp, _vp, _vp, _vp]),
+    "ssa_paged_keep": (
+        _int,
+        [_vp, _vp, _int, _vp, _vp, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i64, _i64, _vp, _i64, _int, _vp, _vp, _i64, _int, _vp, _vp]),
     "ssa_rope_axes": (
         _int,
         [_vp, _vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64,
@@ -228,6 +245,10 @@ def elem_dtype(t: torch.Tensor) -> int:
     if t.dtype == torch.bfloat16:
         return DTYPE_BF16
     raise NotImplementedError(f"dtype {t.dtype} is not supported (float32, bfloat16)")
+
+
+PAGE_DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.int8: DTYPE_I8,
+               torch.float8_e4m3fn: DTYPE_E4M3}
 
 
 def index_dtype(t: torch.Tensor) -> int:

@@ -109,6 +109,14 @@ inline BwdCut bwd_cut(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q,
   return l;
 }
 
+// The most keys of a sequence of max_len that its call reads: with a window, the first keys
+// and those of the window and the new tokens, in whole tiles.
+inline int64_t seen_len(int64_t max_len, int64_t max_new, int64_t window, int64_t sinks) {
+  if (window <= 0 || window >= max_len || sinks >= max_len) return max_len;
+  const int64_t some = div_up(sinks, 128) * 128 + window + max_new + 128;
+  return some < max_len ? some : max_len;
+}
+
 // Parts, tiles and workspace of a call.
 struct PagedPlan {
   int few_splits, row_splits, row_tiles, row_kw;

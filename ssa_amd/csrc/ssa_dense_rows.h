@@ -33,7 +33,17 @@
 // A masked key's weight is 0, but 0 times an infinity or NaN in its value row is
 // not: a row whose accumulators end up other than finite is computed again key
 // by key (exact_row), reading visible keys only.
+//
+// kTwo rows see more than one interval: two given ones, or over pages a sliding window
+// and the first keys, and of drafted tokens in a tree their ancestors.  The block then
+// walks the tiles of the two ranges that its rows see between them and no others, parts
+// of the keys are equal shares of those tiles, and only tiles that some row does not see
+// whole take the mask.  Pages of 8 bits (HELD) are widened to the products' type between
+// the load and the LDS, where they are exact; a key's scale multiplies its score, a
+// value's its weight, both in fp32.
 #pragma once
+
+#include <type_traits>
 
 #include "ssa_tile.h"
 
@@ -48,8 +58,16 @@ struct DenseParams {
   int64_t q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh, o_sb, o_sn, o_sh;
   int64_t n, n_q, q_pos0;  // keys; query tokens; position of query token 0
   int batch, h_q, h_kv, g, d;
-  const int2* spans;  // null: causal by position
+  const int2* spans;  // null: causal by position (kTwo: pairs of them)
   ScoreRule rule;
+  // kTwo over pages: keys back from a row that it sees (0: all) and first keys that all rows
+  // see; parents of drafted tokens (nullable)
+  int window, sinks;
+  const int32_t* parents;
+  // scales of pages of 8 bits, strides as the pools'
+  const float *k_scale, *v_scale;
+  int64_t ks_sb, ks_sn, ks_sh, vs_sb, vs_sn, vs_sh;
+  int e4m3;
   // paged: k and v are the pools [pages][page rows][h_kv][d] (sb = page stride)
   const int32_t *table, *starts, *cached;
   int64_t table_stride;
@@ -92,11 +110,172 @@ __device__ __forceinline__ Seq paged_seq(const DenseParams& p, int b) {
   return s;
 }
 
+enum View { kOne = 0, kTwo = 1 };  // (see the head of the file)
+
+constexpr int kDrafts = 64;  // tokens of a sequence in a tree: an ancestor is a bit
+
+// The keys a row sees: lo <= j < hi, a_lo <= j < a_hi, and new tokens cached + i for the bits i
+// of kin.
+struct Sees {
+  int lo, hi, a_lo, a_hi, cached;
+  uint64_t kin;
+  __device__ __forceinline__ bool key(int j) const {
+    const int i = j - cached;
+    return (j >= lo && j < hi) || (j >= a_lo && j < a_hi) || (i >= 0 && i < kDrafts && (kin >> i & 1) != 0);
+  }
+  // some key of [x, y)
+  __device__ __forceinline__ bool any(int x, int y) const {
+    const int i = min(max(x - cached, 0), kDrafts), z = min(max(y - cached, 0), kDrafts);
+    const uint64_t from = i < kDrafts ? ~uint64_t(0) << i : 0, to = z < kDrafts ? (uint64_t(1) << z) - 1 : ~uint64_t(0);
+    return max(lo, x) < min(hi, y) || max(a_lo, x) < min(a_hi, y) || (kin & from & to) != 0;
+  }
+};
+
+// The bits of 32 keys from the off-th new token on.
+__device__ __forceinline__ uint32_t kin_word(uint64_t kin, int off) {
+  if (off >= kDrafts || off <= -32) return 0u;
+  return off >= 0 ? static_cast<uint32_t>(kin >> off) : static_cast<uint32_t>(kin) << -off;
+}
+
+// The tiles that a block's rows see: [x0, x0 + n1), then [y0, y0 + n - n1), ascending.
+struct Tiles {
+  int x0, n1, y0, n;
+  __device__ __forceinline__ int at(int t) const { return t < n1 ? x0 + t : y0 + t - n1; }
+};
+__device__ __forceinline__ Tiles tiles_of(int a_lo, int a_hi, int b_lo, int b_hi, int kt) {
+  int x0 = a_lo / kt, x1 = a_hi > a_lo ? (a_hi - 1) / kt + 1 : x0;
+  int y0 = b_lo / kt, y1 = b_hi > b_lo ? (b_hi - 1) / kt + 1 : y0;
+  if (x1 == x0) {  // (one range)
+    x0 = y0;
+    x1 = y1;
+    y1 = y0;
+  }
+  if (y1 > y0 && y0 < x0) {
+    const int s0 = x0, s1 = x1;
+    x0 = y0;
+    x1 = y1;
+    y0 = s0;
+    y1 = s1;
+  }
+  if (y1 > y0 && y0 <= x1) {
+    x1 = max(x1, y1);
+    y1 = y0;
+  }
+  return Tiles{x0, x1 - x0, y0, x1 - x0 + y1 - y0};
+}
+
+// Lane i's new token of a sequence with m <= 64 of them: which new tokens it sees (itself and its
+// ancestors; of those its window has left behind, the first keys only) and how many tokens
+// above it (`depth`).  All lanes take part.  The ancestors meet by pointer doubling: after round r
+// a lane knows the next 2^r of them.  A parent that does not come before its child is none.
+__device__ __forceinline__ uint64_t draft_kin(const DenseParams& p, int first, int m, int cached, int& depth) {
+  const int lane = threadIdx.x & 63;
+  int up = -1;
+  if (lane < m) {
+    up = p.parents[first + lane];
+    if (up < -1 || up >= lane) {
+      if (p.error_flag != nullptr) atomicOr(p.error_flag, 1);
+      up = -1;
+    }
+  }
+  uint64_t kin = uint64_t(1) << lane;
+#pragma unroll
+  for (int r = 0; r < 6; ++r) {
+    const int src = max(up, 0);
+    const uint32_t a = static_cast<uint32_t>(__shfl(static_cast<int>(kin & 0xFFFFFFFFu), src, 64));
+    const uint32_t b = static_cast<uint32_t>(__shfl(static_cast<int>(kin >> 32), src, 64));
+    const int next = __shfl(up, src, 64);
+    if (up >= 0) {
+      kin |= static_cast<uint64_t>(b) << 32 | a;
+      up = next;
+    }
+  }
+  depth = __popcll(kin) - 1;
+  if (p.window > 0 && depth >= p.window) {  // (ancestors by rising depth are its bits by rising index)
+    const int keep = min(max(p.sinks - cached, 0), kDrafts);
+    uint64_t rest = kin;
+    for (int e = 0; e <= depth - p.window; ++e) {
+      const uint64_t bit = rest & (~rest + 1);
+      if (e >= keep) kin ^= bit;
+      rest ^= bit;
+    }
+  }
+  return kin;
+}
+__device__ __forceinline__ uint64_t lanes_kin(uint64_t kin, int src) {
+  const uint32_t a = static_cast<uint32_t>(__shfl(static_cast<int>(kin & 0xFFFFFFFFu), src, 64));
+  const uint32_t b = static_cast<uint32_t>(__shfl(static_cast<int>(kin >> 32), src, 64));
+  return static_cast<uint64_t>(b) << 32 | a;
+}
+
+// What a row of a paged call at position pos sees; kin 0: a chain.
+__device__ __forceinline__ Sees paged_sees(const DenseParams& p, int pos, int cached, uint64_t kin) {
+  Sees s;
+  s.lo = p.window > 0 ? max(pos + 1 - p.window, 0) : 0;
+  s.hi = kin != 0 ? cached : pos + 1;
+  s.a_lo = 0;
+  s.a_hi = min(min(p.sinks, s.lo), s.hi);
+  s.cached = cached;
+  s.kin = kin;
+  if (s.lo > s.hi) s.lo = s.hi;
+  return s;
+}
+
+// Eight bits as the value they stand for before the scale, and chunks of them as 16 bytes of T.
+__device__ __forceinline__ float code_value(uint8_t c, int e4m3) {
+  return e4m3 ? __builtin_amdgcn_cvt_f32_fp8(c, 0) : static_cast<float>(static_cast<int8_t>(c));
+}
+template <int I>
+__device__ __forceinline__ float code_of(uint32_t w, int e4m3) {
+  return e4m3 ? __builtin_amdgcn_cvt_f32_fp8(w, I) : static_cast<float>(static_cast<int8_t>(w >> (8 * I)));
+}
+template <typename T>
+struct Codes;
+template <>
+struct Codes<uint16_t> {  // eight codes; int8 and e4m3 are exact in bf16
+  static __device__ __forceinline__ uint4 load(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, static_cast<int>(offset), 0, 0);
+    return make_uint4(x.x, x.y, 0u, 0u);
+  }
+  static __device__ __forceinline__ uint4 load(const uint8_t* p) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    return make_uint4(x.x, x.y, 0u, 0u);
+  }
+  static __device__ __forceinline__ uint4 widen(const uint4& x, int e4m3) {
+    const uint32_t w[2] = {x.x, x.y};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      o[2 * i] = Op<uint16_t>::pack2(code_of<0>(w[i], e4m3), code_of<1>(w[i], e4m3));
+      o[2 * i + 1] = Op<uint16_t>::pack2(code_of<2>(w[i], e4m3), code_of<3>(w[i], e4m3));
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+  }
+};
+template <>
+struct Codes<float> {  // four codes
+  static __device__ __forceinline__ uint4 load(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
+    return make_uint4(__builtin_amdgcn_raw_buffer_load_b32(r, static_cast<int>(offset), 0, 0), 0u, 0u, 0u);
+  }
+  static __device__ __forceinline__ uint4 load(const uint8_t* p) {
+    return make_uint4(*reinterpret_cast<const uint32_t*>(p), 0u, 0u, 0u);
+  }
+  static __device__ __forceinline__ uint4 widen(const uint4& x, int e4m3) {
+    return make_uint4(__float_as_uint(code_of<0>(x.x, e4m3)), __float_as_uint(code_of<1>(x.x, e4m3)),
+                      __float_as_uint(code_of<2>(x.x, e4m3)), __float_as_uint(code_of<3>(x.x, e4m3)));
+  }
+};
+
 // The row of key j: contiguous keys, or the sequence's pages (its new rows where the
-// call brought them).
-template <typename T, bool PAGED>
+// call brought them).  S is what the pages hold: T, or uint8_t for 8-bit codes, whose rows
+// have a scale each.
+template <typename T, bool PAGED, typename S = T>
 struct KeyRows {
-  const T *k, *v;
+  const S *k, *v;
+  const float *k_scale, *v_scale;
+  int64_t ks_sb, ks_sn, vs_sb, vs_sn;
+  int e4m3;
   int64_t k_sn, v_sn, k_sb, v_sb;
   const int32_t* table;
   int page_log2, page_mask, num_pages;
@@ -111,6 +290,22 @@ struct KeyRows {
     if (static_cast<unsigned>(pg) < static_cast<unsigned>(num_pages)) return pg;
     if (error_flag != nullptr) atomicOr(error_flag, 1);
     return 0;
+  }
+  // Pages of 8 bits: whether key j is one of the call's own rows, and where they are.
+  __device__ __forceinline__ bool is_new(int j) const { return j >= new_from; }
+  __device__ __forceinline__ void new_rows(int j, const T*& kr, const T*& vr) const {
+    const int64_t x = j - new_from;
+    kr = k_new + x * kn_st;
+    vr = v_new + x * vn_st;
+  }
+  __device__ __forceinline__ void code_rows(int64_t pg, int j, const S*& kr, const S*& vr) const {
+    const int64_t r = j & page_mask;
+    kr = k + pg * k_sb + r * k_sn;
+    vr = v + pg * v_sb + r * v_sn;
+  }
+  __device__ __forceinline__ float scale_of(bool of_v, int64_t pg, int j) const {
+    const int64_t r = j & page_mask;
+    return of_v ? v_scale[pg * vs_sb + r * vs_sn] : k_scale[pg * ks_sb + r * ks_sn];
   }
   __device__ __forceinline__ void in_page(int64_t pg, int j, const T*& kr, const T*& vr) const {
     const int64_t r = j & page_mask, x = j - new_from;
@@ -128,12 +323,21 @@ struct KeyRows {
   }
 };
 
-template <typename T, bool PAGED>
-__device__ __forceinline__ KeyRows<T, PAGED> key_rows(const DenseParams& p, int b, int kvh, int first, int cached) {
-  KeyRows<T, PAGED> r;
+template <typename T, bool PAGED, typename S = T>
+__device__ __forceinline__ KeyRows<T, PAGED, S> key_rows(const DenseParams& p, int b, int kvh, int first, int cached) {
+  KeyRows<T, PAGED, S> r;
   const int64_t kb = PAGED ? 0 : b * p.k_sb, vb = PAGED ? 0 : b * p.v_sb;
-  r.k = static_cast<const T*>(p.k) + kb + kvh * p.k_sh;
-  r.v = static_cast<const T*>(p.v) + vb + kvh * p.v_sh;
+  r.k = static_cast<const S*>(p.k) + kb + kvh * p.k_sh;
+  r.v = static_cast<const S*>(p.v) + vb + kvh * p.v_sh;
+  if constexpr (!std::is_same_v<S, T>) {
+    r.k_scale = p.k_scale + kvh * p.ks_sh;
+    r.v_scale = p.v_scale + kvh * p.vs_sh;
+    r.ks_sb = p.ks_sb;
+    r.ks_sn = p.ks_sn;
+    r.vs_sb = p.vs_sb;
+    r.vs_sn = p.vs_sn;
+    r.e4m3 = p.e4m3;
+  }
   r.k_sn = p.k_sn;
   r.v_sn = p.v_sn;
   r.k_sb = p.k_sb;
@@ -201,6 +405,75 @@ __device__ __forceinline__ void exact_row(const KeyRows<T, PAGED>& rows, const S
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (lane + 64 * e < d) o[e] = fmaf(wt, ld(vt + lane + 64 * e), o[e]);
+    }
+  }
+}
+
+// exact_row for rows that see more than one interval: adds the keys of [x, y) that the row sees.
+// depth: positions of drafted tokens behind the cached ones (null: a chain).
+template <typename T, typename S, bool PAGED>
+__device__ __forceinline__ void exact_keys(const KeyRows<T, PAGED, S>& rows, const ScoreRule& rule, const Sees& see, const T* q,
+                                           int d, int x, int y, float slope, int pos, const int* depth, float (&o)[4],
+                                           float& m, float& l) {
+  constexpr bool HELD = !std::is_same_v<S, T>;
+  const int lane = threadIdx.x & 63;
+  for (int j0 = x; j0 < y; j0 += 64) {
+    const int j = j0 + lane;
+    const bool ok = j < y && see.key(j);
+    float z = -INFINITY;
+    if (ok) {
+      const int at = depth != nullptr && j >= see.cached ? see.cached + depth[j - see.cached] : j;
+      float dot = 0.0f;
+      if (HELD && !rows.is_new(j)) {
+        const S *kr, *vr;
+        const int64_t pg = rows.checked(rows.entry_of(j));
+        rows.code_rows(pg, j, kr, vr);
+        if constexpr (HELD)
+          for (int e = 0; e < d; ++e) dot = fmaf(ld(q + e), code_value(kr[e], rows.e4m3), dot);
+        dot *= rows.scale_of(false, pg, j);
+      } else {
+        const T *kr, *vr;
+        if constexpr (HELD)
+          rows.new_rows(j, kr, vr);
+        else
+          rows.at(j, kr, vr);
+        dot = row_dot(q, kr, d);
+      }
+      z = rule_of<T>(rule, dot, slope, pos, at);
+    }
+    uint64_t on = __ballot(ok);
+    if (on == 0) continue;
+    const float mn = fmaxf(m, wave_max(z)), ref = mn == -INFINITY ? 0.0f : mn;
+    const float a = exp2_w(m - ref);
+    const float w = ok ? exp2_w(z - ref) : 0.0f;
+    m = mn;
+    l = l * a + wave_sum(w);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= a;
+    while (on != 0) {
+      const int t = __builtin_ctzll(on);
+      on &= on - 1;
+      float wt = lane_value(w, t);
+      const int jt = j0 + t;
+      if (HELD && !rows.is_new(jt)) {
+        const S *kr, *vr;
+        const int64_t pg = rows.checked(rows.entry_of(jt));
+        rows.code_rows(pg, jt, kr, vr);
+        wt *= rows.scale_of(true, pg, jt);
+        if constexpr (HELD)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (lane + 64 * e < d) o[e] = fmaf(wt, code_value(vr[lane + 64 * e], rows.e4m3), o[e]);
+      } else {
+        const T *kr, *vr;
+        if constexpr (HELD)
+          rows.new_rows(jt, kr, vr);
+        else
+          rows.at(jt, kr, vr);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (lane + 64 * e < d) o[e] = fmaf(wt, ld(vr + lane + 64 * e), o[e]);
+      }
     }
   }
 }
@@ -281,8 +554,9 @@ __device__ __forceinline__ int fold_tile(int t, int tiles, int heads) {
 }
 
 // FRESH: tiles of a paged call's own rows are read as contiguous ones are.
-template <typename T, int D, bool PAGED, int RULE, int KW, bool FRESH = false>
+template <typename T, int D, bool PAGED, int RULE, int KW, bool FRESH = false, int VIEW = kOne, typename S = T>
 __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, char* lds) {
+  constexpr bool SETS = VIEW == kTwo, HELD = !std::is_same_v<S, T>, TREE = SETS && PAGED;
   using O = Op<T>;
   using Frag = typename O::Frag;
   constexpr int RB = D * O::kEsize;      // bytes of a tile row
@@ -297,9 +571,11 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
   constexpr int BR = rows_of(KW);        // the block's rows
   constexpr int PS = D + 4;              // floats of a row of sums
   // lds: [2 buffers][K, V][TB], then [4 waves][32][PS]
-  __shared__ int s_range[4][2];
+  __shared__ int s_range[4][SETS ? 4 : 2];
   __shared__ float s_m[4][32], s_l[4][32];
   __shared__ int s_flag[4][32];
+  __shared__ int s_depth[TREE ? kDrafts : 1];
+  __shared__ __align__(16) float s_scale[HELD ? 4 : 1][HELD ? KT : 1];  // [buffer][K, V]
 
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -330,16 +606,53 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
     const bool fold = rows_per_cu<T, D, KW>() == 2 && nbh * tiles * p.splits <= 512;
     tile = tiles - 1 - (fold ? fold_tile(rest, tiles, nbh * p.splits) : rest);
   }
-  const KeyRows<T, PAGED> rows = key_rows<T, PAGED>(p, b, kvh, first, static_cast<int>(n_keys) - m);
+  const KeyRows<T, PAGED, S> rows = key_rows<T, PAGED, S>(p, b, kvh, first, static_cast<int>(n_keys) - m);
 
   // this lane's row
   const int r = tile * BR + rw * 32 + (lane & 31);
   const bool real = r < m * p.g;
   const int tok = real ? r / p.g : 0;
   const int hq = kvh * p.g + (real ? r - tok * p.g : 0);
-  const int pos = PAGED ? static_cast<int>(n_keys) - m + tok : static_cast<int>(p.q_pos0) + tok;
+  int pos = PAGED ? static_cast<int>(n_keys) - m + tok : static_cast<int>(p.q_pos0) + tok;
+  const int cached = PAGED ? static_cast<int>(n_keys) - m : 0;
+  const bool tree = TREE && p.parents != nullptr;
   int lo = 0, hi = 0;
-  if (real) {
+  Sees see{0, 0, 0, 0, cached, 0};
+  int b_lo = 0, b_hi = 0;  // of the second range of tiles: lo and hi, or from there to the drafts' end
+  if constexpr (TREE) {
+    uint64_t kin = 0;
+    if (tree) {
+      int depth;
+      const uint64_t all = draft_kin(p, first, m, cached, depth);
+      if (lane < kDrafts) s_depth[lane] = depth;  // (each wave the same)
+      kin = lanes_kin(all, tok);
+      pos = cached + __shfl(depth, tok, 64);
+    }
+    if (real) {
+      see = paged_sees(p, pos, cached, kin);
+      lo = see.lo;
+      hi = see.hi;
+      b_lo = lo;
+      b_hi = tree ? static_cast<int>(n_keys) : hi;
+    }
+  } else if constexpr (SETS) {
+    if (real) {
+      const int4 s = reinterpret_cast<const int4*>(p.spans)[b * p.n_q + tok];
+      lo = max(s.x, 0);
+      hi = static_cast<int>(min(static_cast<int64_t>(s.y), n_keys));
+      if (hi <= lo) lo = hi = 0;
+      int x = max(s.z, 0), y = static_cast<int>(min(static_cast<int64_t>(s.w), n_keys));
+      if (y <= x) x = y = 0;
+      if (hi == lo) {  // (one interval is the second one)
+        lo = x;
+        hi = y;
+        x = y = 0;
+      }
+      see = Sees{lo, hi, x, y, static_cast<int>(n_keys), 0};
+      b_lo = lo;
+      b_hi = hi;
+    }
+  } else if (real) {
     if (!PAGED && p.spans != nullptr) {
       const int2 s = p.spans[b * p.n_q + tok];
       lo = max(s.x, 0);
@@ -349,14 +662,24 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
     }
     if (hi <= lo) lo = hi = 0;
   }
-  const bool some = real && hi > lo;
+  const bool some = real && (SETS ? b_hi > b_lo : hi > lo);
   const Rule<T, RULE> rule(p.rule);
   const float slope = has_bias(RULE) && real ? slope_of(p.rule, hq) : 0.0f;
-  const int lo_min = wave_min_i(some ? lo : 0x7FFFFFFF), hi_max = wave_max_i(some ? hi : 0);
+  const int lo_min = wave_min_i(some ? (SETS ? b_lo : lo) : 0x7FFFFFFF), hi_max = wave_max_i(some ? (SETS ? b_hi : hi) : 0);
+  int a_min = 0x7FFFFFFF, a_max = 0;
+  if constexpr (SETS) {
+    const bool has = real && see.a_hi > see.a_lo;
+    a_min = wave_min_i(has ? see.a_lo : 0x7FFFFFFF);
+    a_max = wave_max_i(has ? see.a_hi : 0);
+  }
   const int lo_max = wave_max_i(real ? lo : 0), hi_min = wave_min_i(real ? hi : 0x7FFFFFFF);
   if (lane == 0) {
     s_range[wave][0] = lo_min;
     s_range[wave][1] = hi_max;
+    if constexpr (SETS) {
+      s_range[wave][2] = a_min;
+      s_range[wave][3] = a_max;
+    }
   }
   const T* qrow = static_cast<const T*>(p.q) + (PAGED ? first * p.q_sn : b * p.q_sb) + tok * p.q_sn + hq * p.q_sh;
   Frag qf[NC];
@@ -369,15 +692,36 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
   int k_lo = __builtin_amdgcn_readfirstlane(min(min(s_range[0][0], s_range[1][0]), min(s_range[2][0], s_range[3][0])));
   int k_hi = __builtin_amdgcn_readfirstlane(max(max(s_range[0][1], s_range[1][1]), max(s_range[2][1], s_range[3][1])));
   int part_lo = 0, part_hi = 0x7FFFFFFF;
-  if (p.splits > 1) {
+  int first_a = 0;             // keys below it are seen by some row, others from k_lo on
+  Tiles walk{0, 0, 0, 0};      // kTwo: the block's tiles, of which it takes nt from t0 on
+  int part_x[2] = {0, 0}, part_y[2] = {0, 0};  // their keys
+  if constexpr (SETS) {
+    const int a_lo = __builtin_amdgcn_readfirstlane(min(min(s_range[0][2], s_range[1][2]), min(s_range[2][2], s_range[3][2])));
+    first_a = __builtin_amdgcn_readfirstlane(max(max(s_range[0][3], s_range[1][3]), max(s_range[2][3], s_range[3][3])));
+    walk = first_a > a_lo ? tiles_of(a_lo, first_a, k_hi > k_lo ? k_lo : 0, k_hi, KT) : tiles_of(0, 0, k_hi > k_lo ? k_lo : 0, k_hi, KT);
+  } else if (p.splits > 1) {
     const int64_t s0 = split * p.split_len, s1 = s0 + p.split_len;
     part_lo = static_cast<int>(min(s0, static_cast<int64_t>(0x7FFFFFFF)));
     part_hi = static_cast<int>(min(s1, static_cast<int64_t>(0x7FFFFFFF)));
     k_lo = max(k_lo, part_lo);
     k_hi = min(k_hi, part_hi);
   }
-  const int t0 = k_lo / KT;
-  const int nt = k_hi > k_lo ? (k_hi + KT - 1) / KT - t0 : 0;
+  int t0, nt;
+  if constexpr (SETS) {
+    const int per = (walk.n + p.splits - 1) / p.splits;
+    t0 = min(split * per, walk.n);
+    nt = min(per, walk.n - t0);
+    part_x[0] = (walk.x0 + min(t0, walk.n1)) * KT;
+    part_y[0] = (walk.x0 + min(t0 + nt, walk.n1)) * KT;
+    part_x[1] = (walk.y0 + max(t0 - walk.n1, 0)) * KT;
+    part_y[1] = (walk.y0 + max(t0 + nt - walk.n1, 0)) * KT;
+  } else {
+    t0 = k_lo / KT;
+    nt = k_hi > k_lo ? (k_hi + KT - 1) / KT - t0 : 0;
+  }
+  // the first key of the t-th tile; where a key is looked up, one that some row sees
+  auto tile_key = [&](int t) { return SETS ? walk.at(t0 + t) * KT : (t0 + t) * KT; };
+  auto seen_key = [&](int j) { return TREE && j >= first_a ? max(j, k_lo) : j; };
 
   // staging: chunk sc of tile rows sr, sr + RPP, ....  Of paged keys, a wave's rows of
   // a load lie in one page, looked up a tile before; tiles that reach past the pages'
@@ -392,25 +736,68 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
   const uint32_t koff = chunk_ok ? my * ks + sc * 16 : kNoChunk, voff = chunk_ok ? my * vs + sc * 16 : kNoChunk;
   uint4 kreg[NP], vreg[NP];
   int pg[PAGED ? NP : 1];
+  // HELD: the page of the key whose scale this thread fetches (K's of KT threads, then V's), the
+  // scale, and whether the loaded tile is of codes
+  const uint32_t ks8 = static_cast<uint32_t>(rows.k_sn), vs8 = static_cast<uint32_t>(rows.v_sn);
+  const uint32_t koff8 = chunk_ok ? my * ks8 + sc * E : kNoChunk, voff8 = chunk_ok ? my * vs8 + sc * E : kNoChunk;
+  int scale_pg = 0;
+  float scale_reg = 1.0f;
+  bool as_codes = false;
   const int paged_end = PAGED ? min(rows.new_from, static_cast<int>(n_keys)) : 0;
   constexpr int RPW = 64 / NCH;  // rows of a wave's load
   auto find_pages = [&](int t) {
     if constexpr (PAGED) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) pg[i] = rows.entry_of(min((t0 + t) * KT + i * RPP + wave * RPW, last));
+      for (int i = 0; i < NP; ++i) pg[i] = rows.entry_of(min(seen_key(tile_key(t) + i * RPP + wave * RPW), last));
+      if constexpr (HELD) scale_pg = rows.entry_of(min(seen_key(tile_key(t) + (tid & (KT - 1))), last));
     }
   };
   auto load_tile = [&](int t) {
-    const int j0 = (t0 + t) * KT;
+    const int j0 = tile_key(t);
+    if constexpr (HELD) {
+      const int j = min(seen_key(j0 + (tid & (KT - 1))), last);
+      scale_reg = 1.0f;
+      if (tid < 2 * KT && !rows.is_new(j)) scale_reg = rows.scale_of(tid >= KT, rows.checked(scale_pg), j);
+      as_codes = j0 + KT <= paged_end;
+      if (as_codes) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int64_t page = rows.checked(__builtin_amdgcn_readfirstlane(pg[i])), r0 = (j0 + i * RPP + wave * RPW) & rows.page_mask;
+          kreg[i] = Codes<T>::load(row_buffer(rows.k + page * rows.k_sb + r0 * rows.k_sn, kAllBytes), koff8);
+          vreg[i] = Codes<T>::load(row_buffer(rows.v + page * rows.v_sb + r0 * rows.v_sn, kAllBytes), voff8);
+        }
+        return;
+      }
+      if (j0 < rows.new_from) {  // a tile of both
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int x = min(seen_key(j0 + sr + i * RPP), last);
+          kreg[i] = vreg[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (!chunk_ok) continue;
+          if (rows.is_new(x)) {
+            const T *kr, *vr;
+            rows.new_rows(x, kr, vr);
+            kreg[i] = *reinterpret_cast<const uint4*>(kr + sc * E);
+            vreg[i] = *reinterpret_cast<const uint4*>(vr + sc * E);
+          } else {
+            const S *kr, *vr;
+            rows.code_rows(rows.checked(rows.entry_of(x)), x, kr, vr);
+            kreg[i] = Codes<T>::widen(Codes<T>::load(kr + sc * E), rows.e4m3);
+            vreg[i] = Codes<T>::widen(Codes<T>::load(vr + sc * E), rows.e4m3);
+          }
+        }
+        return;
+      }
+    }
     if constexpr (PAGED) {
-      if (j0 + KT <= paged_end) {
+      if (!HELD && j0 + KT <= paged_end) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           const int64_t page = rows.checked(__builtin_amdgcn_readfirstlane(pg[i])), r0 = (j0 + i * RPP + wave * RPW) & rows.page_mask;
           kreg[i] = row_load(row_buffer(rows.k + page * rows.k_sb + r0 * rows.k_sn, kAllBytes), koff);
           vreg[i] = row_load(row_buffer(rows.v + page * rows.v_sb + r0 * rows.v_sn, kAllBytes), voff);
         }
-      } else if (FRESH && j0 >= rows.new_from) {
+      } else if (HELD || (FRESH && j0 >= rows.new_from)) {
         const int left = static_cast<int>(n_keys) - j0, x = j0 - rows.new_from, db = p.d * O::kEsize;
         const uint32_t kn = static_cast<uint32_t>(rows.kn_st * O::kEsize), vn = static_cast<uint32_t>(rows.vn_st * O::kEsize);
         const auto kb = row_buffer(rows.k_new + x * rows.kn_st, left >= KT ? kAllBytes : static_cast<int>((left - 1) * kn) + db);
@@ -421,11 +808,11 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
           kreg[i] = row_load(kb, ko + i * RPP * kn);
           vreg[i] = row_load(vb, vo + i * RPP * vn);
         }
-      } else {
+      } else if constexpr (!HELD) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           const T *kr, *vr;
-          rows.at(min(j0 + sr + i * RPP, last), kr, vr);
+          rows.at(min(seen_key(j0 + sr + i * RPP), last), kr, vr);
           kreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(kr + sc * E) : make_uint4(0u, 0u, 0u, 0u);
           vreg[i] = chunk_ok ? *reinterpret_cast<const uint4*>(vr + sc * E) : make_uint4(0u, 0u, 0u, 0u);
         }
@@ -444,6 +831,18 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
   };
   auto store_tile = [&](int buf) {
     char* kt = lds + buf * 2 * TB;
+    if constexpr (HELD) {
+      if (tid < 2 * KT) s_scale[2 * buf + (tid >= KT ? 1 : 0)][tid & (KT - 1)] = scale_reg;
+      if (as_codes) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int at = chunk_at<RB>(sr + i * RPP, sc);
+          *reinterpret_cast<uint4*>(kt + at) = Codes<T>::widen(kreg[i], rows.e4m3);
+          *reinterpret_cast<uint4*>(kt + TB + at) = Codes<T>::widen(vreg[i], rows.e4m3);
+        }
+        return;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int at = chunk_at<RB>(sr + i * RPP, sc);
@@ -468,8 +867,8 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
     __syncthreads();
     if (t + 1 < nt) load_tile(t + 1);
     if (t + 2 < nt) find_pages(t + 2);
-    const int k0 = (t0 + t) * KT + kw * 32 * NSUB;
-    if (k0 < hi_max && k0 + 32 * NSUB > lo_min) {
+    const int k0 = tile_key(t) + kw * 32 * NSUB;
+    if ((k0 < hi_max && k0 + 32 * NSUB > lo_min) || (SETS && k0 < a_max && k0 + 32 * NSUB > a_min)) {
       const char* kt = lds + (TWO ? (t & 1) * 2 * TB : 0) + kw * 32 * NSUB * RB;
       const char* vt = kt + TB;
       f32x16 s[NSUB];
@@ -482,13 +881,49 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
 
       const int kl = k0 + 4 * half;  // key of register 0
       const float dist = static_cast<float>(kl - pos);
+      [[maybe_unused]] const float* ksc = s_scale[HELD && TWO ? 2 * (t & 1) : 0] + (HELD ? kw * 32 * NSUB + 4 * half : 0);
+      [[maybe_unused]] const float* vsc = s_scale[HELD && TWO ? 2 * (t & 1) + 1 : (HELD ? 1 : 0)] + (HELD ? kw * 32 * NSUB + 4 * half : 0);
+      if constexpr (HELD)
 #pragma unroll
-      for (int u = 0; u < NSUB; ++u)
+        for (int u = 0; u < NSUB; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          s[u][i] = rule.z(p.rule, s[u][i], slope, dist + static_cast<float>(32 * u + 8 * (i >> 2) + (i & 3)));
-      const bool whole = k0 >= lo_max && k0 + 32 * NSUB <= hi_min && k0 >= part_lo && k0 + 32 * NSUB <= part_hi;
-      if (!whole) {
+          for (int e = 0; e < 4; ++e) {
+            const float4 x = *reinterpret_cast<const float4*>(ksc + 32 * u + 8 * e);
+            s[u][4 * e] *= x.x;
+            s[u][4 * e + 1] *= x.y;
+            s[u][4 * e + 2] *= x.z;
+            s[u][4 * e + 3] *= x.w;
+          }
+      if (TREE && has_bias(RULE) && tree && k0 + 32 * NSUB > cached) {  // (drafts lie at cached + depth)
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = kl + 32 * u + 8 * (i >> 2) + (i & 3), x = j - cached;
+            const int at = x < 0 ? j : cached + s_depth[TREE ? min(x, kDrafts - 1) : 0];
+            s[u][i] = rule.z(p.rule, s[u][i], slope, static_cast<float>(at - pos));
+          }
+      } else {
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[u][i] = rule.z(p.rule, s[u][i], slope, dist + static_cast<float>(32 * u + 8 * (i >> 2) + (i & 3)));
+      }
+      const bool whole = k0 >= lo_max && k0 + 32 * NSUB <= hi_min && (SETS || (k0 >= part_lo && k0 + 32 * NSUB <= part_hi));
+      if (SETS && !whole) {
+        const int a = in_branch(lo - kl), z = in_branch(hi - kl), x = in_branch(see.a_lo - kl), y = in_branch(see.a_hi - kl);
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u) {
+          const uint32_t kin = TREE ? kin_word(see.kin, k0 + 32 * u - cached) >> (4 * half) : 0u;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int jj = 8 * (i >> 2) + (i & 3), j = 32 * u + jj;
+            const bool sees = (j >= a && j < z) || (j >= x && j < y) || (TREE && (kin >> jj & 1u) != 0);
+            if (!sees) s[u][i] = Rule<T, RULE>::kHidden;
+          }
+        }
+      } else if (!whole) {
         const int a = in_branch(max(lo, part_lo) - kl), z = in_branch(min(hi, part_hi) - kl);
 #pragma unroll
         for (int u = 0; u < NSUB; ++u)
@@ -520,6 +955,17 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
           s[u][i] = exp2_w(fmaf(s[u][i], rule.a, nref));
           lsum += s[u][i];
         }
+      if constexpr (HELD)
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float4 x = *reinterpret_cast<const float4*>(vsc + 32 * u + 8 * e);
+            s[u][4 * e] *= x.x;
+            s[u][4 * e + 1] *= x.y;
+            s[u][4 * e + 2] *= x.z;
+            s[u][4 * e + 3] *= x.w;
+          }
 #pragma unroll
       for (int u = 0; u < NSUB; ++u)
 #pragma unroll
@@ -563,7 +1009,11 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
       p.lse[(static_cast<int64_t>(b) * p.h_q + h) * p.n_q + tk] = any ? mm + __log2f(l) : INFINITY;
     }
   };
-  const bool here = some && max(lo, part_lo) < min(hi, part_hi);
+  bool here;
+  if constexpr (SETS)
+    here = real && (see.any(part_x[0], part_y[0]) || see.any(part_x[1], part_y[1]));
+  else
+    here = some && max(lo, part_lo) < min(hi, part_hi);
   // no key: zeros, whatever hidden values its tiles' sums met; only keys of score -inf: NaN,
   // as a softmax of them is
   if constexpr (KW == 1) {
@@ -642,9 +1092,24 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
     const int ps = lane_value(pos, src), tk = lane_value(tok, src), h = lane_value(hq, src);
     const float sl = lane_value(slope, src);
     float o[4], mm, ll;
-    exact_row<T, PAGED>(rows, p.rule,
-                        static_cast<const T*>(p.q) + (PAGED ? first * p.q_sn : b * p.q_sb) + tk * p.q_sn + h * p.q_sh, p.d, a,
-                        z, sl, ps, o, mm, ll);
+    bool keys = a < z;
+    const T* qr = static_cast<const T*>(p.q) + (PAGED ? first * p.q_sn : b * p.q_sb) + tk * p.q_sn + h * p.q_sh;
+    if constexpr (SETS) {
+      const uint32_t k0 = lane_value(static_cast<int>(see.kin & 0xFFFFFFFFu), src), k1 = lane_value(static_cast<int>(see.kin >> 32), src);
+      const Sees row{lane_value(lo, src), lane_value(hi, src), lane_value(see.a_lo, src), lane_value(see.a_hi, src), see.cached,
+                     static_cast<uint64_t>(k1) << 32 | k0};
+      mm = -INFINITY;
+      ll = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        exact_keys<T, S, PAGED>(rows, p.rule, row, qr, p.d, part_x[x], min(part_y[x], static_cast<int>(n_keys)), sl, ps,
+                                tree ? s_depth : nullptr, o, mm, ll);
+      keys = row.any(part_x[0], part_y[0]) || row.any(part_x[1], part_y[1]);
+    } else {
+      exact_row<T, PAGED>(rows, p.rule, qr, p.d, a, z, sl, ps, o, mm, ll);
+    }
     const float inv = 1.0f / ll;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -658,7 +1123,7 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
         if (p.out_low != nullptr) O::store1(static_cast<T*>(p.out_low) + at, O::left(o[e] * inv));
       }
     }
-    if (lane == 0) put_sums(tk, h, mm, ll, true, a < z);
+    if (lane == 0) put_sums(tk, h, mm, ll, true, keys);
   }
 }
 

@@ -55,7 +55,16 @@ int attention_entry(const void* q, const void* k, const void* v, int dtype, int6
 
 namespace tile {
 struct ScoreRule;
+struct DenseParams;
 }
+struct PagedPlan;
+
+// ssa_paged_step's kernels of windows and trees (two), and over pages of 8 bits (held); wide:
+// more than 64 features.
+int paged_two_f32(tile::DenseParams& p, const PagedPlan& l, bool wide, bool zero_rows, char* ws, hipStream_t st);
+int paged_two_bf16(tile::DenseParams& p, const PagedPlan& l, bool wide, bool zero_rows, char* ws, hipStream_t st);
+int paged_held_f32(tile::DenseParams& p, const PagedPlan& l, bool wide, bool zero_rows, char* ws, hipStream_t st);
+int paged_held_bf16(tile::DenseParams& p, const PagedPlan& l, bool wide, bool zero_rows, char* ws, hipStream_t st);
 
 // Argument checks and rules of the dense attention entry points (fn names the
 // caller in the message).

@@ -671,13 +671,16 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
                v_pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, cached: torch.Tensor,
                scale_div: Optional[float] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
                max_new: Optional[int] = None, max_len: Optional[int] = None, out: Optional[torch.Tensor] = None,
-               error_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """New tokens of a ragged batch appended to their pages and attended (ssa_paged_step):
-    q [T, h_q, d], k and v [T, h_kv, d] (None: already in the pages), pools
-    [pages, page size, h_kv, d], table int32 [B, width], starts int32 [B + 1], cached int32
-    [B].  ``max_new`` and ``max_len`` bound a sequence's new tokens and keys (defaults: T and
-    what the table holds)."""
-    dev = _on_device(q, k, v, k_pages, v_pages, table, starts, cached, slopes, out, error_flag)
+               error_flag: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0,
+               parents: Optional[torch.Tensor] = None, k_scales: Optional[torch.Tensor] = None,
+               v_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """New tokens of a ragged batch appended to their pages and attended (ssa_paged_step,
+    ssa_paged_step_general): q [T, h_q, d], k and v [T, h_kv, d] (None: already in the pages),
+    pools [pages, page size, h_kv, d], table int32 [B, width], starts int32 [B + 1], cached int32
+    [B].  ``max_new`` and ``max_len`` bound a sequence's new tokens and keys (defaults: T, or 64
+    with ``parents``, and what the table holds).  ``window`` (0: none) with ``sinks``, ``parents``
+    int32 [T], and the scales [pages, page size, h_kv] of pools of 8 bits as in paged.paged_step."""
+    dev = _on_device(q, k, v, k_pages, v_pages, table, starts, cached, slopes, out, error_flag, parents, k_scales, v_scales)
     if (k is None) != (v is None):
         raise ValueError("k and v come together")
     if q.dim() != 3 or k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
@@ -687,21 +690,19 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
     if dp != d or h_kv == 0 or h_q % h_kv != 0:
         raise ValueError(f"q {tuple(q.shape)} does not fit pages {tuple(k_pages.shape)}")
     dtype = q.dtype
-    for name, t in (("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("out", out)):
+    held = k_pages.dtype in HELD_DTYPES
+    for name, t in (("k", k), ("v", v), ("out", out)) if held else (("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("out", out)):
         if t is not None and t.dtype != dtype:
             raise TypeError(f"{name} must have q's dtype {dtype}, got {t.dtype}")
+    general = held or window != 0 or sinks != 0 or parents is not None
     B, width = table.shape
     for name, t, shape in (("table", table, (B, width)), ("starts", starts, (B + 1,)), ("cached", cached, (B,))):
         if t.dtype != torch.int32 or t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
             raise ValueError(f"{name} must be an int32 {list(shape)} tensor with contiguous rows")
-    pools = []
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        rows, st = _rows16(t) if t.numel() else (t, (0, 0, 0))
-        if rows is not t:
-            raise ValueError(f"{name} must have contiguous rows aligned to 16 bytes")
-        if k is not None:
-            _once(t, name)
-        pools += st
+    pools = _pool_strides(k_pages, v_pages, k is not None)
+    scale_steps = _scale_strides(k_pages, v_pages, k_scales, v_scales, k is not None)
+    if parents is not None and (parents.dtype != torch.int32 or parents.shape != (T,) or (T > 1 and parents.stride(0) != 1)):
+        raise ValueError(f"parents must be a contiguous int32 [{T}] tensor")
     slopes = _check_slopes(slopes, h_q)
     if error_flag is not None and (error_flag.dtype != torch.int32 or error_flag.numel() != 1):
         raise ValueError("error_flag must be one int32")
@@ -712,8 +713,8 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
             raise ValueError(f"k must be [{T}, {h_kv}, {d}] and v too, got {tuple(k.shape)} and {tuple(v.shape)}")
         k, ks = _rows16(k)
         v, vs = _rows16(v)
-    name = "ssa_paged_step"
-    if out is None:  # (rows that no sequence has, or that are left out, become zeros)
+    name, zeroed = "ssa_paged_step", out is None
+    if zeroed:  # (rows that no sequence has, or that are left out, become zeros)
         if B == 0:
             return torch.zeros((T, h_q, d), device=q.device, dtype=dtype)
         name, out = "ssa_paged_step_zeroed", torch.empty((T, h_q, d), device=q.device, dtype=dtype)
@@ -721,9 +722,19 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
         if out.shape != (T, h_q, d) or _rows16(out)[0] is not out:
             raise ValueError(f"out must be [{T}, {h_q}, {d}] with rows aligned to 16 bytes")
         _once(out, "out")
-    max_new = T if max_new is None else min(int(max_new), T)
+    max_new = (T if parents is None else min(T, 64)) if max_new is None else min(int(max_new), T)
     max_len = width * page if max_len is None else min(int(max_len), width * page)
     dt = _lib.elem_dtype(q)
+    if general:
+        nbytes = _bytes("ssa_paged_step_general_workspace_bytes", dt, T, B, h_q, h_kv, d, max_new, max_len, window, sinks)
+        ws = _workspace(nbytes, q)
+        _call_on(dev, "ssa_paged_step_general", q.data_ptr(), _at(k), _at(v), dt, T, B, h_q, h_kv, d, *qs, *ks, *vs,
+                 k_pages.data_ptr(), v_pages.data_ptr(), _page_dtype(k_pages), _at(k_scales), _at(v_scales), pages, page,
+                 *pools, *scale_steps, table.data_ptr(), table.stride(0) if B > 1 else 0, width, starts.data_ptr(),
+                 cached.data_ptr(), _at(parents), max_new, max_len, window, sinks,
+                 math.sqrt(d) if scale_div is None else scale_div, softcap, _at(slopes), out.data_ptr(), *_rows16(out)[1],
+                 int(zeroed), _at(error_flag), _at(ws), nbytes)
+        return out
     nbytes = _bytes("ssa_paged_step_workspace_bytes", dt, T, B, h_q, h_kv, d, max_new, max_len)
     ws = _workspace(nbytes, q)
     _call_on(dev, name, q.data_ptr(), _at(k), _at(v), dt, T, B, h_q, h_kv, d, *qs, *ks, *vs, k_pages.data_ptr(),
@@ -731,6 +742,113 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
              starts.data_ptr(), cached.data_ptr(), max_new, max_len, math.sqrt(d) if scale_div is None else scale_div,
              softcap, _at(slopes), out.data_ptr(), *_rows16(out)[1], _at(error_flag), _at(ws), nbytes)
     return out
+
+
+HELD_DTYPES = (torch.int8, torch.float8_e4m3fn)  # of pages whose rows have a scale
+
+
+def _page_dtype(pages: torch.Tensor) -> int:
+    dt = _lib.PAGE_DTYPES.get(pages.dtype)
+    if dt is None:
+        raise TypeError(f"pages hold float32, bfloat16, int8 or float8_e4m3fn, got {pages.dtype}")
+    return dt
+
+
+def _pool_strides(k_pages: torch.Tensor, v_pages: torch.Tensor, written: bool):
+    """Element strides (page, token, head) of both pools, whose rows are contiguous and aligned to 16
+    bytes, of 8-bit codes to 8."""
+    pools = []
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if t.dtype != k_pages.dtype:
+            raise TypeError(f"v_pages must have k_pages' dtype {k_pages.dtype}, got {t.dtype}")
+        if t.dtype in HELD_DTYPES:
+            st = tuple(0 if x == 1 else s for s, x in zip(t.stride(), t.shape))
+            if t.numel() and ((st[-1] != 1 and t.shape[-1] > 1) or any(s % 8 for s in st[:-1]) or t.data_ptr() % 8):
+                raise ValueError(f"{name} must have contiguous rows aligned to 8 bytes")
+            st = st[:-1]
+        else:
+            rows, st = _rows16(t) if t.numel() else (t, (0, 0, 0))
+            if rows is not t:
+                raise ValueError(f"{name} must have contiguous rows aligned to 16 bytes")
+        if written:
+            _once(t, name)
+        pools += st
+    return pools
+
+
+def _scale_strides(k_pages, v_pages, k_scales, v_scales, written: bool):
+    """Element strides of the scales of pools of 8 bits (zeros for others, which have none)."""
+    if k_pages.dtype not in HELD_DTYPES:
+        if k_scales is not None or v_scales is not None:
+            raise ValueError("scales go with pools of int8 or float8_e4m3fn")
+        return (0,) * 6
+    steps = []
+    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if t is None or t.dtype != torch.float32 or t.shape != k_pages.shape[:3]:
+            raise ValueError(f"{name} must be float32 {list(k_pages.shape[:3])} for pools of {k_pages.dtype}")
+        if written:
+            _once(t, name)
+        steps += t.stride()
+    return steps
+
+
+def _check_tables(table, **rows):
+    B = table.shape[0] if table.dim() == 2 else -1
+    for name, (t, n) in {"table": (table, None), **rows}.items():
+        ok = t.dtype == torch.int32 and (t.dim() == 2 if n is None else t.shape == (B + n,))
+        if not ok or (t.shape[-1] > 1 and t.stride(-1) != 1):
+            raise ValueError(f"{name} must be an int32 tensor {'[B, width]' if n is None else [B + n]} with contiguous rows")
+    return B, table.shape[1]
+
+
+def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, first: torch.Tensor,
+               tokens: int, dtype: Optional[torch.dtype] = None, k_scales: Optional[torch.Tensor] = None,
+               v_scales: Optional[torch.Tensor] = None, error_flag: Optional[torch.Tensor] = None
+               ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys first[b] ... of each sequence read back as rows starts[b] ... of two new tensors
+    [tokens, h_kv, d] (ssa_paged_read)."""
+    dev = _on_device(k_pages, v_pages, table, starts, first, k_scales, v_scales, error_flag)
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise ValueError("the pools must be [pages, page size, h_kv, d]")
+    pages, page, h_kv, d = k_pages.shape
+    B, width = _check_tables(table, starts=(starts, 1), first=(first, 0))
+    pools = _pool_strides(k_pages, v_pages, False)
+    steps = _scale_strides(k_pages, v_pages, k_scales, v_scales, False)
+    if dtype is None:
+        dtype = torch.bfloat16 if k_pages.dtype in HELD_DTYPES else k_pages.dtype
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
+    if tokens < 0:
+        raise ValueError(f"tokens must not be negative, got {tokens}")
+    if error_flag is not None and (error_flag.dtype != torch.int32 or error_flag.numel() != 1):
+        raise ValueError("error_flag must be one int32")
+    k, v = (torch.empty((tokens, h_kv, d), device=k_pages.device, dtype=dtype) for _ in "kv")
+    if B == 0:
+        return k.zero_(), v.zero_()
+    _call_on(dev, "ssa_paged_read", k_pages.data_ptr(), v_pages.data_ptr(), _page_dtype(k_pages), _at(k_scales), _at(v_scales),
+             pages, page, h_kv, d, *pools, *steps, B, table.data_ptr(), table.stride(0) if B > 1 else 0, width,
+             starts.data_ptr(), first.data_ptr(), tokens, _lib.elem_dtype(k), k.data_ptr(), v.data_ptr(), _at(error_flag))
+    return k, v
+
+
+def paged_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, cached: torch.Tensor, kept: torch.Tensor,
+               k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None,
+               error_flag: Optional[torch.Tensor] = None) -> None:
+    """Key cached[b] + kept[b, t] of each sequence goes to key cached[b] + t (ssa_paged_keep)."""
+    dev = _on_device(k_pages, v_pages, table, cached, kept, k_scales, v_scales, error_flag)
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise ValueError("the pools must be [pages, page size, h_kv, d]")
+    pages, page, h_kv, d = k_pages.shape
+    B, width = _check_tables(table, cached=(cached, 0))
+    if kept.dtype != torch.int32 or kept.dim() != 2 or kept.shape[0] != B or (kept.shape[1] > 1 and kept.stride(1) != 1):
+        raise ValueError(f"kept must be an int32 [{B}, most kept] tensor with contiguous rows")
+    pools = _pool_strides(k_pages, v_pages, True)
+    steps = _scale_strides(k_pages, v_pages, k_scales, v_scales, True)
+    if error_flag is not None and (error_flag.dtype != torch.int32 or error_flag.numel() != 1):
+        raise ValueError("error_flag must be one int32")
+    _call_on(dev, "ssa_paged_keep", k_pages.data_ptr(), v_pages.data_ptr(), _page_dtype(k_pages), _at(k_scales), _at(v_scales),
+             pages, page, h_kv, d, *pools, *steps, B, table.data_ptr(), table.stride(0) if B > 1 else 0, width,
+             cached.data_ptr(), kept.data_ptr(), kept.stride(0) if B > 1 else 0, kept.shape[1], _at(error_flag))
 
 
 def _steps(t: torch.Tensor):
