@@ -531,6 +531,37 @@ int ssa_masked_attention_backward(
     int64_t o_sb, int64_t o_sn, int64_t o_sh, const void* dout, int64_t do_sb, int64_t do_sn, int64_t do_sh,
     const float* lse, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ssa_mask_spans for causal rows with a sliding window: int32 spans [batch][n_q][4], two key
+ * intervals a row.  A row at position p of a document that starts at a sees the keys
+ * max(a, p - window + 1) .. p (the first interval) and a .. a + sinks - 1 up to its own, with
+ * prefix_lens the first prefix_lens[x] too, whatever its position (the second, empty where
+ * they meet the first, which then holds both).  spans aligned to 16 bytes. */
+int ssa_mask_spans_window(const int32_t* doc_starts, int docs, const int32_t* prefix_lens, int64_t batch, int64_t n,
+                          int64_t n_q, int64_t q_pos0, int64_t window, int64_t sinks, int32_t* spans, void* stream);
+
+/* ssa_masked_attention whose rows see two key intervals: spans int32 [batch][n_q][4] (not
+ * null, aligned to 16 bytes) holds lo, hi, lo2, hi2, each pair clamped to [0, n) and empty
+ * where hi <= lo.  The two may lie in any order and overlap (a key in both counts once).  The
+ * same other arguments and workspace. */
+int ssa_masked_attention_two(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t n,
+                             int64_t n_q, int64_t q_pos0, int h_q, int h_kv, int d, int64_t q_sb, int64_t q_sn,
+                             int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn,
+                             int64_t v_sh, const int32_t* spans, float scale_div, float softcap, const float* slopes,
+                             void* out, int64_t o_sb, int64_t o_sn, int64_t o_sh, void* out_low, float* lse,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradients, as ssa_masked_attention_backward's, with a workspace of
+ * ssa_masked_attention_two_backward_workspace_bytes(...) bytes. */
+size_t ssa_masked_attention_two_backward_workspace_bytes(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q,
+                                                         int h_kv, int d);
+int ssa_masked_attention_two_backward(
+    const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t n, int64_t n_q,
+    int64_t q_pos0, int h_q, int h_kv, int d, int64_t q_sb, int64_t q_sn, int64_t q_sh, int64_t k_sb,
+    int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn, int64_t v_sh, const int32_t* spans,
+    float scale_div, float softcap, const float* slopes, const void* out, const void* out_low,
+    int64_t o_sb, int64_t o_sn, int64_t o_sh, const void* dout, int64_t do_sb, int64_t do_sn, int64_t do_sh,
+    const float* lse, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- paged cache --------------------------------------------------------- */
 
 /* Attention of new tokens over a paged K/V cache, a ragged batch in one call.

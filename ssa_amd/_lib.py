@@ -140,6 +140,18 @@ SIGNATURES = {
         [_vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _int, _int, _int, _i64, _i64, _i64,
          _i64, _i64, _i64, _i64, _i64, _i64, _vp, _flt, _flt, _vp, _vp, _vp, _i64, _i64,
          _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ssa_mask_spans_window": (_int, [_vp, _int, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "ssa_masked_attention_two": (
+        _int,
+        [_vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _int, _int, _int, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i64, _i64, _i64, _vp, _flt, _flt, _vp, _vp, _i64, _i64, _i64,
+         _vp, _vp, _vp, _sz, _vp]),
+    "ssa_masked_attention_two_backward_workspace_bytes": (_sz, [_int, _i64, _i64, _i64, _int, _int, _int]),
+    "ssa_masked_attention_two_backward": (
+        _int,
+        [_vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _int, _int, _int, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i64, _i64, _i64, _vp, _flt, _flt, _vp, _vp, _vp, _i64, _i64,
+         _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ssa_paged_step_workspace_bytes": (_sz, [_int, _i64, _i64, _int, _int, _int, _i64, _i64]),
     "ssa_paged_step": (
         _int,

@@ -109,6 +109,31 @@ inline BwdCut bwd_cut(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q,
   return l;
 }
 
+// The backward of rows that see two intervals: blocks of keys, extra parts that dkv_kernel's plan
+// may give them (as many as fill the device once: bwd_cut's target), and the workspace.
+struct TwoCut {
+  int64_t key_blocks;
+  int extra;
+  size_t counts, entries, cut, part, part_floats, bytes;
+};
+
+inline TwoCut two_cut(const BwdCut& l, int dtype, int64_t batch, int64_t n, int h_kv, int d) {
+  TwoCut t{};
+  const bool f32 = dtype == SSA_DTYPE_F32, wide = d > 64;
+  const int64_t keys = 32 * l.key_groups;
+  t.key_blocks = div_up(n, keys) * batch;
+  t.extra = static_cast<int>(div_up(!f32 && !wide ? 1024 : 512, h_kv));
+  // (no more slots than each block of keys with a part for every group of rows)
+  const int64_t all = t.key_blocks * l.groups, slots = all < 2 * t.extra ? all : 2 * t.extra;
+  t.counts = l.bounds + 2 * static_cast<size_t>(batch) * l.groups * 16;
+  t.entries = (t.counts + static_cast<size_t>(t.key_blocks) * 4 + 15) / 16 * 16;
+  t.cut = t.entries + static_cast<size_t>(t.key_blocks + t.extra) * 16;
+  t.part = t.cut + static_cast<size_t>(t.extra) * 16;
+  t.part_floats = static_cast<size_t>(slots) * h_kv * keys * (wide ? 128 : 64);
+  t.bytes = t.part + 2 * t.part_floats * sizeof(float);
+  return t;
+}
+
 // The most keys of a sequence of max_len that its call reads: with a window, the first keys
 // and those of the window and the new tokens, in whole tiles.
 inline int64_t seen_len(int64_t max_len, int64_t max_new, int64_t window, int64_t sinks) {

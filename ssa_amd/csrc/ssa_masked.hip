@@ -2,11 +2,7 @@
 // (ssa_masked_attention), and the intervals of the usual masks (ssa_mask_spans).
 // The kernel is dense_rows_kernel (ssa_dense_rows.h).
 
-#include <math.h>
-
-#include "ssa_cuts.h"
-#include "ssa_dense_rows.h"
-#include "ssa_internal.h"
+#include "ssa_masked_rows.h"
 
 namespace ssa {
 namespace {
@@ -17,7 +13,7 @@ using namespace tile;
 // by bisection) and the keys it sees there.
 __global__ __launch_bounds__(256) void mask_spans_kernel(const int32_t* starts, int docs, const int32_t* prefix,
                                                          int64_t batch, int64_t n, int64_t n_q, int64_t q_pos0,
-                                                         int causal, int2* out) {
+                                                         int causal, int64_t window, int64_t sinks, int2* out) {
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (t >= batch * n_q) return;
   const int64_t b = t / n_q, pos = q_pos0 + (t - b * n_q);
@@ -35,7 +31,11 @@ __global__ __launch_bounds__(256) void mask_spans_kernel(const int32_t* starts, 
     }
     at = x - 1;
     if (at < 0 || at >= docs) {
-      out[t] = make_int2(0, 0);
+      if (window > 0) {
+        reinterpret_cast<int4*>(out)[t] = make_int4(0, 0, 0, 0);
+      } else {
+        out[t] = make_int2(0, 0);
+      }
       return;
     }
     lo = max(s[at], 0);
@@ -47,54 +47,29 @@ __global__ __launch_bounds__(256) void mask_spans_kernel(const int32_t* starts, 
     if (prefix != nullptr) hi = max(hi, lo + prefix[b * docs + at]);
     hi = min(hi, end);
   }
+  if (window > 0) {  // the window's keys, and the first ones (and the prefix) before it
+    int64_t far = min(lo + sinks, pos + 1);
+    if (prefix != nullptr) far = max(far, lo + prefix[b * docs + at]);
+    int64_t from = max(lo, pos + 1 - window), to = min(pos + 1, end);
+    far = min(far, end);
+    if (far >= from) {  // (they meet)
+      from = lo;
+      to = max(to, far);
+      far = lo;
+    }
+    int4 s = make_int4(0, 0, 0, 0);
+    if (to > from) {
+      s.x = static_cast<int>(from);
+      s.y = static_cast<int>(to);
+    }
+    if (far > lo) {
+      s.z = static_cast<int>(lo);
+      s.w = static_cast<int>(far);
+    }
+    reinterpret_cast<int4*>(out)[t] = s;
+    return;
+  }
   out[t] = hi > lo ? make_int2(static_cast<int>(lo), static_cast<int>(hi)) : make_int2(0, 0);
-}
-
-template <typename T, int D, int RULE, int KW>
-__global__ __launch_bounds__(kThreads, (rows_per_cu<T, D, KW>())) void dense_rows_kernel(DenseParams p) {
-  extern __shared__ __align__(16) char lds[];
-  dense_rows<T, D, false, RULE, KW>(p, blockIdx.x, lds);
-}
-
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void dense_join_kernel(DenseParams p) {
-  dense_join<T, D>(p, static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6));
-}
-
-template <typename T, int D, int RULE, int KW>
-int launch_rows(DenseParams& p, hipStream_t st) {
-  const size_t bytes = rows_lds<T, D, KW>();
-  if (int rc = reserve_lds(reinterpret_cast<const void*>(dense_rows_kernel<T, D, RULE, KW>), bytes + 2048,
-                           "ssa_masked_attention"))
-    return rc;
-  const int64_t blocks = ceil_div(p.n_q * p.g, rows_of(KW)) * p.batch * p.h_kv * p.splits;
-  if (blocks > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "ssa_masked_attention: too many rows");
-  dense_rows_kernel<T, D, RULE, KW><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), bytes, st>>>(p);
-  if (int rc = check_launch("ssa_masked_attention")) return rc;
-  if (p.splits > 1) {
-    dense_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(p.part_rows, kThreads / 64))), dim3(kThreads), 0, st>>>(p);
-    return check_launch("ssa_masked_attention join");
-  }
-  return SSA_OK;
-}
-
-template <typename T, int D, int RULE>
-int launch_kw(DenseParams& p, int kw, hipStream_t st) {
-  if constexpr (most_kw<T, D>() >= 4)
-    if (kw == 4) return launch_rows<T, D, RULE, 4>(p, st);
-  return kw == 2 ? launch_rows<T, D, RULE, 2>(p, st) : launch_rows<T, D, RULE, 1>(p, st);
-}
-
-template <typename T, int D>
-int launch_rule(DenseParams& p, int kw, hipStream_t st) {
-  switch (rule_kind<T>(p.rule)) {
-    case kPlain: return launch_kw<T, D, kPlain>(p, kw, st);
-    case kCap: return launch_kw<T, D, kCap>(p, kw, st);
-    case kBias: return launch_kw<T, D, kBias>(p, kw, st);
-    case kFar:
-      if constexpr (sizeof(T) == 2) return launch_kw<T, D, kFar>(p, kw, st);
-  }
-  return fail(SSA_ERR_UNSUPPORTED, "no kernel for this rule of scores");
 }
 
 }  // namespace
@@ -103,8 +78,8 @@ int launch_rule(DenseParams& p, int kw, hipStream_t st) {
 using namespace ssa;
 using namespace ssa::tile;
 
-extern "C" int ssa_mask_spans(const int32_t* doc_starts, int docs, const int32_t* prefix_lens, int64_t batch,
-                              int64_t n, int64_t n_q, int64_t q_pos0, int causal, int32_t* spans, void* stream) {
+static int mask_spans(const int32_t* doc_starts, int docs, const int32_t* prefix_lens, int64_t batch, int64_t n, int64_t n_q,
+                      int64_t q_pos0, int causal, int64_t window, int64_t sinks, int32_t* spans, void* stream) {
   if (batch < 0 || n < 0 || n_q < 0 || q_pos0 < 0 || n >= (int64_t(1) << 31))
     return fail(SSA_ERR_INVALID_ARGUMENT, "ssa_mask_spans: bad shape batch=%lld n=%lld n_q=%lld q_pos0=%lld",
                 (long long)batch, (long long)n, (long long)n_q, (long long)q_pos0);
@@ -116,8 +91,25 @@ extern "C" int ssa_mask_spans(const int32_t* doc_starts, int docs, const int32_t
   const int64_t grid = ceil_div(batch * n_q, 256);
   if (grid > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "ssa_mask_spans: too many rows");
   mask_spans_kernel<<<dim3(static_cast<unsigned>(grid)), dim3(256), 0, as_stream(stream)>>>(
-      doc_starts, docs, prefix_lens, batch, n, n_q, q_pos0, causal != 0, reinterpret_cast<int2*>(spans));
+      doc_starts, docs, prefix_lens, batch, n, n_q, q_pos0, causal != 0, window, sinks, reinterpret_cast<int2*>(spans));
   return check_launch("ssa_mask_spans");
+}
+
+extern "C" int ssa_mask_spans(const int32_t* doc_starts, int docs, const int32_t* prefix_lens, int64_t batch,
+                              int64_t n, int64_t n_q, int64_t q_pos0, int causal, int32_t* spans, void* stream) {
+  return mask_spans(doc_starts, docs, prefix_lens, batch, n, n_q, q_pos0, causal, 0, 0, spans, stream);
+}
+
+extern "C" int ssa_mask_spans_window(const int32_t* doc_starts, int docs, const int32_t* prefix_lens, int64_t batch,
+                                     int64_t n, int64_t n_q, int64_t q_pos0, int64_t window, int64_t sinks, int32_t* spans,
+                                     void* stream) {
+  const int64_t most = int64_t(1) << 31;  // (past every key)
+  if (window < 1 || sinks < 0)
+    return fail(SSA_ERR_INVALID_ARGUMENT, "ssa_mask_spans_window: window must be positive and sinks not negative");
+  if (reinterpret_cast<uintptr_t>(spans) % 16 != 0)
+    return fail(SSA_ERR_INVALID_ARGUMENT, "ssa_mask_spans_window: spans must be aligned to 16 bytes");
+  return mask_spans(doc_starts, docs, prefix_lens, batch, n, n_q, q_pos0, 1, window < most ? window : most,
+                    sinks < most ? sinks : most, spans, stream);
 }
 
 namespace ssa {
@@ -174,13 +166,12 @@ extern "C" size_t ssa_masked_attention_workspace_bytes(int dtype, int64_t batch,
   return static_cast<size_t>(s) * batch * n_q * h_q * ((d <= 64 ? 64 : 128) + 2) * sizeof(float);
 }
 
-extern "C" int ssa_masked_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t n,
+static int forward(const char* fn, bool two, const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t n,
                                     int64_t n_q, int64_t q_pos0, int h_q, int h_kv, int d, int64_t q_sb, int64_t q_sn,
                                     int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn,
                                     int64_t v_sh, const int32_t* spans, float scale_div, float softcap,
                                     const float* slopes, void* out, int64_t o_sb, int64_t o_sn, int64_t o_sh,
                                     void* out_low, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
-  const char* fn = "ssa_masked_attention";
   if (int rc = check_heads(fn, dtype, h_q, h_kv, d)) return rc;
   if (batch < 0 || n < 0 || n_q < 0 || q_pos0 < 0 || batch > 0x7FFFFFFF)
     return fail(SSA_ERR_INVALID_ARGUMENT, "%s: bad shape batch=%lld n=%lld n_q=%lld q_pos0=%lld", fn, (long long)batch,
@@ -197,6 +188,8 @@ extern "C" int ssa_masked_attention(const void* q, const void* k, const void* v,
   if (int rc = check_aligned(fn, "v", dtype, v, v_sb, v_sn, v_sh)) return rc;
   if (int rc = check_aligned(fn, "out", dtype, out, o_sb, o_sn, o_sh)) return rc;
   if (int rc = check_aligned(fn, "out_low", dtype, out_low, 0, 0, 0)) return rc;
+  if (two && (spans == nullptr || reinterpret_cast<uintptr_t>(spans) % 16 != 0))
+    return fail(SSA_ERR_INVALID_ARGUMENT, "%s: spans must be given, aligned to 16 bytes", fn);
   p.q = q; p.k = k; p.v = v; p.out = out; p.out_low = out_low; p.lse = lse;
   p.q_sb = q_sb; p.q_sn = q_sn; p.q_sh = q_sh;
   p.k_sb = k_sb; p.k_sn = k_sn; p.k_sh = k_sh;
@@ -220,7 +213,30 @@ extern "C" int ssa_masked_attention(const void* q, const void* k, const void* v,
     p.part_ml = p.part_o + static_cast<int64_t>(p.splits) * p.part_rows * (d <= 64 ? 64 : 128);
   }
   hipStream_t st = as_stream(stream);
+  if (two) return dtype == SSA_DTYPE_F32 ? masked_two_f32(p, cut.kw, st) : masked_two_bf16(p, cut.kw, st);
   if (dtype == SSA_DTYPE_F32)
-    return d <= 64 ? launch_rule<float, 64>(p, cut.kw, st) : launch_rule<float, 128>(p, cut.kw, st);
-  return d <= 64 ? launch_rule<uint16_t, 64>(p, cut.kw, st) : launch_rule<uint16_t, 128>(p, cut.kw, st);
+    return d <= 64 ? launch_rows_rule<float, 64, kOne>(p, cut.kw, st) : launch_rows_rule<float, 128, kOne>(p, cut.kw, st);
+  return d <= 64 ? launch_rows_rule<uint16_t, 64, kOne>(p, cut.kw, st) : launch_rows_rule<uint16_t, 128, kOne>(p, cut.kw, st);
+}
+
+extern "C" int ssa_masked_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t n,
+                                    int64_t n_q, int64_t q_pos0, int h_q, int h_kv, int d, int64_t q_sb, int64_t q_sn,
+                                    int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn,
+                                    int64_t v_sh, const int32_t* spans, float scale_div, float softcap,
+                                    const float* slopes, void* out, int64_t o_sb, int64_t o_sn, int64_t o_sh,
+                                    void* out_low, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  return forward("ssa_masked_attention", false, q, k, v, dtype, batch, n, n_q, q_pos0, h_q, h_kv, d, q_sb, q_sn, q_sh, k_sb, k_sn,
+                 k_sh, v_sb, v_sn, v_sh, spans, scale_div, softcap, slopes, out, o_sb, o_sn, o_sh, out_low, lse, workspace,
+                 workspace_bytes, stream);
+}
+
+extern "C" int ssa_masked_attention_two(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t n,
+                                    int64_t n_q, int64_t q_pos0, int h_q, int h_kv, int d, int64_t q_sb, int64_t q_sn,
+                                    int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn,
+                                    int64_t v_sh, const int32_t* spans, float scale_div, float softcap,
+                                    const float* slopes, void* out, int64_t o_sb, int64_t o_sn, int64_t o_sh,
+                                    void* out_low, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  return forward("ssa_masked_attention_two", true, q, k, v, dtype, batch, n, n_q, q_pos0, h_q, h_kv, d, q_sb, q_sn, q_sh, k_sb, k_sn,
+                 k_sh, v_sb, v_sn, v_sh, spans, scale_div, softcap, slopes, out, o_sb, o_sn, o_sh, out_low, lse, workspace,
+                 workspace_bytes, stream);
 }

@@ -1,0 +1,18 @@
+// Dense attention whose rows see two key intervals, forward and backward, f32 (a file of its
+// own, so that the instantiations compile beside the others).
+
+#include "ssa_masked_bwd_rows.h"
+#include "ssa_masked_rows.h"
+
+namespace ssa {
+
+int masked_two_f32(tile::DenseParams& p, int kw, hipStream_t st) {
+  return p.d <= 64 ? launch_rows_rule<float, 64, kTwo>(p, kw, st) : launch_rows_rule<float, 128, kTwo>(p, kw, st);
+}
+
+int masked_two_backward_f32(void* params, const BwdCut& cut, hipStream_t st) {
+  BwdParams& p = *static_cast<BwdParams*>(params);
+  return p.d <= 64 ? launch_rule<float, 64, kTwo>(p, cut, st) : launch_rule<float, 128, kTwo>(p, cut, st);
+}
+
+}  // namespace ssa

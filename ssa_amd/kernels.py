@@ -558,9 +558,10 @@ def _pos0(q_pos0: Optional[int], n: int, n_q: int, spans, slopes) -> int:
 
 
 def mask_spans(n: int, batch: int, n_q: int, q_pos0: int, causal: bool, doc_starts: Optional[torch.Tensor],
-               prefix_lens: Optional[torch.Tensor], device: torch.device) -> torch.Tensor:
-    """Key interval of each row, int32 [batch, n_q, 2] (ssa_mask_spans)."""
-    out = torch.empty((batch, n_q, 2), device=device, dtype=torch.int32)
+               prefix_lens: Optional[torch.Tensor], device: torch.device, window: int = 0, sinks: int = 0) -> torch.Tensor:
+    """Key interval of each row, int32 [batch, n_q, 2] (ssa_mask_spans), or two of them,
+    [batch, n_q, 4], with a ``window`` (ssa_mask_spans_window)."""
+    out = torch.empty((batch, n_q, 4 if window else 2), device=device, dtype=torch.int32)
     dev = _on_device(out, doc_starts, prefix_lens)
     docs = 1 if doc_starts is None else doc_starts.shape[-1] - 1
     if doc_starts is not None:
@@ -571,6 +572,10 @@ def mask_spans(n: int, batch: int, n_q: int, q_pos0: int, causal: bool, doc_star
         if tuple(prefix_lens.shape) != (batch, docs):
             raise ValueError(f"prefix_lens must be [{batch}, {docs}], got {tuple(prefix_lens.shape)}")
         prefix_lens = _index32(prefix_lens, "prefix_lens")
+    if window:
+        _call_on(dev, "ssa_mask_spans_window", _at(doc_starts), docs, _at(prefix_lens), batch, n, n_q, q_pos0, window, sinks,
+                 out.data_ptr())
+        return out
     _call_on(dev, "ssa_mask_spans", _at(doc_starts), docs, _at(prefix_lens), batch, n, n_q, q_pos0, int(bool(causal)),
              out.data_ptr())
     return out
@@ -596,9 +601,16 @@ def _check_dense(q, k, v, spans):
         raise ValueError(f"k and v must be [{B}, n, h_kv, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
     if h_kv == 0 or h_q % h_kv != 0:
         raise ValueError(f"{h_q} query heads are not divisible by {h_kv} KV heads")
-    if spans is not None and (spans.dtype != torch.int32 or tuple(spans.shape) != (B, n_q, 2) or not spans.is_contiguous()):
-        raise ValueError(f"spans must be a contiguous int32 [{B}, {n_q}, 2] tensor")
+    if spans is not None:
+        if spans.dtype != torch.int32 or spans.shape not in ((B, n_q, 2), (B, n_q, 4)) or not spans.is_contiguous():
+            raise ValueError(f"spans must be a contiguous int32 [{B}, {n_q}, 2] or [{B}, {n_q}, 4] tensor")
+        if spans.shape[-1] == 4 and spans.data_ptr() % 16:
+            raise ValueError("spans of two intervals must be aligned to 16 bytes")
     return B, n_q, h_q, d, n, h_kv
+
+
+def _two(spans: Optional[torch.Tensor]) -> bool:
+    return spans is not None and spans.shape[-1] == 4
 
 
 def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: Optional[torch.Tensor] = None,
@@ -607,7 +619,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: O
     """Dense attention over each row's key interval (ssa_masked_attention): [B, n_q, h_q, d]
     in q's dtype.  ``with_lse`` returns (out, out_low, lse) for the backward: what rounding left of a
     bf16 output (None for float32) and the float32 [B, h_q, n_q] log2 sums.
-    ``spans`` None: causal.  Query row i sits at key position ``q_pos0 + i`` (default n - n_q)."""
+    ``spans`` None: causal; of four columns: two intervals a row (ssa_masked_attention_two).  Query row i sits at key position ``q_pos0 + i`` (default n - n_q)."""
     dev = _on_device(q, k, v, spans, slopes)
     B, n_q, h_q, d, n, h_kv = _check_dense(q, k, v, spans)
     slopes = _check_slopes(slopes, h_q)
@@ -622,7 +634,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: O
         low = torch.empty_like(out) if dt == _lib.DTYPE_BF16 else None
     nbytes = _bytes("ssa_masked_attention_workspace_bytes", dt, B, n, n_q, h_q, h_kv, d)
     ws = _workspace(nbytes, q)
-    _call_on(dev, "ssa_masked_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, n, n_q,
+    _call_on(dev, "ssa_masked_attention_two" if _two(spans) else "ssa_masked_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, n, n_q,
              _pos0(q_pos0, n, n_q, spans, slopes), h_q, h_kv, d, *qs, *ks, *vs, _at(spans),
              math.sqrt(d) if scale_div is None else scale_div, softcap, _at(slopes), out.data_ptr(), n_q * h_q * d, h_q * d, d,
              _at(low), _at(lse), _at(ws), nbytes)
@@ -658,9 +670,10 @@ def masked_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     dout, dos = _group_rows16(dout, h_q // h_kv)
     out_low = None if out_low is None else _rows16(out_low)[0]
     dt = _lib.elem_dtype(q)
-    nbytes = _bytes("ssa_masked_attention_backward_workspace_bytes", dt, B, n, n_q, h_q, h_kv, d)
+    name = "ssa_masked_attention_two_backward" if _two(spans) else "ssa_masked_attention_backward"
+    nbytes = _bytes(name + "_workspace_bytes", dt, B, n, n_q, h_q, h_kv, d)
     ws = _workspace(nbytes, q)
-    _call_on(dev, "ssa_masked_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, n, n_q,
+    _call_on(dev, name, q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, n, n_q,
              _pos0(q_pos0, n, n_q, spans, slopes), h_q, h_kv, d, *qs, *ks, *vs, _at(spans),
              math.sqrt(d) if scale_div is None else scale_div, softcap, _at(slopes), out.data_ptr(), _at(out_low), *os,
              dout.data_ptr(), *dos, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(ws), nbytes)

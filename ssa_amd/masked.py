@@ -1,9 +1,9 @@
-"""Dense attention whose rows each see one interval of keys, with capped scores and a
+"""Dense attention whose rows each see one or two intervals of keys, with capped scores and a
 distance bias, forward and backward on HIP kernels.
 
 ``dense_attention`` (ssa/attention.py:118-158) takes an ``[n, n]`` bool mask and forms
 all n x n scores.  The masks of packed, prefixed and causal sequences are an interval
-of keys per row, which is what ``masked_attention`` takes: nothing of size n x n exists,
+of keys per row, two behind a sliding window with first keys that stay visible, which is what ``masked_attention`` takes: nothing of size n x n exists,
 and keys that no row of a tile sees are not read.
 """
 
@@ -19,8 +19,9 @@ from . import _lib, kernels
 
 def mask_spans(seq_len: int, batch: int = 1, *, causal: bool = True, doc_starts: Optional[torch.Tensor] = None,
                prefix_lens: Optional[torch.Tensor] = None, num_queries: Optional[int] = None,
-               q_pos0: Optional[int] = None, device=None) -> torch.Tensor:
-    """Key interval [lo, hi) of every row for ``masked_attention``: int32 [batch, num_queries, 2].
+               q_pos0: Optional[int] = None, device=None, window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
+    """Key interval [lo, hi) of every row for ``masked_attention``: int32 [batch, num_queries, 2],
+    or with ``window`` two of them: [batch, num_queries, 4].
 
     ``causal``: keys up to the row's own position, else all.  ``doc_starts`` (int [batch,
     documents + 1], ascending) packs documents: document x is the keys ``doc_starts[b, x]``
@@ -29,6 +30,8 @@ def mask_spans(seq_len: int, batch: int = 1, *, causal: bool = True, doc_starts:
     ``prefix_lens`` (int [batch, documents]) opens each document with that many keys that all
     its rows see, whatever their position (an image before its text).  With ``num_queries``
     rows fewer than keys, row i sits at key position ``q_pos0 + i`` (default: the last ones).
+    ``window`` w (with causal rows) leaves a row the w keys up to its own, and the first
+    ``sinks`` keys of its document (up to its own; of a prefix all).
 
     Made once for a batch, it serves every layer's forward and backward."""
     n_q = seq_len if num_queries is None else num_queries
@@ -36,6 +39,10 @@ def mask_spans(seq_len: int, batch: int = 1, *, causal: bool = True, doc_starts:
         q_pos0 = seq_len - n_q
     if prefix_lens is not None and not causal:
         raise ValueError("prefix_lens goes with causal=True: without it every row sees its whole document")
+    if window is not None and (window < 1 or not causal):
+        raise ValueError(f"window must be positive and goes with causal=True, got window={window}")
+    if sinks < 0 or (sinks > 0 and window is None):
+        raise ValueError(f"sinks must not be negative and go with a window, got sinks={sinks}, window={window}")
     if device is None:
         device = next((t.device for t in (doc_starts, prefix_lens) if t is not None), torch.device("cuda"))
     device = torch.device(device)
@@ -45,7 +52,8 @@ def mask_spans(seq_len: int, batch: int = 1, *, causal: bool = True, doc_starts:
         device = torch.device("cuda", torch.cuda.current_device())
     if prefix_lens is not None and prefix_lens.dim() == 1 and doc_starts is None:
         prefix_lens = prefix_lens[:, None]
-    return kernels.mask_spans(seq_len, batch, n_q, q_pos0, causal, doc_starts, prefix_lens, device)
+    return kernels.mask_spans(seq_len, batch, n_q, q_pos0, causal, doc_starts, prefix_lens, device,
+                              0 if window is None else min(int(window), 1 << 31), min(int(sinks), 1 << 31))
 
 
 class _MaskedAttention(torch.autograd.Function):
@@ -75,7 +83,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, spans: O
 
     ``q [B, n_q, h_q, d]``, ``k, v [B, n, h_kv, d]`` (query head j uses KV head
     ``j // (h_q // h_kv)``; unbatched shapes too); ``spans`` from ``mask_spans`` or any int32
-    ``[B, n_q, 2]`` of key intervals [lo, hi), None for causal.  Scores are q.k / scale
+    ``[B, n_q, 2]`` of key intervals [lo, hi), or ``[B, n_q, 4]`` of two each (lo, hi, lo2, hi2,
+    in any order; a key in both counts once), None for causal.  Scores are q.k / scale
     (sqrt(d)); ``softcap`` c makes them c tanh(s / c); ``slopes`` (float32 [h_q]) subtracts
     slopes[h] |position - key|, row i at position ``q_pos0 + i`` (default n - n_q).  Slopes
     get no gradient.
