@@ -221,18 +221,26 @@ __device__ __forceinline__ Sees paged_sees(const DenseParams& p, int pos, int ca
   return s;
 }
 
-// Eight bits as the value they stand for before the scale, and chunks of them as 16 bytes of T.
+// Eight bits as the value they stand for before the scale.
 __device__ __forceinline__ float code_value(uint8_t c, int e4m3) {
   return e4m3 ? __builtin_amdgcn_cvt_f32_fp8(c, 0) : static_cast<float>(static_cast<int8_t>(c));
 }
-template <int I>
-__device__ __forceinline__ float code_of(uint32_t w, int e4m3) {
-  return e4m3 ? __builtin_amdgcn_cvt_f32_fp8(w, I) : static_cast<float>(static_cast<int8_t>(w >> (8 * I)));
+// Four codes as floats.
+template <bool E4M3>
+__device__ __forceinline__ void code_floats(uint32_t w, float (&f)[4]) {
+  if constexpr (E4M3) {
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+  }
 }
+// The codes of 16 bytes of T, exact in bf16 too: eight (two words of them) or four.
 template <typename T>
 struct Codes;
 template <>
-struct Codes<uint16_t> {  // eight codes; int8 and e4m3 are exact in bf16
+struct Codes<uint16_t> {
   static __device__ __forceinline__ uint4 load(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, static_cast<int>(offset), 0, 0);
@@ -242,30 +250,34 @@ struct Codes<uint16_t> {  // eight codes; int8 and e4m3 are exact in bf16
     const uint2 x = *reinterpret_cast<const uint2*>(p);
     return make_uint4(x.x, x.y, 0u, 0u);
   }
-  static __device__ __forceinline__ uint4 widen(const uint4& x, int e4m3) {
-    const uint32_t w[2] = {x.x, x.y};
-    uint32_t o[4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      o[2 * i] = Op<uint16_t>::pack2(code_of<0>(w[i], e4m3), code_of<1>(w[i], e4m3));
-      o[2 * i + 1] = Op<uint16_t>::pack2(code_of<2>(w[i], e4m3), code_of<3>(w[i], e4m3));
-    }
-    return make_uint4(o[0], o[1], o[2], o[3]);
+  template <bool E4M3>
+  static __device__ __forceinline__ uint4 widen(uint32_t x, uint32_t y) {
+    float a[4], b[4];
+    code_floats<E4M3>(x, a);
+    code_floats<E4M3>(y, b);
+    return make_uint4(Op<uint16_t>::pack2(a[0], a[1]), Op<uint16_t>::pack2(a[2], a[3]), Op<uint16_t>::pack2(b[0], b[1]),
+                      Op<uint16_t>::pack2(b[2], b[3]));
   }
 };
 template <>
-struct Codes<float> {  // four codes
+struct Codes<float> {
   static __device__ __forceinline__ uint4 load(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
     return make_uint4(__builtin_amdgcn_raw_buffer_load_b32(r, static_cast<int>(offset), 0, 0), 0u, 0u, 0u);
   }
   static __device__ __forceinline__ uint4 load(const uint8_t* p) {
     return make_uint4(*reinterpret_cast<const uint32_t*>(p), 0u, 0u, 0u);
   }
-  static __device__ __forceinline__ uint4 widen(const uint4& x, int e4m3) {
-    return make_uint4(__float_as_uint(code_of<0>(x.x, e4m3)), __float_as_uint(code_of<1>(x.x, e4m3)),
-                      __float_as_uint(code_of<2>(x.x, e4m3)), __float_as_uint(code_of<3>(x.x, e4m3)));
+  template <bool E4M3>
+  static __device__ __forceinline__ uint4 widen(uint32_t x, uint32_t) {
+    float a[4];
+    code_floats<E4M3>(x, a);
+    return make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
   }
 };
+template <typename T>
+__device__ __forceinline__ uint4 widen_one(const uint4& x, int e4m3) {
+  return e4m3 ? Codes<T>::template widen<true>(x.x, x.y) : Codes<T>::template widen<false>(x.x, x.y);
+}
 
 // The row of key j: contiguous keys, or the sequence's pages (its new rows where the
 // call brought them).  S is what the pages hold: T, or uint8_t for 8-bit codes, whose rows
@@ -782,8 +794,8 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
           } else {
             const S *kr, *vr;
             rows.code_rows(rows.checked(rows.entry_of(x)), x, kr, vr);
-            kreg[i] = Codes<T>::widen(Codes<T>::load(kr + sc * E), rows.e4m3);
-            vreg[i] = Codes<T>::widen(Codes<T>::load(vr + sc * E), rows.e4m3);
+            kreg[i] = widen_one<T>(Codes<T>::load(kr + sc * E), rows.e4m3);
+            vreg[i] = widen_one<T>(Codes<T>::load(vr + sc * E), rows.e4m3);
           }
         }
         return;
@@ -833,13 +845,20 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
     char* kt = lds + buf * 2 * TB;
     if constexpr (HELD) {
       if (tid < 2 * KT) s_scale[2 * buf + (tid >= KT ? 1 : 0)][tid & (KT - 1)] = scale_reg;
-      if (as_codes) {
+      auto put = [&](auto kind) {
+        constexpr bool E4M3 = decltype(kind)::value;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           const int at = chunk_at<RB>(sr + i * RPP, sc);
-          *reinterpret_cast<uint4*>(kt + at) = Codes<T>::widen(kreg[i], rows.e4m3);
-          *reinterpret_cast<uint4*>(kt + TB + at) = Codes<T>::widen(vreg[i], rows.e4m3);
+          *reinterpret_cast<uint4*>(kt + at) = Codes<T>::template widen<E4M3>(kreg[i].x, kreg[i].y);
+          *reinterpret_cast<uint4*>(kt + TB + at) = Codes<T>::template widen<E4M3>(vreg[i].x, vreg[i].y);
         }
+      };
+      if (as_codes) {
+        if (rows.e4m3)
+          put(std::true_type());
+        else
+          put(std::false_type());
         return;
       }
     }

@@ -283,7 +283,11 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
   char* vt = kt + TB;
   const int sc = lane % NCH, sr = lane / NCH;
   const bool chunk_ok = sc * E < p.d;
-  uint4 kreg[NP], vreg[NP];
+  // HELD: a load covers eight rows of one page, eight lanes a row (16 codes each, or 8 of 64 features)
+  constexpr int CB = D / 8, NW = CB / 4;  // bytes and words of a lane's chunk
+  uint4 kreg[HELD ? 4 : NP], vreg[HELD ? 4 : NP];
+  const int my_row = lane >> 3, my_at = (lane & 7) * CB;
+  const uint32_t ks8 = static_cast<uint32_t>(rows.k_sn), vs8 = static_cast<uint32_t>(rows.v_sn);
   // kTwo: a key of the sequence that stands for key j where j is looked up, one that some row sees
   auto seen_key = [&](int j) { return min(j >= first_a ? max(j, from) : j, k_end - 1); };
   // HELD: the last key in the pages where j is a new one
@@ -300,12 +304,26 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
       const int j = seen_key(k0 + rr);
       scale_reg = rows.is_new(j) ? 1.0f : rows.scale_of(half != 0, pg, j);
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int r = sr + i * RPW;
-        const S *kr, *vr;
-        rows.code_rows(__shfl(pg, r, 64), min(seen_key(k0 + r), paged_last), kr, vr);
-        kreg[i] = chunk_ok ? Codes<T>::load(kr + sc * E) : make_uint4(0u, 0u, 0u, 0u);
-        vreg[i] = chunk_ok ? Codes<T>::load(vr + sc * E) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < 4; ++i) {
+        const int64_t page = lane_value(pg, 8 * i), r0 = (k0 + 8 * i) & rows.page_mask;
+        const auto kb = row_buffer(rows.k + page * rows.k_sb + r0 * rows.k_sn, kAllBytes);
+        const auto vb = row_buffer(rows.v + page * rows.v_sb + r0 * rows.v_sn, kAllBytes);
+        const uint32_t ko = my_row * ks8 + my_at, vo = my_row * vs8 + my_at;
+        if constexpr (CB == 16) {
+          if (p.d & 8) {  // (rows of 8 bytes more than 16s: a chunk's second half may lie past the row)
+            const bool a = my_at < p.d, b = my_at + 8 < p.d;
+            const uint4 k0_ = Codes<uint16_t>::load(kb, a ? ko : kNoChunk), k1_ = Codes<uint16_t>::load(kb, b ? ko + 8 : kNoChunk);
+            const uint4 v0_ = Codes<uint16_t>::load(vb, a ? vo : kNoChunk), v1_ = Codes<uint16_t>::load(vb, b ? vo + 8 : kNoChunk);
+            kreg[i] = make_uint4(k0_.x, k0_.y, k1_.x, k1_.y);
+            vreg[i] = make_uint4(v0_.x, v0_.y, v1_.x, v1_.y);
+          } else {
+            kreg[i] = row_load(kb, my_at < p.d ? ko : kNoChunk);
+            vreg[i] = row_load(vb, my_at < p.d ? vo : kNoChunk);
+          }
+        } else {
+          kreg[i] = Codes<uint16_t>::load(kb, my_at < p.d ? ko : kNoChunk);
+          vreg[i] = Codes<uint16_t>::load(vb, my_at < p.d ? vo : kNoChunk);
+        }
       }
       return;
     }
@@ -336,15 +354,35 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
   settle(qf);
   for (; x < x_end; x += STEP) {
     const int k0 = key_at(x);
+    if constexpr (!HELD) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int at = chunk_at<RB>(sr + i * RPW, sc);
-      *reinterpret_cast<uint4*>(kt + at) = HELD ? Codes<T>::widen(kreg[i], rows.e4m3) : kreg[i];
-      *reinterpret_cast<uint4*>(vt + at) = HELD ? Codes<T>::widen(vreg[i], rows.e4m3) : vreg[i];
-    }
-    if constexpr (HELD) {
+      for (int i = 0; i < NP; ++i) {
+        const int at = chunk_at<RB>(sr + i * RPW, sc);
+        *reinterpret_cast<uint4*>(kt + at) = kreg[i];
+        *reinterpret_cast<uint4*>(vt + at) = vreg[i];
+      }
+    } else {
+      auto put = [&](auto kind) {
+        constexpr bool E4M3 = decltype(kind)::value;
+        constexpr int W = sizeof(T) == 2 ? 2 : 1;  // words of codes that make 16 bytes of T
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t kw[4] = {kreg[i].x, kreg[i].y, kreg[i].z, kreg[i].w}, vw[4] = {vreg[i].x, vreg[i].y, vreg[i].z, vreg[i].w};
+#pragma unroll
+          for (int c = 0; c < NW / W; ++c) {
+            const int at = chunk_at<RB>(8 * i + my_row, (lane & 7) * (NW / W) + c);
+            *reinterpret_cast<uint4*>(kt + at) = Codes<T>::template widen<E4M3>(kw[W * c], kw[(W * c + 1) & 3]);
+            *reinterpret_cast<uint4*>(vt + at) = Codes<T>::template widen<E4M3>(vw[W * c], vw[(W * c + 1) & 3]);
+          }
+        }
+      };
+      if (rows.e4m3)
+        put(std::true_type());
+      else
+        put(std::false_type());
       s_scale[wave][half][rr] = scale_reg;
       if (k0 + 32 > rows.new_from) {  // the call's own rows, as they are given
+        wave_lds_sync();  // (over what other lanes have put there)
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           const int r = sr + i * RPW, j = seen_key(k0 + r);
