@@ -109,11 +109,12 @@ inline BwdCut bwd_cut(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q,
   return l;
 }
 
-// The backward of rows that see two intervals: blocks of keys, extra parts that dkv_kernel's plan
-// may give them (as many as fill the device once: bwd_cut's target), and the workspace.
+// The backward of rows that see two intervals: blocks of keys, how many of a head run at a time
+// (slots), the parts that dkv_kernel's plan may cut blocks into (extra, and one more for each that
+// it cuts), and the workspace.
 struct TwoCut {
   int64_t key_blocks;
-  int extra;
+  int slots, extra, most;
   size_t counts, entries, cut, part, part_floats, bytes;
 };
 
@@ -122,23 +123,26 @@ inline TwoCut two_cut(const BwdCut& l, int dtype, int64_t batch, int64_t n, int 
   const bool f32 = dtype == SSA_DTYPE_F32, wide = d > 64;
   const int64_t keys = 32 * l.key_groups;
   t.key_blocks = div_up(n, keys) * batch;
-  t.extra = static_cast<int>(div_up(!f32 && !wide ? 1024 : 512, h_kv));
-  // (no more slots than each block of keys with a part for every group of rows)
-  const int64_t all = t.key_blocks * l.groups, slots = all < 2 * t.extra ? all : 2 * t.extra;
+  // a CU holds one block of bf16 at 128 features (its K and V lie in the LDS), two of the others
+  t.slots = static_cast<int>(div_up(!f32 && wide ? 256 : 512, h_kv));
+  t.extra = 4 * t.slots;
+  t.most = t.extra + 2 * t.slots;
+  // (no more parts than each block of keys with one for every group of rows)
+  const int64_t all = t.key_blocks * l.groups, parts = all < t.most ? all : t.most;
   t.counts = l.bounds + 2 * static_cast<size_t>(batch) * l.groups * 16;
   t.entries = (t.counts + static_cast<size_t>(t.key_blocks) * 4 + 15) / 16 * 16;
-  t.cut = t.entries + static_cast<size_t>(t.key_blocks + t.extra) * 16;
-  t.part = t.cut + static_cast<size_t>(t.extra) * 16;
-  t.part_floats = static_cast<size_t>(slots) * h_kv * keys * (wide ? 128 : 64);
+  t.cut = t.entries + static_cast<size_t>(t.key_blocks + t.most) * 16;
+  t.part = t.cut + static_cast<size_t>(2 * t.slots + 1) * 16;
+  t.part_floats = static_cast<size_t>(parts) * h_kv * keys * (wide ? 128 : 64);
   t.bytes = t.part + 2 * t.part_floats * sizeof(float);
   return t;
 }
 
 // The most keys of a sequence of max_len that its call reads: with a window, the first keys
-// and those of the window and the new tokens, in whole tiles.
+// and those of the window and the new tokens, in whole tiles of up to 128.
 inline int64_t seen_len(int64_t max_len, int64_t max_new, int64_t window, int64_t sinks) {
   if (window <= 0 || window >= max_len || sinks >= max_len) return max_len;
-  const int64_t some = div_up(sinks, 128) * 128 + window + max_new + 128;
+  const int64_t some = div_up(sinks, 128) * 128 + window + max_new + 256;
   return some < max_len ? some : max_len;
 }
 
@@ -149,7 +153,9 @@ struct PagedPlan {
   size_t few_o, few_ml, row_o, row_ml, bytes;
 };
 
-inline PagedPlan paged_plan(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t max_new, int64_t max_len) {
+// whole_tiles: parts of the keys of many rows are multiples of as many.
+inline PagedPlan paged_plan(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t max_new, int64_t max_len,
+                            int64_t whole_tiles = 64) {
   PagedPlan l{};
   max_new = max_new < tokens ? max_new : tokens;
   const int64_t g = h_q / h_kv, D = d <= 64 ? 64 : 128;
@@ -172,7 +178,7 @@ inline PagedPlan paged_plan(int dtype, int64_t tokens, int64_t batch, int h_q, i
     l.row_kw = cut.kw;
     l.row_tiles = static_cast<int>(by_seq < ragged ? by_seq : ragged);
     l.row_splits = cut.parts;
-    l.row_len = div_up(div_up(max_len, l.row_splits), 64) * 64;
+    l.row_len = div_up(div_up(max_len, l.row_splits), whole_tiles) * whole_tiles;
   }
   if (l.few_splits > 1) {
     const size_t rows = static_cast<size_t>(l.few_splits) * batch * h_kv * kFew;

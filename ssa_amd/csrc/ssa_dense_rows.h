@@ -720,9 +720,17 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
   }
   int t0, nt;
   if constexpr (SETS) {
-    const int per = (walk.n + p.splits - 1) / p.splits;
-    t0 = min(split * per, walk.n);
+    // parts are equal shares of the block's tiles; over pages as long as each other (p.split_len keys),
+    // so that short sequences have few
+    const int per = TREE ? (p.splits > 1 ? static_cast<int>(p.split_len / KT) : walk.n) : (walk.n + p.splits - 1) / p.splits;
+    t0 = static_cast<int>(min(static_cast<int64_t>(split) * per, static_cast<int64_t>(walk.n)));
     nt = min(per, walk.n - t0);
+    if (p.splits > 1 && nt == 0) {  // (a part without a key: the join wants its sums alone)
+      const int64_t at = (PAGED ? first : static_cast<int64_t>(b) * p.n_q) + tok;
+      if (real && half == 0 && kw == 0)
+        *reinterpret_cast<float2*>(p.part_ml + (split * p.part_rows + at * p.h_q + hq) * 2) = make_float2(-INFINITY, 0.0f);
+      return;
+    }
     part_x[0] = (walk.x0 + min(t0, walk.n1)) * KT;
     part_y[0] = (walk.x0 + min(t0 + nt, walk.n1)) * KT;
     part_x[1] = (walk.y0 + max(t0 - walk.n1, 0)) * KT;

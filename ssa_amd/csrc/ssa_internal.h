@@ -59,16 +59,19 @@ struct DenseParams;
 }
 struct PagedPlan;
 struct BwdCut;
+struct TwoCut;
 
 // ssa_masked_attention_two's kernels, and its backward's (params: the BwdParams of
 // ssa_masked_bwd_rows.h, the same type in every file that includes it).
 int masked_two_f32(tile::DenseParams& p, int kw, hipStream_t st);
 int masked_two_bf16(tile::DenseParams& p, int kw, hipStream_t st);
-int masked_two_backward_f32(void* params, const BwdCut& cut, hipStream_t st);
-int masked_two_backward_bf16(void* params, const BwdCut& cut, hipStream_t st);
+int masked_two_backward_f32(void* params, const BwdCut& cut, const TwoCut& two, hipStream_t st);
+int masked_two_backward_bf16(void* params, const BwdCut& cut, const TwoCut& two, hipStream_t st);
 
-// ssa_paged_step's kernels of windows and trees (two), and over pages of 8 bits (held); wide:
-// more than 64 features.
+// ssa_paged_step's kernels (one), those of windows and trees (two), and those over pages of 8 bits
+// (held); wide: more than 64 features.
+int paged_one_f32(tile::DenseParams& p, const PagedPlan& l, bool wide, bool zero_rows, char* ws, hipStream_t st);
+int paged_one_bf16(tile::DenseParams& p, const PagedPlan& l, bool wide, bool zero_rows, char* ws, hipStream_t st);
 int paged_two_f32(tile::DenseParams& p, const PagedPlan& l, bool wide, bool zero_rows, char* ws, hipStream_t st);
 int paged_two_bf16(tile::DenseParams& p, const PagedPlan& l, bool wide, bool zero_rows, char* ws, hipStream_t st);
 int paged_held_f32(tile::DenseParams& p, const PagedPlan& l, bool wide, bool zero_rows, char* ws, hipStream_t st);

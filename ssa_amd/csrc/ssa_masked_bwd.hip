@@ -108,14 +108,14 @@ static int backward(
     p.cut = reinterpret_cast<int4*>(ws + two_l.cut);
     p.part_k = reinterpret_cast<float*>(ws + two_l.part);
     p.part_v = p.part_k + two_l.part_floats;
-    return dtype == SSA_DTYPE_F32 ? masked_two_backward_f32(&p, l, st) : masked_two_backward_bf16(&p, l, st);
+    return dtype == SSA_DTYPE_F32 ? masked_two_backward_f32(&p, l, two_l, st) : masked_two_backward_bf16(&p, l, two_l, st);
   }
   if (l.splits > 1) {
     p.part_k = reinterpret_cast<float*>(ws + l.part);
     p.part_v = p.part_k + static_cast<int64_t>(l.splits) * batch * n * h_kv * (d <= 64 ? 64 : 128);
   }
-  if (dtype == SSA_DTYPE_F32) return d <= 64 ? launch_rule<float, 64, kOne>(p, l, st) : launch_rule<float, 128, kOne>(p, l, st);
-  return d <= 64 ? launch_rule<uint16_t, 64, kOne>(p, l, st) : launch_rule<uint16_t, 128, kOne>(p, l, st);
+  if (dtype == SSA_DTYPE_F32) return d <= 64 ? launch_rule<float, 64, kOne>(p, l, two_l, st) : launch_rule<float, 128, kOne>(p, l, two_l, st);
+  return d <= 64 ? launch_rule<uint16_t, 64, kOne>(p, l, two_l, st) : launch_rule<uint16_t, 128, kOne>(p, l, two_l, st);
 }
 
 extern "C" int ssa_masked_attention_backward(

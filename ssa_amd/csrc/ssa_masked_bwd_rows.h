@@ -30,10 +30,9 @@
 // the tiles of both.  For dK and dV the first keys of a document are seen by all of its rows
 // and others by a window of them, 14 times as few where 16384 rows see 1024 keys back, so that
 // blocks of equal keys are not blocks of equal work.  Two small kernels look at the groups'
-// bounds first: plan_count counts the row tiles that see each block of keys, plan_list gives
-// blocks with more than a share of all of them several parts (and their slots in the workspace),
-// the cut ones first, so that no part is longer than what a CU has to do anyway.  Only cut
-// blocks of keys go through fp32 parts.
+// bounds first: plan_count counts the row tiles that see each block of keys, plan_list cuts blocks
+// with more than their share of all of them into parts (and gives these slots of the workspace).
+// Only cut blocks of keys go through fp32 parts.
 //
 // Masked rows or keys that hold infinities or NaN: as in the forward, sums that
 // end up other than finite are computed again pair by pair, visible pairs only.
@@ -69,8 +68,8 @@ struct BwdParams {
   // batch elements, how many tiles of rows see each, and what the blocks of dkv_kernel take
   int key_blocks, key_tiles, extra;
   int32_t* counts;  // [key_blocks]
-  int4* entries;    // [key_blocks + extra]: block of keys (-1: nothing), part, parts, first slot
-  int4* cut;        // [extra]: block of keys (-1: none), parts, first slot
+  int4* entries;    // [key_blocks + most]: block of keys (-1: nothing), part, parts, first slot
+  int4* cut;        // how many, then of each its block of keys (-1: in one part), parts, first slot
 };
 
 constexpr int kBlk = 128;  // rows or keys of a block
@@ -904,82 +903,160 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(BwdParams p) {
   if (threadIdx.x == 0) p.counts[at] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
 }
 
-// The blocks of dkv_kernel, by one block: a block of keys that more than C tiles see takes one
-// part for every C of them, C the share of `extra` parts (and at least `least`).  Those cut come
-// first.  At most key_blocks + extra entries, extra cut blocks and 2 extra slots.
-constexpr int kPlan = 1024;
-[[maybe_unused]] __global__ __launch_bounds__(kPlan) void plan_list_kernel(BwdParams p, int least) {
-  __shared__ int s_wave[2][kPlan / 64];
-  __shared__ int64_t s_total[kPlan / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int64_t mine = 0;
-  for (int x = tid; x < p.key_blocks; x += kPlan) mine += p.counts[x];
+// The blocks of dkv_kernel, by one block.  A slot is a block of keys, of one head, that runs at a
+// time; share = what each of `slots` has to do on average.
+//   h tiles > share   cut into parts of a tenth of the share (the more of them there are, the
+//                     longer, up to a quarter: `extra` parts in all)
+//   the others        whole, the longest first, so that the device's last blocks are short ones;
+//                     where those of the last round would leave a good part of it idle they are cut
+//                     until they fill it
+// parts come after whole blocks (16001 rows that see 1000 keys back and 4 first ones, 16 / 4 heads,
+// d = 128: dK and dV 640 us with parts first and as long as whole blocks, MEASURED so).
+// At most key_blocks + most entries, most parts, 2 slots cut blocks.
+constexpr int kPlan = 1024, kSorted = 2 * kPlan;
+struct PlanSums {
+  int64_t wave[kPlan / 64];
+};
+__device__ __forceinline__ int64_t plan_sum(int64_t x, PlanSums& s) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o, 64);
-  if (lane == 0) s_total[wave] = mine;
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
   __syncthreads();
-  int64_t total = 0;
-  for (int x = 0; x < kPlan / 64; ++x) total += s_total[x];
-  const int64_t share = (total + p.extra - 1) / p.extra;
-  const int C = static_cast<int>(share > least ? share : least);
-  int at_part = 0, at_cut = 0, at_one = 0;  // entries of cut blocks, cut blocks, entries of others so far
-  for (int pass = 0; pass < 2; ++pass) {    // the cut ones, then the others
-    for (int x0 = 0; x0 < p.key_blocks; x0 += kPlan) {
-      const int x = x0 + tid, h = x < p.key_blocks ? p.counts[x] : 0;
-      const int parts = x < p.key_blocks ? (h > C ? (h + C - 1) / C : 1) : 0;
-      const int put = pass == 0 ? (parts > 1 ? parts : 0) : (parts == 1 ? 1 : 0), one = put > 0 ? 1 : 0;
-      const int i1 = wave_incl_scan(put), i2 = wave_incl_scan(one);
-      __syncthreads();
-      if (lane == 63) {
-        s_wave[0][wave] = i1;
-        s_wave[1][wave] = i2;
-      }
-      __syncthreads();
-      int b1 = 0, b2 = 0, all1 = 0, all2 = 0;
-      for (int y = 0; y < kPlan / 64; ++y) {
-        const int v = s_wave[0][y], u = s_wave[1][y];
-        if (y < wave) {
-          b1 += v;
-          b2 += u;
-        }
-        all1 += v;
-        all2 += u;
-      }
-      if (pass == 0) {
-        const int from = at_part + b1 + i1 - put;
-        if (put > 0) p.cut[at_cut + b2 + i2 - one] = make_int4(x, parts, from, 0);
-        for (int y = 0; y < put; ++y) p.entries[from + y] = make_int4(x, y, parts, from);
-        at_part += all1;
-        at_cut += all2;
-      } else {
-        if (put > 0) p.entries[at_part + at_one + b1 + i1 - put] = make_int4(x, 0, 1, 0);
-        at_one += all1;
-      }
-    }
+  if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = x;
+  __syncthreads();
+  int64_t all = 0;
+  for (int y = 0; y < kPlan / 64; ++y) all += s.wave[y];
+  return all;
+}
+// Exclusive sums over the block's threads, and the whole block's.
+__device__ __forceinline__ int plan_scan(int x, int (&s)[kPlan / 64], int& all) {
+  const int incl = wave_incl_scan(x), wave = threadIdx.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) s[wave] = incl;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+  for (int y = 0; y < kPlan / 64; ++y) {
+    if (y < wave) before += s[y];
+    all += s[y];
   }
-  for (int x = at_part + at_one + tid; x < p.key_blocks + p.extra; x += kPlan) p.entries[x] = make_int4(-1, 0, 0, 0);
-  for (int x = at_cut + tid; x < p.extra; x += kPlan) p.cut[x] = make_int4(-1, 0, 0, 0);
+  return before + incl - x;
 }
 
-// dk and dv of the cut blocks of keys, four features a thread, in part order.
-constexpr int kJoinPieces = 8;  // blocks a head of a cut block
+[[maybe_unused]] __global__ __launch_bounds__(kPlan) void plan_list_kernel(BwdParams p, int least, int slots, int most) {
+  __shared__ PlanSums s_sums;
+  __shared__ int s_scan[kPlan / 64];
+  __shared__ __align__(16) int s_h[kSorted + 16];
+  const int tid = threadIdx.x, N = p.key_blocks;
+  const bool sorted = N <= kSorted;
+  int64_t mine = 0;
+  for (int x = tid; x < N; x += kPlan) {
+    const int h = p.counts[x];
+    mine += h;
+    if (sorted) s_h[x] = h;
+  }
+  if (sorted && tid < 16) s_h[N + tid] = 0x7FFFFFFF;
+  const int64_t total = plan_sum(mine, s_sums);
+  const int64_t share = max((total + slots - 1) / slots, static_cast<int64_t>(least));
+  int64_t big = 0, n_big = 0;
+  for (int x = tid; x < N; x += kPlan) {
+    const int h = p.counts[x];
+    if (h > share) {
+      big += h;
+      ++n_big;
+    }
+  }
+  big = plan_sum(big << 24 | n_big, s_sums);  // (few are big: fewer than 2^24 of them, and tiles below 2^39)
+  n_big = big & 0xFFFFFF;
+  big >>= 24;
+  const int P = static_cast<int>(max(max(static_cast<int64_t>(least), (big + p.extra - 1) / p.extra), share / 10));
+  // whole blocks of the last round
+  const int n_one = N - static_cast<int>(n_big), left = n_one % slots;
+  const bool cut_left = sorted && n_one > slots && n_one < 4 * slots && left > 0 && 10 * left < 7 * slots;
+  const int n_whole = n_one - (cut_left ? left : 0);
+  int rank[kSorted / kPlan];
+#pragma unroll
+  for (int c = 0; c < kSorted / kPlan; ++c) {
+    rank[c] = 0;
+    const int x = c * kPlan + tid;
+    if (!sorted || x >= N || s_h[x] > share) continue;
+    const int h = s_h[x], top = static_cast<int>(share);
+    int n = 0;
+#pragma unroll 4
+    for (int y = 0; y < N; y += 4) {  // (s_h is padded with blocks past any share)
+      const int4 o = *reinterpret_cast<const int4*>(&s_h[y]);
+      n += (o.x <= top && (o.x > h || (o.x == h && y < x))) + (o.y <= top && (o.y > h || (o.y == h && y + 1 < x))) +
+           (o.z <= top && (o.z > h || (o.z == h && y + 2 < x))) + (o.w <= top && (o.w > h || (o.w == h && y + 3 < x)));
+    }
+    rank[c] = n;
+  }
+  int P2 = P;
+  if (cut_left) {
+    int64_t sum = 0;
+#pragma unroll
+    for (int c = 0; c < kSorted / kPlan; ++c) {
+      const int x = c * kPlan + tid;
+      if (x < N && s_h[x] <= share && rank[c] >= n_whole) sum += s_h[x];
+    }
+    sum = plan_sum(sum, s_sums);
+    P2 = static_cast<int>(max(static_cast<int64_t>(least), (sum + slots - 1) / slots));
+  }
+  int at_part = 0, at_cut = 0, at_one = 0;
+  for (int x0 = 0, c = 0; x0 < N; x0 += kPlan, ++c) {
+    const int x = x0 + tid, h = x < N ? p.counts[x] : 0;
+    const bool is_big = x < N && h > share;
+    const int rk = sorted ? (c == 0 ? rank[0] : rank[1]) : 0;
+    const bool is_left = cut_left && x < N && !is_big && rk >= n_whole;
+    int parts = is_big ? (h + P - 1) / P : (is_left ? (h + P2 - 1) / P2 : 0);
+    if (is_left && parts < 1) parts = 1;  // (nobody sees it: its zeros go through a part)
+    const int whole = x < N && !is_big && !is_left ? 1 : 0;
+    int all_parts, all_cut, all_one;
+    const int b_part = plan_scan(parts, s_scan, all_parts), b_cut = plan_scan(parts > 0 ? 1 : 0, s_scan, all_cut);
+    const int b_one = plan_scan(whole, s_scan, all_one);
+    if (whole) p.entries[sorted ? rk : at_one + b_one] = make_int4(x, 0, 1, 0);
+    if (parts > 0) {
+      const int from = at_part + b_part;
+      // (a block in one part is whole: it needs no join)
+      p.cut[1 + at_cut + b_cut] = make_int4(parts > 1 ? x : -1, parts, from, 0);
+      for (int y = 0; y < parts; ++y) p.entries[n_whole + from + y] = make_int4(x, y, parts, from);
+    }
+    at_part += all_parts;
+    at_cut += all_cut;
+    at_one += all_one;
+  }
+  if (tid == 0) p.cut[0] = make_int4(at_cut, 0, 0, 0);
+  for (int x = n_whole + at_part + tid; x < N + most; x += kPlan) p.entries[x] = make_int4(-1, 0, 0, 0);
+}
+
+// dk and dv of the cut blocks of keys, four features a thread, in part order, four parts' loads
+// in flight.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void dkv_two_join_kernel(BwdParams p, int keys) {
-  const int4 c = p.cut[blockIdx.x / p.h_kv];
-  if (c.x < 0) return;
-  const int kvh = blockIdx.x % p.h_kv, b = c.x / p.key_tiles, k0 = (c.x - b * p.key_tiles) * keys, per = p.d / 4;
-  for (int x = blockIdx.y * 256 + threadIdx.x; x < 2 * keys * per; x += kJoinPieces * 256) {
+  const int per = p.d / 4, work = 2 * keys * per, pieces = (work + 255) / 256;
+  const int items = p.cut[0].x * p.h_kv * pieces;
+  for (int it = blockIdx.x; it < items; it += gridDim.x) {
+    const int rest = it / pieces, x = (it - rest * pieces) * 256 + threadIdx.x;
+    const int4 c = p.cut[1 + rest / p.h_kv];
+    const int kvh = rest % p.h_kv;
+    if (c.x < 0 || x >= work) continue;
+    const int b = c.x / p.key_tiles, k0 = (c.x - b * p.key_tiles) * keys;
     const bool isv = x >= keys * per;
     const int u = isv ? x - keys * per : x, key = u / per, dd = (u - key * per) * 4;
     if (k0 + key >= p.n) continue;
+    const int64_t step = static_cast<int64_t>(p.h_kv) * keys * D;
     const float* part = (isv ? p.part_v : p.part_k) + ((static_cast<int64_t>(c.z) * p.h_kv + kvh) * keys + key) * D + dd;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int y = 0; y < c.y; ++y) {
-      const float4 a = *reinterpret_cast<const float4*>(part + static_cast<int64_t>(y) * p.h_kv * keys * D);
-      s.x += a.x;
-      s.y += a.y;
-      s.z += a.z;
-      s.w += a.w;
+    for (int y0 = 0; y0 < c.y; y0 += 4) {
+      float4 a[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) a[y] = *reinterpret_cast<const float4*>(part + min(y0 + y, c.y - 1) * step);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        if (y0 + y >= c.y) continue;
+        s.x += a[y].x;
+        s.y += a[y].y;
+        s.z += a[y].z;
+        s.w += a[y].w;
+      }
     }
     const int64_t id = (static_cast<int64_t>(b) * p.n + k0 + key) * p.h_kv + kvh;
     Op<T>::store4(static_cast<T*>(isv ? p.dv : p.dk) + id * p.d + dd, s.x, s.y, s.z, s.w);
@@ -998,21 +1075,21 @@ int launch_dq(BwdParams& p, hipStream_t st) {
 }
 
 template <typename T, int D, int RULE, int KG, int RW, int VIEW>
-int launch_dkv(BwdParams& p, hipStream_t st) {
+int launch_dkv(BwdParams& p, const TwoCut& cut, hipStream_t st) {
   const char* fn = "ssa_masked_attention_backward";
   using S = DkvShape<T, D, KG, RW>;
   if (int rc = reserve_lds(reinterpret_cast<const void*>(dkv_kernel<T, D, RULE, KG, RW, VIEW>), S::lds + (VIEW == kTwo ? 32 : 24) * S::QT * 2 + 1024, fn)) return rc;
   if constexpr (VIEW == kTwo) {
     // (parts of at least 128 rows, as of one interval)
     constexpr int least = S::QT < 128 ? 128 / S::QT : 1;
-    const int64_t grid = static_cast<int64_t>(p.key_blocks + p.extra) * p.h_kv;
+    const int64_t grid = static_cast<int64_t>(p.key_blocks + cut.most) * p.h_kv;
     if (grid > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many keys", fn);
     plan_count_kernel<<<dim3(static_cast<unsigned>(p.key_blocks)), dim3(256), 0, st>>>(p, 32 * KG, S::SG);
-    plan_list_kernel<<<dim3(1), dim3(kPlan), 0, st>>>(p, least);
+    plan_list_kernel<<<dim3(1), dim3(kPlan), 0, st>>>(p, least, cut.slots, cut.most);
     if (int rc = check_launch("ssa_masked_attention_backward plan")) return rc;
     dkv_kernel<T, D, RULE, KG, RW, VIEW><<<dim3(static_cast<unsigned>(grid)), dim3(S::kThr), S::lds, st>>>(p);
     if (int rc = check_launch("ssa_masked_attention_backward dkv")) return rc;
-    dkv_two_join_kernel<T, D><<<dim3(static_cast<unsigned>(p.extra * p.h_kv), kJoinPieces), dim3(256), 0, st>>>(p, 32 * KG);
+    dkv_two_join_kernel<T, D><<<dim3(1024), dim3(256), 0, st>>>(p, 32 * KG);
     return check_launch("ssa_masked_attention_backward join");
   }
   const int64_t nbh = static_cast<int64_t>(p.batch) * p.h_kv;
@@ -1029,7 +1106,7 @@ int launch_dkv(BwdParams& p, hipStream_t st) {
 }
 
 template <typename T, int D, int RULE, int VIEW>
-int launch_bwd(BwdParams& p, const BwdCut& cut, hipStream_t st) {
+int launch_bwd(BwdParams& p, const BwdCut& cut, const TwoCut& two, hipStream_t st) {
   int rc;
   if (most_kw<T, D>() >= 4 && cut.kw == 4)
     rc = launch_dq<T, D, RULE, most_kw<T, D>(), VIEW>(p, st);
@@ -1037,22 +1114,22 @@ int launch_bwd(BwdParams& p, const BwdCut& cut, hipStream_t st) {
     rc = cut.kw >= 2 ? launch_dq<T, D, RULE, 2, VIEW>(p, st) : launch_dq<T, D, RULE, 1, VIEW>(p, st);
   if (rc) return rc;
   if constexpr (sizeof(T) == 2 && D == 128) {
-    return cut.key_groups == 4 ? launch_dkv<T, D, RULE, 4, 2, VIEW>(p, st) : launch_dkv<T, D, RULE, 2, 2, VIEW>(p, st);
+    return cut.key_groups == 4 ? launch_dkv<T, D, RULE, 4, 2, VIEW>(p, two, st) : launch_dkv<T, D, RULE, 2, 2, VIEW>(p, two, st);
   } else {
     if constexpr (D == 64)
-      if (cut.key_groups == 1) return launch_dkv<T, D, RULE, 1, 4, VIEW>(p, st);
-    return cut.key_groups == 4 ? launch_dkv<T, D, RULE, 4, 1, VIEW>(p, st) : launch_dkv<T, D, RULE, 2, 2, VIEW>(p, st);
+      if (cut.key_groups == 1) return launch_dkv<T, D, RULE, 1, 4, VIEW>(p, two, st);
+    return cut.key_groups == 4 ? launch_dkv<T, D, RULE, 4, 1, VIEW>(p, two, st) : launch_dkv<T, D, RULE, 2, 2, VIEW>(p, two, st);
   }
 }
 
 template <typename T, int D, int VIEW>
-int launch_rule(BwdParams& p, const BwdCut& cut, hipStream_t st) {
+int launch_rule(BwdParams& p, const BwdCut& cut, const TwoCut& two, hipStream_t st) {
   switch (rule_kind<T>(p.rule)) {
-    case kPlain: return launch_bwd<T, D, kPlain, VIEW>(p, cut, st);
-    case kCap: return launch_bwd<T, D, kCap, VIEW>(p, cut, st);
-    case kBias: return launch_bwd<T, D, kBias, VIEW>(p, cut, st);
+    case kPlain: return launch_bwd<T, D, kPlain, VIEW>(p, cut, two, st);
+    case kCap: return launch_bwd<T, D, kCap, VIEW>(p, cut, two, st);
+    case kBias: return launch_bwd<T, D, kBias, VIEW>(p, cut, two, st);
     case kFar:
-      if constexpr (sizeof(T) == 2) return launch_bwd<T, D, kFar, VIEW>(p, cut, st);
+      if constexpr (sizeof(T) == 2) return launch_bwd<T, D, kFar, VIEW>(p, cut, two, st);
   }
   return fail(SSA_ERR_UNSUPPORTED, "no kernel for this rule of scores");
 }

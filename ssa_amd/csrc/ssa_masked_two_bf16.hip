@@ -10,9 +10,9 @@ int masked_two_bf16(tile::DenseParams& p, int kw, hipStream_t st) {
   return p.d <= 64 ? launch_rows_rule<uint16_t, 64, kTwo>(p, kw, st) : launch_rows_rule<uint16_t, 128, kTwo>(p, kw, st);
 }
 
-int masked_two_backward_bf16(void* params, const BwdCut& cut, hipStream_t st) {
+int masked_two_backward_bf16(void* params, const BwdCut& cut, const TwoCut& two, hipStream_t st) {
   BwdParams& p = *static_cast<BwdParams*>(params);
-  return p.d <= 64 ? launch_rule<uint16_t, 64, kTwo>(p, cut, st) : launch_rule<uint16_t, 128, kTwo>(p, cut, st);
+  return p.d <= 64 ? launch_rule<uint16_t, 64, kTwo>(p, cut, two, st) : launch_rule<uint16_t, 128, kTwo>(p, cut, two, st);
 }
 
 }  // namespace ssa

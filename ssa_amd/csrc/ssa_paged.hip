@@ -23,10 +23,15 @@
 // one of 131072, 16 / 2 heads: 28 us, 4.8 TB/s, and 9 us for the join of its 256 parts.
 // One short sequence waits for memory four times in a row (table, page, K and V, out):
 // 203 tokens, 8 / 2 heads, fp32, 12.4 us.
+//
+// The kernels are in ssa_paged_rows.h; ssa_paged_one_*.hip, ssa_paged_two_*.hip and
+// ssa_paged_held_*.hip compile them.
 
 #include <math.h>
 
-#include "ssa_paged_rows.h"
+#include "ssa_cuts.h"
+#include "ssa_dense_rows.h"
+#include "ssa_internal.h"
 
 using namespace ssa;
 
@@ -115,7 +120,11 @@ static int paged_step(const char* fn, bool zero_rows, const General& x, const vo
   if (x.parents != nullptr && max_new > tile::kDrafts)
     return fail(SSA_ERR_UNSUPPORTED, "%s: a tree has at most %d new tokens a sequence, max_new is %lld", fn, tile::kDrafts,
                 (long long)max_new);
-  const PagedPlan l = paged_plan(dtype, tokens, batch, h_q, h_kv, d, max_new, seen_len(max_len, max_new, x.window, x.sinks));
+  // (a window that no sequence reaches is none)
+  const int64_t window = x.window < max_len ? x.window : 0;
+  const bool two = held || window > 0 || x.parents != nullptr;
+  const PagedPlan l = paged_plan(dtype, tokens, batch, h_q, h_kv, d, max_new, seen_len(max_len, max_new, x.window, x.sinks),
+                                 two ? 128 : 64);
   if (l.bytes > 0 && (workspace == nullptr || workspace_bytes < l.bytes))
     return fail(SSA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", fn, l.bytes,
                 workspace == nullptr ? size_t(0) : workspace_bytes);
@@ -136,8 +145,7 @@ static int paged_step(const char* fn, bool zero_rows, const General& x, const vo
   p.error_flag = error_flag;
   p.k_new = k; p.v_new = v;
   p.kn_st = k_st; p.kn_sh = k_sh; p.vn_st = v_st; p.vn_sh = v_sh;
-  // (a window that no sequence reaches is none)
-  p.window = x.window < max_len ? static_cast<int>(x.window) : 0;
+  p.window = static_cast<int>(window);
   p.sinks = p.window > 0 ? static_cast<int>(x.sinks < 0x7FFFFFFF ? x.sinks : 0x7FFFFFFF) : 0;
   p.parents = x.parents;
   p.k_scale = x.k_scales; p.v_scale = x.v_scales;
@@ -148,10 +156,9 @@ static int paged_step(const char* fn, bool zero_rows, const General& x, const vo
   char* ws = static_cast<char*>(workspace);
   const bool f32 = dtype == SSA_DTYPE_F32, wide = d > 64;
   if (held) return f32 ? paged_held_f32(p, l, wide, zero_rows, ws, st) : paged_held_bf16(p, l, wide, zero_rows, ws, st);
-  if (p.window > 0 || p.parents != nullptr)
+  if (two)
     return f32 ? paged_two_f32(p, l, wide, zero_rows, ws, st) : paged_two_bf16(p, l, wide, zero_rows, ws, st);
-  if (f32) return wide ? launch_rule<float, 128, kOne>(p, l, zero_rows, ws, st) : launch_rule<float, 64, kOne>(p, l, zero_rows, ws, st);
-  return wide ? launch_rule<uint16_t, 128, kOne>(p, l, zero_rows, ws, st) : launch_rule<uint16_t, 64, kOne>(p, l, zero_rows, ws, st);
+  return f32 ? paged_one_f32(p, l, wide, zero_rows, ws, st) : paged_one_bf16(p, l, wide, zero_rows, ws, st);
 }
 
 extern "C" int ssa_paged_step(const void* q, const void* k, const void* v, int dtype, int64_t tokens, int64_t batch,

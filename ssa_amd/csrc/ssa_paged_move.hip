@@ -100,72 +100,77 @@ __global__ __launch_bounds__(256) void read_kernel(MoveParams p) {
   for (unsigned i = 0; i < sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(dst)[i] = w[i];
 }
 
-// Moves one piece (of type U) of every kept row of a sequence, eight rows' loads in flight.  Kept
+// Moves one piece (of type U) of every kept row of a sequence, sixteen rows' loads in flight.  Kept
 // rows ascend, so that the t-th lies at or behind its place: what is written is never read later.
 template <typename U>
-__device__ __forceinline__ void keep_piece(const MoveParams& p, int b, int first, int n, const int32_t* s_kept, char* base,
-                                           int64_t sp, int64_t st) {
-  const int mask = (1 << p.page_log2) - 1;
-  for (int t0 = 0; t0 < n; t0 += 8) {
-    U x[8];
+__device__ __forceinline__ void keep_piece(int n, const int2* s_from, const int2* s_to, char* base, int64_t sp, int64_t st) {
+  constexpr int kAtOnce = 16;
+  for (int t0 = 0; t0 < n; t0 += kAtOnce) {
+    U x[kAtOnce];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (t0 + i >= n) continue;
-      const int64_t j = static_cast<int64_t>(first) + s_kept[t0 + i], pg = page_of(p, b, j);
-      if (pg >= 0)
-        x[i] = *reinterpret_cast<const U*>(base + pg * sp + (j & mask) * st);
-      else
-        flag(p);
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int2 a = s_from[min(t0 + i, n - 1)];
+      x[i] = *reinterpret_cast<const U*>(base + a.x * sp + a.y * st);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (t0 + i >= n || s_kept[t0 + i] == t0 + i) continue;
-      const int64_t j = static_cast<int64_t>(first) + t0 + i, from = static_cast<int64_t>(first) + s_kept[t0 + i];
-      const int64_t pg = page_of(p, b, j);
-      if (pg >= 0 && page_of(p, b, from) >= 0)
-        *reinterpret_cast<U*>(base + pg * sp + (j & mask) * st) = x[i];
-      else
-        flag(p);
-    }
+    for (int i = 0; i < kAtOnce; ++i)
+      if (t0 + i < n) {
+        const int2 a = s_to[t0 + i];
+        *reinterpret_cast<U*>(base + a.x * sp + a.y * st) = x[i];
+      }
   }
 }
 
 constexpr int kMostKept = 64;
 
-// A thread takes a piece of a head's rows of K or V, of all kept tokens; E bytes an element.
+// A thread takes a piece of a head's rows of K or V, of all kept tokens; E bytes an element.  The
+// first wave looks the rows up: rows that are in their place already, or that have no page at one
+// end, are left out.
 template <int E>
 __global__ __launch_bounds__(256) void keep_kernel(MoveParams p) {
   using U = std::conditional_t<E == 1, uint2, uint4>;
-  __shared__ int32_t s_kept[kMostKept];
+  __shared__ int2 s_from[kMostKept], s_to[kMostKept];  // page, row of it
   __shared__ int s_n;
   const int b = blockIdx.y;
-  const int first = p.cached[b];
   if (threadIdx.x < 64) {  // the kept tokens up to the first one below 0, or the first that does not ascend
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x, first = p.cached[b];
     const int x = lane < p.most ? p.kept[b * p.kept_stride + lane] : -1;
     const int before = __shfl_up(x, 1, 64);
     const uint64_t end = __ballot(x < 0), fall = __ballot(lane > 0 && x >= 0 && x <= before);
     const int n = end != 0 ? __builtin_ctzll(end) : 64, good = fall != 0 ? __builtin_ctzll(fall) : 64;
-    if (lane == 0) {
-      if (first < 0 || good < n) flag(p);
-      s_n = first < 0 ? 0 : (n < good ? n : good);
+    bool on = first >= 0 && lane < min(n, good), bad = first < 0 || good < n;
+    const int64_t from = static_cast<int64_t>(first) + x, to = static_cast<int64_t>(first) + lane;
+    int pg = 0, pt = 0;
+    if (on) {
+      pg = page_of(p, b, from);
+      pt = page_of(p, b, to);
+      bad |= pg < 0 || pt < 0;
+      on = pg >= 0 && pt >= 0 && x != lane;
     }
-    s_kept[lane] = x;
+    const uint64_t go = __ballot(on);
+    const int at = __popcll(go & ((uint64_t(1) << lane) - 1)), mask = (1 << p.page_log2) - 1;
+    if (on) {
+      s_from[at] = make_int2(pg, static_cast<int>(from & mask));
+      s_to[at] = make_int2(pt, static_cast<int>(to & mask));
+    }
+    if (bad) flag(p);
+    if (lane == 0) s_n = __popcll(go);
   }
   __syncthreads();
   const int n = s_n, per = p.d * E / static_cast<int>(sizeof(U)), rows = 2 * p.h_kv;
   const int at = blockIdx.x * 256 + threadIdx.x;
+  if (n == 0) return;
   if (at < rows * per) {
     const int row = at / per, c = at - row * per;
     const bool isv = row >= p.h_kv;
     const Pool& pool = isv ? p.v : p.k;
     char* base = static_cast<char*>(pool.at) + (isv ? row - p.h_kv : row) * pool.sh * E + c * static_cast<int>(sizeof(U));
-    keep_piece<U>(p, b, first, n, s_kept, base, pool.sp * E, pool.st * E);
+    keep_piece<U>(n, s_from, s_to, base, pool.sp * E, pool.st * E);
   } else if (E == 1 && at < rows * (per + 1)) {
     const int row = at - rows * per;
     const bool isv = row >= p.h_kv;
     const Pool& pool = isv ? p.v : p.k;
-    keep_piece<uint32_t>(p, b, first, n, s_kept, reinterpret_cast<char*>(pool.scale + (isv ? row - p.h_kv : row) * pool.c_sh),
+    keep_piece<uint32_t>(n, s_from, s_to, reinterpret_cast<char*>(pool.scale + (isv ? row - p.h_kv : row) * pool.c_sh),
                          pool.c_sp * 4, pool.c_st * 4);
   }
 }

@@ -704,7 +704,8 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
         raise ValueError(f"q {tuple(q.shape)} does not fit pages {tuple(k_pages.shape)}")
     dtype = q.dtype
     held = k_pages.dtype in HELD_DTYPES
-    for name, t in (("k", k), ("v", v), ("out", out)) if held else (("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("out", out)):
+    like_q = (("k", k), ("v", v), ("out", out))
+    for name, t in like_q if held else like_q + (("k_pages", k_pages), ("v_pages", v_pages)):
         if t is not None and t.dtype != dtype:
             raise TypeError(f"{name} must have q's dtype {dtype}, got {t.dtype}")
     general = held or window != 0 or sinks != 0 or parents is not None
@@ -730,9 +731,10 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
     if zeroed:  # (rows that no sequence has, or that are left out, become zeros)
         if B == 0:
             return torch.zeros((T, h_q, d), device=q.device, dtype=dtype)
-        name, out = "ssa_paged_step_zeroed", torch.empty((T, h_q, d), device=q.device, dtype=dtype)
+        name, out, os = "ssa_paged_step_zeroed", torch.empty((T, h_q, d), device=q.device, dtype=dtype), (h_q * d, d)
     else:
-        if out.shape != (T, h_q, d) or _rows16(out)[0] is not out:
+        rows, os = _rows16(out)
+        if out.shape != (T, h_q, d) or rows is not out:
             raise ValueError(f"out must be [{T}, {h_q}, {d}] with rows aligned to 16 bytes")
         _once(out, "out")
     max_new = (T if parents is None else min(T, 64)) if max_new is None else min(int(max_new), T)
@@ -745,7 +747,7 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
                  k_pages.data_ptr(), v_pages.data_ptr(), _page_dtype(k_pages), _at(k_scales), _at(v_scales), pages, page,
                  *pools, *scale_steps, table.data_ptr(), table.stride(0) if B > 1 else 0, width, starts.data_ptr(),
                  cached.data_ptr(), _at(parents), max_new, max_len, window, sinks,
-                 math.sqrt(d) if scale_div is None else scale_div, softcap, _at(slopes), out.data_ptr(), *_rows16(out)[1],
+                 math.sqrt(d) if scale_div is None else scale_div, softcap, _at(slopes), out.data_ptr(), *os,
                  int(zeroed), _at(error_flag), _at(ws), nbytes)
         return out
     nbytes = _bytes("ssa_paged_step_workspace_bytes", dt, T, B, h_q, h_kv, d, max_new, max_len)
@@ -753,7 +755,7 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
     _call_on(dev, name, q.data_ptr(), _at(k), _at(v), dt, T, B, h_q, h_kv, d, *qs, *ks, *vs, k_pages.data_ptr(),
              v_pages.data_ptr(), pages, page, *pools, table.data_ptr(), table.stride(0) if B > 1 else 0, width,
              starts.data_ptr(), cached.data_ptr(), max_new, max_len, math.sqrt(d) if scale_div is None else scale_div,
-             softcap, _at(slopes), out.data_ptr(), *_rows16(out)[1], _at(error_flag), _at(ws), nbytes)
+             softcap, _at(slopes), out.data_ptr(), *os, _at(error_flag), _at(ws), nbytes)
     return out
 
 
@@ -770,11 +772,17 @@ def _page_dtype(pages: torch.Tensor) -> int:
 def _pool_strides(k_pages: torch.Tensor, v_pages: torch.Tensor, written: bool):
     """Element strides (page, token, head) of both pools, whose rows are contiguous and aligned to 16
     bytes, of 8-bit codes to 8."""
+    dtype = k_pages.dtype
+    if v_pages.dtype != dtype:
+        raise TypeError(f"v_pages must have k_pages' dtype {dtype}, got {v_pages.dtype}")
+    held = dtype in HELD_DTYPES
+    _, page, h, d = k_pages.shape
+    if k_pages.is_contiguous() and v_pages.is_contiguous() and d % 8 == 0 and not (k_pages.data_ptr() | v_pages.data_ptr()) % 16:
+        st = (page * h * d, h * d, d)
+        return st + st
     pools = []
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.dtype != k_pages.dtype:
-            raise TypeError(f"v_pages must have k_pages' dtype {k_pages.dtype}, got {t.dtype}")
-        if t.dtype in HELD_DTYPES:
+        if held:
             st = tuple(0 if x == 1 else s for s, x in zip(t.stride(), t.shape))
             if t.numel() and ((st[-1] != 1 and t.shape[-1] > 1) or any(s % 8 for s in st[:-1]) or t.data_ptr() % 8):
                 raise ValueError(f"{name} must have contiguous rows aligned to 8 bytes")
@@ -794,24 +802,27 @@ def _scale_strides(k_pages, v_pages, k_scales, v_scales, written: bool):
     if k_pages.dtype not in HELD_DTYPES:
         if k_scales is not None or v_scales is not None:
             raise ValueError("scales go with pools of int8 or float8_e4m3fn")
-        return (0,) * 6
-    steps = []
+        return (0, 0, 0, 0, 0, 0)
+    if k_scales is None or v_scales is None:
+        raise ValueError(f"pools of {k_pages.dtype} need k_scales and v_scales")
+    shape = k_pages.shape[:3]
     for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
-        if t is None or t.dtype != torch.float32 or t.shape != k_pages.shape[:3]:
-            raise ValueError(f"{name} must be float32 {list(k_pages.shape[:3])} for pools of {k_pages.dtype}")
-        if written:
+        if t.dtype != torch.float32 or t.shape != shape:
+            raise ValueError(f"{name} must be float32 {list(shape)} for pools of {k_pages.dtype}")
+        if written and 0 in t.stride():
             _once(t, name)
-        steps += t.stride()
-    return steps
+    return k_scales.stride() + v_scales.stride()
 
 
-def _check_tables(table, **rows):
-    B = table.shape[0] if table.dim() == 2 else -1
-    for name, (t, n) in {"table": (table, None), **rows}.items():
-        ok = t.dtype == torch.int32 and (t.dim() == 2 if n is None else t.shape == (B + n,))
-        if not ok or (t.shape[-1] > 1 and t.stride(-1) != 1):
-            raise ValueError(f"{name} must be an int32 tensor {'[B, width]' if n is None else [B + n]} with contiguous rows")
-    return B, table.shape[1]
+def _table_rows(t: torch.Tensor, name: str, shape) -> None:
+    """Checks an int32 [..., n] tensor with contiguous rows."""
+    if t.dtype != torch.int32 or t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name} must be an int32 {list(shape)} tensor with contiguous rows")
+
+
+def _check_flag(t: Optional[torch.Tensor]) -> None:
+    if t is not None and (t.dtype != torch.int32 or t.numel() != 1):
+        raise ValueError("error_flag must be one int32")
 
 
 def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, first: torch.Tensor,
@@ -824,7 +835,13 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
         raise ValueError("the pools must be [pages, page size, h_kv, d]")
     pages, page, h_kv, d = k_pages.shape
-    B, width = _check_tables(table, starts=(starts, 1), first=(first, 0))
+    if table.dim() != 2:
+        raise ValueError(f"table must be [B, width], got {tuple(table.shape)}")
+    B, width = table.shape
+    _table_rows(table, "table", (B, width))
+    _table_rows(starts, "starts", (B + 1,))
+    _table_rows(first, "first", (B,))
+    _check_flag(error_flag)
     pools = _pool_strides(k_pages, v_pages, False)
     steps = _scale_strides(k_pages, v_pages, k_scales, v_scales, False)
     if dtype is None:
@@ -833,9 +850,8 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
         raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
     if tokens < 0:
         raise ValueError(f"tokens must not be negative, got {tokens}")
-    if error_flag is not None and (error_flag.dtype != torch.int32 or error_flag.numel() != 1):
-        raise ValueError("error_flag must be one int32")
-    k, v = (torch.empty((tokens, h_kv, d), device=k_pages.device, dtype=dtype) for _ in "kv")
+    k = torch.empty((tokens, h_kv, d), device=k_pages.device, dtype=dtype)
+    v = torch.empty_like(k)
     if B == 0:
         return k.zero_(), v.zero_()
     _call_on(dev, "ssa_paged_read", k_pages.data_ptr(), v_pages.data_ptr(), _page_dtype(k_pages), _at(k_scales), _at(v_scales),
@@ -852,13 +868,16 @@ def paged_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
         raise ValueError("the pools must be [pages, page size, h_kv, d]")
     pages, page, h_kv, d = k_pages.shape
-    B, width = _check_tables(table, cached=(cached, 0))
+    if table.dim() != 2:
+        raise ValueError(f"table must be [B, width], got {tuple(table.shape)}")
+    B, width = table.shape
+    _table_rows(table, "table", (B, width))
+    _table_rows(cached, "cached", (B,))
+    _check_flag(error_flag)
     if kept.dtype != torch.int32 or kept.dim() != 2 or kept.shape[0] != B or (kept.shape[1] > 1 and kept.stride(1) != 1):
         raise ValueError(f"kept must be an int32 [{B}, most kept] tensor with contiguous rows")
     pools = _pool_strides(k_pages, v_pages, True)
     steps = _scale_strides(k_pages, v_pages, k_scales, v_scales, True)
-    if error_flag is not None and (error_flag.dtype != torch.int32 or error_flag.numel() != 1):
-        raise ValueError("error_flag must be one int32")
     _call_on(dev, "ssa_paged_keep", k_pages.data_ptr(), v_pages.data_ptr(), _page_dtype(k_pages), _at(k_scales), _at(v_scales),
              pages, page, h_kv, d, *pools, *steps, B, table.data_ptr(), table.stride(0) if B > 1 else 0, width,
              cached.data_ptr(), kept.data_ptr(), kept.stride(0) if B > 1 else 0, kept.shape[1], _at(error_flag))
