@@ -579,13 +579,392 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
   }
 }
 
+// few_rows for at most 16 rows over pages of 8 bits, bf16 queries.  Widening the codes, 1.5
+// instructions a code, is most of the work beside memory's, so that the rest is kept small and
+// more waves share a SIMD (two of few_rows do, whose tiles of bf16 fill the LDS): the LDS
+// holds codes, widened as they are read, and 16x16x32 products, whose 16 columns spend half the
+// softmax that 32 do.  A product's contraction takes the features in the order in which 16 bytes a
+// lane bring them, and Q is loaded in that order too; V is transposed by its reads
+// (ds_read_b64_tr_b8).  The call's own rows,
+// which have no codes yet, are added one by one at the end, by one wave of the last part.
+// 32 sequences of up to 8191 cached tokens, 32 / 8 heads: MEASURED.
+constexpr int kCols = 16;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// 16 codes (8 of rows of at most 64) at a lane's and the wave's offset.
+template <int D>
+__device__ __forceinline__ uint4 load_codes(__amdgpu_buffer_rsrc_t rows, uint32_t lane_at, int at) {
+  if constexpr (D == 128) {
+    const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rows, static_cast<int>(lane_at), at, 0);
+    return make_uint4(x.x, x.y, x.z, x.w);
+  } else {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rows, static_cast<int>(lane_at), at, 0);
+    return make_uint4(x.x, x.y, 0u, 0u);
+  }
+}
+
+template <int D, int RULE>
+__device__ __forceinline__ void few_codes(const DenseParams& p, const int block, char* lds) {
+  using T = uint16_t;
+  using S = uint8_t;
+  using O = Op<T>;
+  using Frag = typename O::Frag;
+  constexpr int NS = D / 32, NH = D / 64, NF = D / 16;  // products of a score, a lane's loads of a row, tiles of features
+  constexpr int CB = 32 * D, PS = D + 4;
+  // lds: [4 waves][K, V][codes], then [4][16][PS] sums
+  __shared__ float s_m[4][kCols], s_l[4][kCols];
+  __shared__ int s_bad[4][kCols];
+  __shared__ uint64_t s_kin[kDrafts];
+  __shared__ int s_depth[kDrafts];
+  __shared__ __align__(16) float s_scale[4][2][32];
+
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = block % p.h_kv, rest = block / p.h_kv;
+  const int split = rest % p.splits, b = rest / p.splits;
+  const Seq sq = paged_seq(p, b);
+  const int R = sq.m * p.g;
+  if (R == 0 || R > kCols) return;
+  const int cached = sq.len - sq.m;
+  const Tiles walk = seq_tiles(p, sq);
+  const int per = static_cast<int>(p.split_len / 32);
+  const int t_begin = static_cast<int>(min(static_cast<int64_t>(split) * per, static_cast<int64_t>(walk.n)));
+  const int t_end = min(t_begin + per, walk.n);
+  if (t_begin >= t_end) return;  // (a part past the sequence's tiles, which the join does not read)
+  const int part_x[2] = {(walk.x0 + min(t_begin, walk.n1)) * 32, (walk.y0 + max(t_begin - walk.n1, 0)) * 32};
+  const int part_y[2] = {(walk.x0 + min(t_end, walk.n1)) * 32, (walk.y0 + max(t_end - walk.n1, 0)) * 32};
+  const int first_a = p.window > 0 ? min(p.sinks, max(sq.len - p.window, 0)) : 0;
+  const int from = p.window > 0 ? max(cached + 1 - p.window, 0) : 0;
+  const KeyRows<T, true, S> rows = key_rows<T, true, S>(p, b, kvh, sq.first, cached);
+
+  const bool real = n < R;
+  const int tok = real ? n / p.g : 0;
+  const int hq = kvh * p.g + (real ? n - tok * p.g : 0);
+  const bool tree = p.parents != nullptr;
+  int pos = cached + tok;
+  uint64_t kin = 0;
+  if (tree) {
+    int depth;
+    const uint64_t all = draft_kin(p, sq.first, sq.m, cached, depth);
+    if (lane < kDrafts) {  // (each wave the same)
+      s_kin[lane] = all;
+      s_depth[lane] = depth;
+    }
+    wave_lds_sync();
+    kin = s_kin[tok];
+    pos = cached + s_depth[tok];
+  }
+  const Sees see = paged_sees(p, pos, cached, kin);
+  const int lo_max = p.window > 0 ? max(sq.len - p.window, 0) : 0, hi_min = min(rows.new_from, tree ? cached : cached + 1);
+  const Rule<T, RULE> rule(p.rule);
+  const float slope = has_bias(RULE) && real ? slope_of(p.rule, hq) : 0.0f;
+  const T* qrow = static_cast<const T*>(p.q) + (sq.first + tok) * p.q_sn + hq * p.q_sh;
+  auto feature = [&](int s) { return 64 * (s >> 1) + 16 * quad + 8 * (s & 1); };  // of product s, this lane's first
+  Frag qf[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) qf[s] = real && feature(s) < p.d ? O::load(qrow + feature(s)) : O::zero();
+
+  char* kt = lds + wave * 2 * CB;
+  char* vt = kt + CB;
+  // (the banks of a tile's rows: 16-byte chunk c of row r lies at chunk c ^ f(r))
+  auto chunk = [&](int r, int c) { return r * D + ((c ^ (D == 128 ? r & 7 : (r >> 2) & 3)) << 4); };
+  auto seen_key = [&](int j) { return min(j >= first_a ? max(j, from) : j, sq.len - 1); };
+  const int paged_last = max(min(rows.new_from, sq.len) - 1, 0);
+  // tiles of new keys alone are left out: they have no codes
+  auto key_at = [&](int x) { return x < t_end ? walk.at(x) * 32 : 0x7FFFFFFF; };
+  const int codes_end = min(rows.new_from, sq.len);
+  const int my_row = lane >> 3, my_at = (lane & 7) * (D / 8), key32 = lane & 31;
+  const uint32_t ko = my_at < p.d ? my_row * static_cast<uint32_t>(rows.k_sn) + my_at : kNoChunk;
+  const uint32_t vo = my_at < p.d ? my_row * static_cast<uint32_t>(rows.v_sn) + my_at : kNoChunk;
+  uint4 kreg[4], vreg[4];
+  float scale_reg = 1.0f;  // of K's key lane, from lane 32 on of V's key lane - 32
+  auto find = [&](int k0) { return k0 < codes_end ? rows.entry_of(min(seen_key(k0 + key32), paged_last)) : 0; };
+  auto load = [&](int k0, int entry) {
+    const int pg = rows.checked(entry);
+    scale_reg = rows.scale_of(lane >= 32, pg, min(seen_key(k0 + key32), paged_last));
+    auto fetch = [&](int i, __amdgpu_buffer_rsrc_t kb, __amdgpu_buffer_rsrc_t vb, int ks, int vs) {
+      kreg[i] = load_codes<D>(kb, ko, ks);
+      vreg[i] = load_codes<D>(vb, vo, vs);
+    };
+    if (rows.page_mask >= 31) {  // (one page holds the tile)
+      const int64_t page = lane_value(pg, 0), r0 = k0 & rows.page_mask;
+      const auto kb = row_buffer(rows.k + page * rows.k_sb + r0 * rows.k_sn, kAllBytes);
+      const auto vb = row_buffer(rows.v + page * rows.v_sb + r0 * rows.v_sn, kAllBytes);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fetch(i, kb, vb, 8 * i * static_cast<int>(rows.k_sn), 8 * i * static_cast<int>(rows.v_sn));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t page = lane_value(pg, 8 * i), r0 = (k0 + 8 * i) & rows.page_mask;
+        fetch(i, row_buffer(rows.k + page * rows.k_sb + r0 * rows.k_sn, kAllBytes),
+              row_buffer(rows.v + page * rows.v_sb + r0 * rows.v_sn, kAllBytes), 0, 0);
+      }
+    }
+  };
+  auto put = [&](char* tile, const uint4 (&reg)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      char* at = tile + chunk(8 * i + my_row, my_at >> 4) + (my_at & 15);
+      if constexpr (D == 128)
+        *reinterpret_cast<uint4*>(at) = reg[i];
+      else
+        *reinterpret_cast<uint2*>(at) = make_uint2(reg[i].x, reg[i].y);
+    }
+  };
+
+  const int vr = 16 * (n >> 3) + 4 * quad + ((n >> 1) & 3);
+  const int k_base = chunk(n, quad), v_base = chunk(vr, 0) + 8 * (n & 1);
+
+  f32x4 acc[NF];
+#pragma unroll
+  for (int i = 0; i < NF; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float mref = -INFINITY, lsum = 0.0f;
+  auto rescale = [&](float top) {  // moves the reference to at least top
+    const float mn = fmaxf(mref, top);
+    const float alpha = mref == mn ? 1.0f : exp2_w(mref - mn);
+    mref = mn;
+    lsum *= alpha;
+#pragma unroll
+    for (int i = 0; i < NF; ++i) acc[i] *= alpha;
+  };
+
+  int x = t_begin + wave;
+  int entry = find(key_at(x));
+  if (key_at(x) < codes_end) load(key_at(x), entry);
+  entry = find(key_at(x + 4));
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    settle(qf[s].v.x);
+    settle(qf[s].v.y);
+    settle(qf[s].v.z);
+    settle(qf[s].v.w);
+  }
+  auto walk_tiles = [&](auto kind) {
+    constexpr bool E4M3 = decltype(kind)::value;
+    for (; key_at(x) < codes_end; x += 4) {
+      const int k0 = key_at(x);
+      // (addresses that differ by an exclusive or are formed anew: kept, they take twelve registers)
+      const int k_at = in_branch(k_base), v_at = in_branch(v_base);
+      put(kt, kreg);
+      put(vt, vreg);
+      s_scale[wave][lane >> 5][key32] = scale_reg;
+      wave_lds_sync();
+      if (key_at(x + 4) < codes_end) load(key_at(x + 4), entry);
+      entry = find(key_at(x + 8));
+      f32x4 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          const uint4 k = *reinterpret_cast<const uint4*>(kt + (k_at ^ (h << 6)) + 16 * D * u);
+          const uint4 a = Codes<T>::template widen<E4M3>(k.x, k.y), c = Codes<T>::template widen<E4M3>(k.z, k.w);
+          s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, qf[2 * h].v), s[u], 0, 0, 0);
+          s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c), __builtin_bit_cast(bf16x8, qf[2 * h + 1].v), s[u], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);  // (widened any earlier, the codes take the registers of a wave)
+        }
+      }
+      const int kl = k0 + 4 * quad;  // key of register 0
+      float top = Rule<T, RULE>::kHidden;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float4 f = *reinterpret_cast<const float4*>(&s_scale[wave][0][16 * u + 4 * quad]);
+        const float fs[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[u][r] = rule.z(p.rule, s[u][r] * fs[r], slope, static_cast<float>(kl + 16 * u + r - pos));
+      }
+      if (k0 < lo_max || k0 + 32 > hi_min) {  // (new keys come later)
+        const int a = in_branch(see.lo - kl), z = in_branch(min(see.hi, rows.new_from) - kl), y = in_branch(min(see.a_hi, rows.new_from) - kl);
+        const uint32_t kin = rows.new_from < sq.len ? 0u : kin_word(see.kin, k0 - cached) >> (4 * quad);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = 16 * u + r;
+            if (!((j >= a && j < z) || j < y || (kin >> j & 1u) != 0)) s[u][r] = Rule<T, RULE>::kHidden;
+          }
+        if (has_bias(RULE) && tree && rows.new_from >= sq.len && k0 + 32 > cached) {  // (drafts that the pages hold lie at cached + depth)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int j = kl + 16 * u + r - cached;
+              if (j >= 0 && j < kDrafts && (kin >> (16 * u + r) & 1u) != 0)
+                s[u][r] += slope * (fabsf(static_cast<float>(cached + j - pos)) - fabsf(static_cast<float>(cached + s_depth[j] - pos)));
+            }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = rule.better(top, s[u][r]);
+      top = rule.better(top, __shfl_xor(top, 16, 64));
+      top = fmaf(rule.better(top, __shfl_xor(top, 32, 64)), rule.a, rule.b);
+      if (__ballot(top > mref + 8.0f) != 0) rescale(top);
+      const float nref = rule.b - (mref == -INFINITY ? 0.0f : mref);
+      uint32_t pk[4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float4 f = *reinterpret_cast<const float4*>(&s_scale[wave][1][16 * u + 4 * quad]);
+        const float fs[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[u][r] = exp2_w(fmaf(s[u][r], rule.a, nref));
+          lsum += s[u][r];
+          s[u][r] *= fs[r];
+        }
+        pk[2 * u] = O::pack2(s[u][0], s[u][1]);
+        pk[2 * u + 1] = O::pack2(s[u][2], s[u][3]);
+      }
+      const uint4 pf = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+      // lane i of a quad's 16 reads 8 bytes of the quad's keys 4 quad + {0..3, 16..19}, the (i / 2)-th,
+      // and gets feature i of all eight
+      typedef int v2i __attribute__((ext_vector_type(2)));
+      typedef __attribute__((address_space(3))) v2i* lds_v2i;
+#pragma unroll
+      for (int i = 0; i < NF; ++i) {
+        const v2i c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(vt + (v_at ^ (i << 4))));
+        const uint4 a = Codes<T>::template widen<E4M3>(static_cast<uint32_t>(c.x), static_cast<uint32_t>(c.y));
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pf), acc[i], 0, 0, 0);
+        if (i & 1) __builtin_amdgcn_sched_barrier(0);
+      }
+      wave_lds_sync();
+    }
+  };
+  if (rows.e4m3)
+    walk_tiles(std::true_type());
+  else
+    walk_tiles(std::false_type());
+
+  // the call's own rows, as they are given
+  if (t_end == walk.n && rows.new_from < sq.len && wave == 3) {
+    for (int i = 0; i < sq.m; ++i) {
+      const int j = cached + i;
+      const T *kr, *vr;
+      rows.new_rows(j, kr, vr);
+      float dot = 0.0f;
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        if (feature(s) < p.d) dot = O::dot(qf[s], O::load(kr + feature(s)), dot);
+      dot += __shfl_xor(dot, 16, 64);
+      dot += __shfl_xor(dot, 32, 64);
+      const bool on = real && see.key(j);
+      const int at = tree ? cached + s_depth[i] : j;
+      const float sc = fmaf(rule.z(p.rule, dot, slope, static_cast<float>(at - pos)), rule.a, rule.b);
+      if (on) rescale(sc);
+      const float w = on ? exp2_w(sc - (mref == -INFINITY ? 0.0f : mref)) : 0.0f;
+      lsum += quad == 0 ? w : 0.0f;
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const int c = 16 * f + 4 * quad;
+        if (c >= p.d || !on) continue;
+        const uint2 v = *reinterpret_cast<const uint2*>(vr + c);
+        acc[f][0] = fmaf(w, __uint_as_float(v.x << 16), acc[f][0]);
+        acc[f][1] = fmaf(w, __uint_as_float(v.x & 0xFFFF0000u), acc[f][1]);
+        acc[f][2] = fmaf(w, __uint_as_float(v.y << 16), acc[f][2]);
+        acc[f][3] = fmaf(w, __uint_as_float(v.y & 0xFFFF0000u), acc[f][3]);
+      }
+    }
+  }
+
+  lsum += __shfl_xor(lsum, 16, 64);
+  lsum += __shfl_xor(lsum, 32, 64);
+  float worst = finite(lsum) ? 0.0f : 1.0f;
+#pragma unroll
+  for (int i = 0; i < NF; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) worst = finite(acc[i][e]) ? worst : 1.0f;
+  worst = fmaxf(worst, __shfl_xor(worst, 16, 64));
+  worst = fmaxf(worst, __shfl_xor(worst, 32, 64));
+  if (quad == 0) {
+    s_m[wave][n] = mref;
+    s_l[wave][n] = lsum;
+    s_bad[wave][n] = worst != 0.0f;
+  }
+  __syncthreads();  // every wave is past its tiles: their LDS holds the sums now
+  float* sums = reinterpret_cast<float*>(lds);
+  if (real) {
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+      *reinterpret_cast<float4*>(sums + (wave * kCols + n) * PS + 16 * i + 4 * quad) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+  }
+  __syncthreads();
+  const int64_t part_row = (static_cast<int64_t>(b) * p.h_kv + kvh) * kFew;
+  const int quads = p.d / 4;
+  auto sees_of = [&](int t) { return paged_sees(p, cached + (tree ? s_depth[t] : t), cached, tree ? s_kin[t] : 0); };
+  // whether the part holds a key that token t sees
+  auto here_of = [&](int t) {
+    const Sees w = sees_of(t);
+    return w.any(part_x[0], part_y[0]) || w.any(part_x[1], part_y[1]);
+  };
+  for (int e = tid; e < R * quads; e += kThreads) {
+    const int r = e / quads, dd = (e - r * quads) * 4;
+    if (s_bad[0][r] | s_bad[1][r] | s_bad[2][r] | s_bad[3][r]) continue;
+    const float m = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.0f;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const float a = exp2_w(s_m[y][r] - ref);
+      const float4 w = *reinterpret_cast<const float4*>(sums + (y * kCols + r) * PS + dd);
+      l = fmaf(a, s_l[y][r], l);
+      o.x = fmaf(a, w.x, o.x);
+      o.y = fmaf(a, w.y, o.y);
+      o.z = fmaf(a, w.z, o.z);
+      o.w = fmaf(a, w.w, o.w);
+    }
+    const int t = r / p.g, h = kvh * p.g + r - t * p.g;
+    if (p.splits > 1) {
+      const int64_t pr = split * p.part_rows + part_row + r;
+      *reinterpret_cast<float4*>(p.part_o + pr * D + dd) = o;
+      if (dd == 0) {
+        // (a part whose visible keys all scored -inf says so by a finite m)
+        p.part_ml[pr * 2] = here_of(t) && m == -INFINITY ? -3.0e38f : m;
+        p.part_ml[pr * 2 + 1] = l;
+      }
+    } else {
+      const float inv = 1.0f / l;
+      O::store4(static_cast<T*>(p.out) + (sq.first + t) * p.o_sn + h * p.o_sh + dd, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    }
+  }
+  for (int r = wave; r < R; r += 4) {  // rows to compute again, key by key
+    if (!(s_bad[0][r] | s_bad[1][r] | s_bad[2][r] | s_bad[3][r])) continue;
+    const int t = r / p.g, h = kvh * p.g + r - t * p.g, ps = cached + (tree ? s_depth[t] : t);
+    const float sl = has_bias(RULE) ? slope_of(p.rule, h) : 0.0f;
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+      exact_keys<T, S, true>(rows, p.rule, sees_of(t), static_cast<const T*>(p.q) + (sq.first + t) * p.q_sn + h * p.q_sh, p.d,
+                             part_x[y], min(part_y[y], sq.len), sl, ps, tree ? s_depth : nullptr, o, m, l);
+    const int64_t pr = split * p.part_rows + part_row + r;
+    T* orow = static_cast<T*>(p.out) + (sq.first + t) * p.o_sn + h * p.o_sh;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+      const int dd = lane + 64 * e;
+      if (dd >= p.d) continue;
+      if (p.splits > 1)
+        p.part_o[pr * D + dd] = o[e];
+      else
+        O::store1(orow + dd, o[e] * (1.0f / l));
+    }
+    if (p.splits > 1 && lane == 0) {
+      p.part_ml[pr * 2] = here_of(t) && m == -INFINITY ? -3.0e38f : m;
+      p.part_ml[pr * 2 + 1] = l;
+    }
+  }
+}
+
 // Everything of a call in one launch: blocks of many rows (the longest) first, then
-// few rows, then the blocks that append.  KW 0: no sequence has many rows; its call may
+// few rows, then the blocks that append.  KW 0: no sequence has many rows (KW -1: none more than
+// 16 of them, over pages of 8 bits); its call may
 // have no second launch, so that the blocks of no rows stand here (beside dense_rows they
 // cost 2048 rows behind 30720 cached 12%: 1215 to 1350 us).
 template <typename T, int D, int KW>
 constexpr int paged_per_cu() {
   if constexpr (KW > 0) return rows_per_cu<T, D, KW>();
+  if constexpr (KW < 0) return 3;
   return sizeof(T) == 2 || D == 64 ? 2 : 1;
 }
 
@@ -597,7 +976,10 @@ __global__ __launch_bounds__(kThreads, (paged_per_cu<T, D, KW>())) void paged_ke
   if (w < row_blocks) {
     if constexpr (KW > 0) dense_rows<T, D, true, RULE, KW, FRESH, VIEW, S>(rows, w, lds);
   } else if (w < row_blocks + few_blocks) {
-    few_rows<T, D, RULE, VIEW, S>(few, w - row_blocks, lds);
+    if constexpr (KW < 0)
+      few_codes<D, RULE>(few, w - row_blocks, lds);
+    else
+      few_rows<T, D, RULE, VIEW, S>(few, w - row_blocks, lds);
   } else if (KW > 0 || w < row_blocks + few_blocks + copy_blocks) {
     const int64_t t = static_cast<int64_t>(w - row_blocks - few_blocks) * kAppend + threadIdx.x;
     for (int i = 0; i < kAppend; i += kThreads) {
@@ -607,7 +989,7 @@ __global__ __launch_bounds__(kThreads, (paged_per_cu<T, D, KW>())) void paged_ke
         append_row<T>(few, t + i);
     }
   } else {
-    if constexpr (KW == 0) no_rows<T>(few, w - row_blocks - few_blocks - copy_blocks);
+    if constexpr (KW <= 0) no_rows<T>(few, w - row_blocks - few_blocks - copy_blocks);
   }
 }
 
@@ -716,6 +1098,7 @@ int launch_paged(DenseParams& p, const PagedPlan& l, bool zero_rows, char* ws, h
   const size_t tiles = static_cast<size_t>(8) * 32 * D * sizeof(T), sums = static_cast<size_t>(4) * kFew * (D + 4) * sizeof(float);
   size_t bytes = tiles > sums ? tiles : sums;
   if constexpr (KW > 0) bytes = bytes > rows_lds<T, D, KW>() ? bytes : rows_lds<T, D, KW>();
+  if constexpr (KW < 0) bytes = static_cast<size_t>(4) * kCols * (D + 4) * sizeof(float);  // (more than V's codes take)
   if (int rc = reserve_lds(reinterpret_cast<const void*>(kernel), bytes + (VIEW == kTwo ? 8192 : 4096), fn)) return rc;
   const int64_t rblocks = static_cast<int64_t>(l.row_tiles) * p.h_kv * r.splits;
   const int64_t fblocks = static_cast<int64_t>(p.batch) * p.h_kv * f.splits;
@@ -725,7 +1108,7 @@ int launch_paged(DenseParams& p, const PagedPlan& l, bool zero_rows, char* ws, h
   const int per = f.splits <= 8 ? 1 : (f.splits <= 32 ? 4 : 16);  // waves a row: one round of loads, or 16 waves
   const int64_t few_join_blocks = f.splits > 1 ? ceil_div(static_cast<int64_t>(p.batch) * p.h_kv * most, kJoinWaves / per) : 0;
   const int64_t join_blocks = few_join_blocks + (l.row_tiles > 0 && r.splits > 1 ? ceil_div(r.part_rows, kJoinWaves) : 0);
-  const bool zero_here = zero_rows && KW == 0 && join_blocks == 0;
+  const bool zero_here = zero_rows && KW <= 0 && join_blocks == 0;
   const int64_t second = join_blocks + (zero_rows && !zero_here ? ceil_div(p.n_q, kJoinWaves * 64) : 0);
   if (second > 0x7FFFFFFF) return fail(SSA_ERR_UNSUPPORTED, "%s: too many sequences", fn);
   const int64_t cblocks = ceil_div(chunks, kAppend);
@@ -745,6 +1128,9 @@ int launch_paged(DenseParams& p, const PagedPlan& l, bool zero_rows, char* ws, h
 // The kernel for a call's cut and score rule.
 template <typename T, int D, int RULE, int VIEW, typename S>
 int launch_kw(DenseParams& p, const PagedPlan& l, bool zero, char* ws, hipStream_t st) {
+  // (16 rows a sequence and fewer: MEASURED with few_rows)
+  if constexpr (!std::is_same_v<S, T> && sizeof(T) == 2)
+    if (p.max_new * p.g <= kCols && (D == 64 || p.d % 16 == 0)) return launch_paged<T, D, RULE, -1, false, VIEW, S>(p, l, zero, ws, st);
   if (l.row_tiles == 0) return launch_paged<T, D, RULE, 0, false, VIEW, S>(p, l, zero, ws, st);
   // Where a good part of the keys are the call's own rows, their tiles are read as
   // contiguous ones (four prompts of 1000 tokens, 32 / 8 heads: 117 to 81 us); the
