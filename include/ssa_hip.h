@@ -630,8 +630,9 @@ int ssa_paged_step_zeroed(const void* q, const void* k, const void* v, int dtype
  *   zero_rows != 0: as ssa_paged_step_zeroed.
  * The other arguments and what is refused as ssa_paged_step; the workspace is
  * ssa_paged_step_general_workspace_bytes(...) bytes.  No reference counterpart. */
-size_t ssa_paged_step_general_workspace_bytes(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv, int d,
-                                              int64_t max_new, int64_t max_len, int64_t window, int64_t sinks);
+size_t ssa_paged_step_general_workspace_bytes(int dtype, int page_dtype, int64_t tokens, int64_t batch, int h_q,
+                                              int h_kv, int d, int64_t max_new, int64_t max_len, int64_t window,
+                                              int64_t sinks);
 int ssa_paged_step_general(const void* q, const void* k, const void* v, int dtype, int64_t tokens, int64_t batch,
                            int h_q, int h_kv, int d, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
                            int64_t v_st, int64_t v_sh, void* k_pages, void* v_pages, int page_dtype,

@@ -163,7 +163,7 @@ SIGNATURES = {
         [_vp, _vp, _vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64,
          _i64, _vp, _vp, _i64, _int, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _int,
          _vp, _vp, _i64, _i64, _flt, _flt, _vp, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
-    "ssa_paged_step_general_workspace_bytes": (_sz, [_int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64]),
+    "ssa_paged_step_general_workspace_bytes": (_sz, [_int, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64]),
     "ssa_paged_step_general": (
         _int,
         [_vp, _vp, _vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64,

@@ -111,8 +111,10 @@ inline BwdCut bwd_cut(int dtype, int64_t batch, int64_t n, int64_t n_q, int h_q,
 
 // The backward of rows that see two intervals: blocks of keys, how many of a head run at a time
 // (slots), the parts that dkv_kernel's plan may cut blocks into (extra, and one more for each that
-// it cuts), and the workspace.
+// it cuts), and the workspace.  Few blocks of keys are all cut alike, as those of one interval are,
+// with no plan (1024 x 2 rows of 8 / 2 heads, fp32, d = 64: the plan's two kernels take 13 us of 163).
 struct TwoCut {
+  bool planned;
   int64_t key_blocks;
   int slots, extra, most;
   size_t counts, entries, cut, part, part_floats, bytes;
@@ -126,11 +128,18 @@ inline TwoCut two_cut(const BwdCut& l, int dtype, int64_t batch, int64_t n, int 
   // a CU holds one block of bf16 at 128 features (its K and V lie in the LDS), two of the others
   t.slots = static_cast<int>(div_up(!f32 && wide ? 256 : 512, h_kv));
   t.extra = 4 * t.slots;
-  t.most = t.extra + 2 * t.slots;
+  t.most = t.extra + 3 * t.slots;
+  t.planned = 4 * t.key_blocks > t.slots;
   // (no more parts than each block of keys with one for every group of rows)
   const int64_t all = t.key_blocks * l.groups, parts = all < t.most ? all : t.most;
   t.counts = l.bounds + 2 * static_cast<size_t>(batch) * l.groups * 16;
-  t.entries = (t.counts + static_cast<size_t>(t.key_blocks) * 4 + 15) / 16 * 16;
+  if (!t.planned) {
+    t.part = t.counts;
+    t.part_floats = l.splits > 1 ? static_cast<size_t>(l.splits) * batch * n * h_kv * (wide ? 128 : 64) : 0;
+    t.bytes = t.part + 2 * t.part_floats * sizeof(float);
+    return t;
+  }
+  t.entries = (t.counts + static_cast<size_t>(t.key_blocks) * 8 + 15) / 16 * 16;
   t.cut = t.entries + static_cast<size_t>(t.key_blocks + t.most) * 16;
   t.part = t.cut + static_cast<size_t>(2 * t.slots + 1) * 16;
   t.part_floats = static_cast<size_t>(parts) * h_kv * keys * (wide ? 128 : 64);
@@ -146,6 +155,14 @@ inline int64_t seen_len(int64_t max_len, int64_t max_new, int64_t window, int64_
   return some < max_len ? some : max_len;
 }
 
+// Whether a call over pages of 8 bits is one for few_codes: bf16 queries, at most 16 rows a sequence
+// (32 sequences of up to 8191 tokens, 32 / 8 heads: 101 us against few_rows' 129), and rows of
+// whole 16-byte pieces where a lane loads 16.
+inline bool codes_call(int dtype, int page_dtype, int64_t max_new, int64_t g, int d) {
+  const bool held = page_dtype == SSA_DTYPE_I8 || page_dtype == SSA_DTYPE_E4M3;
+  return held && dtype == SSA_DTYPE_BF16 && max_new * g <= 16 && (d <= 64 || d % 16 == 0);
+}
+
 // Parts, tiles and workspace of a call.
 struct PagedPlan {
   int few_splits, row_splits, row_tiles, row_kw;
@@ -153,16 +170,18 @@ struct PagedPlan {
   size_t few_o, few_ml, row_o, row_ml, bytes;
 };
 
-// whole_tiles: parts of the keys of many rows are multiples of as many.
+// whole_tiles: parts of the keys of many rows are multiples of as many; codes: few_codes takes the call.
 inline PagedPlan paged_plan(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv, int d, int64_t max_new, int64_t max_len,
-                            int64_t whole_tiles = 64) {
+                            int64_t whole_tiles = 64, bool codes = false) {
   PagedPlan l{};
   max_new = max_new < tokens ? max_new : tokens;
   const int64_t g = h_q / h_kv, D = d <= 64 ? 64 : 128;
   // Few rows: parts of at least 256 keys, enough for two blocks a CU twice over
   // where the batch has sequences of unlike lengths to even out, once for one.
   const int64_t blocks = batch * h_kv;
-  int64_t s = div_up(batch > 1 ? 1024 : 512, blocks), most = div_up(max_len, 256);
+  // (few_codes runs three blocks a CU: 1536 of them take the 32 ragged sequences of int8 111 to 98 us,
+  // 2048 or 3072 the same or more, 32 of 8191 tokens 138 to 129 and 141)
+  int64_t s = div_up(batch > 1 ? (codes ? 1536 : 1024) : 512, blocks), most = div_up(max_len, 256);
   s = s < most ? s : most;
   s = s > 1 ? s : 1;
   l.few_len = div_up(div_up(max_len, s), 128) * 128;

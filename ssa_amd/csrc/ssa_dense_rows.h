@@ -252,6 +252,14 @@ struct Codes<uint16_t> {
   }
   template <bool E4M3>
   static __device__ __forceinline__ uint4 widen(uint32_t x, uint32_t y) {
+    if constexpr (E4M3) {  // (two codes an instruction)
+      auto two = [](uint32_t w, auto high) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, decltype(high)::value));
+      };
+      const std::false_type lo;
+      const std::true_type hi;
+      return make_uint4(two(x, lo), two(x, hi), two(y, lo), two(y, hi));
+    }
     float a[4], b[4];
     code_floats<E4M3>(x, a);
     code_floats<E4M3>(y, b);

@@ -99,13 +99,14 @@ static int backward(
   p.splits = l.splits;
   hipStream_t st = as_stream(stream);
   if (two) {
-    p.splits = 1;
-    p.key_blocks = static_cast<int>(two_l.key_blocks);
-    p.key_tiles = static_cast<int>(two_l.key_blocks / batch);
-    p.extra = two_l.extra;
-    p.counts = reinterpret_cast<int32_t*>(ws + two_l.counts);
-    p.entries = reinterpret_cast<int4*>(ws + two_l.entries);
-    p.cut = reinterpret_cast<int4*>(ws + two_l.cut);
+    if (two_l.planned) {
+      p.key_blocks = static_cast<int>(two_l.key_blocks);
+      p.key_tiles = static_cast<int>(two_l.key_blocks / batch);
+      p.extra = two_l.extra;
+      p.counts = reinterpret_cast<int2*>(ws + two_l.counts);
+      p.entries = reinterpret_cast<int4*>(ws + two_l.entries);
+      p.cut = reinterpret_cast<int4*>(ws + two_l.cut);
+    }
     p.part_k = reinterpret_cast<float*>(ws + two_l.part);
     p.part_v = p.part_k + two_l.part_floats;
     return dtype == SSA_DTYPE_F32 ? masked_two_backward_f32(&p, l, two_l, st) : masked_two_backward_bf16(&p, l, two_l, st);

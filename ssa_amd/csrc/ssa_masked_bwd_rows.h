@@ -67,7 +67,7 @@ struct BwdParams {
   // kTwo (spans hold two intervals a row, bounds two records a group): blocks of keys of all
   // batch elements, how many tiles of rows see each, and what the blocks of dkv_kernel take
   int key_blocks, key_tiles, extra;
-  int32_t* counts;  // [key_blocks]
+  int2* counts;     // [key_blocks]: how many, and the first of them
   int4* entries;    // [key_blocks + most]: block of keys (-1: nothing), part, parts, first slot
   int4* cut;        // how many, then of each its block of keys (-1: in one part), parts, first slot
 };
@@ -436,8 +436,9 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = wave % RW, kg = wave / RW;
-  int b, kvh, split, splits, tile, slot = 0;
-  if constexpr (SETS) {
+  int b, kvh, split, splits, tile, slot = 0, from = 0;  // from: no tile of rows before it sees the keys
+  const bool planned = SETS && p.entries != nullptr;
+  if (planned) {
     kvh = blockIdx.x % p.h_kv;
     const int4 entry = p.entries[blockIdx.x / p.h_kv];
     if (entry.x < 0) return;
@@ -446,6 +447,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
     split = entry.y;
     splits = entry.z;
     slot = entry.w;
+    from = p.counts[entry.x].y & ~63;
   } else {
     const int nbh = p.batch * p.h_kv;
     const int bh = blockIdx.x % nbh;
@@ -490,7 +492,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
   // whatever the mask)
   const int t_end = (p.groups + SG - 1) / SG;
   const int4* bounds = p.bounds + static_cast<int64_t>(b) * p.groups * (SETS ? 2 : 1);
-  int t_base = -64, t_seen = 0;
+  int t_base = from - 64, t_seen = 0;
   uint64_t t_mask = 0;
   int4 bd[SG];
   int2 ba[SETS ? SG : 1];
@@ -763,7 +765,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
   T* dvrow = static_cast<T*>(p.dv) + kid * p.d;
   // where a key's parts go: by part and key, or (kTwo) by slot, head and key of the block
   auto part_at = [&](int64_t id, int key_) {
-    if constexpr (SETS) return ((static_cast<int64_t>(slot + split) * p.h_kv + kvh) * (32 * KG) + (key_ - kb0)) * D;
+    if (planned) return ((static_cast<int64_t>(slot + split) * p.h_kv + kvh) * (32 * KG) + (key_ - kb0)) * D;
     return (split * kids + id) * D;
   };
   float* pk = splits > 1 ? p.part_k + part_at(kid, real ? key : kb0) : nullptr;
@@ -887,8 +889,8 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(BwdParams p) {
   const int at = blockIdx.x, b = at / p.key_tiles, k0 = (at - b * p.key_tiles) * keys;
   const int tiles = (p.groups + sg - 1) / sg;
   const int4* bounds = p.bounds + static_cast<int64_t>(b) * p.groups * 2;
-  __shared__ int s_sum[4];
-  int n = 0;
+  __shared__ int s_sum[4], s_first[4];
+  int n = 0, at0 = 0x7FFFFFFF;
   for (int t = threadIdx.x; t < tiles; t += 256) {
     bool hit = false;
     for (int g = t * sg; g < min((t + 1) * sg, p.groups); ++g) {
@@ -896,11 +898,17 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(BwdParams p) {
       hit |= (x.x < k0 + keys && x.y > k0) || (a.x < k0 + keys && a.y > k0);
     }
     n += hit ? 1 : 0;
+    if (hit) at0 = min(at0, t);
   }
-  const int w = lane_value(wave_incl_scan(n), 63);
-  if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = w;
+  const int w = lane_value(wave_incl_scan(n), 63), f = wave_min_i(at0);
+  if ((threadIdx.x & 63) == 0) {
+    s_sum[threadIdx.x >> 6] = w;
+    s_first[threadIdx.x >> 6] = f;
+  }
   __syncthreads();
-  if (threadIdx.x == 0) p.counts[at] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+  if (threadIdx.x == 0)
+    p.counts[at] = make_int2(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3],
+                             min(min(s_first[0], s_first[1]), min(min(s_first[2], s_first[3]), tiles)));
 }
 
 // The blocks of dkv_kernel, by one block.  A slot is a block of keys, of one head, that runs at a
@@ -911,7 +919,7 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(BwdParams p) {
 //                     where those of the last round would leave a good part of it idle they are cut
 //                     until they fill it
 // parts come after whole blocks (16001 rows that see 1000 keys back and 4 first ones, 16 / 4 heads,
-// d = 128: dK and dV 640 us with parts first and as long as whole blocks, MEASURED so).
+// d = 128: dK and dV 640 us with parts first and as long as whole blocks, 525 so).
 // At most key_blocks + most entries, most parts, 2 slots cut blocks.
 constexpr int kPlan = 1024, kSorted = 2 * kPlan;
 struct PlanSums {
@@ -950,7 +958,7 @@ __device__ __forceinline__ int plan_scan(int x, int (&s)[kPlan / 64], int& all) 
   const bool sorted = N <= kSorted;
   int64_t mine = 0;
   for (int x = tid; x < N; x += kPlan) {
-    const int h = p.counts[x];
+    const int h = p.counts[x].x;
     mine += h;
     if (sorted) s_h[x] = h;
   }
@@ -959,7 +967,7 @@ __device__ __forceinline__ int plan_scan(int x, int (&s)[kPlan / 64], int& all) 
   const int64_t share = max((total + slots - 1) / slots, static_cast<int64_t>(least));
   int64_t big = 0, n_big = 0;
   for (int x = tid; x < N; x += kPlan) {
-    const int h = p.counts[x];
+    const int h = p.counts[x].x;
     if (h > share) {
       big += h;
       ++n_big;
@@ -1002,7 +1010,7 @@ __device__ __forceinline__ int plan_scan(int x, int (&s)[kPlan / 64], int& all) 
   }
   int at_part = 0, at_cut = 0, at_one = 0;
   for (int x0 = 0, c = 0; x0 < N; x0 += kPlan, ++c) {
-    const int x = x0 + tid, h = x < N ? p.counts[x] : 0;
+    const int x = x0 + tid, h = x < N ? p.counts[x].x : 0;
     const bool is_big = x < N && h > share;
     const int rk = sorted ? (c == 0 ? rank[0] : rank[1]) : 0;
     const bool is_left = cut_left && x < N && !is_big && rk >= n_whole;
@@ -1079,7 +1087,7 @@ int launch_dkv(BwdParams& p, const TwoCut& cut, hipStream_t st) {
   const char* fn = "ssa_masked_attention_backward";
   using S = DkvShape<T, D, KG, RW>;
   if (int rc = reserve_lds(reinterpret_cast<const void*>(dkv_kernel<T, D, RULE, KG, RW, VIEW>), S::lds + (VIEW == kTwo ? 32 : 24) * S::QT * 2 + 1024, fn)) return rc;
-  if constexpr (VIEW == kTwo) {
+  if (VIEW == kTwo && p.entries != nullptr) {
     // (parts of at least 128 rows, as of one interval)
     constexpr int least = S::QT < 128 ? 128 / S::QT : 1;
     const int64_t grid = static_cast<int64_t>(p.key_blocks + cut.most) * p.h_kv;

@@ -43,11 +43,14 @@ extern "C" size_t ssa_paged_step_workspace_bytes(int dtype, int64_t tokens, int6
   return paged_plan(dtype, tokens, batch, h_q, h_kv, d, max_new, max_len).bytes;
 }
 
-extern "C" size_t ssa_paged_step_general_workspace_bytes(int dtype, int64_t tokens, int64_t batch, int h_q, int h_kv, int d,
-                                                         int64_t max_new, int64_t max_len, int64_t window, int64_t sinks) {
-  if (max_new <= 0 || max_len <= 0 || tokens <= 0 || window < 0 || sinks < 0) return 0;
-  return ssa_paged_step_workspace_bytes(dtype, tokens, batch, h_q, h_kv, d, max_new,
-                                        seen_len(max_len, max_new < tokens ? max_new : tokens, window, sinks));
+extern "C" size_t ssa_paged_step_general_workspace_bytes(int dtype, int page_dtype, int64_t tokens, int64_t batch, int h_q,
+                                                         int h_kv, int d, int64_t max_new, int64_t max_len, int64_t window,
+                                                         int64_t sinks) {
+  if (tokens <= 0 || batch <= 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0 || max_new <= 0 || max_len <= 0) return 0;
+  if (tokens > 0x7FFFFF00 || batch > 0x7FFFFF || max_len > 0x7FFFFF00 || window < 0 || sinks < 0) return 0;  // (what the call refuses)
+  max_new = max_new < tokens ? max_new : tokens;
+  return paged_plan(dtype, tokens, batch, h_q, h_kv, d, max_new, seen_len(max_len, max_new, window, sinks), 128,
+                    codes_call(dtype, page_dtype, max_new, h_q / h_kv, d)).bytes;
 }
 
 namespace {
@@ -124,7 +127,7 @@ static int paged_step(const char* fn, bool zero_rows, const General& x, const vo
   const int64_t window = x.window < max_len ? x.window : 0;
   const bool two = held || window > 0 || x.parents != nullptr;
   const PagedPlan l = paged_plan(dtype, tokens, batch, h_q, h_kv, d, max_new, seen_len(max_len, max_new, x.window, x.sinks),
-                                 two ? 128 : 64);
+                                 two ? 128 : 64, codes_call(dtype, x.page_dtype, max_new, h_q / h_kv, d));
   if (l.bytes > 0 && (workspace == nullptr || workspace_bytes < l.bytes))
     return fail(SSA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", fn, l.bytes,
                 workspace == nullptr ? size_t(0) : workspace_bytes);

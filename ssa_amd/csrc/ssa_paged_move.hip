@@ -123,16 +123,16 @@ __device__ __forceinline__ void keep_piece(int n, const int2* s_from, const int2
 
 constexpr int kMostKept = 64;
 
-// A thread takes a piece of a head's rows of K or V, of all kept tokens; E bytes an element.  The
-// first wave looks the rows up: rows that are in their place already, or that have no page at one
+// A thread takes a piece of a head's rows of K or V, of all kept tokens; E bytes an element.  Blocks of
+// one wave, which looks the rows up for itself: rows that are in their place already, or that have no page at one
 // end, are left out.
 template <int E>
-__global__ __launch_bounds__(256) void keep_kernel(MoveParams p) {
+__global__ __launch_bounds__(64) void keep_kernel(MoveParams p) {
   using U = std::conditional_t<E == 1, uint2, uint4>;
   __shared__ int2 s_from[kMostKept], s_to[kMostKept];  // page, row of it
   __shared__ int s_n;
   const int b = blockIdx.y;
-  if (threadIdx.x < 64) {  // the kept tokens up to the first one below 0, or the first that does not ascend
+  {  // the kept tokens up to the first one below 0, or the first that does not ascend
     const int lane = threadIdx.x, first = p.cached[b];
     const int x = lane < p.most ? p.kept[b * p.kept_stride + lane] : -1;
     const int before = __shfl_up(x, 1, 64);
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(256) void keep_kernel(MoveParams p) {
   }
   __syncthreads();
   const int n = s_n, per = p.d * E / static_cast<int>(sizeof(U)), rows = 2 * p.h_kv;
-  const int at = blockIdx.x * 256 + threadIdx.x;
+  const int at = blockIdx.x * 64 + threadIdx.x;
   if (n == 0) return;
   if (at < rows * per) {
     const int row = at / per, c = at - row * per;
@@ -290,13 +290,13 @@ extern "C" int ssa_paged_keep(void* k_pages, void* v_pages, int page_dtype, floa
     part.table += b0 * table_stride;
     part.cached += b0;
     part.kept += b0 * kept_stride;
-    const dim3 grid(static_cast<unsigned>(ceil_div(pieces, 256)), static_cast<unsigned>(batch - b0 < 65535 ? batch - b0 : 65535));
+    const dim3 grid(static_cast<unsigned>(ceil_div(pieces, 64)), static_cast<unsigned>(batch - b0 < 65535 ? batch - b0 : 65535));
     if (held)
-      keep_kernel<1><<<grid, dim3(256), 0, st>>>(part);
+      keep_kernel<1><<<grid, dim3(64), 0, st>>>(part);
     else if (page_dtype == SSA_DTYPE_F32)
-      keep_kernel<4><<<grid, dim3(256), 0, st>>>(part);
+      keep_kernel<4><<<grid, dim3(64), 0, st>>>(part);
     else
-      keep_kernel<2><<<grid, dim3(256), 0, st>>>(part);
+      keep_kernel<2><<<grid, dim3(64), 0, st>>>(part);
     if (int rc = check_launch(fn)) return rc;
   }
   return SSA_OK;

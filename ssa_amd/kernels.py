@@ -741,11 +741,12 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
     max_len = width * page if max_len is None else min(int(max_len), width * page)
     dt = _lib.elem_dtype(q)
     if general:
-        nbytes = _bytes("ssa_paged_step_general_workspace_bytes", dt, T, B, h_q, h_kv, d, max_new, max_len, window, sinks)
+        page_dt = _page_dtype(k_pages)
+        nbytes = _bytes("ssa_paged_step_general_workspace_bytes", dt, page_dt, T, B, h_q, h_kv, d, max_new, max_len, window, sinks)
         ws = _workspace(nbytes, q)
         _call_on(dev, "ssa_paged_step_general", q.data_ptr(), _at(k), _at(v), dt, T, B, h_q, h_kv, d, *qs, *ks, *vs,
-                 k_pages.data_ptr(), v_pages.data_ptr(), _page_dtype(k_pages), _at(k_scales), _at(v_scales), pages, page,
-                 *pools, *scale_steps, table.data_ptr(), table.stride(0) if B > 1 else 0, width, starts.data_ptr(),
+                 k_pages.data_ptr(), v_pages.data_ptr(), page_dt, _at(k_scales), _at(v_scales), pages, page, *pools,
+                 *scale_steps, table.data_ptr(), table.stride(0) if B > 1 else 0, width, starts.data_ptr(),
                  cached.data_ptr(), _at(parents), max_new, max_len, window, sinks,
                  math.sqrt(d) if scale_div is None else scale_div, softcap, _at(slopes), out.data_ptr(), *os,
                  int(zeroed), _at(error_flag), _at(ws), nbytes)
