@@ -693,6 +693,24 @@ int ssa_rope_axes(const void* q, const void* k, int dtype, int64_t batch, int64_
                   int64_t qo_sn, int64_t qo_sh, void* k_out, int64_t ko_sb, int64_t ko_sn, int64_t ko_sh,
                   void* stream);
 
+/* ---- calls with packed arguments ----------------------------------------- */
+
+/* Calls one of the entry points below with its arguments from an array, in order, eight bytes
+ * each: integers and pointers as int64_t, floats as double.  For callers to whom each argument
+ * costs (a Python call of 50 arguments takes 5 microseconds, one of a packed array 2). */
+#define SSA_CALL_MASK_SPANS 0
+#define SSA_CALL_MASK_SPANS_WINDOW 1
+#define SSA_CALL_MASKED_ATTENTION 2
+#define SSA_CALL_MASKED_ATTENTION_TWO 3
+#define SSA_CALL_MASKED_ATTENTION_BACKWARD 4
+#define SSA_CALL_MASKED_ATTENTION_TWO_BACKWARD 5
+#define SSA_CALL_PAGED_STEP 6
+#define SSA_CALL_PAGED_STEP_ZEROED 7
+#define SSA_CALL_PAGED_STEP_GENERAL 8
+#define SSA_CALL_PAGED_READ 9
+#define SSA_CALL_PAGED_KEEP 10
+int ssa_call(int function, const int64_t* arguments);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from typing import Optional
 
@@ -185,6 +186,15 @@ SIGNATURES = {
          _i64, _i64, _i64, _vp]),
 }
 
+SIGNATURES["ssa_call"] = (_int, [_int, _vp])
+
+# Entry points that ssa_call takes with packed arguments, in its numbering: name -> (number, packer).
+_SLOT = {_flt: "d"}  # (integers, sizes and pointers: q)
+PACKED = {name: (i, struct.Struct("".join(_SLOT.get(a, "q") for a in SIGNATURES[name][1])).pack) for i, name in enumerate((
+    "ssa_mask_spans", "ssa_mask_spans_window", "ssa_masked_attention", "ssa_masked_attention_two",
+    "ssa_masked_attention_backward", "ssa_masked_attention_two_backward", "ssa_paged_step", "ssa_paged_step_zeroed",
+    "ssa_paged_step_general", "ssa_paged_read", "ssa_paged_keep"))}
+
 _lib = None
 _lock = threading.Lock()
 
@@ -220,7 +230,19 @@ def load(path: Optional[str] = None):
 
 def call(name: str, *args) -> None:
     L = load()
-    st = getattr(L, name)(*args)
+    _raise(L, name, getattr(L, name)(*args))
+
+
+def call_packed(name: str, *args) -> None:
+    """``call`` through ssa_call: one array in place of each argument.  Null pointers are 0 here."""
+    L = _lib or load()
+    number, pack = PACKED[name]
+    st = L.ssa_call(number, pack(*args))
+    if st != SSA_OK:
+        _raise(L, name, st)
+
+
+def _raise(L, name: str, st: int) -> None:
     if st != SSA_OK:
         detail = (L.ssa_last_error() or b"").decode(errors="replace")
         if st == SSA_ERR_UNSUPPORTED:

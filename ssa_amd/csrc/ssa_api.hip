@@ -1,6 +1,9 @@
 // Status plumbing shared by every entry point of libssa_hip.
 #include <stdarg.h>
 #include <stdio.h>
+#include <string.h>
+
+#include <utility>
 
 #include "ssa_common.h"
 
@@ -53,3 +56,48 @@ extern "C" const char* ssa_status_str(int status) {
 }
 
 extern "C" const char* ssa_last_error(void) { return ssa::g_last_error; }
+
+// ssa_call: a slot of eight bytes as an argument of type T.
+namespace {
+
+template <typename T>
+T argument(int64_t slot) {
+  if constexpr (std::is_pointer_v<T>) {
+    return reinterpret_cast<T>(static_cast<uintptr_t>(slot));
+  } else if constexpr (std::is_floating_point_v<T>) {
+    double x;
+    memcpy(&x, &slot, sizeof(x));
+    return static_cast<T>(x);
+  } else {
+    return static_cast<T>(slot);
+  }
+}
+
+template <typename... A, size_t... I>
+int spread(int (*f)(A...), const int64_t* a, std::index_sequence<I...>) {
+  return f(argument<A>(a[I])...);
+}
+template <typename... A>
+int spread(int (*f)(A...), const int64_t* a) {
+  return spread(f, a, std::make_index_sequence<sizeof...(A)>());
+}
+
+}  // namespace
+
+extern "C" int ssa_call(int function, const int64_t* arguments) {
+  if (arguments == nullptr) return ssa::fail(SSA_ERR_INVALID_ARGUMENT, "ssa_call: null pointer");
+  switch (function) {
+    case SSA_CALL_MASK_SPANS: return spread(ssa_mask_spans, arguments);
+    case SSA_CALL_MASK_SPANS_WINDOW: return spread(ssa_mask_spans_window, arguments);
+    case SSA_CALL_MASKED_ATTENTION: return spread(ssa_masked_attention, arguments);
+    case SSA_CALL_MASKED_ATTENTION_TWO: return spread(ssa_masked_attention_two, arguments);
+    case SSA_CALL_MASKED_ATTENTION_BACKWARD: return spread(ssa_masked_attention_backward, arguments);
+    case SSA_CALL_MASKED_ATTENTION_TWO_BACKWARD: return spread(ssa_masked_attention_two_backward, arguments);
+    case SSA_CALL_PAGED_STEP: return spread(ssa_paged_step, arguments);
+    case SSA_CALL_PAGED_STEP_ZEROED: return spread(ssa_paged_step_zeroed, arguments);
+    case SSA_CALL_PAGED_STEP_GENERAL: return spread(ssa_paged_step_general, arguments);
+    case SSA_CALL_PAGED_READ: return spread(ssa_paged_read, arguments);
+    case SSA_CALL_PAGED_KEEP: return spread(ssa_paged_keep, arguments);
+    default: return ssa::fail(SSA_ERR_INVALID_ARGUMENT, "ssa_call: no function %d", function);
+  }
+}

@@ -483,8 +483,8 @@ def _on_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> int:
     return dev
 
 
-def _call_on(dev: int, name: str, *args) -> None:
-    """``call`` on the current stream of device ``dev``, with it current (launches go to the
+def _call_on(dev: int, name: str, *args, call=_lib.call_packed) -> None:
+    """``call_packed`` on the current stream of device ``dev``, with it current (launches go to the
     current device)."""
     stream = torch._C._cuda_getCurrentRawStream(dev)
     if dev == torch._C._cuda_getDevice():
@@ -494,8 +494,8 @@ def _call_on(dev: int, name: str, *args) -> None:
             call(name, *args, stream)
 
 
-def _at(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _rows16(t: torch.Tensor):
@@ -704,22 +704,24 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
         raise ValueError(f"q {tuple(q.shape)} does not fit pages {tuple(k_pages.shape)}")
     dtype = q.dtype
     held = k_pages.dtype in HELD_DTYPES
-    like_q = (("k", k), ("v", v), ("out", out))
-    for name, t in like_q if held else like_q + (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t is not None and t.dtype != dtype:
-            raise TypeError(f"{name} must have q's dtype {dtype}, got {t.dtype}")
+    if (not held and k_pages.dtype != dtype) or (k is not None and (k.dtype != dtype or v.dtype != dtype)) or (
+            out is not None and out.dtype != dtype):
+        for name, t in (("k", k), ("v", v), ("out", out), ("k_pages", k_pages)):
+            if t is not None and t.dtype != dtype:
+                raise TypeError(f"{name} must have q's dtype {dtype}, got {t.dtype}")
     general = held or window != 0 or sinks != 0 or parents is not None
     B, width = table.shape
-    for name, t, shape in (("table", table, (B, width)), ("starts", starts, (B + 1,)), ("cached", cached, (B,))):
-        if t.dtype != torch.int32 or t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
-            raise ValueError(f"{name} must be an int32 {list(shape)} tensor with contiguous rows")
+    if not (table.dtype == starts.dtype == cached.dtype == torch.int32 and starts.shape == (B + 1,) and cached.shape == (B,)
+            and table.is_contiguous() and starts.is_contiguous() and cached.is_contiguous()):
+        _table_rows(table, "table", (B, width))
+        _table_rows(starts, "starts", (B + 1,))
+        _table_rows(cached, "cached", (B,))
     pools = _pool_strides(k_pages, v_pages, k is not None)
     scale_steps = _scale_strides(k_pages, v_pages, k_scales, v_scales, k is not None)
     if parents is not None and (parents.dtype != torch.int32 or parents.shape != (T,) or (T > 1 and parents.stride(0) != 1)):
         raise ValueError(f"parents must be a contiguous int32 [{T}] tensor")
     slopes = _check_slopes(slopes, h_q)
-    if error_flag is not None and (error_flag.dtype != torch.int32 or error_flag.numel() != 1):
-        raise ValueError("error_flag must be one int32")
+    _check_flag(error_flag)
     q, qs = _rows16(q)
     ks = vs = (0, 0)
     if k is not None:
@@ -940,7 +942,7 @@ def axes_run(plan: AxesPlan, q: torch.Tensor, k: Optional[torch.Tensor], inverse
         k_at, ks, ko_at = k.data_ptr(), _steps(k), ko.data_ptr()
     _call_on(plan.dev, "ssa_rope_axes", q.data_ptr(), k_at, plan.dtype, B, n, h_q, h_k, d, *_steps(q), *ks,
              plan.positions.data_ptr(), *plan.turn, plan.freqs.data_ptr(), 2 * plan.freqs.shape[0], inverse, qo.data_ptr(),
-             n * h_q * d, h_q * d, d, ko_at, n * h_k * d, h_k * d, d)
+             n * h_q * d, h_q * d, d, ko_at, n * h_k * d, h_k * d, d, call=call)
     return qo, ko
 
 

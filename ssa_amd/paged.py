@@ -61,10 +61,11 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
     page_size a power of 2 from 8 to 4096.  No gradient: inputs that want one are refused (call
     it under ``torch.no_grad()``, or detach them)."""
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or
-                                    any([t.requires_grad for t in (k, v, slopes, out, k_scales, v_scales) if t is not None])):
+                                    (k is not None and (k.requires_grad or v is not None and v.requires_grad)) or
+                                    any([t.requires_grad for t in (slopes, out, k_scales, v_scales) if t is not None])):
         raise NotImplementedError("paged_step has no gradient: call it under torch.no_grad(), or detach its inputs")
     _lib.refuse_tangents("paged_step", q, k, v, k_pages, v_pages, slopes)
-    window = _window(window, sinks)
+    window = 0 if window is None and sinks == 0 else _window(window, sinks)
     if softcap is not None and not softcap > 0:
         raise ValueError(f"softcap must be positive, got {softcap}")
     flag = torch.zeros(1, device=q.device, dtype=torch.int32) if check else None
