@@ -362,6 +362,11 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
         *reinterpret_cast<uint4*>(vt + at) = vreg[i];
       }
     } else {
+      if (k0 + 32 > min(rows.new_from, k_end)) {  // (rows without a key may hold a code for NaN, which a weight of 0 does not silence)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (k0 + 8 * i + my_row >= min(rows.new_from, k_end)) vreg[i] = make_uint4(0u, 0u, 0u, 0u);
+      }
       auto put = [&](auto kind) {
         constexpr bool E4M3 = decltype(kind)::value;
         constexpr int W = sizeof(T) == 2 ? 2 : 1;  // words of codes that make 16 bytes of T
@@ -586,7 +591,8 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
 // softmax that 32 do.  A product's contraction takes the features in the order in which 16 bytes a
 // lane bring them, and Q is loaded in that order too; V is transposed by its reads
 // (ds_read_b64_tr_b8).  The call's own rows,
-// which have no codes yet, are added one by one at the end, by one wave of the last part.
+// which have no codes yet, are added one by one at the end, by one wave of the last part, wherever
+// they lie.
 // 64 sequences of 8191 cached tokens, 32 / 8 heads, int8: 233 us, 4.8 TB/s of codes and scales (few_rows
 // 279); 32 ragged ones 98 us, 3.5 TB/s: their blocks end at unlike times.
 constexpr int kCols = 16;
@@ -747,6 +753,11 @@ __device__ __forceinline__ void few_codes(const DenseParams& p, const int block,
       const int k0 = key_at(x);
       // (addresses that differ by an exclusive or are formed anew: kept, they take twelve registers)
       const int k_at = in_branch(k_base), v_at = in_branch(v_base);
+      if (k0 + 32 > codes_end) {  // (rows without a key may hold a code for NaN, which a weight of 0 does not silence)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (k0 + 8 * i + my_row >= codes_end) vreg[i] = make_uint4(0u, 0u, 0u, 0u);
+      }
       put(kt, kreg);
       put(vt, vreg);
       s_scale[wave][lane >> 5][key32] = scale_reg;
@@ -894,10 +905,12 @@ __device__ __forceinline__ void few_codes(const DenseParams& p, const int block,
   const int64_t part_row = (static_cast<int64_t>(b) * p.h_kv + kvh) * kFew;
   const int quads = p.d / 4;
   auto sees_of = [&](int t) { return paged_sees(p, cached + (tree ? s_depth[t] : t), cached, tree ? s_kin[t] : 0); };
-  // whether the part holds a key that token t sees
+  // whether the part holds a key that token t sees: of its tiles those with codes, of the last part
+  // the call's own rows too
+  const int own = t_end == walk.n && codes_end < sq.len ? sq.len : 0;
   auto here_of = [&](int t) {
     const Sees w = sees_of(t);
-    return w.any(part_x[0], part_y[0]) || w.any(part_x[1], part_y[1]);
+    return w.any(part_x[0], min(part_y[0], codes_end)) || w.any(part_x[1], min(part_y[1], codes_end)) || w.any(codes_end, own);
   };
   for (int e = tid; e < R * quads; e += kThreads) {
     const int r = e / quads, dd = (e - r * quads) * 4;
@@ -935,10 +948,11 @@ __device__ __forceinline__ void few_codes(const DenseParams& p, const int block,
     const int t = r / p.g, h = kvh * p.g + r - t * p.g, ps = cached + (tree ? s_depth[t] : t);
     const float sl = has_bias(RULE) ? slope_of(p.rule, h) : 0.0f;
     float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
+    const T* qr = static_cast<const T*>(p.q) + (sq.first + t) * p.q_sn + h * p.q_sh;
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
-      exact_keys<T, S, true>(rows, p.rule, sees_of(t), static_cast<const T*>(p.q) + (sq.first + t) * p.q_sn + h * p.q_sh, p.d,
-                             part_x[y], min(part_y[y], sq.len), sl, ps, tree ? s_depth : nullptr, o, m, l);
+    for (int y = 0; y < 3; ++y)
+      exact_keys<T, S, true>(rows, p.rule, sees_of(t), qr, p.d, y < 2 ? part_x[y & 1] : codes_end,
+                             y < 2 ? min(part_y[y & 1], codes_end) : own, sl, ps, tree ? s_depth : nullptr, o, m, l);
     const int64_t pr = split * p.part_rows + part_row + r;
     T* orow = static_cast<T*>(p.out) + (sq.first + t) * p.o_sn + h * p.o_sh;
 #pragma unroll

@@ -141,6 +141,15 @@ CASES = [
     (F32, E4M3, [(40, 100), (1, 64), (33, 0)], False, 6, 2, 96, 16, 0, 0, 2.0, False),
     (F32, I8, [(90, 1000)], False, 4, 2, 120, 16, 0, 0, 0.0, False),
     (BF16, I8, [(200, 3000), (1, 64)], False, 16, 4, 128, 64, 0, 0, 0.0, True),
+    # few rows over 8 bits, of every width, group and number of tokens
+    (BF16, I8, [(1, 31), (1, 700)], False, 2, 1, 8, 8, 0, 0, 0.0, False),
+    (BF16, E4M3, [(1, 100), (2, 1), (1, 33)], False, 4, 2, 24, 16, 0, 0, 0.0, True),
+    (BF16, E4M3, [(1, 600), (1, 0)], False, 16, 1, 112, 32, 0, 0, 3.0, False),
+    (BF16, I8, [(16, 505), (9, 100), (1, 64)], False, 2, 2, 128, 64, 0, 0, 0.0, False),
+    (BF16, I8, [(7, 300), (8, 1030)], True, 4, 2, 80, 16, 0, 0, 0.0, True),
+    (BF16, E4M3, [(16, 60), (16, 3), (11, 520)], True, 3, 3, 64, 8, 9, 5, 2000.0, True),
+    (BF16, I8, [(1, 5000), (1, 40), (1, 900)], False, 14, 1, 128, 32, 300, 40, 0.0, True),
+    (F32, I8, [(16, 505), (9, 100), (1, 64)], False, 2, 2, 128, 64, 0, 0, 0.0, False),
     # all together
     (BF16, I8, [(1, 600), (45, 2000), (0, 0), (1, 9), (130, 31)], False, 28, 4, 128, 32, 256, 4, 5.0, True),
     (BF16, E4M3, [(20, 4), (64, 700), (8, 0)], True, 8, 4, 128, 16, 5, 6, 0.0, True),
@@ -625,3 +634,82 @@ def test_cache(dev, dtype, hold, window, sinks):
     for s in list(rows):
         cache.free(s)
     assert cache.free_pages == 60
+
+
+@pytest.mark.parametrize("hold", [I8, E4M3])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_own_rows_across_parts(dev, dtype, hold):
+    """New tokens on both sides of a border between parts, with hidden keys in the window's first tile whose
+    codes stand for NaN: the rows that are computed again count every key once."""
+    from ssa_amd import paged_step
+
+    for m, window in ((14, 300), (3, 290), (16, 520)):
+        for cached in range(560, 660, 4):
+            s, keys, parents = batch(63, dtype, [(m, cached)], 2, 2, 64, 8, hold, window, 0)
+            x = {n: t.clone() for n, t in s.items()}
+            lo = cached + 1 - window
+            for j in range(lo // 8 * 8, lo):   # (of the page that holds the window's first key)
+                x["v_scales"][x["table"][0, j // 8], j % 8] = math.nan
+            out = paged_step(**{n: t.to(dev) for n, t in x.items()}, window=window, check=True)
+            (_, _, _, (value, bound)), = expect(s, keys, parents, [(m, cached)], window=window)
+            check(out, value, bound, f"{m} {window} {cached}")
+
+
+@pytest.mark.parametrize("dtype,m,g", [(BF16, 1, 4), (BF16, 9, 2), (F32, 1, 4), (BF16, 30, 1), (BF16, 40, 4)])
+def test_rows_without_a_key_are_not_looked_at(dev, dtype, m, g):
+    """Pages of e4m3 whose other rows hold codes for NaN take no longer than pages of zeros (the rows
+    that such a code reached would be computed again, key by key)."""
+    from ssa_amd import paged_step
+
+    seqs, h_kv = [(m, 4001)] * 4, 2
+    s, _, _ = batch(64, dtype, seqs, h_kv * g, h_kv, 128, 64, E4M3)
+    x = {n: t.to(dev) for n, t in s.items()}
+    took = []
+    for fill in (0, 0x7F):
+        y = {n: t.clone() for n, t in x.items()}
+        for n in ("k_pages", "v_pages"):
+            flat = y[n].view(I8)
+            for b in range(4):
+                last = int(s["table"][b, 4001 // 64])
+                flat[last, 4001 % 64:] = fill
+        for keys_there in (False, True):
+            if keys_there:
+                y["k"] = y["v"] = None  # (the pages hold them now)
+            z = dict(y, max_new=m, max_len=4001 + m)
+            for _ in range(3):
+                paged_step(**z)
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            best = 1e9
+            for _ in range(5):
+                a.record()
+                for _ in range(10):
+                    paged_step(**z)
+                b.record()
+                b.synchronize()
+                best = min(best, a.elapsed_time(b))
+            took.append(best)
+    assert took[2] < 3 * took[0] and took[3] < 3 * took[1], took
+
+
+def test_rows_aligned_to_8_bytes(dev):
+    """Codes whose rows lie at odd multiples of 8 bytes."""
+    from ssa_amd import paged_keep, paged_read, paged_step
+
+    for dtype, m in ((BF16, 1), (BF16, 12), (BF16, 40), (F32, 3)):
+        seqs = [(m, 300), (1, 70)]
+        s, keys, parents = batch(65, dtype, seqs, 8, 2, 64, 16, I8)
+        x = {n: t.to(dev) for n, t in s.items()}
+        pages, page, h, d = x["k_pages"].shape
+        for i, n in enumerate(("k_pages", "v_pages")):
+            wide = torch.zeros(pages * page * h * (d + 8) + 8, device=dev, dtype=I8)[8:].view(pages, page, h, d + 8)
+            wide[..., :d] = x[n]
+            x[n] = wide[..., :d]
+        out = paged_step(**x, check=True)
+        for b, at, n, (value, bound) in expect(s, keys, parents, seqs):
+            check(out[at:at + n], value, bound, f"sequence {b}")
+        kept = torch.tensor([[0, 2] if m > 2 else [0, -1], [0, -1]], device=dev, dtype=torch.int32)
+        scales = {n: x[n] for n in ("k_scales", "v_scales")}
+        paged_keep(x["k_pages"], x["v_pages"], x["table"], x["cached"], kept, check=True, **scales)
+        k, _ = paged_read(x["k_pages"], x["v_pages"], x["table"], x["starts"], x["cached"], m + 1, dtype=F32, check=True, **scales)
+        want = s["k"][[0, 2] if m > 2 else [0]]
+        assert torch.equal(k[:len(want)].cpu(), values(*held(want, I8)).float())
