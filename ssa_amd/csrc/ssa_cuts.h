@@ -139,7 +139,7 @@ inline TwoCut two_cut(const BwdCut& l, int dtype, int64_t batch, int64_t n, int 
     t.bytes = t.part + 2 * t.part_floats * sizeof(float);
     return t;
   }
-  t.entries = (t.counts + static_cast<size_t>(t.key_blocks) * 8 + 15) / 16 * 16;
+  t.entries = (t.counts + static_cast<size_t>(t.key_blocks) * 4 + 15) / 16 * 16;
   t.cut = t.entries + static_cast<size_t>(t.key_blocks + t.most) * 16;
   t.part = t.cut + static_cast<size_t>(2 * t.slots + 1) * 16;
   t.part_floats = static_cast<size_t>(parts) * h_kv * keys * (wide ? 128 : 64);

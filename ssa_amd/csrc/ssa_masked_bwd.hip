@@ -103,7 +103,7 @@ static int backward(
       p.key_blocks = static_cast<int>(two_l.key_blocks);
       p.key_tiles = static_cast<int>(two_l.key_blocks / batch);
       p.extra = two_l.extra;
-      p.counts = reinterpret_cast<int2*>(ws + two_l.counts);
+      p.counts = reinterpret_cast<int*>(ws + two_l.counts);
       p.entries = reinterpret_cast<int4*>(ws + two_l.entries);
       p.cut = reinterpret_cast<int4*>(ws + two_l.cut);
     }

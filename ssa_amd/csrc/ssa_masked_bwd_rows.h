@@ -67,7 +67,7 @@ struct BwdParams {
   // kTwo (spans hold two intervals a row, bounds two records a group): blocks of keys of all
   // batch elements, how many tiles of rows see each, and what the blocks of dkv_kernel take
   int key_blocks, key_tiles, extra;
-  int2* counts;     // [key_blocks]: how many, and the first of them
+  int* counts;      // [key_blocks]: row tiles that see it
   int4* entries;    // [key_blocks + most]: block of keys (-1: nothing), part, parts, first slot
   int4* cut;        // how many, then of each its block of keys (-1: in one part), parts, first slot
 };
@@ -436,7 +436,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = wave % RW, kg = wave / RW;
-  int b, kvh, split, splits, tile, slot = 0, from = 0;  // from: no tile of rows before it sees the keys
+  int b, kvh, split, splits, tile, slot = 0;
   const bool planned = SETS && p.entries != nullptr;
   if (planned) {
     kvh = blockIdx.x % p.h_kv;
@@ -447,7 +447,6 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
     split = entry.y;
     splits = entry.z;
     slot = entry.w;
-    from = p.counts[entry.x].y & ~63;
   } else {
     const int nbh = p.batch * p.h_kv;
     const int bh = blockIdx.x % nbh;
@@ -492,7 +491,7 @@ __global__ __launch_bounds__(64 * KG * RW, (DkvShape<T, D, KG, RW>::kPerSimd * 4
   // whatever the mask)
   const int t_end = (p.groups + SG - 1) / SG;
   const int4* bounds = p.bounds + static_cast<int64_t>(b) * p.groups * (SETS ? 2 : 1);
-  int t_base = from - 64, t_seen = 0;
+  int t_base = -64, t_seen = 0;
   uint64_t t_mask = 0;
   int4 bd[SG];
   int2 ba[SETS ? SG : 1];
@@ -889,8 +888,8 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(BwdParams p) {
   const int at = blockIdx.x, b = at / p.key_tiles, k0 = (at - b * p.key_tiles) * keys;
   const int tiles = (p.groups + sg - 1) / sg;
   const int4* bounds = p.bounds + static_cast<int64_t>(b) * p.groups * 2;
-  __shared__ int s_sum[4], s_first[4];
-  int n = 0, at0 = 0x7FFFFFFF;
+  __shared__ int s_sum[4];
+  int n = 0;
   for (int t = threadIdx.x; t < tiles; t += 256) {
     bool hit = false;
     for (int g = t * sg; g < min((t + 1) * sg, p.groups); ++g) {
@@ -898,17 +897,12 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(BwdParams p) {
       hit |= (x.x < k0 + keys && x.y > k0) || (a.x < k0 + keys && a.y > k0);
     }
     n += hit ? 1 : 0;
-    if (hit) at0 = min(at0, t);
   }
-  const int w = lane_value(wave_incl_scan(n), 63), f = wave_min_i(at0);
-  if ((threadIdx.x & 63) == 0) {
-    s_sum[threadIdx.x >> 6] = w;
-    s_first[threadIdx.x >> 6] = f;
-  }
+  const int w = lane_value(wave_incl_scan(n), 63);
+  if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = w;
   __syncthreads();
   if (threadIdx.x == 0)
-    p.counts[at] = make_int2(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3],
-                             min(min(s_first[0], s_first[1]), min(min(s_first[2], s_first[3]), tiles)));
+    p.counts[at] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
 }
 
 // The blocks of dkv_kernel, by one block.  A slot is a block of keys, of one head, that runs at a
@@ -958,7 +952,7 @@ __device__ __forceinline__ int plan_scan(int x, int (&s)[kPlan / 64], int& all) 
   const bool sorted = N <= kSorted;
   int64_t mine = 0;
   for (int x = tid; x < N; x += kPlan) {
-    const int h = p.counts[x].x;
+    const int h = p.counts[x];
     mine += h;
     if (sorted) s_h[x] = h;
   }
@@ -967,7 +961,7 @@ __device__ __forceinline__ int plan_scan(int x, int (&s)[kPlan / 64], int& all) 
   const int64_t share = max((total + slots - 1) / slots, static_cast<int64_t>(least));
   int64_t big = 0, n_big = 0;
   for (int x = tid; x < N; x += kPlan) {
-    const int h = p.counts[x].x;
+    const int h = p.counts[x];
     if (h > share) {
       big += h;
       ++n_big;
@@ -1010,7 +1004,7 @@ __device__ __forceinline__ int plan_scan(int x, int (&s)[kPlan / 64], int& all) 
   }
   int at_part = 0, at_cut = 0, at_one = 0;
   for (int x0 = 0, c = 0; x0 < N; x0 += kPlan, ++c) {
-    const int x = x0 + tid, h = x < N ? p.counts[x].x : 0;
+    const int x = x0 + tid, h = x < N ? p.counts[x] : 0;
     const bool is_big = x < N && h > share;
     const int rk = sorted ? (c == 0 ? rank[0] : rank[1]) : 0;
     const bool is_left = cut_left && x < N && !is_big && rk >= n_whole;
