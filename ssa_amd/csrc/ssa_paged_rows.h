@@ -289,12 +289,10 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
   const int my_row = lane >> 3, my_at = (lane & 7) * CB;
   const uint32_t ks8 = static_cast<uint32_t>(rows.k_sn), vs8 = static_cast<uint32_t>(rows.v_sn);
   // kTwo: a key of the sequence that stands for key j where j is looked up, one that some row sees
+  // (or a new one, whose page the table has too)
   auto seen_key = [&](int j) { return min(j >= first_a ? max(j, from) : j, k_end - 1); };
-  // HELD: the last key in the pages where j is a new one
-  const int paged_last = HELD ? max(min(rows.new_from, k_end) - 1, 0) : 0;
   float scale_reg = 1.0f;  // HELD: of K's key lane, from lane 32 on of V's key lane - 32
   auto pages_at = [&](int k0) {
-    if constexpr (HELD) return k0 >= 0 ? rows.entry_of(min(seen_key(k0 + rr), paged_last)) : 0;
     if constexpr (SETS) return k0 >= 0 ? rows.entry_of(seen_key(k0 + rr)) : 0;
     return k0 < k_end ? rows.entry_of(min(k0 + rr, k_end - 1)) : 0;
   };
@@ -677,7 +675,6 @@ __device__ __forceinline__ void few_codes(const DenseParams& p, const int block,
   // (the banks of a tile's rows: 16-byte chunk c of row r lies at chunk c ^ f(r))
   auto chunk = [&](int r, int c) { return r * D + ((c ^ (D == 128 ? r & 7 : (r >> 2) & 3)) << 4); };
   auto seen_key = [&](int j) { return min(j >= first_a ? max(j, from) : j, sq.len - 1); };
-  const int paged_last = max(min(rows.new_from, sq.len) - 1, 0);
   // tiles of new keys alone are left out: they have no codes
   auto key_at = [&](int x) { return x < t_end ? walk.at(x) * 32 : 0x7FFFFFFF; };
   const int codes_end = min(rows.new_from, sq.len);
@@ -686,10 +683,11 @@ __device__ __forceinline__ void few_codes(const DenseParams& p, const int block,
   const uint32_t vo = my_at < p.d ? my_row * static_cast<uint32_t>(rows.v_sn) + my_at : kNoChunk;
   uint4 kreg[4], vreg[4];
   float scale_reg = 1.0f;  // of K's key lane, from lane 32 on of V's key lane - 32
-  auto find = [&](int k0) { return k0 < codes_end ? rows.entry_of(min(seen_key(k0 + key32), paged_last)) : 0; };
+  auto find = [&](int k0) { return k0 < codes_end ? rows.entry_of(seen_key(k0 + key32)) : 0; };
   auto load = [&](int k0, int entry) {
     const int pg = rows.checked(entry);
-    scale_reg = rows.scale_of(lane >= 32, pg, min(seen_key(k0 + key32), paged_last));
+    const int j = seen_key(k0 + key32);
+    scale_reg = j < codes_end ? rows.scale_of(lane >= 32, pg, j) : 1.0f;
     auto fetch = [&](int i, __amdgpu_buffer_rsrc_t kb, __amdgpu_buffer_rsrc_t vb, int ks, int vs) {
       kreg[i] = load_codes<D>(kb, ko, ks);
       vreg[i] = load_codes<D>(vb, vo, vs);

@@ -655,6 +655,15 @@ def test_own_rows_across_parts(dev, dtype, hold):
             check(out, value, bound, f"{m} {window} {cached}")
 
 
+@pytest.mark.parametrize("hold", [None, I8, E4M3])
+@pytest.mark.parametrize("dtype,h_q,m,trees", [(BF16, 2, 1, False), (F32, 2, 3, False), (BF16, 8, 9, False), (F32, 4, 30, True), (BF16, 1, 16, True)])
+def test_windows_that_leave_no_cached_key(dev, dtype, hold, h_q, m, trees):
+    """A window of one key: no page of the cached keys is looked up, wherever the new ones begin."""
+    seqs = [(m, 128), (1, 32), (m, 40), (m, 0), (1, 56), (0, 64), (2, 127)]
+    for sinks in (0, 1):
+        test_step(dev, (dtype, hold, seqs, trees, h_q, 1, 64, 8, 1, sinks, 0.0, False))
+
+
 @pytest.mark.parametrize("dtype,m,g", [(BF16, 1, 4), (BF16, 9, 2), (F32, 1, 4), (BF16, 30, 1), (BF16, 40, 4)])
 def test_rows_without_a_key_are_not_looked_at(dev, dtype, m, g):
     """Pages of e4m3 whose other rows hold codes for NaN take no longer than pages of zeros (the rows
