@@ -233,7 +233,7 @@ __device__ __forceinline__ void code_floats(uint32_t w, float (&f)[4]) {
     f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+    for (int i = 0; i < 4; ++i) f[i] = static_cast<float>(static_cast<int>(__builtin_amdgcn_sbfe(w, 8 * i, 8)));  // (one instruction a code)
   }
 }
 // The codes of 16 bytes of T, exact in bf16 too: eight (two words of them) or four.
@@ -310,6 +310,16 @@ struct KeyRows {
     if (static_cast<unsigned>(pg) < static_cast<unsigned>(num_pages)) return pg;
     if (error_flag != nullptr) atomicOr(error_flag, 1);
     return 0;
+  }
+  // The same for the tiles of a loop, behind which `report` says what was outside the pool (with a
+  // check that sets the flag itself, 2048 tokens over 30720 of int8 take 1690 us for 1650).
+  __device__ __forceinline__ int noted(int pg, int& outside) const {
+    const bool in = static_cast<unsigned>(pg) < static_cast<unsigned>(num_pages);
+    outside |= in ? 0 : 1;
+    return in ? pg : 0;
+  }
+  __device__ __forceinline__ void report(int outside) const {
+    if (outside != 0 && error_flag != nullptr) atomicOr(error_flag, 1);
   }
   // Pages of 8 bits: whether key j is one of the call's own rows, and where they are.
   __device__ __forceinline__ bool is_new(int j) const { return j >= new_from; }
@@ -573,6 +583,10 @@ __device__ __forceinline__ int fold_tile(int t, int tiles, int heads) {
   return round * per + (left < per ? left : per) - 1 - at;
 }
 
+// What a tile over pages of 8 bits holds: codes, or some of the call's own rows.  Each kind has a loop
+// of its own in dense_rows.
+enum { kGiven, kI8, kE4m3 };
+
 // FRESH: tiles of a paged call's own rows are read as contiguous ones are.
 template <typename T, int D, bool PAGED, int RULE, int KW, bool FRESH = false, int VIEW = kOne, typename S = T>
 __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, char* lds) {
@@ -764,33 +778,37 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
   const uint32_t koff = chunk_ok ? my * ks + sc * 16 : kNoChunk, voff = chunk_ok ? my * vs + sc * 16 : kNoChunk;
   uint4 kreg[NP], vreg[NP];
   int pg[PAGED ? NP : 1];
-  // HELD: the page of the key whose scale this thread fetches (K's of KT threads, then V's), the
-  // scale, and whether the loaded tile is of codes
+  // HELD: the scale that this thread fetches, of key `scale_key` of a tile (K's by SW waves, V's by the
+  // next), and its page
+  constexpr int SW = KT > 64 ? KT / 64 : 1;
+  const int scale_key = KT < 64 ? lane : tid & (KT - 1);
+  const bool scale_here = wave < 2 * SW && (KT >= 64 || lane < KT), scale_of_v = wave >= SW;
   const uint32_t ks8 = static_cast<uint32_t>(rows.k_sn), vs8 = static_cast<uint32_t>(rows.v_sn);
   const uint32_t koff8 = chunk_ok ? my * ks8 + sc * E : kNoChunk, voff8 = chunk_ok ? my * vs8 + sc * E : kNoChunk;
   int scale_pg = 0;
   float scale_reg = 1.0f;
-  bool as_codes = false;
+  int outside = 0;  // whether a page of a tile was outside the pool
   const int paged_end = PAGED ? min(rows.new_from, static_cast<int>(n_keys)) : 0;
   constexpr int RPW = 64 / NCH;  // rows of a wave's load
   auto find_pages = [&](int t) {
     if constexpr (PAGED) {
 #pragma unroll
       for (int i = 0; i < NP; ++i) pg[i] = rows.entry_of(min(seen_key(tile_key(t) + i * RPP + wave * RPW), last));
-      if constexpr (HELD) scale_pg = rows.entry_of(min(seen_key(tile_key(t) + (tid & (KT - 1))), last));
+      if (HELD && scale_here) scale_pg = rows.entry_of(min(seen_key(tile_key(t) + scale_key), last));
     }
   };
-  auto load_tile = [&](int t) {
+  // (kind: of HELD tiles whether they are codes alone, int8 or e4m3, or have the call's own rows)
+  auto load_tile = [&](auto kind, int t) {
+    constexpr int KIND = decltype(kind)::value;
     const int j0 = tile_key(t);
     if constexpr (HELD) {
-      const int j = min(seen_key(j0 + (tid & (KT - 1))), last);
+      const int j = min(seen_key(j0 + scale_key), last);
       scale_reg = 1.0f;
-      if (tid < 2 * KT && !rows.is_new(j)) scale_reg = rows.scale_of(tid >= KT, rows.checked(scale_pg), j);
-      as_codes = j0 + KT <= paged_end;
-      if (as_codes) {
+      if (scale_here && !rows.is_new(j)) scale_reg = rows.scale_of(scale_of_v, rows.noted(scale_pg, outside), j);
+      if constexpr (KIND != kGiven) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          const int64_t page = rows.checked(__builtin_amdgcn_readfirstlane(pg[i])), r0 = (j0 + i * RPP + wave * RPW) & rows.page_mask;
+          const int64_t page = rows.noted(__builtin_amdgcn_readfirstlane(pg[i]), outside), r0 = (j0 + i * RPP + wave * RPW) & rows.page_mask;
           kreg[i] = Codes<T>::load(row_buffer(rows.k + page * rows.k_sb + r0 * rows.k_sn, kAllBytes), koff8);
           vreg[i] = Codes<T>::load(row_buffer(rows.v + page * rows.v_sb + r0 * rows.v_sn, kAllBytes), voff8);
         }
@@ -809,7 +827,7 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
             vreg[i] = *reinterpret_cast<const uint4*>(vr + sc * E);
           } else {
             const S *kr, *vr;
-            rows.code_rows(rows.checked(rows.entry_of(x)), x, kr, vr);
+            rows.code_rows(rows.noted(rows.entry_of(x), outside), x, kr, vr);
             kreg[i] = widen_one<T>(Codes<T>::load(kr + sc * E), rows.e4m3);
             vreg[i] = widen_one<T>(Codes<T>::load(vr + sc * E), rows.e4m3);
           }
@@ -821,7 +839,7 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
       if (!HELD && j0 + KT <= paged_end) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          const int64_t page = rows.checked(__builtin_amdgcn_readfirstlane(pg[i])), r0 = (j0 + i * RPP + wave * RPW) & rows.page_mask;
+          const int64_t page = rows.noted(__builtin_amdgcn_readfirstlane(pg[i]), outside), r0 = (j0 + i * RPP + wave * RPW) & rows.page_mask;
           kreg[i] = row_load(row_buffer(rows.k + page * rows.k_sb + r0 * rows.k_sn, kAllBytes), koff);
           vreg[i] = row_load(row_buffer(rows.v + page * rows.v_sb + r0 * rows.v_sn, kAllBytes), voff);
         }
@@ -857,24 +875,18 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
       }
     }
   };
-  auto store_tile = [&](int buf) {
+  auto store_tile = [&](auto kind, int buf) {
+    constexpr int KIND = decltype(kind)::value;
     char* kt = lds + buf * 2 * TB;
     if constexpr (HELD) {
-      if (tid < 2 * KT) s_scale[2 * buf + (tid >= KT ? 1 : 0)][tid & (KT - 1)] = scale_reg;
-      auto put = [&](auto kind) {
-        constexpr bool E4M3 = decltype(kind)::value;
+      if (scale_here) s_scale[2 * buf + (scale_of_v ? 1 : 0)][scale_key] = scale_reg;
+      if constexpr (KIND != kGiven) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           const int at = chunk_at<RB>(sr + i * RPP, sc);
-          *reinterpret_cast<uint4*>(kt + at) = Codes<T>::template widen<E4M3>(kreg[i].x, kreg[i].y);
-          *reinterpret_cast<uint4*>(kt + TB + at) = Codes<T>::template widen<E4M3>(vreg[i].x, vreg[i].y);
+          *reinterpret_cast<uint4*>(kt + at) = Codes<T>::template widen<KIND == kE4m3>(kreg[i].x, kreg[i].y);
+          *reinterpret_cast<uint4*>(kt + TB + at) = Codes<T>::template widen<KIND == kE4m3>(vreg[i].x, vreg[i].y);
         }
-      };
-      if (as_codes) {
-        if (rows.e4m3)
-          put(std::true_type());
-        else
-          put(std::false_type());
         return;
       }
     }
@@ -891,128 +903,143 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
   for (int i = 0; i < ND; ++i) acc[i] = f32x16{};
   float mref = -INFINITY, lsum = 0.0f;
 
-  if (nt > 0) {
-    find_pages(0);
-    load_tile(0);
-    if (nt > 1) find_pages(1);
-    store_tile(0);
-  }
-  settle(qf);
-  for (int t = 0; t < nt; ++t) {
-    __syncthreads();
-    if (t + 1 < nt) load_tile(t + 1);
-    if (t + 2 < nt) find_pages(t + 2);
-    const int k0 = tile_key(t) + kw * 32 * NSUB;
-    if ((k0 < hi_max && k0 + 32 * NSUB > lo_min) || (SETS && k0 < a_max && k0 + 32 * NSUB > a_min)) {
-      const char* kt = lds + (TWO ? (t & 1) * 2 * TB : 0) + kw * 32 * NSUB * RB;
-      const char* vt = kt + TB;
-      f32x16 s[NSUB];
-#pragma unroll
-      for (int u = 0; u < NSUB; ++u) s[u] = f32x16{};
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int u = 0; u < NSUB; ++u) s[u] = O::mfma(O::template row_frag<RB>(kt, 32 * u, c, lane), qf[c], s[u]);
-
-      const int kl = k0 + 4 * half;  // key of register 0
-      const float dist = static_cast<float>(kl - pos);
-      [[maybe_unused]] const float* ksc = s_scale[HELD && TWO ? 2 * (t & 1) : 0] + (HELD ? kw * 32 * NSUB + 4 * half : 0);
-      [[maybe_unused]] const float* vsc = s_scale[HELD && TWO ? 2 * (t & 1) + 1 : (HELD ? 1 : 0)] + (HELD ? kw * 32 * NSUB + 4 * half : 0);
-      if constexpr (HELD)
-#pragma unroll
-        for (int u = 0; u < NSUB; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float4 x = *reinterpret_cast<const float4*>(ksc + 32 * u + 8 * e);
-            s[u][4 * e] *= x.x;
-            s[u][4 * e + 1] *= x.y;
-            s[u][4 * e + 2] *= x.z;
-            s[u][4 * e + 3] *= x.w;
-          }
-      if (TREE && has_bias(RULE) && tree && k0 + 32 * NSUB > cached) {  // (drafts lie at cached + depth)
-#pragma unroll
-        for (int u = 0; u < NSUB; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int j = kl + 32 * u + 8 * (i >> 2) + (i & 3), x = j - cached;
-            const int at = x < 0 ? j : cached + s_depth[TREE ? min(x, kDrafts - 1) : 0];
-            s[u][i] = rule.z(p.rule, s[u][i], slope, static_cast<float>(at - pos));
-          }
-      } else {
-#pragma unroll
-        for (int u = 0; u < NSUB; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            s[u][i] = rule.z(p.rule, s[u][i], slope, dist + static_cast<float>(32 * u + 8 * (i >> 2) + (i & 3)));
-      }
-      const bool whole = k0 >= lo_max && k0 + 32 * NSUB <= hi_min && (SETS || (k0 >= part_lo && k0 + 32 * NSUB <= part_hi));
-      if (SETS && !whole) {
-        const int a = in_branch(lo - kl), z = in_branch(hi - kl), x = in_branch(see.a_lo - kl), y = in_branch(see.a_hi - kl);
-#pragma unroll
-        for (int u = 0; u < NSUB; ++u) {
-          const uint32_t kin = TREE ? kin_word(see.kin, k0 + 32 * u - cached) >> (4 * half) : 0u;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int jj = 8 * (i >> 2) + (i & 3), j = 32 * u + jj;
-            const bool sees = (j >= a && j < z) || (j >= x && j < y) || (TREE && (kin >> jj & 1u) != 0);
-            if (!sees) s[u][i] = Rule<T, RULE>::kHidden;
-          }
-        }
-      } else if (!whole) {
-        const int a = in_branch(max(lo, part_lo) - kl), z = in_branch(min(hi, part_hi) - kl);
-#pragma unroll
-        for (int u = 0; u < NSUB; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int j = 32 * u + 8 * (i >> 2) + (i & 3);
-            if (j < a || j >= z) s[u][i] = Rule<T, RULE>::kHidden;
-          }
-      }
-      float top = Rule<T, RULE>::kHidden;
-#pragma unroll
-      for (int u = 0; u < NSUB; ++u)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = rule.better(top, s[u][i]);
-      top = fmaf(rule.better(top, other_half(top)), rule.a, rule.b);
-      if (__ballot(top > mref + 8.0f) != 0) {
-        const float mn = fmaxf(mref, top);
-        const float alpha = mref == mn ? 1.0f : exp2_w(mref - mn);
-        mref = mn;
-        lsum *= alpha;
-#pragma unroll
-        for (int i = 0; i < ND; ++i) acc[i] *= alpha;
-      }
-      const float nref = rule.b - (mref == -INFINITY ? 0.0f : mref);
-#pragma unroll
-      for (int u = 0; u < NSUB; ++u)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[u][i] = exp2_w(fmaf(s[u][i], rule.a, nref));
-          lsum += s[u][i];
-        }
-      if constexpr (HELD)
-#pragma unroll
-        for (int u = 0; u < NSUB; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float4 x = *reinterpret_cast<const float4*>(vsc + 32 * u + 8 * e);
-            s[u][4 * e] *= x.x;
-            s[u][4 * e + 1] *= x.y;
-            s[u][4 * e + 2] *= x.z;
-            s[u][4 * e + 3] *= x.w;
-          }
-#pragma unroll
-      for (int u = 0; u < NSUB; ++u)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const Frag pf = O::pack(s[u], c);
-#pragma unroll
-          for (int i = 0; i < ND; ++i) acc[i] = O::mfma(O::template col_frag<RB>(vt, 32 * u + 16 * c, 32 * i, lane), pf, acc[i]);
-        }
+  auto walk_tiles = [&](auto kind, const int from, const int to) {
+    if (to > from) {
+      find_pages(from);
+      load_tile(kind, from);
+      if (to > from + 1) find_pages(from + 1);
+      store_tile(kind, TWO ? from & 1 : 0);
     }
-    if constexpr (!TWO) __syncthreads();
-    if (t + 1 < nt) store_tile(TWO ? (t + 1) & 1 : 0);
+    settle(qf);
+    for (int t = from; t < to; ++t) {
+      __syncthreads();
+      if (t + 1 < to) load_tile(kind, t + 1);
+      if (t + 2 < to) find_pages(t + 2);
+      const int k0 = tile_key(t) + kw * 32 * NSUB;
+      if ((k0 < hi_max && k0 + 32 * NSUB > lo_min) || (SETS && k0 < a_max && k0 + 32 * NSUB > a_min)) {
+        const char* kt = lds + (TWO ? (t & 1) * 2 * TB : 0) + kw * 32 * NSUB * RB;
+        const char* vt = kt + TB;
+        f32x16 s[NSUB];
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u) s[u] = f32x16{};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int u = 0; u < NSUB; ++u) s[u] = O::mfma(O::template row_frag<RB>(kt, 32 * u, c, lane), qf[c], s[u]);
+
+        const int kl = k0 + 4 * half;  // key of register 0
+        const float dist = static_cast<float>(kl - pos);
+        [[maybe_unused]] const float* ksc = s_scale[HELD && TWO ? 2 * (t & 1) : 0] + (HELD ? kw * 32 * NSUB + 4 * half : 0);
+        [[maybe_unused]] const float* vsc = s_scale[HELD && TWO ? 2 * (t & 1) + 1 : (HELD ? 1 : 0)] + (HELD ? kw * 32 * NSUB + 4 * half : 0);
+        if constexpr (HELD)
+#pragma unroll
+          for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float4 x = *reinterpret_cast<const float4*>(ksc + 32 * u + 8 * e);
+              s[u][4 * e] *= x.x;
+              s[u][4 * e + 1] *= x.y;
+              s[u][4 * e + 2] *= x.z;
+              s[u][4 * e + 3] *= x.w;
+            }
+        if (TREE && has_bias(RULE) && tree && k0 + 32 * NSUB > cached) {  // (drafts lie at cached + depth)
+#pragma unroll
+          for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int j = kl + 32 * u + 8 * (i >> 2) + (i & 3), x = j - cached;
+              const int at = x < 0 ? j : cached + s_depth[TREE ? min(x, kDrafts - 1) : 0];
+              s[u][i] = rule.z(p.rule, s[u][i], slope, static_cast<float>(at - pos));
+            }
+        } else {
+#pragma unroll
+          for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              s[u][i] = rule.z(p.rule, s[u][i], slope, dist + static_cast<float>(32 * u + 8 * (i >> 2) + (i & 3)));
+        }
+        const bool whole = k0 >= lo_max && k0 + 32 * NSUB <= hi_min && (SETS || (k0 >= part_lo && k0 + 32 * NSUB <= part_hi));
+        if (SETS && !whole) {
+          const int a = in_branch(lo - kl), z = in_branch(hi - kl), x = in_branch(see.a_lo - kl), y = in_branch(see.a_hi - kl);
+#pragma unroll
+          for (int u = 0; u < NSUB; ++u) {
+            const uint32_t kin = TREE ? kin_word(see.kin, k0 + 32 * u - cached) >> (4 * half) : 0u;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int jj = 8 * (i >> 2) + (i & 3), j = 32 * u + jj;
+              const bool sees = (j >= a && j < z) || (j >= x && j < y) || (TREE && (kin >> jj & 1u) != 0);
+              if (!sees) s[u][i] = Rule<T, RULE>::kHidden;
+            }
+          }
+        } else if (!whole) {
+          const int a = in_branch(max(lo, part_lo) - kl), z = in_branch(min(hi, part_hi) - kl);
+#pragma unroll
+          for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int j = 32 * u + 8 * (i >> 2) + (i & 3);
+              if (j < a || j >= z) s[u][i] = Rule<T, RULE>::kHidden;
+            }
+        }
+        float top = Rule<T, RULE>::kHidden;
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = rule.better(top, s[u][i]);
+        top = fmaf(rule.better(top, other_half(top)), rule.a, rule.b);
+        if (__ballot(top > mref + 8.0f) != 0) {
+          const float mn = fmaxf(mref, top);
+          const float alpha = mref == mn ? 1.0f : exp2_w(mref - mn);
+          mref = mn;
+          lsum *= alpha;
+#pragma unroll
+          for (int i = 0; i < ND; ++i) acc[i] *= alpha;
+        }
+        const float nref = rule.b - (mref == -INFINITY ? 0.0f : mref);
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            s[u][i] = exp2_w(fmaf(s[u][i], rule.a, nref));
+            lsum += s[u][i];
+          }
+        if constexpr (HELD)
+#pragma unroll
+          for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float4 x = *reinterpret_cast<const float4*>(vsc + 32 * u + 8 * e);
+              s[u][4 * e] *= x.x;
+              s[u][4 * e + 1] *= x.y;
+              s[u][4 * e + 2] *= x.z;
+              s[u][4 * e + 3] *= x.w;
+            }
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const Frag pf = O::pack(s[u], c);
+#pragma unroll
+            for (int i = 0; i < ND; ++i) acc[i] = O::mfma(O::template col_frag<RB>(vt, 32 * u + 16 * c, 32 * i, lane), pf, acc[i]);
+          }
+      }
+      if constexpr (!TWO) __syncthreads();
+      if (t + 1 < to) store_tile(kind, TWO ? (t + 1) & 1 : 0);
+    }
+  };
+  if constexpr (HELD) {
+    int held = nt;  // the tiles of codes alone, which come first
+    while (held > 0 && tile_key(held - 1) + KT > paged_end) --held;
+    if (rows.e4m3)
+      walk_tiles(std::integral_constant<int, kE4m3>(), 0, held);
+    else
+      walk_tiles(std::integral_constant<int, kI8>(), 0, held);
+    walk_tiles(std::integral_constant<int, kGiven>(), held, nt);
+  } else {
+    walk_tiles(std::integral_constant<int, kGiven>(), 0, nt);
   }
+
+  if constexpr (PAGED) rows.report(outside);
 
   // the row's sums, joined over the half-waves (they share the reference)
   lsum += other_half(lsum);

@@ -291,13 +291,14 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
   // kTwo: a key of the sequence that stands for key j where j is looked up, one that some row sees
   // (or a new one, whose page the table has too)
   auto seen_key = [&](int j) { return min(j >= first_a ? max(j, from) : j, k_end - 1); };
+  int outside = 0;  // whether a page of a tile was outside the pool
   float scale_reg = 1.0f;  // HELD: of K's key lane, from lane 32 on of V's key lane - 32
   auto pages_at = [&](int k0) {
     if constexpr (SETS) return k0 >= 0 ? rows.entry_of(seen_key(k0 + rr)) : 0;
     return k0 < k_end ? rows.entry_of(min(k0 + rr, k_end - 1)) : 0;
   };
   auto load_tile = [&](int k0, int entry) {
-    const int pg = rows.checked(entry);
+    const int pg = rows.noted(entry, outside);
     if constexpr (HELD) {
       const int j = seen_key(k0 + rr);
       scale_reg = rows.is_new(j) ? 1.0f : rows.scale_of(half != 0, pg, j);
@@ -481,6 +482,7 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
     }
     wave_lds_sync();
   }
+  rows.report(outside);
 
   lsum += other_half(lsum);
   float worst = finite(lsum) ? 0.0f : 1.0f;
