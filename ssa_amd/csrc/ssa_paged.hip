@@ -8,6 +8,7 @@
 //   few rows     sequences with at most 32 rows (tokens x heads of a group) per KV
 //                head, single tokens above all: few_rows
 //   many rows    chunks: dense_rows (ssa_dense_rows.h) over pages
+//   few codes    at most 16 bf16 rows over pages of 8 bits: few_codes
 //
 // all in one launch, and the parts that sequences were cut into joined in a second.  Where
 // the caller says that out holds nothing, blocks of the second (of the first, of calls
@@ -23,6 +24,9 @@
 // one of 131072, 16 / 2 heads: 28 us, 4.8 TB/s, and 9 us for the join of its 256 parts.
 // One short sequence waits for memory four times in a row (table, page, K and V, out):
 // 203 tokens, 8 / 2 heads, fp32, 12.4 us.
+//
+// ssa_paged_step_general adds windows, drafted trees and pages of 8 bits to the same launch: rows
+// that see two intervals of keys (and, of a tree, a word of drafts) walk the tiles of both.
 //
 // The kernels are in ssa_paged_rows.h; ssa_paged_one_*.hip, ssa_paged_two_*.hip and
 // ssa_paged_held_*.hip compile them.
