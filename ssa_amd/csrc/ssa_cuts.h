@@ -180,7 +180,7 @@ inline PagedPlan paged_plan(int dtype, int64_t tokens, int64_t batch, int h_q, i
   // where the batch has sequences of unlike lengths to even out, once for one.
   const int64_t blocks = batch * h_kv;
   // (few_codes runs three blocks a CU: 1536 of them take the 32 ragged sequences of int8 111 to 98 us,
-  // 2048 or 3072 the same or more, 32 of 8191 tokens 138 to 129 and 141)
+  // 2048 or more the same or worse, 32 of 8191 tokens 138 to 129 and 141)
   int64_t s = div_up(batch > 1 ? (codes ? 1536 : 1024) : 512, blocks), most = div_up(max_len, 256);
   s = s < most ? s : most;
   s = s > 1 ? s : 1;
