@@ -64,7 +64,7 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
                                     (k is not None and (k.requires_grad or v is not None and v.requires_grad)) or
                                     any([t.requires_grad for t in (slopes, out, k_scales, v_scales) if t is not None])):
         raise NotImplementedError("paged_step has no gradient: call it under torch.no_grad(), or detach its inputs")
-    _lib.refuse_tangents("paged_step", q, k, v, k_pages, v_pages, slopes)
+    _lib.refuse_tangents("paged_step", q, k, v, k_pages, v_pages, slopes, k_scales, v_scales, out)
     window = 0 if window is None and sinks == 0 else _window(window, sinks)
     if softcap is not None and not softcap > 0:
         raise ValueError(f"softcap must be positive, got {softcap}")
