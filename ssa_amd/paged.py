@@ -161,6 +161,7 @@ class PagedKVCache:
         self._gone = {}    # sequence -> which of them were
         self._len = {}     # sequence -> its keys
         self._drafts = {}  # sequence -> drafted tokens at its end, of which keep says what stays
+        self._parents = {}  # sequence -> those tokens' parents
         self._next = 0
 
     def add(self) -> int:
@@ -173,6 +174,7 @@ class PagedKVCache:
     def free(self, seq: int) -> None:
         """Closes a sequence; its pages are used again."""
         del self._len[seq], self._drafts[seq]
+        self._parents.pop(seq, None)
         gone = self._gone.pop(seq)
         self._free.extend(reversed([x for i, x in enumerate(self._pages.pop(seq)) if i not in gone]))
 
@@ -263,21 +265,25 @@ class PagedKVCache:
                 while len(self._pages[s]) > before[s]:
                     self._free.append(self._pages[s].pop())
             raise
-        for s, c in zip(seqs, counts):
+        for i, (s, c) in enumerate(zip(seqs, counts)):
             self._len[s] += c
             if parents is not None:
-                self._drafts[s] = c
+                self._drafts[s], self._parents[s] = c, list(parents[i])
         return out
 
     def keep(self, seqs: Sequence[int], kept: Sequence[Sequence[int]]) -> None:
         """Says which of the tokens that the last ``step`` of each sequence drafted stay: ``kept[i]``
         are their numbers, ascending, a path from a root of the tree on (empty: none).  The rest is
-        dropped, and pages it had filled go back."""
+        dropped, and pages it had filled go back.  Raises ValueError, with nothing changed, for
+        tokens that are no such path: each but the first follows the one before it."""
         if len(seqs) != len(kept) or len(set(seqs)) != len(seqs) or any(s not in self._len for s in seqs):
             raise ValueError("seqs and kept must pair distinct open sequences with tokens")
         for s, x in zip(seqs, kept):
             if any(not a < b for a, b in zip([-1, *x], [*x, self._drafts[s]])):
                 raise ValueError(f"kept tokens must ascend and lie among the {self._drafts[s]} drafted ones")
+            up = self._parents.get(s)
+            if up is not None and any(up[b] != a for a, b in zip([-1, *x], x)):
+                raise ValueError(f"kept tokens must be a path from a root of the tree on, not {list(x)} of parents {up}")
         if not seqs:
             return
         base = {s: self._len[s] - self._drafts[s] for s in seqs}
@@ -288,6 +294,7 @@ class PagedKVCache:
             paged_keep(self.k_pages, self.v_pages, table, cached, rows.view(len(seqs), most), **self._scales())
         for s, x in zip(seqs, kept):
             self._len[s], self._drafts[s] = base[s] + len(x), 0
+            self._parents.pop(s, None)
             while len(self._pages[s]) > -(-self._len[s] // self.page_size):
                 self._free.append(self._pages[s].pop())
 

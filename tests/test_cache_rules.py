@@ -20,3 +20,44 @@ def test_step_refuses_every_tangent_that_it_would_drop():
                 ssa_amd.paged_step(**{**floats, **rest, name: fwAD.make_dual(t, torch.ones_like(t))})
         with pytest.raises(RuntimeError, match="GPU"):  # (no tangent: the device is what is wrong)
             ssa_amd.paged_step(**floats, **rest)
+
+
+def _drafted(monkeypatch, parents, dtype=torch.bfloat16):
+    """A cache on the host after a step that drafted trees of these parents (no kernel runs)."""
+    moved = []
+    monkeypatch.setattr(ssa_amd.paged, "paged_step", lambda q, *a, **kw: torch.zeros_like(q))
+    monkeypatch.setattr(ssa_amd.paged, "paged_keep", lambda *a, **kw: moved.append(a))
+    c = ssa_amd.PagedKVCache(20, 16, 2, 64, dtype=dtype, device="cpu")
+    seqs = [c.add() for _ in parents]
+    for s in seqs:
+        x = torch.zeros(5, 2, 64, dtype=dtype)
+        c.step(torch.zeros(5, 4, 64, dtype=dtype), x, x, [s], [5])
+    T = sum(len(p) for p in parents)
+    x = torch.zeros(T, 2, 64, dtype=dtype)
+    c.step(torch.zeros(T, 4, 64, dtype=dtype), x, x, seqs, [len(p) for p in parents], parents=parents)
+    return c, seqs, moved
+
+
+def test_keep_takes_a_path_of_the_tree_alone(monkeypatch):
+    tree = [-1, 0, 0, 1, -1, 4, 3]
+    for bad in ([0, 1, 2], [1], [0, 3], [0, 4], [4, 6], [0, 1, 3, 5], [2, 6]):
+        c, (a, b), moved = _drafted(monkeypatch, [tree, [-1, 0]])
+        books = (c.length(a), c.length(b), c.free_pages)
+        with pytest.raises(ValueError, match="path"):
+            c.keep([b, a], [[0], bad])
+        assert not moved and books == (c.length(a), c.length(b), c.free_pages)
+        c.keep([a, b], [[], [0, 1]])  # (and may still say what stays)
+        assert (c.length(a), c.length(b)) == (5, 7)
+    for good in ([], [0], [4], [0, 2], [4, 5], [0, 1, 3, 6]):
+        c, (a, b), moved = _drafted(monkeypatch, [tree, [-1, 0]])
+        c.keep([a, b], [good, [0, 1]])
+        assert c.length(a) == 5 + len(good) and len(moved) == (0 if good in ([], [0]) else 1)
+        # the next step drafts another tree, of which another path stays
+        x = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+        c.step(torch.zeros(3, 4, 64, dtype=torch.bfloat16), x, x, [a], [3], parents=[[-1, -1, 1]])
+        with pytest.raises(ValueError, match="path"):
+            c.keep([a], [[0, 1]])
+        c.keep([a], [[1, 2]])
+        assert c.length(a) == 7 + len(good)
+        c.free(a)
+        assert a not in c._parents
