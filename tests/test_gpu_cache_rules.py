@@ -57,3 +57,39 @@ def test_codes_are_read_in_one_rounding(dev, hold):
         assert float(exact[0, 0, 0, 0]) == 17 * float(torch.tensor(0.022805606946349144))
         assert float(nearest_bf16(exact)[0, 0, 0, 0]) == 0.388671875
     assert not torch.equal(torch.nan_to_num(nearest_bf16(exact)), torch.nan_to_num(exact.float().to(BF16))), "no product tells them apart"
+
+
+@pytest.mark.parametrize("dtype,m,g", [(BF16, 1, 4), (BF16, 9, 2), (F32, 1, 4), (BF16, 30, 1), (BF16, 40, 4), (F32, 40, 2)])
+@pytest.mark.parametrize("cached", [13, 4001])
+def test_codes_of_rows_without_a_key_change_no_bit(dev, dtype, m, g, cached):
+    """Pages of e4m3 whose rows behind the last key hold codes for NaN give the bits that zeros there give: a
+    row that one of them reached would be computed again key by key, in another order of its sums."""
+    from ssa_amd import paged_step
+    from tests.cache_oracle import attend_set, held, sees, values
+    from tests.dense_oracle import check
+    from tests.test_gpu_bounded_cache import batch
+
+    seqs, h_kv, page = [(m, cached)] * 4, 2, 64
+    s, keys, _ = batch(82, dtype, seqs, h_kv * g, h_kv, 128, page, E4M3)
+    see, qpos, kpos = sees(m, cached)
+    for given in (True, False):  # (else the pages hold the call's own rows, from the call before)
+        outs = []
+        for fill in (0, 0x7F):
+            x = {n: t.to(dev) for n, t in s.items()}
+            if not given:
+                paged_step(**x)
+            for n in ("k_pages", "v_pages"):
+                flat = x[n].view(I8)
+                for b in range(4):
+                    at = cached if given else cached + m
+                    if at % page:
+                        flat[int(s["table"][b, at // page]), at % page:] = fill
+            if not given:
+                x["k"] = x["v"] = None
+            outs.append(paged_step(**x, max_new=m, max_len=cached + m, check=True))
+        assert torch.equal(*outs), given
+        for b in range(4):
+            full = keys[b]
+            if not given:
+                full = [torch.cat([t[:cached], values(*held(t[cached:].to(dtype), E4M3))]) for t in full]
+            check(outs[0][b * m:(b + 1) * m], *attend_set(s["q"][b * m:(b + 1) * m], *full, see, qpos, kpos)["out"], f"{given} {b}")
