@@ -1,11 +1,18 @@
-// How the dense attention calls are cut into blocks, and the workspaces that follow: host
-// rules on sizes and types alone, in plain C++, so that a host test can ask for a call's cut.
+// How the dense attention calls are cut into blocks, and the workspaces that follow: rules on
+// sizes and types alone, in plain C++, so that a host test can ask for a call's cut.  Those that
+// the kernels follow too (SSA_BOTH) stand here for both.
 #pragma once
 
 #include <stddef.h>
 #include <stdint.h>
 
 #include "ssa_hip.h"
+
+#ifdef __HIPCC__
+#define SSA_BOTH __host__ __device__ inline __attribute__((always_inline))
+#else
+#define SSA_BOTH inline
+#endif
 
 namespace ssa {
 
@@ -145,6 +152,69 @@ inline TwoCut two_cut(const BwdCut& l, int dtype, int64_t batch, int64_t n, int 
   t.part_floats = static_cast<size_t>(parts) * h_kv * keys * (wide ? 128 : 64);
   t.bytes = t.part + 2 * t.part_floats * sizeof(float);
   return t;
+}
+
+// What plan_list_kernel makes of a call whose blocks of keys are seen by `h` tiles of rows each,
+// `total` in all.  A block with more than `share` of them is big, and cut into parts of plan_part
+// tiles; of the others, whole ones, plan_left of the last round are cut into parts of plan_left_part.
+SSA_BOTH int64_t plan_share(int64_t total, int slots, int least) {
+  const int64_t share = (total + slots - 1) / slots;
+  return share > least ? share : least;
+}
+// big: tiles of the big blocks
+SSA_BOTH int plan_part(int64_t big, int extra, int least, int64_t share) {
+  int64_t p = (big + extra - 1) / extra;
+  p = p > least ? p : least;
+  return static_cast<int>(p > share / 10 ? p : share / 10);
+}
+// How many of the `one` blocks that are not big, the shortest, are cut so that they fill a last round
+// (0: none).  Blocks are sorted up to kSorted of them.
+constexpr int kSorted = 2048;
+SSA_BOTH int plan_left(int blocks, int one, int slots) {
+  const int left = one % slots;
+  return blocks <= kSorted && one > slots && one < 4 * slots && 10 * left < 7 * slots ? left : 0;
+}
+// sum: tiles of those
+SSA_BOTH int plan_left_part(int64_t sum, int slots, int least) {
+  const int64_t p = (sum + slots - 1) / slots;
+  return static_cast<int>(p > least ? p : least);
+}
+// Parts of a block of h tiles that is cut (one at least: nobody sees it, and its zeros go through a part).
+SSA_BOTH int plan_parts(int h, int part) { return h > part ? (h + part - 1) / part : 1; }
+
+// The tiles of kt keys that the rows of a block see, [a_lo, a_hi) and [b_lo, b_hi) between them:
+// [x0, x0 + n1), then [y0, y0 + n - n1), ascending.
+struct Tiles {
+  int x0, n1, y0, n;
+  SSA_BOTH int at(int t) const { return t < n1 ? x0 + t : y0 + t - n1; }
+};
+SSA_BOTH Tiles tiles_of(int a_lo, int a_hi, int b_lo, int b_hi, int kt) {
+  int x0 = a_lo / kt, x1 = a_hi > a_lo ? (a_hi - 1) / kt + 1 : x0;
+  int y0 = b_lo / kt, y1 = b_hi > b_lo ? (b_hi - 1) / kt + 1 : y0;
+  if (x1 == x0) {  // (one range)
+    x0 = y0;
+    x1 = y1;
+    y1 = y0;
+  }
+  if (y1 > y0 && y0 < x0) {
+    const int s0 = x0, s1 = x1;
+    x0 = y0;
+    x1 = y1;
+    y0 = s0;
+    y1 = s1;
+  }
+  if (y1 > y0 && y0 <= x1) {
+    x1 = x1 > y1 ? x1 : y1;
+    y1 = y0;
+  }
+  return Tiles{x0, x1 - x0, y0, x1 - x0 + y1 - y0};
+}
+// Those of a sequence's new tokens, at positions cached to len - 1, behind a window (0: none) with
+// first keys.
+SSA_BOTH Tiles seen_tiles(int cached, int len, int window, int sinks, int kt) {
+  const int lo = window > 0 && cached + 1 - window > 0 ? cached + 1 - window : 0;
+  const int far = window > 0 && len - window > 0 ? len - window : 0;
+  return tiles_of(0, sinks < far ? sinks : far, lo, len, kt);
 }
 
 // The most keys of a sequence of max_len that its call reads: with a window, the first keys

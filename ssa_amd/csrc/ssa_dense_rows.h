@@ -45,6 +45,7 @@
 
 #include <type_traits>
 
+#include "ssa_cuts.h"
 #include "ssa_tile.h"
 
 namespace ssa {
@@ -135,33 +136,6 @@ struct Sees {
 __device__ __forceinline__ uint32_t kin_word(uint64_t kin, int off) {
   if (off >= kDrafts || off <= -32) return 0u;
   return off >= 0 ? static_cast<uint32_t>(kin >> off) : static_cast<uint32_t>(kin) << -off;
-}
-
-// The tiles that a block's rows see: [x0, x0 + n1), then [y0, y0 + n - n1), ascending.
-struct Tiles {
-  int x0, n1, y0, n;
-  __device__ __forceinline__ int at(int t) const { return t < n1 ? x0 + t : y0 + t - n1; }
-};
-__device__ __forceinline__ Tiles tiles_of(int a_lo, int a_hi, int b_lo, int b_hi, int kt) {
-  int x0 = a_lo / kt, x1 = a_hi > a_lo ? (a_hi - 1) / kt + 1 : x0;
-  int y0 = b_lo / kt, y1 = b_hi > b_lo ? (b_hi - 1) / kt + 1 : y0;
-  if (x1 == x0) {  // (one range)
-    x0 = y0;
-    x1 = y1;
-    y1 = y0;
-  }
-  if (y1 > y0 && y0 < x0) {
-    const int s0 = x0, s1 = x1;
-    x0 = y0;
-    x1 = y1;
-    y0 = s0;
-    y1 = s1;
-  }
-  if (y1 > y0 && y0 <= x1) {
-    x1 = max(x1, y1);
-    y1 = y0;
-  }
-  return Tiles{x0, x1 - x0, y0, x1 - x0 + y1 - y0};
 }
 
 // Lane i's new token of a sequence with m <= 64 of them: which new tokens it sees (itself and its

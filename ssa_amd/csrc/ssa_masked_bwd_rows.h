@@ -915,7 +915,8 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(BwdParams p) {
 // parts come after whole blocks (16001 rows that see 1000 keys back and 4 first ones, 16 / 4 heads,
 // d = 128: dK and dV 640 us with parts first and as long as whole blocks, 525 so).
 // At most key_blocks + most entries, most parts, 2 slots cut blocks.
-constexpr int kPlan = 1024, kSorted = 2 * kPlan;
+constexpr int kPlan = 1024;  // (the rules are in ssa_cuts.h)
+static_assert(kSorted == 2 * kPlan, "a thread ranks two blocks");
 struct PlanSums {
   int64_t wave[kPlan / 64];
 };
@@ -958,7 +959,7 @@ __device__ __forceinline__ int plan_scan(int x, int (&s)[kPlan / 64], int& all) 
   }
   if (sorted && tid < 16) s_h[N + tid] = 0x7FFFFFFF;
   const int64_t total = plan_sum(mine, s_sums);
-  const int64_t share = max((total + slots - 1) / slots, static_cast<int64_t>(least));
+  const int64_t share = plan_share(total, slots, least);
   int64_t big = 0, n_big = 0;
   for (int x = tid; x < N; x += kPlan) {
     const int h = p.counts[x];
@@ -970,11 +971,10 @@ __device__ __forceinline__ int plan_scan(int x, int (&s)[kPlan / 64], int& all) 
   big = plan_sum(big << 24 | n_big, s_sums);  // (few are big: fewer than 2^24 of them, and tiles below 2^39)
   n_big = big & 0xFFFFFF;
   big >>= 24;
-  const int P = static_cast<int>(max(max(static_cast<int64_t>(least), (big + p.extra - 1) / p.extra), share / 10));
+  const int P = plan_part(big, p.extra, least, share);
   // whole blocks of the last round
-  const int n_one = N - static_cast<int>(n_big), left = n_one % slots;
-  const bool cut_left = sorted && n_one > slots && n_one < 4 * slots && left > 0 && 10 * left < 7 * slots;
-  const int n_whole = n_one - (cut_left ? left : 0);
+  const int n_one = N - static_cast<int>(n_big), left = plan_left(N, n_one, slots), n_whole = n_one - left;
+  const bool cut_left = left > 0;
   int rank[kSorted / kPlan];
 #pragma unroll
   for (int c = 0; c < kSorted / kPlan; ++c) {
@@ -1000,7 +1000,7 @@ __device__ __forceinline__ int plan_scan(int x, int (&s)[kPlan / 64], int& all) 
       if (x < N && s_h[x] <= share && rank[c] >= n_whole) sum += s_h[x];
     }
     sum = plan_sum(sum, s_sums);
-    P2 = static_cast<int>(max(static_cast<int64_t>(least), (sum + slots - 1) / slots));
+    P2 = plan_left_part(sum, slots, least);
   }
   int at_part = 0, at_cut = 0, at_one = 0;
   for (int x0 = 0, c = 0; x0 < N; x0 += kPlan, ++c) {
@@ -1008,8 +1008,7 @@ __device__ __forceinline__ int plan_scan(int x, int (&s)[kPlan / 64], int& all) 
     const bool is_big = x < N && h > share;
     const int rk = sorted ? (c == 0 ? rank[0] : rank[1]) : 0;
     const bool is_left = cut_left && x < N && !is_big && rk >= n_whole;
-    int parts = is_big ? (h + P - 1) / P : (is_left ? (h + P2 - 1) / P2 : 0);
-    if (is_left && parts < 1) parts = 1;  // (nobody sees it: its zeros go through a part)
+    const int parts = is_big || is_left ? plan_parts(h, is_big ? P : P2) : 0;
     const int whole = x < N && !is_big && !is_left ? 1 : 0;
     int all_parts, all_cut, all_one;
     const int b_part = plan_scan(parts, s_scan, all_parts), b_cut = plan_scan(parts > 0 ? 1 : 0, s_scan, all_cut);

@@ -190,9 +190,7 @@ __device__ __forceinline__ void no_rows(const DenseParams& p, const int block) {
 
 // kTwo: the 32-key tiles that a sequence's new tokens see.
 __device__ __forceinline__ Tiles seq_tiles(const DenseParams& p, const Seq& s) {
-  const int cached = s.len - s.m;
-  const int lo = p.window > 0 ? max(cached + 1 - p.window, 0) : 0, far = p.window > 0 ? max(s.len - p.window, 0) : 0;
-  return tiles_of(0, min(p.sinks, far), lo, s.len, 32);
+  return seen_tiles(s.len - s.m, s.len, p.window, p.sinks, 32);
 }
 
 template <typename T, int D, int RULE, int VIEW = kOne, typename S = T>
