@@ -558,8 +558,20 @@ __device__ __forceinline__ int fold_tile(int t, int tiles, int heads) {
 }
 
 // What a tile over pages of 8 bits holds: codes, or some of the call's own rows.  Each kind has a loop
-// of its own in dense_rows.
-enum { kGiven, kI8, kE4m3 };
+// of its own in dense_rows; kAny: one loop for all, which asks of each tile.
+enum { kGiven, kI8, kE4m3, kAny };
+
+// Whether bf16 rows of 8-bit pages walk them in one loop: three of them with a rule of scores that takes
+// many registers spill up to 183 of them.  2048 tokens over 30720, 32 / 8 heads, three loops and one:
+//   d = 128, distance bias   2368 and 2358 us of int8, 2702 and 2266 of e4m3
+//            far caps        2950 and 2631            3185 and 2582
+//   d = 64, far caps         2220 and 2167            2156 and 2115
+// (512 over 8192, d = 128, bias: 253 and 265, 299 and 258; d = 64, where nothing spills: 187 and 209, 183 and
+// 206).  The other rules gain by three: plain scores, d = 128, 1694 to 1556 and 1546 to 1517.
+template <typename T, int D, int RULE>
+constexpr bool one_loop() {
+  return sizeof(T) == 2 && (RULE == kFar || (RULE == kBias && D == 128));
+}
 
 // FRESH: tiles of a paged call's own rows are read as contiguous ones are.
 template <typename T, int D, bool PAGED, int RULE, int KW, bool FRESH = false, int VIEW = kOne, typename S = T>
@@ -762,6 +774,7 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
   int scale_pg = 0;
   float scale_reg = 1.0f;
   int outside = 0;  // whether a page of a tile was outside the pool
+  [[maybe_unused]] bool as_codes = false;  // kAny: whether the loaded tile is of codes alone
   const int paged_end = PAGED ? min(rows.new_from, static_cast<int>(n_keys)) : 0;
   constexpr int RPW = 64 / NCH;  // rows of a wave's load
   auto find_pages = [&](int t) {
@@ -779,7 +792,8 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
       const int j = min(seen_key(j0 + scale_key), last);
       scale_reg = 1.0f;
       if (scale_here && !rows.is_new(j)) scale_reg = rows.scale_of(scale_of_v, rows.noted(scale_pg, outside), j);
-      if constexpr (KIND != kGiven) {
+      if (KIND == kAny) as_codes = j0 + KT <= paged_end;
+      if (KIND == kAny ? as_codes : KIND != kGiven) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           const int64_t page = rows.noted(__builtin_amdgcn_readfirstlane(pg[i]), outside), r0 = (j0 + i * RPP + wave * RPW) & rows.page_mask;
@@ -854,13 +868,20 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
     char* kt = lds + buf * 2 * TB;
     if constexpr (HELD) {
       if (scale_here) s_scale[2 * buf + (scale_of_v ? 1 : 0)][scale_key] = scale_reg;
-      if constexpr (KIND != kGiven) {
+      auto widened = [&](auto e4m3) {
+        constexpr bool E4M3 = decltype(e4m3)::value;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           const int at = chunk_at<RB>(sr + i * RPP, sc);
-          *reinterpret_cast<uint4*>(kt + at) = Codes<T>::template widen<KIND == kE4m3>(kreg[i].x, kreg[i].y);
-          *reinterpret_cast<uint4*>(kt + TB + at) = Codes<T>::template widen<KIND == kE4m3>(vreg[i].x, vreg[i].y);
+          *reinterpret_cast<uint4*>(kt + at) = Codes<T>::template widen<E4M3>(kreg[i].x, kreg[i].y);
+          *reinterpret_cast<uint4*>(kt + TB + at) = Codes<T>::template widen<E4M3>(vreg[i].x, vreg[i].y);
         }
+      };
+      if (KIND == kAny ? as_codes : KIND != kGiven) {
+        if (KIND == kE4m3 || (KIND == kAny && rows.e4m3))
+          widened(std::true_type());
+        else
+          widened(std::false_type());
         return;
       }
     }
@@ -1001,7 +1022,9 @@ __device__ __forceinline__ void dense_rows(const DenseParams& p, const int w, ch
       if (t + 1 < to) store_tile(kind, TWO ? (t + 1) & 1 : 0);
     }
   };
-  if constexpr (HELD) {
+  if constexpr (HELD && one_loop<T, D, RULE>()) {
+    walk_tiles(std::integral_constant<int, kAny>(), 0, nt);
+  } else if constexpr (HELD) {
     int held = nt;  // the tiles of codes alone, which come first
     while (held > 0 && tile_key(held - 1) + KT > paged_end) --held;
     if (rows.e4m3)

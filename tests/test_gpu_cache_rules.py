@@ -93,3 +93,16 @@ def test_codes_of_rows_without_a_key_change_no_bit(dev, dtype, m, g, cached):
             if not given:
                 full = [torch.cat([t[:cached], values(*held(t[cached:].to(dtype), E4M3))]) for t in full]
             check(outs[0][b * m:(b + 1) * m], *attend_set(s["q"][b * m:(b + 1) * m], *full, see, qpos, kpos)["out"], f"{given} {b}")
+
+
+@pytest.mark.parametrize("hold", [I8, E4M3])
+@pytest.mark.parametrize("d", [128, 64, 72])
+@pytest.mark.parametrize("cap,bias", [(0.0, True), (3000.0, False), (3000.0, True), (5.0, False)])
+def test_chunks_of_every_rule(dev, hold, d, cap, bias):
+    """Chunks whose tiles are codes alone, some of the call's own rows or both, with one, two and four waves that
+    share rows (528 blocks of 128 rows; 65 sequences; one)."""
+    from tests.test_gpu_bounded_cache import test_step
+
+    for seqs, h_q, h_kv, window in (([(128, 3 * i) for i in range(66)], 8, 2, 0), ([(40, 200 + i) for i in range(64)] + [(5, 60)], 16, 4, 0),
+                                    ([(301, 700), (60, 33)], 8, 2, 0), ([(301, 700), (60, 0)], 8, 2, 97)):
+        test_step(dev, (BF16, hold, seqs, False, h_q, h_kv, d, 16, window, 5 if window else 0, cap, bias))
