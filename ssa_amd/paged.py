@@ -136,7 +136,8 @@ class PagedKVCache:
 
     ``dtype`` int8 or float8_e4m3fn holds the rows in 8 bits with a scale each (135 M tokens).
     With ``window`` (and ``sinks``) every step attends as ``paged_step`` does with them, and a
-    sequence's pages that no later token sees go back to the pool as it grows.  ``step`` with
+    sequence's pages that no later token sees go back to the pool as it grows (its table keeps their
+    entries, 4 bytes a page that are copied with a step).  ``step`` with
     ``parents`` verifies drafted trees, and ``keep`` then says what stays of them."""
 
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
@@ -191,7 +192,10 @@ class PagedKVCache:
             return []
         P = self.page_size
         first, last = -(-self.sinks // P), (self._len[seq] + 1 - self.window) // P  # (whole pages before the window)
-        return [i for i in range(first, min(last, len(self._pages[seq]))) if i not in self._gone[seq]]
+        at = end = min(last, len(self._pages[seq]))
+        while at > first and at - 1 not in self._gone[seq]:  # (those given back are the ones from `first` on)
+            at -= 1
+        return list(range(at, end))
 
     def _tables(self, seqs: Sequence[int], *rows: Sequence[int]):
         """The sequences' table [B, width] and the given rows of numbers, on the device by one copy."""
@@ -204,7 +208,11 @@ class PagedKVCache:
             at += len(r)
         table = host[at:].view(B, width)
         for i, s in enumerate(seqs):
-            table[i, :len(self._pages[s])] = torch.tensor(self._pages[s], dtype=torch.int32)
+            pages, gone = self._pages[s], len(self._gone[s])
+            first = -(-self.sinks // self.page_size) if gone else len(pages)
+            table[i, :first] = torch.tensor(pages[:first], dtype=torch.int32)
+            if gone:  # (entries of pages that were given back stay 0: only live ones are walked)
+                table[i, first + gone:len(pages)] = torch.tensor(pages[first + gone:], dtype=torch.int32)
         dev = host.to(self.k_pages.device)
         return dev[at:].view(B, width), *dev[:at].split(sizes)
 

@@ -61,3 +61,43 @@ def test_keep_takes_a_path_of_the_tree_alone(monkeypatch):
         assert c.length(a) == 7 + len(good)
         c.free(a)
         assert a not in c._parents
+
+
+class _Counted(set):
+    asked = 0
+
+    def __contains__(self, x):
+        type(self).asked += 1
+        return super().__contains__(x)
+
+
+@pytest.mark.parametrize("window,sinks", [(40, 17), (1, 0), (100, 16), (33, 1)])
+def test_a_step_behind_a_window_walks_live_pages_alone(monkeypatch, window, sinks):
+    """The host's work of a step does not grow with the pages that its sequence has left behind, and the table
+    that it makes has every page that some token sees."""
+    tables = []
+    monkeypatch.setattr(ssa_amd.paged, "paged_step", lambda q, k, v, kp, vp, table, *a, **kw: (tables.append(table.clone()), torch.zeros_like(q))[1])
+    c = ssa_amd.PagedKVCache(40, 16, 2, 64, device="cpu", window=window, sinks=sinks)
+    s, other = c.add(), c.add()
+    c._gone[s] = _Counted()
+    q, k = torch.zeros(17, 4, 64), torch.zeros(17, 2, 64)
+    length, given = 0, set()
+    for step in range(400):
+        m = (1, 17, 5)[step % 3]
+        _Counted.asked = 0
+        c.step(q[:m], k[:m], k[:m], [other, s], [0, m])
+        assert _Counted.asked <= 4, "pages behind the window are asked for again"
+        pages, table = c._pages[s], tables.pop()
+        live = {j // 16 for j in range(length, length + m)}  # (new keys are written)
+        for p in range(length, length + m):
+            live |= {j // 16 for j in range(max(0, p + 1 - window), p + 1)} | {j // 16 for j in range(min(sinks, p + 1))}
+        given |= {i for i in range(len(pages)) if i in set(c._gone[s])}
+        assert not live & given
+        assert [int(x) for x in table[1][sorted(live)]] == [pages[i] for i in sorted(live)]
+        assert len({pages[i] for i in live}) == len(live), "a page twice"
+        length += m
+        assert c.length(s) == length and len(pages) - len(c._gone[s]) + c.free_pages == 40
+        assert len(pages) - len(c._gone[s]) <= (window + sinks + 17) // 16 + 4
+    assert len(c._pages[s]) > 150
+    c.free(s)
+    assert c.free_pages == 40
