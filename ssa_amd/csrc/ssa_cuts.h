@@ -225,12 +225,19 @@ inline int64_t seen_len(int64_t max_len, int64_t max_new, int64_t window, int64_
   return some < max_len ? some : max_len;
 }
 
-// Whether a call over pages of 8 bits is one for few_codes: bf16 queries, at most 16 rows a sequence
-// (32 sequences of up to 8191 tokens, 32 / 8 heads: 101 us against few_rows' 129), and rows of
-// whole 16-byte pieces where a lane loads 16.
+// Whether a call over pages of 8 bits is one for few_codes: bf16 queries, rows of whole 16-byte pieces
+// where a lane loads 16, at most 16 rows a sequence, and of those at most two new tokens, which it adds one
+// by one.  us of few_rows and few_codes, int8, d = 128, groups of 4 or 1 heads:
+//   new tokens                 1              2             4             8
+//   32 ragged, up to 8191      102, 69
+//   32 sequences of 4000       51.4, 45.2     52.5, 46.0    54.3, 55.4    55.3, 57.3
+//   32 of 200                  12.8, 12.2     13.0, 12.3    13.8, 15.4    13.1, 20.6
+//   one of 8191                17.8, 18.6     17.9, 16.9    19.0, 19.8    17.8, 24.6
+// (32 and 64 equal ones of 8191 129 and 130, 231 and 240.)  A call with a longer sequence takes few_rows for
+// its single tokens too: 32 ragged ones beside a chunk of 40 over 4096 137 us, by themselves 69 and 35.
 inline bool codes_call(int dtype, int page_dtype, int64_t max_new, int64_t g, int d) {
   const bool held = page_dtype == SSA_DTYPE_I8 || page_dtype == SSA_DTYPE_E4M3;
-  return held && dtype == SSA_DTYPE_BF16 && max_new * g <= 16 && (d <= 64 || d % 16 == 0);
+  return held && dtype == SSA_DTYPE_BF16 && max_new <= 2 && max_new * g <= 16 && (d <= 64 || d % 16 == 0);
 }
 
 // Parts, tiles and workspace of a call.

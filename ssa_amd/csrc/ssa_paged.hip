@@ -8,7 +8,7 @@
 //   few rows     sequences with at most 32 rows (tokens x heads of a group) per KV
 //                head, single tokens above all: few_rows
 //   many rows    chunks: dense_rows (ssa_dense_rows.h) over pages
-//   few codes    at most 16 bf16 rows over pages of 8 bits: few_codes
+//   few codes    at most 16 bf16 rows of one or two new tokens over pages of 8 bits: few_codes
 //
 // all in one launch, and the parts that sequences were cut into joined in a second.  Where
 // the caller says that out holds nothing, blocks of the second (of the first, of calls

@@ -582,7 +582,7 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
   }
 }
 
-// few_rows for at most 16 rows over pages of 8 bits, bf16 queries.  Widening the codes, 1.5
+// few_rows for at most 16 rows of one or two new tokens over pages of 8 bits, bf16 queries.  Widening the codes, 1.5
 // instructions a code, is most of the work beside memory's, so that the rest is kept small and
 // more waves share a SIMD (two of few_rows do, whose tiles of bf16 fill the LDS): the LDS
 // holds codes, widened as they are read, and 16x16x32 products, whose 16 columns spend half the
@@ -591,8 +591,8 @@ __device__ __forceinline__ void few_rows(const DenseParams& p, const int block, 
 // (ds_read_b64_tr_b8).  The call's own rows,
 // which have no codes yet, are added one by one at the end, by one wave of the last part, wherever
 // they lie.
-// 64 sequences of 8191 cached tokens, 32 / 8 heads, int8: 233 us, 4.8 TB/s of codes and scales (few_rows
-// 279); 32 ragged ones 98 us, 3.5 TB/s: their blocks end at unlike times.
+// 64 sequences of 8191 cached tokens, 32 / 8 heads, int8: 233 to 240 us, 4.8 to 4.6 TB/s of codes and scales;
+// ragged ones end at unlike times.  ssa_cuts.h's codes_call has both kernels' times.
 constexpr int kCols = 16;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 

@@ -182,3 +182,27 @@ def test_the_list_of_the_backward_holds_every_block_once(tmp_path):
 def test_windowed_rows_walk_the_tiles_that_they_see(tmp_path):
     """Those and no others, in order, and the parts of a call hold them all."""
     assert build_and_run(TILES, tmp_path) == "ok\n"
+
+
+CODES = r"""
+#include <stdio.h>
+#include "ssa_cuts.h"
+using namespace ssa;
+int main() {
+  for (int dtype = 0; dtype < 2; ++dtype)
+    for (int page = 0; page < 4; ++page)
+      for (int64_t m = 1; m <= 64; ++m)
+        for (int64_t g = 1; g <= 32; ++g)
+          for (int d = 8; d <= 128; d += 8) {
+            const bool want = dtype == SSA_DTYPE_BF16 && page >= 2 && m <= 2 && m * g <= 16 && (d <= 64 || d % 16 == 0);
+            if (codes_call(dtype, page, m, g, d) != want) { printf("%d %d %d %d %d\n", dtype, page, int(m), int(g), d); return 1; }
+          }
+  printf("ok\n");
+  return 0;
+}
+"""
+
+
+def test_few_codes_takes_one_or_two_tokens(tmp_path):
+    """(Sixteen drafts of one head took 13 us by few_rows and 32 by few_codes.)"""
+    assert build_and_run(CODES, tmp_path) == "ok\n"

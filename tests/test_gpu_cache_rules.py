@@ -106,3 +106,67 @@ def test_chunks_of_every_rule(dev, hold, d, cap, bias):
     for seqs, h_q, h_kv, window in (([(128, 3 * i) for i in range(66)], 8, 2, 0), ([(40, 200 + i) for i in range(64)] + [(5, 60)], 16, 4, 0),
                                     ([(301, 700), (60, 33)], 8, 2, 0), ([(301, 700), (60, 0)], 8, 2, 97)):
         test_step(dev, (BF16, hold, seqs, False, h_q, h_kv, d, 16, window, 5 if window else 0, cap, bias))
+
+
+@pytest.mark.parametrize("hold", [I8, E4M3])
+@pytest.mark.parametrize("m,trees", [(1, False), (2, False), (2, True)])
+def test_one_and_two_tokens_around_borders_between_parts(dev, hold, m, trees):
+    """The own rows of calls that few_codes takes, wherever the last part begins, and with codes for NaN in rows
+    of the window's first page that nobody sees; and the same calls with their rows in the pages already."""
+    from ssa_amd import paged_step
+    from tests.cache_oracle import attend_set, held, sees, values
+    from tests.dense_oracle import check
+    from tests.test_gpu_bounded_cache import batch
+
+    for window, g, d in ((0, 4, 128), (300, 8, 64), (520, 1, 128)):
+        for cached in [*range(248, 264), *range(504, 520, 3), *range(1016, 1032, 5)]:
+            s, keys, parents = batch(83, BF16, [(m, cached), (m, 3)], 2 * g, 2, d, 8, hold, window, 0, trees=trees)
+            if window:
+                lo = max(0, cached + 1 - window)
+                for j in range(lo // 8 * 8, lo):
+                    s["v_scales"][s["table"][0, j // 8], j % 8] = math.nan
+            slopes = torch.tensor([2.0 ** (-4.0 * (i + 1) / (2 * g)) for i in range(2 * g)])
+            kw = dict(window=window or None, slopes=slopes.to(dev), max_new=m, check=True)
+            x = {n: t.to(dev) for n, t in s.items()}
+            out = paged_step(**x, **kw)
+            x["k"] = x["v"] = None
+            again = paged_step(**x, **kw)
+            for b, c in enumerate((cached, 3)):
+                see, qpos, kpos = sees(m, c, parents[b], window, 0)
+                rows = slice(b * m, (b + 1) * m)
+                check(out[rows], *attend_set(s["q"][rows], *keys[b], see, qpos, kpos, 0.0, slopes)["out"], f"{window} {c}")
+                full = [torch.cat([t[:c], values(*held(t[c:].to(BF16), hold))]) for t in keys[b]]
+                check(again[rows], *attend_set(s["q"][rows], *full, see, qpos, kpos, 0.0, slopes)["out"], f"{window} {c} held")
+
+
+@pytest.mark.parametrize("hold", [I8, E4M3])
+@pytest.mark.parametrize("seqs,trees,h_q,h_kv,d,page,window,sinks,cap,bias", [
+    ([(1, 31), (1, 32), (1, 33), (1, 500), (0, 40), (1, 127), (1, 0)], False, 8, 2, 128, 16, 0, 0, 0.0, False),
+    ([(2, 1000), (1, 77), (2, 1), (2, 63)], False, 32, 4, 128, 64, 0, 0, 4.0, True),
+    ([(1, 3000), (1, 100), (1, 2047)], False, 16, 1, 128, 128, 0, 0, 0.0, False),
+    ([(2, 90), (1, 0), (2, 700)], False, 8, 2, 64, 8, 0, 0, 2000.0, True),
+    ([(1, 500), (1, 70)], False, 2, 1, 8, 8, 0, 0, 0.0, True),
+    ([(2, 100), (2, 1), (1, 33)], True, 4, 2, 24, 16, 0, 0, 0.0, True),
+    ([(1, 600), (1, 0)], False, 16, 1, 112, 32, 0, 0, 3.0, False),
+    ([(2, 300), (2, 1030), (2, 0)], True, 6, 2, 80, 16, 0, 0, 0.0, True),
+    ([(2, 60), (2, 3), (1, 520)], True, 8, 8, 64, 8, 9, 5, 2000.0, True),
+    ([(1, 5000), (1, 40), (1, 900)], False, 14, 1, 128, 32, 300, 40, 0.0, True),
+    ([(2, 5000), (2, 40), (2, 900)], True, 8, 1, 128, 8, 1, 1, 0.0, False),
+    ([(1, 900 + 37 * i) for i in range(40)], False, 8, 2, 64, 64, 0, 0, 5.0, False)])
+def test_one_and_two_tokens_over_codes(dev, hold, seqs, trees, h_q, h_kv, d, page, window, sinks, cap, bias):
+    """Calls that few_codes takes: outputs, the pages' new rows, and rows of no sequence."""
+    from ssa_amd import paged_step
+    from tests.dense_oracle import check
+    from tests.test_gpu_bounded_cache import batch, bits, expect, pools_after
+
+    s, keys, parents = batch(84, BF16, seqs, h_q, h_kv, d, page, hold, window, sinks, trees, behind=2)
+    slopes = torch.tensor([2.0 ** (-4.0 * (i + 1) / h_q) for i in range(h_q)]) if bias else None
+    x = {n: t.to(dev) for n, t in s.items()}
+    T = int(s["starts"][-1])
+    out = paged_step(**x, softcap=cap or None, slopes=None if slopes is None else slopes.to(dev), window=window or None, sinks=sinks,
+                     max_new=max(m for m, _ in seqs), max_len=max(m + c for m, c in seqs), check=True)
+    assert not out[T:].any()
+    for b, at, m, (value, bound) in expect(s, keys, parents, seqs, cap=cap, slopes=slopes, window=window, sinks=sinks):
+        check(out[at:at + m], value, bound, f"sequence {b}")
+    for name, want in pools_after(s, seqs, page, hold).items():
+        assert torch.equal(bits(x[name].cpu()), bits(want)), name
