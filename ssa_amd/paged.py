@@ -65,7 +65,7 @@ def paged_step(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Ten
                                     any([t.requires_grad for t in (slopes, out, k_scales, v_scales) if t is not None])):
         raise NotImplementedError("paged_step has no gradient: call it under torch.no_grad(), or detach its inputs")
     _lib.refuse_tangents("paged_step", q, k, v, k_pages, v_pages, slopes, k_scales, v_scales, out)
-    window = 0 if window is None and sinks == 0 else _window(window, sinks)
+    window, sinks = (0, 0) if window is None and sinks == 0 else (_window(window, sinks), min(int(sinks), 1 << 31))
     if softcap is not None and not softcap > 0:
         raise ValueError(f"softcap must be positive, got {softcap}")
     flag = torch.zeros(1, device=q.device, dtype=torch.int32) if check else None

@@ -170,3 +170,26 @@ def test_one_and_two_tokens_over_codes(dev, hold, seqs, trees, h_q, h_kv, d, pag
         check(out[at:at + m], value, bound, f"sequence {b}")
     for name, want in pools_after(s, seqs, page, hold).items():
         assert torch.equal(bits(x[name].cpu()), bits(want)), name
+
+
+@pytest.mark.parametrize("window,sinks", [(1 << 70, 0), (3, 1 << 70), (1 << 31, 1 << 31), (1, 1 << 63)])
+def test_windows_and_first_keys_past_every_key(dev, window, sinks):
+    """They see what a step without them does."""
+    from ssa_amd import PagedKVCache, paged_step
+    from tests.test_gpu_bounded_cache import batch
+
+    for hold in (None, I8):
+        s, _, _ = batch(85, BF16, [(3, 70), (1, 300), (60, 9)], 4, 2, 64, 16, hold)
+        outs = []
+        for kw in ({}, dict(window=window, sinks=sinks)):
+            x = {n: t.to(dev) for n, t in s.items()}
+            outs.append(paged_step(**x, check=True, **kw))
+        assert torch.equal(*outs)
+    x = [torch.randn(40, h, 64, device=dev, dtype=BF16, generator=torch.Generator(device=dev).manual_seed(1)) for h in (4, 2, 2)]
+    outs = []
+    for kw in ({}, dict(window=window, sinks=sinks)):
+        cache = PagedKVCache(10, 16, 2, 64, **kw)
+        a = cache.add()
+        outs.append(torch.cat([cache.step(*x, [a], [40]), cache.step(*[t[:1] for t in x], [a], [1])]))
+        assert cache.free_pages == 7
+    assert torch.equal(*outs)
