@@ -43,6 +43,8 @@ def test_codes_are_read_in_one_rounding(dev, hold):
     scales[:, 0] = 0.022805606946349144
     codes[:, 0, :, 0] = 17
     scales[:, 1], scales[:, 2], scales[:, 3], scales[:, 4], scales[:, 5] = 2.0 ** -126, 1.3e-42, 3.1e36, math.nan, 0.0
+    scales[:, 6:200] = torch.exp2(torch.rand(2, 194, h, generator=g) * 60 - 149)  # (products around 2^-100 and below fp32's)
+    scales[:, 200] = -scales[:, 201]
     pools = [x.view(hold).view(-1, page, h, d).to(dev) for x in codes]
     both = [x.view(-1, page, h).to(dev) for x in scales]
     at = dict(table=torch.arange(T // page, device=dev, dtype=torch.int32)[None],
