@@ -695,7 +695,7 @@ int ssa_rope_axes(const void* q, const void* k, int dtype, int64_t batch, int64_
 
 /* ---- calls with packed arguments ----------------------------------------- */
 
-/* Calls one of the entry points below with its arguments from an array, in order, eight bytes
+/* Calls one of these entry points with its arguments from an array, in order, eight bytes
  * each: integers and pointers as int64_t, floats as double.  For callers to whom each argument
  * costs (a Python call of 50 arguments takes 5 microseconds, one of a packed array 2). */
 #define SSA_CALL_MASK_SPANS 0

@@ -227,14 +227,15 @@ inline int64_t seen_len(int64_t max_len, int64_t max_new, int64_t window, int64_
 
 // Whether a call over pages of 8 bits is one for few_codes: bf16 queries, rows of whole 16-byte pieces
 // where a lane loads 16, at most 16 rows a sequence, and of those at most two new tokens, which it adds one
-// by one.  us of few_rows and few_codes, int8, d = 128, groups of 4 or 1 heads:
+// by one.  us a call (repeated on the same pages) by few_rows and few_codes, int8, d = 128, 4 KV heads of 4
+// query heads, of 1 where 8 tokens are new:
 //   new tokens                 1              2             4             8
-//   32 ragged, up to 8191      102, 69
 //   32 sequences of 4000       51.4, 45.2     52.5, 46.0    54.3, 55.4    55.3, 57.3
 //   32 of 200                  12.8, 12.2     13.0, 12.3    13.8, 15.4    13.1, 20.6
 //   one of 8191                17.8, 18.6     17.9, 16.9    19.0, 19.8    17.8, 24.6
-// (32 and 64 equal ones of 8191 129 and 130, 231 and 240.)  A call with a longer sequence takes few_rows for
-// its single tokens too: 32 ragged ones beside a chunk of 40 over 4096 137 us, by themselves 69 and 35.
+// and single tokens of 32 / 8 heads: 32 ragged sequences of up to 8191 115, 102, 32 and 64 equal ones 129, 130
+// and 231, 240.  A longer sequence in the call sends its single tokens to few_rows too: 32 ragged ones (of
+// 268 MB, which the caches hold in part) and a chunk of 40 over 4096 137 us in one call, 69 and 35 in two.
 inline bool codes_call(int dtype, int page_dtype, int64_t max_new, int64_t g, int d) {
   const bool held = page_dtype == SSA_DTYPE_I8 || page_dtype == SSA_DTYPE_E4M3;
   return held && dtype == SSA_DTYPE_BF16 && max_new <= 2 && max_new * g <= 16 && (d <= 64 || d % 16 == 0);
@@ -256,8 +257,8 @@ inline PagedPlan paged_plan(int dtype, int64_t tokens, int64_t batch, int h_q, i
   // Few rows: parts of at least 256 keys, enough for two blocks a CU twice over
   // where the batch has sequences of unlike lengths to even out, once for one.
   const int64_t blocks = batch * h_kv;
-  // (few_codes runs three blocks a CU: 1536 of them take the 32 ragged sequences of int8 111 to 98 us,
-  // 2048 or more the same or worse, 32 of 8191 tokens 138 to 129 and 141)
+  // (few_codes runs three blocks a CU: 1536 of them take 0.88 of 1024's time for 32 ragged sequences of int8,
+  // 0.93 for 32 of 8191 tokens, 2048 or more the same or worse)
   int64_t s = div_up(batch > 1 ? (codes ? 1536 : 1024) : 512, blocks), most = div_up(max_len, 256);
   s = s < most ? s : most;
   s = s > 1 ? s : 1;

@@ -30,6 +30,11 @@
 // than 8 (in log2): weights then reach 2^8, which costs fp32 sums and bf16
 // weights no relative precision, and most tiles rescale nothing.
 //
+// Of bf16 calls a weight (over 8-bit pages times its value's scale) is rounded to bf16 for its
+// product with V, half a step of 2^-8 of it, as few_rows and few_codes do; scores, sums of weights and the
+// products' sums are fp32.  An output is within 0.0024 of its scale of 64 bits so, its own rounding
+// alone is 0.0017; products of fp32 weights run at an eighth of the rate.
+//
 // A masked key's weight is 0, but 0 times an infinity or NaN in its value row is
 // not: a row whose accumulators end up other than finite is computed again key
 // by key (exact_row), reading visible keys only.

@@ -26,6 +26,9 @@
 // and on packed documents by blocks of unlike lengths: twelve in 8192 tokens 0.22 ms
 // (dQ) and 0.44 ms (dK, dV), 0.43 PFLOP/s.
 //
+// Of bf16 calls P and dS are rounded to bf16 (half a step, 2^-8 of each) for the products that make dV, dQ
+// and dK, whose sums are fp32; scores, dO . V and D are fp32.
+//
 // Rows that see two intervals (kTwo: a sliding window and a document's first keys): dQ walks
 // the tiles of both.  For dK and dV the first keys of a document are seen by all of its rows
 // and others by a window of them, 14 times as few where 16384 rows see 1024 keys back, so that
